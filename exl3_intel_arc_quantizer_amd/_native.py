@@ -78,6 +78,23 @@ _SIGNATURES = {
     "exl3_block_fold": (_c_int, [_c_vp, _c_vp, _c_vp, _c_i64, _c_vp]),
     "exl3_ldlq_gather": (_c_int, [_c_vp, _c_int, _c_i64, _c_vp, _c_vp]),
     "exl3_ldlq_scatter": (_c_int, [_c_vp, _c_int, _c_i64, _c_vp, _c_vp, _c_vp]),
+    # the attention cache of include/exl3_layer.h
+    "exl3_rotary": (_c_int, [_c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_int,
+                             _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_int, _c_i64,
+                             _c_int, _c_int, _c_vp, _c_int, _c_vp, _c_int, _c_int, _c_float,
+                             _c_int, _c_vp]),
+    "exl3_plan_step": (_c_int, [_c_vp, _c_vp, _c_int, _c_vp, _c_int, _c_vp, _c_int, _c_vp, _c_int,
+                                _c_i64, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp]),
+    "exl3_cache_append": (_c_int, [_c_vp, _c_i64, _c_i64, _c_vp, _c_int, _c_vp, _c_i64, _c_i64,
+                                   _c_vp, _c_i64, _c_i64, _c_i64, _c_int, _c_vp, _c_vp, _c_int,
+                                   _c_vp, _c_int, _c_int, _c_float, _c_vp, _c_i64, _c_int, _c_int,
+                                   _c_int, _c_vp]),
+    "exl3_cache_read": (_c_int, [_c_vp, _c_i64, _c_int, _c_int, _c_int, _c_vp, _c_i64, _c_int,
+                                 _c_vp, _c_vp, _c_vp]),
+    "exl3_cache_attention_workspace": (_c_i64, [_c_int, _c_int]),
+    "exl3_cache_attention": (_c_int, [_c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_int, _c_int, _c_vp,
+                                      _c_i64, _c_int, _c_int, _c_int, _c_vp, _c_int, _c_vp, _c_vp,
+                                      _c_int, _c_float, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp]),
 }
 
 
@@ -887,3 +904,214 @@ def extension() -> QuantizeExtension:
     if _EXT is None:
         _EXT = QuantizeExtension()
     return _EXT
+
+
+# ------------------------------------------------- the 4-bit attention cache
+
+def _types() -> dict:
+    torch = _torch()
+    return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _rows(t, name: str, like=None, heads=None, dim=None) -> None:
+    """A (tokens, heads, head_dim) GPU tensor whose last axis is contiguous."""
+    torch = _torch()
+    if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.dim() != 3:
+        raise RuntimeError(f"{name} must be a 3-D GPU (cuda) tensor (tokens, heads, head_dim)")
+    if t.dtype not in _types():
+        raise RuntimeError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
+    if t.size(2) > 1 and t.stride(2) != 1:
+        raise RuntimeError(f"the last axis of {name} must be contiguous")
+    if like is not None and (t.device != like.device or t.dtype != like.dtype
+                             or t.size(0) != like.size(0)):
+        raise RuntimeError(f"{name} must have the device, type and tokens of the other rows")
+    if (heads is not None and t.size(1) != heads) or (dim is not None and t.size(2) != dim):
+        raise RuntimeError(f"{name} must have {heads if heads is not None else 'any'} heads of "
+                           f"{dim} values, got {tuple(t.shape)}")
+
+
+def _vector(t, name: str, dtypes: tuple, numel, device) -> None:
+    torch = _torch()
+    if (not isinstance(t, torch.Tensor) or t.device != device or t.dtype not in dtypes
+            or t.dim() != 1 or not t.is_contiguous() or (numel is not None and t.numel() != numel)):
+        raise RuntimeError(f"{name} must be a contiguous vector of "
+                           f"{'any length' if numel is None else numel}, "
+                           f"{' or '.join(map(str, dtypes))}, on {device}")
+
+
+def _pages(pages) -> tuple:
+    """(pages, page size, kv heads, head dim) of a cache."""
+    torch = _torch()
+    if (not isinstance(pages, torch.Tensor) or pages.device.type != "cuda" or pages.dim() != 4
+            or pages.dtype != torch.uint8 or not pages.is_contiguous()):
+        raise RuntimeError("pages must be a contiguous 4-D uint8 GPU (cuda) tensor "
+                           "(pages, kv_heads, page_size / 32, 36 * head_dim)")
+    n, heads, tiles, size = pages.shape
+    if size not in (2304, 4608, 9216) or tiles not in (1, 2, 4, 8) or heads < 1:
+        raise RuntimeError(f"pages of shape {tuple(pages.shape)} are no cache: head_dim 64, 128 "
+                           "or 256 (36 * head_dim bytes a tile), page_size 32, 64, 128 or 256")
+    return n, 32 * tiles, heads, size // 36
+
+
+def _run(device, what: str, call, *args) -> None:
+    """One C call on the current stream of ``device``."""
+    torch = _torch()
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            _check(call(*args, torch.cuda.current_stream(device).cuda_stream), what)
+    else:
+        _check(call(*args, torch.cuda.current_stream(device).cuda_stream), what)
+
+
+def rotary(q, k, positions, frequencies, layout: int, magnitude: float, inverse: bool,
+           out=None) -> tuple:
+    """q and k turned by their positions (exl3_rotary); k may be None."""
+    torch = _torch()
+    _rows(q, "q")
+    tokens, heads, dim = q.shape
+    if k is not None:
+        _rows(k, "k", q, None, dim)
+    _vector(positions, "positions", (torch.int32, torch.int64), tokens, q.device)
+    _vector(frequencies, "frequencies", (torch.float64,), None, q.device)
+    pairs = frequencies.numel()
+    if not 1 <= pairs <= dim // 2:
+        raise RuntimeError(f"frequencies must hold 1 to {dim // 2} pairs, got {pairs}")
+    if out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    else:
+        q_out, k_out = out
+        _rows(q_out, "out[0]", q, heads, dim)
+        if k is not None:
+            _rows(k_out, "out[1]", q, k.size(1), dim)
+    sq, so = q.stride(), q_out.stride()
+    if k is None:
+        k_args = (None, 0, 0, None, 0, 0, 0)
+    else:
+        sk, sp = k.stride(), k_out.stride()
+        k_args = (k.data_ptr(), sk[0], sk[1], k_out.data_ptr(), sp[0], sp[1], k.size(1))
+    _run(q.device, "apply_rotary", load_library().exl3_rotary, q.data_ptr(), sq[0], sq[1],
+         q_out.data_ptr(), so[0], so[1], heads, *k_args, tokens, dim, _types()[q.dtype],
+         positions.data_ptr(), int(positions.dtype == torch.int64), frequencies.data_ptr(), pairs,
+         layout, float(magnitude), int(inverse))
+    return q_out, k_out if k is not None else None
+
+
+def plan_step(cached, new, tables, free_pages, taken, page_size: int, max_tokens: int) -> tuple:
+    """Slots, positions, starts, lengths, taken and status (exl3_plan_step)."""
+    torch = _torch()
+    dev = tables.device if isinstance(tables, torch.Tensor) else None
+    if (dev is None or dev.type != "cuda" or tables.dim() != 2 or tables.dtype != torch.int32
+            or not tables.is_contiguous()):
+        raise RuntimeError("tables must be a contiguous 2-D int32 GPU (cuda) tensor")
+    requests, width = tables.shape
+    _vector(cached, "cached", (torch.int32,), requests, dev)
+    _vector(new, "new", (torch.int32,), requests, dev)
+    _vector(free_pages, "free_pages", (torch.int32,), None, dev)
+    _vector(taken, "taken", (torch.int32,), 1, dev)
+    if not 0 <= max_tokens < 2 ** 31:
+        raise RuntimeError(f"max_tokens must be in 0..2^31 - 1, got {max_tokens}")
+    slots = torch.empty(max_tokens, dtype=torch.int64, device=dev)
+    ints = torch.empty(max_tokens + 2 * requests + 3, dtype=torch.int32, device=dev)
+    positions, starts, lengths, taken_out, status = ints.split(
+        [max_tokens, requests + 1, requests, 1, 1])
+    _run(dev, "plan_step", load_library().exl3_plan_step, cached.data_ptr(), new.data_ptr(),
+         requests, tables.data_ptr(), width, free_pages.data_ptr(), free_pages.numel(),
+         taken.data_ptr(), page_size, max_tokens, slots.data_ptr(), positions.data_ptr(),
+         starts.data_ptr(), lengths.data_ptr(), taken_out.data_ptr(), status.data_ptr())
+    return slots, positions, starts, lengths, taken_out, status
+
+
+def cache_append(pages, k, v, slots, q, positions, frequencies, layout: int, magnitude: float):
+    """k and v into the cache, k (and q) turned first (exl3_cache_append);
+    returns the turned q."""
+    torch = _torch()
+    n, page_size, heads, dim = _pages(pages)
+    _rows(k, "k", None, heads, dim)
+    _rows(v, "v", k, heads, dim)
+    tokens = k.size(0)
+    if k.device != pages.device:
+        raise RuntimeError("k and v must be on the cache's device")
+    _vector(slots, "slots", (torch.int64,), tokens, pages.device)
+    # The kernel reads 16 bytes at a time; rows that start elsewhere are copied.
+    k, v = _wide(k), _wide(v)
+    pairs, wide, freq, at = 0, 0, None, None
+    q_out, q_args = None, (None, 0, 0, None, 0)
+    if frequencies is not None:
+        _vector(frequencies, "frequencies", (torch.float64,), None, pages.device)
+        pairs = frequencies.numel()
+        if pairs % 8 or not 8 <= pairs <= dim // 2:
+            raise RuntimeError(f"frequencies must hold a multiple of 8 pairs up to {dim // 2}, got "
+                               f"{pairs}: turn with apply_rotary first")
+        _vector(positions, "positions", (torch.int32, torch.int64), tokens, pages.device)
+        wide, freq, at = int(positions.dtype == torch.int64), frequencies.data_ptr(), positions.data_ptr()
+        if q is not None:
+            _rows(q, "q", k, None, dim)
+            q = _wide(q)
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            q_args = (q.data_ptr(), q.stride(0), q.stride(1), q_out.data_ptr(), q.size(1))
+    elif q is not None or positions is not None:
+        raise RuntimeError("q and positions are only taken with frequencies")
+    _run(pages.device, "append_tokens", load_library().exl3_cache_append, *q_args,
+         k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), tokens,
+         _types()[k.dtype], slots.data_ptr(), at, wide, freq, pairs, layout, float(magnitude),
+         pages.data_ptr(), n, page_size, heads, dim)
+    return q_out
+
+
+def _wide(t):
+    """``t``, or a copy of it, with every row 16-byte aligned."""
+    size = t.element_size()
+    if t.data_ptr() % 16 or t.stride(0) * size % 16 or t.stride(1) * size % 16:
+        return t.clone(memory_format=_torch().contiguous_format)
+    return t
+
+
+def cache_read(pages, slots, dtype) -> tuple:
+    """Keys and values at ``slots`` (exl3_cache_read)."""
+    torch = _torch()
+    n, page_size, heads, dim = _pages(pages)
+    _vector(slots, "slots", (torch.int64,), None, pages.device)
+    if dtype not in _types():
+        raise RuntimeError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
+    tokens = slots.numel()
+    k = torch.empty((tokens, heads, dim), dtype=dtype, device=pages.device)
+    v = torch.empty_like(k)
+    _run(pages.device, "read_tokens", load_library().exl3_cache_read, pages.data_ptr(), n,
+         page_size, heads, dim, slots.data_ptr(), tokens, _types()[dtype], k.data_ptr(),
+         v.data_ptr())
+    return k, v
+
+
+def cache_attention(q, pages, tables, starts, lengths, scale, window, max_new):
+    """Attention over the cache (exl3_cache_attention)."""
+    torch = _torch()
+    n, page_size, heads, dim = _pages(pages)
+    dev = pages.device
+    _rows(q, "q", None, None, dim)
+    if q.dtype == torch.float32 or q.device != dev:
+        raise RuntimeError("q must be float16 or bfloat16, on the cache's device")
+    tokens, q_heads, _ = q.shape
+    if q_heads < 1 or q_heads % heads:
+        raise RuntimeError(f"q must have a multiple of the cache's {heads} heads, got {q_heads}")
+    if (not isinstance(tables, torch.Tensor) or tables.device != dev or tables.dim() != 2
+            or tables.dtype != torch.int32 or not tables.is_contiguous()):
+        raise RuntimeError(f"tables must be a contiguous 2-D int32 tensor on {dev}")
+    requests, width = tables.shape
+    _vector(starts, "starts", (torch.int32,), requests + 1, dev)
+    _vector(lengths, "lengths", (torch.int32,), requests, dev)
+    if window is not None and window < 1:
+        raise RuntimeError(f"window must be positive, got {window}")
+    if max_new is not None and max_new < 0:
+        raise RuntimeError(f"max_new must not be negative, got {max_new}")
+    q = _wide(q)
+    lib = load_library()
+    out = torch.empty((tokens, q_heads, dim), dtype=q.dtype, device=dev)
+    size = lib.exl3_cache_attention_workspace(requests, dim)
+    workspace = torch.empty(max(size, 0), dtype=torch.uint8, device=dev)
+    _run(dev, "cache_attention", lib.exl3_cache_attention, q.data_ptr(), q.stride(0), q.stride(1),
+         out.data_ptr(), tokens, q_heads, _types()[q.dtype], pages.data_ptr(), n, page_size, heads,
+         dim, tables.data_ptr(), width, starts.data_ptr(), lengths.data_ptr(), requests,
+         dim ** -0.5 if scale is None else float(scale), 2 ** 31 - 1 if window is None else
+         int(window), tokens if max_new is None else int(max_new), workspace.data_ptr(), size)
+    return out

@@ -6,6 +6,8 @@
  * buffers owned by the caller, nothing allocated, work enqueued on `stream`
  * (a hipStream_t, NULL = the null stream), 0 on success and a message in
  * exl3_last_error() otherwise. Matrices are float32, row-major, contiguous.
+ * The last section holds the operators of a served model's 4-bit attention
+ * cache.
  */
 #ifndef EXL3_LAYER_H
 #define EXL3_LAYER_H
@@ -200,6 +202,94 @@ int exl3_ldlq_gather(const exl3_ldlq_block* blocks, int nblocks, int64_t tiles, 
  * states[t][p] = idx[tile0 + t][p]. */
 int exl3_ldlq_scatter(const exl3_ldlq_block* blocks, int nblocks, int64_t tiles,
                       const float* recon, const int16_t* idx, void* stream);
+
+/* ---- The 4-bit attention cache of a served model (no counterpart in the
+ * reference). Element types: 0 float32, 1 float16, 2 bfloat16. Rows are
+ * (tokens, heads, head_dim) tensors whose last axis is contiguous, given by
+ * their first element and the strides of tokens and heads in elements.
+ *
+ * A cache is num_pages x kv_heads x (page_size / 32) tiles of 36 head_dim
+ * bytes: page_size 32, 64, 128 or 256 tokens, head_dim 64, 128 or 256. A group
+ * of 32 values x is held as y = H x / 8 (H the Sylvester matrix of order 32,
+ * entries +-1), s = float16(bfloat16(max|y| / 7)), at most 9344, and codes
+ * clamp(rint(y / s), -7, 7) + 8 in 4 bits; it stands for H ((code - 8) s) / 4.
+ * A group with an infinity or a NaN is held as NaN. A tile of 32 tokens of one
+ * kv head:
+ *   16 head_dim bytes  key codes: dwords [token][j 0..3][group] of dims
+ *                      32 group + 8 j .. + 7, dim 2 u in nibble u and
+ *                      dim 2 u + 1 in nibble u + 4
+ *   16 head_dim bytes  value codes: dwords [token / 8][r][token % 8] of dims
+ *                      8 r .. 8 r + 7 in nibble order
+ *    2 head_dim bytes  key scales: float16 [token][group]
+ *    2 head_dim bytes  value scales: float16 [token / 8][group][token % 8]
+ * The slot of a token is page * page_size + its position in the page. ---- */
+
+/* Rotary positions of queries and keys in one launch: of every head's values
+ * the pairs (i, i + pairs) (layout 0) or (2 i, 2 i + 1) (layout 1), i < pairs,
+ *   y1 = magnitude (x1 cos a - x2 sin a), y2 = magnitude (x2 cos a + x1 sin a),
+ * a = position * frequencies[i] (`inverse`: -a, which gives the gradient);
+ * the other head_dim - 2 pairs values are copied. positions: int32, or int64
+ * if wide_positions. Angles are taken in 64 bits, sums in 32. Outputs may be
+ * the inputs. q_heads or k_heads may be 0, its pointers NULL. */
+int exl3_rotary(const void* q, int64_t q_token, int64_t q_head, void* q_out, int64_t qo_token,
+                int64_t qo_head, int q_heads, const void* k, int64_t k_token, int64_t k_head,
+                void* k_out, int64_t ko_token, int64_t ko_head, int k_heads, int64_t tokens,
+                int head_dim, int type, const void* positions, int wide_positions,
+                const double* frequencies, int pairs, int layout, float magnitude, int inverse,
+                void* stream);
+
+/* The tables of one serving step from the requests' lengths (cached: tokens
+ * held, fresh: new ones; negative counts as 0; at most 4096 requests). A
+ * request holds ceil(cached / page_size) pages in its row of `tables`
+ * (requests x width) and takes those its new tokens need from free_pages,
+ * from *taken on; the new entries are written into the row, -1 once the
+ * free_count entries are used up. Writes, for token t of max_tokens in request
+ * order, slots[t] and positions[t] (its place in the request); -1 and 0 past
+ * the last, slot -1 where no page is; starts [requests + 1], the prefix sums
+ * of fresh; lengths [requests] = cached + fresh; taken_out = *taken plus the
+ * pages used; status: 1 pages ran out, 2 a request outgrew its row, 4 more
+ * tokens than max_tokens, added up. */
+int exl3_plan_step(const int32_t* cached, const int32_t* fresh, int requests, int32_t* tables,
+                   int width, const int32_t* free_pages, int free_count, const int32_t* taken,
+                   int page_size, int64_t max_tokens, int64_t* slots, int32_t* positions,
+                   int32_t* starts, int32_t* lengths, int32_t* taken_out, int32_t* status,
+                   void* stream);
+
+/* Writes token t's keys and values to slots[t]; slots outside the cache are
+ * skipped, and no slot may be given twice. With pairs > 0 (a multiple of 8)
+ * the keys, and q_heads queries beside them into q_out (contiguous), first
+ * turn by their positions as in exl3_rotary; keys stay in 32 bits between.
+ * Rows are 16-byte aligned. */
+int exl3_cache_append(const void* q, int64_t q_token, int64_t q_head, void* q_out, int q_heads,
+                      const void* k, int64_t k_token, int64_t k_head, const void* v,
+                      int64_t v_token, int64_t v_head, int64_t tokens, int type,
+                      const int64_t* slots, const void* positions, int wide_positions,
+                      const double* frequencies, int pairs, int layout, float magnitude,
+                      void* pages, int64_t num_pages, int page_size, int kv_heads, int head_dim,
+                      void* stream);
+
+/* The keys and values that the entries at `slots` stand for, contiguous
+ * (tokens, kv_heads, head_dim); zeros for slots outside the cache. */
+int exl3_cache_read(const void* pages, int64_t num_pages, int page_size, int kv_heads, int head_dim,
+                    const int64_t* slots, int64_t tokens, int type, void* k, void* v, void* stream);
+
+/* Bytes of workspace that exl3_cache_attention needs, or -1. */
+int64_t exl3_cache_attention_workspace(int requests, int head_dim);
+
+/* Attention of new tokens over the cache. Request r's queries are rows
+ * starts[r] .. starts[r + 1] - 1 of q (float16 or bfloat16), its last of
+ * lengths[r] positions; each attends its own position and the window - 1
+ * before it: out = sum softmax(scale q . k) v, (tokens, q_heads, head_dim)
+ * contiguous. Query head h reads kv head h / (q_heads / kv_heads). Rows that
+ * attend nothing and rows of no request are 0; positions whose table entry
+ * names no page of the cache are not attended. max_new, the most new tokens of
+ * a request, only chooses kernels: results do not depend on it. */
+int exl3_cache_attention(const void* q, int64_t q_token, int64_t q_head, void* out, int64_t tokens,
+                         int q_heads, int type, const void* pages, int64_t num_pages, int page_size,
+                         int kv_heads, int head_dim, const int32_t* tables, int width,
+                         const int32_t* starts, const int32_t* lengths, int requests, float scale,
+                         int64_t window, int64_t max_new, void* workspace, int64_t workspace_bytes,
+                         void* stream);
 
 #ifdef __cplusplus
 }
