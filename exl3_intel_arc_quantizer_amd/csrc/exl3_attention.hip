@@ -18,6 +18,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "../../include/exl3_layer.h"
@@ -41,18 +42,27 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr float NONE = -__builtin_inff();
 constexpr int THREADS = 256, WAVES = THREADS / 64;
 
+// One launch of a kernel over the requests with `low` to `high` query rows to
+// a kv head, in blocks of `rows`.
+struct Class {
+  int low, high, rows;
+  int whole;                     // every owner takes one segment, none is cut
+  int owners;                    // else: shares that the work is cut into
+  float* partials;               // [2 owners][rows][D + 2]: values, then maximum and sum
+  int64_t* shares;               // [requests + 1] prefix of the work, for the join
+};
+
 struct AttendArgs {
   const uint16_t* q;
   uint16_t* out;                 // (tokens, q_heads, D) contiguous
   const uint8_t* pages;
   const int32_t *tables, *starts, *lengths;
-  float* partials;               // [2 shares][rows][D + 2]: values, then maximum and sum
-  int64_t* shares;               // [requests + 1] prefix of the work, for the join
   int64_t q_token, q_head, tokens, window;
   CacheShape cache;
   int requests, width, q_heads, group;
-  int waves;                     // shares that the work is cut into
   float scale;
+  int classes;
+  Class of[2];
 };
 
 // What a request asks for, every figure bounded by the arrays' sizes whatever
@@ -75,24 +85,33 @@ __device__ __forceinline__ Request request_of(const AttendArgs& a, int r) {
   return q;
 }
 
-// A segment is one kv head and block of ROWS query rows of a request. Its work
-// is its tiles, and before them what beginning and ending it costs, as tiles:
-// a share of many short segments would end late without.
+// A segment is one kv head and block of query rows of a request. Its work is
+// its tiles, and before them what beginning and ending it costs, as tiles: a
+// share of many short segments would end late without. (A ragged batch of 128
+// requests: 107 us at 8, 115 at 4, 130 at 2, 108 at 12.) Where segments are
+// taken whole the work is their number.
 constexpr int SEGMENT_COST = 8;
-template <int ROWS>
-__device__ __forceinline__ int64_t work_of(const AttendArgs& a, const Request& q) {
-  const int64_t blocks = ((int64_t)q.n * a.group + ROWS - 1) / ROWS;
-  return q.tiles ? blocks * a.cache.kv_heads * (q.tiles + SEGMENT_COST) : 0;
+__device__ __forceinline__ int blocks_of(const AttendArgs& a, const Class& c, const Request& q) {
+  return (int)(((int64_t)q.n * a.group + c.rows - 1) / c.rows);
+}
+__device__ __forceinline__ bool takes(const AttendArgs& a, const Class& c, const Request& q) {
+  const int64_t rows = (int64_t)q.n * a.group;
+  return q.tiles && rows >= c.low && rows <= c.high;
+}
+__device__ __forceinline__ int64_t work_of(const AttendArgs& a, const Class& c, const Request& q) {
+  if (!takes(a, c, q)) return 0;
+  const int64_t blocks = blocks_of(a, c, q);
+  return a.cache.kv_heads * blocks * (c.whole ? 1 : q.tiles + SEGMENT_COST);
 }
 
 // prefix[r] = work before request r, prefix[requests] = all of it.
-template <int ROWS>
-__device__ __forceinline__ void sum_work(const AttendArgs& a, int64_t* prefix, int64_t* parts) {
+template <int NTHREADS>
+__device__ __forceinline__ void sum_work(const AttendArgs& a, const Class& c, int64_t* prefix, int64_t* parts) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int64_t base = 0;
-  for (int r0 = 0; r0 < a.requests; r0 += THREADS) {
+  for (int r0 = 0; r0 < a.requests; r0 += NTHREADS) {
     const int r = r0 + tid;
-    int64_t v = r < a.requests ? work_of<ROWS>(a, request_of(a, r)) : 0;
+    int64_t v = r < a.requests ? work_of(a, c, request_of(a, r)) : 0;
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) {
       const int64_t w = __shfl_up(v, o);
@@ -103,7 +122,7 @@ __device__ __forceinline__ void sum_work(const AttendArgs& a, int64_t* prefix, i
     __syncthreads();
     int64_t before = base;
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) {
+    for (int i = 0; i < NTHREADS / 64; ++i) {
       if (i < wave) before += parts[i];
       base += parts[i];
     }
@@ -120,10 +139,10 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
   return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
-// The work is cut into equal shares, one a wave, of LEAST at least.
+// The work is cut into equal shares, one an owner, of LEAST at least.
 constexpr int LEAST = 2;
-__device__ __forceinline__ int64_t share_of(const AttendArgs& a, int64_t all) {
-  return max((all + a.waves - 1) / a.waves, (int64_t)LEAST);
+__device__ __forceinline__ int64_t share_of(const Class& c, int64_t all) {
+  return max((all + c.owners - 1) / c.owners, (int64_t)LEAST);
 }
 
 // Last index i of [0, n) with at[i] <= x; at[0] <= x.
@@ -201,6 +220,14 @@ __device__ __forceinline__ void lane_butterfly(float& x, float& y) {
   swap(x, y);
 }
 
+// A tile as a buffer: loads then take its base from scalar registers and a
+// 32-bit offset, where pointers cost two registers and an addition a load. The
+// buffer ends with the tile.
+template <int D>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_resource(const uint8_t* tile) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(tile), 0, 36 * D, 0x00027000);
+}
+
 // One tile's registers of a lane: row token of quarter j for the keys; dword
 // columns r (and r + 16) of octet j for the values.
 template <int D>
@@ -244,8 +271,13 @@ struct Tile {
   }
 };
 
-// Workgroups of a compute unit that a variant's registers allow.
-constexpr int resident(int d, int ct) { return d == 64 ? (ct == 1 ? 4 : 3) : d == 128 ? (ct == 1 ? 3 : 2) : (ct == 1 ? 2 : 1); }
+// The variants of attend_rows_kernel: CT column tiles of 8 rows, each with
+// what float16 leaves of it beside it, or (WIDE) of 16 rows. Workgroups of a
+// compute unit that a variant's registers allow:
+constexpr int resident(int d, bool wide, int ct) {
+  if (wide) return 2;
+  return d == 64 ? (ct == 1 ? 4 : 3) : d == 128 ? (ct == 1 ? 3 : 2) : (ct == 1 ? 2 : 1);
+}
 
 // Every wave takes one share of all work, an equal run of tiles that may end
 // one segment and begin others: segments that it holds whole it finishes,
@@ -259,25 +291,30 @@ constexpr int resident(int d, int ct) { return d == 64 ? (ct == 1 ? 4 : 3) : d =
 // No score crosses lanes but for the maximum. A block of 8 rows fills half of
 // the 16 columns; the other half takes what float16 leaves of the same rows:
 // q = hi + lo and p = hi + lo in columns n and n + 8, so queries and weights
-// count with 22 bits at no further product. The running maximum moves only
-// where a row's tile maximum passes it by 8 (in powers of two: weights stay
-// under 2^8), one vote a tile; then the rows agree across lanes on a new one.
-// Sums and outputs are float32.
+// count with 22 bits at no further product. WIDE blocks have all columns for
+// rows: weights count with 11 bits, and so do bfloat16 queries, which have 8
+// of their own (errors under 2^-11 of the output's terms, which its own
+// rounding of 2^-9 covers); float16 queries keep their rest in products of
+// their own. The running maximum moves only where a row's tile maximum passes
+// it by 8 (in powers of two: weights stay under 2^8), one vote a tile; then
+// the rows agree across lanes on a new one. Sums and outputs are float32.
 //
 // Two tiles' registers take turns: one is loaded while the other is
 // multiplied, and table entries are read a tile further ahead.
-template <int D, int CT, bool BF16>
-__global__ void __launch_bounds__(THREADS, resident(D, CT)) attend_rows_kernel(AttendArgs a) {
-  constexpr int ROWS = 8 * CT, GROUPS = D / 32, SETS = Tile<D>::SETS, NIB = D == 64 ? 4 : 8;
+template <int D, bool WIDE, int CT, bool BF16>
+__global__ void __launch_bounds__(THREADS, resident(D, WIDE, CT)) attend_rows_kernel(AttendArgs a, int index) {
+  constexpr int PER = WIDE ? 16 : 8, ROWS = PER * CT, GROUPS = D / 32, SETS = Tile<D>::SETS, NIB = D == 64 ? 4 : 8;
+  constexpr bool REST = WIDE && !BF16;                   // products of the queries' rest
   extern __shared__ int64_t prefix[];                    // [requests + 1]
   __shared__ int64_t parts[WAVES];
 
+  const Class& cls = a.of[index];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Magic magic;
-  sum_work<ROWS>(a, prefix, parts);
+  sum_work<THREADS>(a, cls, prefix, parts);
   if (blockIdx.x == 0)
-    for (int r = tid; r <= a.requests; r += THREADS) a.shares[r] = prefix[r];
-  const int64_t all = uniform(prefix[a.requests]), share = share_of(a, all);
+    for (int r = tid; r <= a.requests; r += THREADS) cls.shares[r] = prefix[r];
+  const int64_t all = uniform(prefix[a.requests]), share = share_of(cls, all);
   const int owner = (int)blockIdx.x * WAVES + wave;
   const int64_t begin = owner * share, end = min(begin + share, all);
 
@@ -288,21 +325,44 @@ __global__ void __launch_bounds__(THREADS, resident(D, CT)) attend_rows_kernel(A
     asm volatile("" : "+v"(lane));
     const int n = lane & 15, j = lane >> 4;
     // The minus one of columns 8..15, which take what columns 0..7 leave.
-    const float rest = n & 8 ? -1.0f : 0.0f;
-    // The segment (request, head, block of rows) that `at` lies in.
+    const float rest = !WIDE && n & 8 ? -1.0f : 0.0f;
+    // The segment (request, head, block of rows) that `at` lies in, and the
+    // tiles of it that are this wave's.
     const int r = __builtin_amdgcn_readfirstlane(last_at_most(prefix, a.requests + 1, at));
     const Request req = request_of(a, r);
+    const int blocks = blocks_of(a, cls, req), rows = req.n * a.group;
     const int64_t before = uniform(prefix[r]);
-    const uint32_t in_request = (uint32_t)(at - before);
-    const int segment = (int)(in_request / (uint32_t)(req.tiles + SEGMENT_COST));
-    const int blocks = (req.n * a.group + ROWS - 1) / ROWS;
+    const int segment = (int)((uint32_t)(at - before) / (uint32_t)(req.tiles + SEGMENT_COST));
     const int head = segment / blocks, block = segment - head * blocks;
     const int64_t seg0 = before + (int64_t)segment * (req.tiles + SEGMENT_COST) + SEGMENT_COST;
-    const int64_t seg1 = seg0 + req.tiles;               // its tiles in the row of all work
+    const int64_t seg1 = seg0 + req.tiles;
     const int first = (int)max(at - seg0, (int64_t)0), past = (int)(min(end, seg1) - seg0);
     at = min(end, seg1);
     if (past <= first) continue;
-    const int t0 = req.tile0 + first, t1 = req.tile0 + past;
+    const bool whole = past - first == req.tiles;
+    float* part = cls.partials + ((int64_t)owner * 2 + (first == 0)) * (ROWS * (D + 2));
+    // The block's rows attend positions low .. last; what all of them attend,
+    // most_from .. least_last, needs no mask.
+    const int row0 = block * ROWS, row1 = min(row0 + ROWS, rows) - 1;
+    const int least_last = req.length - req.n + row0 / a.group, most_last = req.length - req.n + row1 / a.group;
+    const int low = (int)max((int64_t)least_last - a.window + 1, (int64_t)0);
+    const int most_from = (int)max((int64_t)most_last - a.window + 1, (int64_t)0);
+    const int t0 = max(req.tile0 + first, low / CACHE_TILE);
+    const int t1 = min(req.tile0 + past, most_last < 0 ? 0 : most_last / CACHE_TILE + 1);
+    if (t1 <= t0) {
+      // Nothing to attend in this share.
+      for (int i = lane; i <= row1 - row0; i += 64) {
+        if (!whole) part[ROWS * D + 2 * i] = NONE, part[ROWS * D + 2 * i + 1] = 0.0f;
+      }
+      if (whole) {
+        for (int i = lane; i < (row1 - row0 + 1) * (D / 4); i += 64) {
+          const int of = row0 + i / (D / 4);
+          uint16_t* out = a.out + ((int64_t)(req.first + of / a.group) * a.q_heads + head * a.group + of % a.group) * D;
+          reinterpret_cast<u32x2*>(out)[i % (D / 4)] = u32x2{0u, 0u};
+        }
+      }
+      continue;
+    }
 
     // In the constant address space: read by the scalar unit.
     const auto* table = (const __attribute__((address_space(4))) int32_t*)(a.tables + (int64_t)r * a.width);
@@ -319,15 +379,14 @@ __global__ void __launch_bounds__(THREADS, resident(D, CT)) attend_rows_kernel(A
     int page_even = page_of(t0), page_odd = page_of(t0 + 1);
     even.load(tile_at(t0, page_even), lane);
 
-    // Queries: hi in columns 0..7, lo in 8..15, scaled by a power of two so
-    // that float16 holds them whatever the type's range.
-    u32x4 qf[CT][GROUPS];
+    // Queries, scaled by a power of two so that float16 holds them whatever
+    // the type's range; hi in columns 0..7 and lo in 8..15 of narrow blocks.
+    u32x4 qf[CT][GROUPS], ql[REST ? CT : 1][REST ? GROUPS : 1];
     float qs[CT], rise[CT];
     int last[CT], from[CT];                              // positions this lane's row attends
-    const int rows = req.n * a.group;
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
-      const int row = block * ROWS + c * 8 + (n & 7);
+      const int row = row0 + c * PER + (WIDE ? n : n & 7);
       const bool there = row < rows;
       const int i = there ? row / a.group : 0, g = there ? row - i * a.group : 0;
       const uint16_t* src = a.q + (int64_t)(req.first + i) * a.q_token +
@@ -360,22 +419,23 @@ __global__ void __launch_bounds__(THREADS, resident(D, CT)) attend_rows_kernel(A
         for (int e = 0; e < 4; ++e) {
           const float y0 = flip * ldexpf(x[k][2 * e], -power), y1 = flip * ldexpf(x[k][2 * e + 1], -power);
           const f16x2 hi = {(_Float16)y0, (_Float16)y1};
-          qf[c][k][e] = bits_of(f16x2{(_Float16)__builtin_fmaf((float)hi[0], rest, y0),
-                                      (_Float16)__builtin_fmaf((float)hi[1], rest, y1)});
+          if constexpr (WIDE)
+            qf[c][k][e] = bits_of(hi);
+          else
+            qf[c][k][e] = bits_of(f16x2{(_Float16)__builtin_fmaf((float)hi[0], rest, y0),
+                                        (_Float16)__builtin_fmaf((float)hi[1], rest, y1)});
+          if constexpr (REST) ql[c][k][e] = bits_of(f16x2{(_Float16)(y0 - (float)hi[0]), (_Float16)(y1 - (float)hi[1])});
         }
       }
       // An eighth from the query's transform, 2 from both; log2(e) for powers
       // of two.
-      qs[c] = ldexpf(fabsf(a.scale) * 0.25f * 1.4426950408889634f, power);
+      // (At least 2^-120: a scale of 0 weighs all positions alike.)
+      qs[c] = fmaxf(ldexpf(fabsf(a.scale) * 0.25f * 1.4426950408889634f, power), 0x1p-120f);
       rise[c] = 8.0f / qs[c];
       last[c] = there ? req.length - req.n + i : -1;
-      const int64_t low = there ? (int64_t)last[c] - a.window + 1 : 0;
-      from[c] = (int)max(low, (int64_t)0);
+      const int64_t from64 = there ? (int64_t)last[c] - a.window + 1 : 0;
+      from[c] = (int)max(from64, (int64_t)0);
     }
-    // Positions that all rows of the block attend need no mask.
-    const int row0 = block * ROWS, row1 = min(row0 + ROWS, rows) - 1;
-    const int least_last = req.length - req.n + row0 / a.group;
-    const int most_from = (int)max((int64_t)(req.length - req.n + row1 / a.group) - a.window + 1, (int64_t)0);
 
     float run[CT], sum[CT];                              // run: the maximum before the factor qs
     f32x4 o[CT][SETS * NIB];
@@ -408,7 +468,10 @@ __global__ void __launch_bounds__(THREADS, resident(D, CT)) attend_rows_kernel(A
           f[2] = values_of<true>(w >> 8, scale, magic);
           f[3] = values_of<false>(w >> 8, scale, magic);
 #pragma unroll
-          for (int c = 0; c < CT; ++c) s[c][u] = mfma(f, qf[c][k], s[c][u]);
+          for (int c = 0; c < CT; ++c) {
+            s[c][u] = mfma(f, qf[c][k], s[c][u]);
+            if constexpr (REST) s[c][u] = mfma(f, ql[c][k], s[c][u]);
+          }
         }
       }
 
@@ -420,7 +483,7 @@ __global__ void __launch_bounds__(THREADS, resident(D, CT)) attend_rows_kernel(A
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float v = s[c][e >> 2][e & 3];
-          x[e] = v + other_half(v);
+          x[e] = WIDE ? v : v + other_half(v);
         }
         if (masked) {
           attended[c] = 0;
@@ -455,8 +518,11 @@ __global__ void __launch_bounds__(THREADS, resident(D, CT)) attend_rows_kernel(A
             sum[c] += w[h];
           }
           const f16x2 hi = {(_Float16)w[0], (_Float16)w[1]};
-          p[c][e] = bits_of(f16x2{(_Float16)__builtin_fmaf((float)hi[0], rest, w[0]),
-                                  (_Float16)__builtin_fmaf((float)hi[1], rest, w[1])});
+          if constexpr (WIDE)
+            p[c][e] = bits_of(hi);
+          else
+            p[c][e] = bits_of(f16x2{(_Float16)__builtin_fmaf((float)hi[0], rest, w[0]),
+                                    (_Float16)__builtin_fmaf((float)hi[1], rest, w[1])});
         }
       }
 
@@ -487,8 +553,8 @@ __global__ void __launch_bounds__(THREADS, resident(D, CT)) attend_rows_kernel(A
           u32x4 lo, hi;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const uint32_t first = tile.v[d][e >> 1][(2 * e) & 3], second = tile.v[d][e >> 1][(2 * e + 1) & 3];
-            const uint32_t w = __builtin_amdgcn_perm(first, second, pick);
+            const uint32_t one = tile.v[d][e >> 1][(2 * e) & 3], other = tile.v[d][e >> 1][(2 * e + 1) & 3];
+            const uint32_t w = __builtin_amdgcn_perm(one, other, pick);
             const f16x2 scale = halves_of(scales[e]);
             lo[e] = values_of<true>(w, scale, magic);
             hi[e] = values_of<false>(w, scale, magic);
@@ -534,15 +600,13 @@ __global__ void __launch_bounds__(THREADS, resident(D, CT)) attend_rows_kernel(A
     // The result: hi and lo columns together, taken back from the transformed
     // basis. Lane (n, j) holds dims 8 (4 j + e) + m of row n: whole groups of
     // D >= 128, half a group of D = 64.
-    const bool whole = past - first == req.tiles;
-    float* part = a.partials + ((int64_t)owner * 2 + (first == 0)) * (ROWS * (D + 2));
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       sum[c] += __shfl_xor(sum[c], 16);
       sum[c] += __shfl_xor(sum[c], 32);
       const float inverse = sum[c] == 0.0f ? 0.0f : 1.0f / sum[c];
-      const int row = c * 8 + n, of = block * ROWS + row;
-      const bool writes = n < 8 && of < rows;
+      const int row = c * PER + n, of = row0 + row;
+      const bool writes = n < PER && of < rows;
       if (writes && !whole && j == 0) {
         part[ROWS * D + 2 * row] = run[c] == NONE ? NONE : run[c] * qs[c];
         part[ROWS * D + 2 * row + 1] = sum[c];
@@ -551,10 +615,12 @@ __global__ void __launch_bounds__(THREADS, resident(D, CT)) attend_rows_kernel(A
 #pragma unroll
       for (int d = 0; d < SETS; ++d) {
         f32x4* v = &o[c][d * NIB];
+        if constexpr (!WIDE) {
 #pragma unroll
-        for (int m = 0; m < NIB; ++m)
+          for (int m = 0; m < NIB; ++m)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[m][e] += other_half(v[m][e]);
+            for (int e = 0; e < 4; ++e) v[m][e] += other_half(v[m][e]);
+        }
 #pragma unroll
         for (int h = 1; h < NIB; h *= 2)
 #pragma unroll
@@ -596,111 +662,584 @@ __global__ void __launch_bounds__(THREADS, resident(D, CT)) attend_rows_kernel(A
   }
 }
 
-// The partial results of an output row (token, query head) that more than one
-// wave has taken, joined in the order of the tiles; rows of no work are 0;
-// whole ones are left. The maxima are read first, 64 at once, so that the
-// values are then summed by known weights and no load waits for another.
-// SPREAD waves take one row's partials in turn: all four of a workgroup where
-// there are few rows, each with many partials (one token of 4097 positions, 32
-// rows: 5.6 us, with one wave a row 9.8), one where there are many rows (128
-// tokens, 4096 rows: 13.7 us with four).
-template <int D, int CT, bool BF16, int SPREAD>
-__global__ void __launch_bounds__(THREADS) attend_join_kernel(AttendArgs a) {
-  constexpr int ROWS = 8 * CT, PER = D / 64, STRIDE = ROWS * (D + 2);
-  typedef float values __attribute__((ext_vector_type(PER)));
-  __shared__ float held[WAVES][SPREAD > 1 ? D : 1], sums[WAVES];
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Many query rows to a kv head (chunks and prompts): a workgroup takes a block
+// of 32 rows a wave, and unpacks two tiles at a time, as float16, into shared
+// memory, where all its waves read them.
+//
+// The same products as above at 32 x 32 x 16: S^T = K Q^T in one accumulator
+// of 32 tokens x 32 rows a tile, O^T += V^T P^T in D / 32. Lane (n, h) of S^T
+// holds row n's scores of positions 8 b + 4 h + x of the product's rows; keys
+// lie in shared memory with bits 2 and 3 of their token exchanged, so that
+// these are tokens 16 c + 8 h .. + 7, the eight that the lane's operand of P^T
+// wants. Sixteen-byte vectors of a key row (of a value dim) are permuted by the
+// low bits of the row (the dim), so that the sixteen lanes that read in one
+// cycle read different banks. Two tiles a step, because the products of one tile's scores
+// wait for each other. Two buffers and one barrier a step: while one is
+// multiplied the next is unpacked, and the codes after it are on their way.
+//
+// Weights, and bfloat16 queries, count with 11 bits (errors under 2^-11 of the
+// output's terms); float16 queries keep their rest in products of their own.
+constexpr int tile_waves(int d) { return d == 128 ? 8 : 4; }
+constexpr int tile_groups(int d) { return d == 64 ? 3 : 1; }  // workgroups of a compute unit
+template <int D, bool BF16>
+__global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_waves(D) / 4)
+    attend_tiles_kernel(AttendArgs a, int index) {
+  constexpr int NW = tile_waves(D), NT = 64 * NW, ROWS = 32 * NW, GROUPS = D / 32, STEPS = D / 16;
+  constexpr bool REST = !BF16;
+  // Parts of a step's two tiles: a dword of key codes, and two dims (a byte) of
+  // four tokens' values. A thread takes KN of them, a wave's always of one tile.
+  constexpr int AHEAD = 2;
+  constexpr int PARTS = 4 * D, KN = 2 * PARTS / NT, INNER = PARTS > NT ? PARTS / NT : 1;
+  constexpr int SPAN = D == 64 ? 7 : 15;                 // vectors of a key row that are permuted, less one
+  constexpr uint32_t TILE = 64 * D;                      // bytes of a tile's keys, and of its values
+  extern __shared__ int64_t prefix[];                    // [requests + 1]
+  __shared__ int64_t parts[NW];
+  __shared__ u32x4 keys[4 * TILE / 16], values[4 * TILE / 16];  // [buffer][tile]
+  __shared__ int poison[2];
+
+  const Class& cls = a.of[index];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t at = (int64_t)blockIdx.x * (WAVES / SPREAD) + wave / SPREAD;
-  if (at >= a.tokens * a.q_heads) return;
-  const int64_t token = at / a.q_heads;
-  const int qh = (int)(at - token * a.q_heads);
-  uint16_t* out = a.out + at * D + PER * lane;
-  auto write = [&](const float (&x)[PER], float l) {
+  const int n = lane & 31, h = lane >> 5;
+  const Magic magic;
+  sum_work<NT>(a, cls, prefix, parts);
+  const int64_t all = uniform(prefix[a.requests]);
+  const int owner = blockIdx.x;
+  int64_t begin = owner, end = min(begin + 1, all);
+  if (!cls.whole) {
+    if (owner == 0)
+      for (int r = tid; r <= a.requests; r += NT) cls.shares[r] = prefix[r];
+    const int64_t share = share_of(cls, all);
+    begin = owner * share, end = min(begin + share, all);
+  }
+  // A thread's places in a tile (byte, half of the octet, dword column and
+  // octet of a value part) and its operands' in shared memory, opaque so that
+  // they stay one register each.
+  const uint32_t part0 = tid % PARTS;
+  uint32_t key_at = 4 * part0, key_scale_at = 32 * D + (part0 / (D / 8) * GROUPS + part0 % GROUPS) * 2;
+  uint32_t value_at = 16 * D + part0 / 4 * 16;
+  uint32_t value_scale_at = 34 * D + ((part0 / D * GROUPS + part0 / 8 % (D / 8) / 4) * 2 + (part0 / 4 & 1)) * 8;
+  uint32_t key_row = n * (2 * D) + (h ^ (n & SPAN)) * 16, value_row = n * 64 + (h ^ (n >> 2 & 3)) * 16;
+  asm volatile("" : "+v"(key_at), "+v"(key_scale_at), "+v"(value_at), "+v"(value_scale_at), "+v"(key_row), "+v"(value_row));
+  if (tid < 2) poison[tid] = -1;
+  int count = 0;                                         // steps so far; names a buffer's content
+
+  for (int64_t at = begin; at < end;) {
+    const int r = __builtin_amdgcn_readfirstlane(last_at_most(prefix, a.requests + 1, at));
+    const Request req = request_of(a, r);
+    const int blocks = blocks_of(a, cls, req), rows = req.n * a.group;
+    const int64_t before = uniform(prefix[r]);
+    int head, block, first = 0, past = req.tiles;
+    if (cls.whole) {
+      // The longest blocks first, heads next to each other: workgroups are
+      // dealt to the chip's eight dies in turn, so that 8 kv heads' keys and
+      // values lie in one die's cache each.
+      const uint32_t unit = (uint32_t)(at - before), heads = (uint32_t)a.cache.kv_heads;
+      block = blocks - 1 - (int)(unit / heads), head = (int)(unit % heads);
+      at = end;
+    } else {
+      const int segment = (int)((uint32_t)(at - before) / (uint32_t)(req.tiles + SEGMENT_COST));
+      head = segment / blocks, block = segment - head * blocks;
+      const int64_t seg0 = before + (int64_t)segment * (req.tiles + SEGMENT_COST) + SEGMENT_COST;
+      const int64_t seg1 = seg0 + req.tiles;
+      first = (int)max(at - seg0, (int64_t)0), past = (int)(min(end, seg1) - seg0);
+      at = min(end, seg1);
+      if (past <= first) continue;
+    }
+    const bool whole = past - first == req.tiles;
+    float* part = cls.partials + ((int64_t)owner * 2 + (first == 0)) * (ROWS * (D + 2));
+    const int row0 = block * ROWS, row1 = min(row0 + ROWS, rows) - 1;
+    const int offset = req.length - req.n;
+    const int least_last = offset + row0 / a.group, most_last = offset + row1 / a.group;
+    const int low = (int)max((int64_t)least_last - a.window + 1, (int64_t)0);
+    const int most_from = (int)max((int64_t)most_last - a.window + 1, (int64_t)0);
+    const int t0 = max(req.tile0 + first, low / CACHE_TILE);
+    const int t1 = min(req.tile0 + past, most_last < 0 ? 0 : most_last / CACHE_TILE + 1);
+
+    // This wave's rows and what they attend.
+    const int row = 32 * wave + n;
+    const bool there = row0 + row < rows;
+    const int token = there ? (row0 + row) / a.group : 0, of_group = there ? row0 + row - token * a.group : 0;
+    const int last = there ? offset + token : -1;
+    const int from = there ? (int)max((int64_t)last - a.window + 1, (int64_t)0) : 0;
+    const int wave0 = min(row0 + 32 * wave, row1), wave1 = min(row0 + 32 * wave + 31, row1);
+    const int wave_least = offset + wave0 / a.group, wave_most = offset + wave1 / a.group;
+    const int wave_from = (int)max((int64_t)wave_most - a.window + 1, (int64_t)0);
+
+    const auto* table = (const __attribute__((address_space(4))) int32_t*)(a.tables + (int64_t)r * a.width);
+    // The page of a tile; -1 past the share's tiles and where the table names
+    // no page of the cache: none of its positions is attended.
+    auto page_of = [&](int t) {
+      const int id = table[min(t, t1 - 1) >> a.cache.tile_shift];
+      return t < t1 && (uint32_t)id < (uint64_t)a.cache.pages ? id : -1;
+    };
+    auto bytes_of = [&](int t, int page) {
+      return a.pages + exl3::cache_tile_at(a.cache, max(page, 0), head, min(t, t1 - 1) & ((1 << a.cache.tile_shift) - 1));
+    };
+    // The codes and scales of this thread's parts of a step.
+    uint32_t kc[KN], ks[KN];
+    u32x4 vc[KN];
+    u32x2 vs[KN];
+    auto tile_of = [&](int u) { return (u * NT + 64 * wave) / PARTS; };
+    auto fetch = [&](int t, int page0, int page1) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < KN; ++u) {
+        const auto tile = tile_resource<D>(bytes_of(t + tile_of(u), tile_of(u) ? page1 : page0));
+        const int i = u % INNER;
+        kc[u] = __builtin_amdgcn_raw_buffer_load_b32(tile, key_at + i * (4 * NT), 0, 0);
+        ks[u] = __builtin_amdgcn_raw_buffer_load_b16(tile, key_scale_at + i * (NT / (D / 8) * GROUPS * 2), 0, 0);
+        vc[u] = __builtin_amdgcn_raw_buffer_load_b128(tile, value_at + i * (4 * NT), 0, 0);
+        vs[u] = __builtin_amdgcn_raw_buffer_load_b64(tile, value_scale_at + i * (NT / D * GROUPS * 16), 0, 0);
+      }
+    };
+    auto unpack = [&](int buffer) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < KN; ++u) {
+        const uint32_t d = part0 + u % INNER * NT, base = (2 * buffer + tile_of(u)) * (TILE / 16);
+        {
+          const uint32_t token = d / (D / 8), inside = d % (D / 8);
+          const uint32_t vector = 4 * (inside % GROUPS) + inside / GROUPS;
+          // Bits 2 and 3 of the token exchanged.
+          const uint32_t to = (token & 0x13) | (token & 4) << 1 | (token & 8) >> 1;
+          const f16x2 scale = halves_of(ks[u] | ks[u] << 16);
+          u32x4 f;
+          f[0] = values_of<true>(kc[u], scale, magic);
+          f[1] = values_of<false>(kc[u], scale, magic);
+          f[2] = values_of<true>(kc[u] >> 8, scale, magic);
+          f[3] = values_of<false>(kc[u] >> 8, scale, magic);
+          keys[base + to * (D / 8) + (vector ^ (to & SPAN))] = f;
+        }
+        const uint32_t byte = d & 3, four = d / 4, octet = d / D, column = d / 8 % (D / 8);
+        const uint32_t pick = 0x0c000c04u | byte << 16 | byte;
+        u32x2 lo, hi;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t w = __builtin_amdgcn_perm(vc[u][2 * e], vc[u][2 * e + 1], pick);
+          const f16x2 scale = halves_of(vs[u][e]);
+          lo[e] = values_of<true>(w, scale, magic);
+          hi[e] = values_of<false>(w, scale, magic);
+        }
+        const uint32_t dim = 8 * column + 2 * byte;      // dims 4 x .. 4 x + 3 permute alike
+        u32x2* to = reinterpret_cast<u32x2*>(&values[base + dim * 4 + (octet ^ (dim >> 2 & 3))]) + (four & 1);
+        to[0] = lo, to[8] = hi;
+      }
+    };
+    // A weight of 0 must not meet a NaN or infinity: in steps that some row
+    // does not attend whole, such scales of values count as 0, and the rows
+    // that do attend their tokens are seen to after the product.
+    auto partial = [&](int t, int page0, int page1) {
+      return t * CACHE_TILE < most_from || t * CACHE_TILE + 2 * CACHE_TILE - 1 > least_last || (page0 | page1) < 0;
+    };
+    auto clean = [&](int buffer, int name) {
+#pragma unroll
+      for (int u = 0; u < KN; ++u) {
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t bits = vs[u][e / 2] >> (16 * (e & 1)) & 0x7fffu;
+          if (bits >= 0x7c00u) {
+            bad = true;
+            vs[u][e / 2] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
+          }
+        }
+        if (bad) poison[buffer] = name;
+        asm volatile("" : "+v"(vs[u]));
+      }
+    };
+
+    // Pages of this step's tiles and of the next two steps'.
+    int page0[3], page1[3];
+    if (t0 < t1) {
+#pragma unroll
+      for (int i = 0; i < 3; ++i) page0[i] = page_of(t0 + 2 * i), page1[i] = page_of(t0 + 2 * i + 1);
+      fetch(t0, page0[0], page1[0]);
+    }
+
+    // Queries, scaled by a power of two so that float16 holds them.
+    u32x4 qf[STEPS], ql[REST ? STEPS : 1];
+    float qs, rise;
+    {
+      const uint16_t* src = a.q + (int64_t)(req.first + token) * a.q_token + (int64_t)(head * a.group + of_group) * a.q_head;
+      float x[STEPS][8], top = 0.0f;
+#pragma unroll
+      for (int k = 0; k < STEPS; ++k) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(src + 16 * k + 8 * h);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[k][e] = there ? widen<BF16>(w[e / 2] >> (16 * (e & 1)) & 0xffffu) : 0.0f;
+        exl3::butterfly8(x[k]);
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) lane_butterfly<32>(x[k][e], x[k][e + 1]);
+      }
+#pragma unroll
+      for (int k = 0; k < STEPS; k += 2)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float y = x[k][e], z = x[k + 1][e];
+          x[k][e] = y + z, x[k + 1][e] = y - z;
+          top = fmaxf(top, fmaxf(fabsf(y + z), fabsf(y - z)));
+        }
+      top = fmaxf(top, __shfl_xor(top, 32));
+      int power = 0;
+      if (top > 0.0f && top < __builtin_inff()) frexpf(top, &power);
+      const float flip = a.scale < 0.0f ? -1.0f : 1.0f;
+#pragma unroll
+      for (int k = 0; k < STEPS; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float y0 = flip * ldexpf(x[k][2 * e], -power), y1 = flip * ldexpf(x[k][2 * e + 1], -power);
+          const f16x2 hi = {(_Float16)y0, (_Float16)y1};
+          qf[k][e] = bits_of(hi);
+          if constexpr (REST) ql[k][e] = bits_of(f16x2{(_Float16)(y0 - (float)hi[0]), (_Float16)(y1 - (float)hi[1])});
+        }
+      qs = fmaxf(ldexpf(fabsf(a.scale) * 0.25f * 1.4426950408889634f, power), 0x1p-120f);
+      rise = 8.0f / qs;
+    }
+
+    float run = NONE, sum = 0.0f;
+    f32x16 o[GROUPS];
+#pragma unroll
+    for (int d = 0; d < GROUPS; ++d) o[d] = f32x16{};
+
+    // This lane's vectors of a key row and a value dim: the permutation is an
+    // exclusive or of address bits, so one address serves all of a buffer.
+    auto key = [&](int k, uint32_t place) {
+      return *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(keys) + ((key_row + place) ^ (2 * k & SPAN) << 4) + (2 * k & ~SPAN) * 16);
+    };
+    auto value = [&](int v, uint32_t place) {
+      return *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(values) + ((value_row + place) ^ (v & 1) << 5) + (v >> 1) * 2048);
+    };
+    if (t0 < t1) {
+      if (partial(t0, page0[0], page1[0])) clean(count & 1, count);
+      unpack(count & 1);
+      fetch(t0 + 2, page0[1], page1[1]);
+      __syncthreads();
+    }
+    for (int t = t0; t < t1; t += 2) {
+      const int now = count & 1, then = now ^ 1, pos = t * CACHE_TILE;
+      const int page0_after = page_of(t + 6), page1_after = page_of(t + 7);
+      if (partial(t + 2, page0[1], page1[1])) clean(then, count + 1);
+      const uint32_t place = now * (2 * TILE);
+      // Operands are read from shared memory AHEAD products before their use.
+      // The barriers to the scheduler keep that: left alone it reads each right
+      // before its product, to save registers, and every product waits for the
+      // whole latency (a prompt of 8192 tokens: 647 us).
+      f32x16 s[2] = {};
+      u32x4 f[2][AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) f[0][k] = key(k, place), f[1][k] = key(k, place + TILE);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int k = 0; k < STEPS; ++k) {
+        s[0] = mfma32(f[0][k % AHEAD], qf[k], s[0]);
+        s[1] = mfma32(f[1][k % AHEAD], qf[k], s[1]);
+        if constexpr (REST) {
+          s[0] = mfma32(f[0][k % AHEAD], ql[k], s[0]);
+          s[1] = mfma32(f[1][k % AHEAD], ql[k], s[1]);
+        }
+        if (k + AHEAD < STEPS) {
+          f[0][k % AHEAD] = key(k + AHEAD, place), f[1][k % AHEAD] = key(k + AHEAD, place + TILE);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      float x[32];
+#pragma unroll
+      for (int e = 0; e < 32; ++e) x[e] = s[e >> 4][e & 15];
+      if (pos < wave_from || pos + 2 * CACHE_TILE - 1 > wave_least || (page0[0] | page1[0]) < 0) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const int p = pos + 16 * (e >> 3) + 8 * h + (e & 7);
+          x[e] = p >= from && p <= last && (e < 16 ? page0[0] : page1[0]) >= 0 ? x[e] : NONE;
+          asm volatile("" : "+v"(x[e]));
+        }
+      }
+      float top = x[0];
+#pragma unroll
+      for (int e = 1; e < 32; ++e) top = fmaxf(top, x[e]);
+      if (__any(top > run + rise)) {
+        top = fmaxf(top, run);
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float shrink = top == run ? 1.0f : __builtin_amdgcn_exp2f((run - top) * qs);
+        run = top;
+        sum *= shrink;
+#pragma unroll
+        for (int d = 0; d < GROUPS; ++d) o[d] *= shrink;
+      }
+      const float ref = run == NONE ? 0.0f : -run * qs;
+      // Product v of the output: 16 tokens v / GROUPS, dims of group v % GROUPS.
+      auto operand = [&](int v) { return value(2 * (v % GROUPS) + (v / GROUPS & 1), place + v / GROUPS / 2 * TILE); };
+#pragma unroll
+      for (int v = 0; v < 2 * AHEAD; ++v) f[v & 1][v / 2] = operand(v);
+      __builtin_amdgcn_sched_barrier(0);
+      unpack(then);
+      fetch(t + 4, page0[2], page1[2]);
+      u32x4 p[4];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const f16x2 w = {(_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * e], qs, ref)),
+                         (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * e + 1], qs, ref))};
+        sum = __builtin_amdgcn_fdot2(w, f16x2{1, 1}, sum, false);
+        p[e >> 2][e & 3] = bits_of(w);
+      }
+#pragma unroll
+      for (int v = 0; v < 4 * GROUPS; ++v) {
+        u32x4& w = f[v & 1][v / 2 % AHEAD];
+        o[v % GROUPS] = mfma32(w, p[v / GROUPS], o[v % GROUPS]);
+        if (v + 2 * AHEAD < 4 * GROUPS) {
+          w = operand(v + 2 * AHEAD);
+          if (v & 1) __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+
+      if (poison[now] == count) {
+        // Rows that attend a token whose values of a group are NaN.
+#pragma unroll 1
+        for (int k = 0; k < 2 * CACHE_TILE; ++k) {
+          const int page = k < CACHE_TILE ? page0[0] : page1[0];
+          if (page < 0) continue;
+          const uint8_t* scales = bytes_of(t + k / CACHE_TILE, page) + 34 * D;
+          const bool in = pos + k >= from && pos + k <= last;
+#pragma unroll
+          for (int d = 0; d < GROUPS; ++d) {
+            const uint32_t bits = reinterpret_cast<const uint16_t*>(scales)[((k % CACHE_TILE >> 3) * GROUPS + d) * 8 + (k & 7)];
+            if (in && (bits & 0x7fffu) >= 0x7c00u) o[d] = f32x16{} + __builtin_nanf("");
+          }
+        }
+      }
+      page0[0] = page0[1], page0[1] = page0[2], page0[2] = page0_after;
+      page1[0] = page1[1], page1[1] = page1[2], page1[2] = page1_after;
+      ++count;
+      __syncthreads();
+    }
+
+    // Taken back from the transformed basis: a lane holds dims 32 d + 8 b +
+    // 4 h + x of its row.
+    sum += __shfl_xor(sum, 32);
+    if (there && !whole && h == 0) {
+      part[ROWS * D + 2 * row] = run == NONE ? NONE : run * qs;
+      part[ROWS * D + 2 * row + 1] = sum;
+    }
+    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+    // (From the row again, which is cheaper than two registers in the loop.)
+    int of = row0 + row;
+    asm volatile("" : "+v"(of));
+    uint16_t* out = a.out + ((int64_t)(req.first + of / a.group) * a.q_heads + head * a.group + of % a.group) * D;
+#pragma unroll
+    for (int d = 0; d < GROUPS; ++d) {
+      float v[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] = o[d][e];
+#pragma unroll
+      for (int level = 1; level < 16; level *= 2)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (!(e & level)) {
+            const float y = v[e], z = v[e + level];
+            v[e] = y + z, v[e + level] = y - z;
+          }
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) lane_butterfly<32>(v[e], v[e + 1]);
+      if (!there) continue;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const f32x4 y = 0.25f * f32x4{v[4 * b], v[4 * b + 1], v[4 * b + 2], v[4 * b + 3]};
+        const int dim = 32 * d + 8 * b + 4 * h;
+        if (whole) {
+          u32x2 w;
+          w[0] = narrow<BF16>(y[0] * inverse) | narrow<BF16>(y[1] * inverse) << 16;
+          w[1] = narrow<BF16>(y[2] * inverse) | narrow<BF16>(y[3] * inverse) << 16;
+          *reinterpret_cast<u32x2*>(out + dim) = w;
+        } else {
+          *reinterpret_cast<f32x4*>(part + row * D + dim) = y;
+        }
+      }
+    }
+  }
+}
+
+// The partial results of an output row (token, query head) that more than one
+// owner has taken, joined; rows of no work are 0; whole ones are left. Partials
+// are taken four at a time with a running maximum, so that a row of few waits
+// for memory once. SPREAD waves share one row's partials where there are few
+// rows, each with many; otherwise a wave takes `run` rows one after another
+// (a prompt's are all whole: it only has to see that).
+template <int D, bool BF16, int SPREAD>
+__global__ void __launch_bounds__(SPREAD > 1 ? 64 * SPREAD : THREADS) attend_join_kernel(AttendArgs a, int run) {
+  constexpr int PER = D / 64, BATCH = 4;
+  __shared__ float held[SPREAD][SPREAD > 1 ? D : 1], tops[SPREAD], sums[SPREAD];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t first = SPREAD > 1 ? (int64_t)blockIdx.x : ((int64_t)blockIdx.x * WAVES + wave) * run;
+  const int64_t past = min(first + run, a.tokens * a.q_heads);
+  int64_t token = -1;
+  int r = 0;
+  Request req{};
+  bool work = false;
+  for (int64_t at = first; at < past; ++at) {
+    const int64_t of_token = at / a.q_heads;
+    const int qh = (int)(at - of_token * a.q_heads);
+    if (of_token != token) {
+      // The request: as many starts after the first as are not past the token.
+      token = of_token;
+      r = 0;
+      for (int r0 = 0; r0 < a.requests; r0 += 64)
+        r += __popcll(__ballot(r0 + lane < a.requests && a.starts[r0 + lane + 1] <= token));
+      work = false;
+      if (r < a.requests) {
+        req = request_of(a, r);
+        work = req.tiles && token >= req.first && token < req.first + req.n;
+      }
+    }
+    float x[PER], top = NONE, l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) x[e] = 0.0f;
+    if (work) {
+      const Class& cls = a.of[a.classes == 1 || takes(a, a.of[0], req) ? 0 : 1];
+      if (cls.whole) {
+        // Nor are the token's other rows: on to the next token's first.
+        at = (token + 1) * a.q_heads - 1;
+        continue;
+      }
+      const int head = qh / a.group, of = (int)(token - req.first) * a.group + qh % a.group;
+      const int blocks = blocks_of(a, cls, req), row = of % cls.rows, stride = cls.rows * (D + 2);
+      const int64_t share = share_of(cls, cls.shares[a.requests]);
+      const int64_t seg0 = cls.shares[r] + ((int64_t)head * blocks + of / cls.rows) * (req.tiles + SEGMENT_COST) + SEGMENT_COST;
+      const int64_t seg1 = seg0 + req.tiles;
+      const int w0 = __builtin_amdgcn_readfirstlane((int)(seg0 / share));
+      const int w1 = __builtin_amdgcn_readfirstlane((int)((seg1 - 1) / share));
+      if (w0 == w1) continue;
+      const int stats = cls.rows * D + 2 * row;           // a row's maximum and sum in a slot
+      for (int w = w0 + wave % SPREAD; w <= w1; w += BATCH * SPREAD) {
+        float peak[BATCH], sum[BATCH], v[BATCH][PER];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+          // The first owner's share ends in this segment (slot 1), the others'
+          // begin in it (slot 0).
+          const int own = min(w + i * SPREAD, w1);
+          const float* part = cls.partials + (2 * (int64_t)own + (own == w0)) * stride;
+          peak[i] = part[stats], sum[i] = part[stats + 1];
+#pragma unroll
+          for (int e = 0; e < PER; ++e) v[i][e] = part[row * D + PER * lane + e];
+        }
+        float newer = top;
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) newer = fmaxf(newer, peak[i]);
+        const float keep = top == newer ? 1.0f : __builtin_amdgcn_exp2f(top - newer);
+        top = newer;
+        l *= keep;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) x[e] *= keep;
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+          // A share without an attended position leaves its values unwritten.
+          const bool holds = w + i * SPREAD <= w1 && (peak[i] != NONE || sum[i] != 0.0f);
+          const float weight = peak[i] == NONE ? 1.0f : __builtin_amdgcn_exp2f(peak[i] - newer);
+          l += holds ? sum[i] * weight : 0.0f;
+#pragma unroll
+          for (int e = 0; e < PER; ++e) x[e] += holds ? v[i][e] * weight : 0.0f;
+        }
+      }
+    }
+    if constexpr (SPREAD > 1) {
+      // One row a workgroup: all its waves are here together.
+#pragma unroll
+      for (int e = 0; e < PER; ++e) held[wave][PER * lane + e] = x[e];
+      if (lane == 0) tops[wave] = top, sums[wave] = l;
+      __syncthreads();
+      if (wave != 0) return;
+      top = NONE, l = 0.0f;
+#pragma unroll
+      for (int i = 0; i < SPREAD; ++i) top = fmaxf(top, tops[i]);
+#pragma unroll
+      for (int e = 0; e < PER; ++e) x[e] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < SPREAD; ++i) {
+        const float weight = tops[i] == NONE ? 1.0f : __builtin_amdgcn_exp2f(tops[i] - top);
+        l += sums[i] * weight;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) x[e] += held[i][PER * lane + e] * weight;
+      }
+    }
     const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-    for (int e = 0; e < PER; ++e) out[e] = (uint16_t)narrow<BF16>(x[e] * inverse);
-  };
-  // The request: as many starts after the first as are not past the token.
-  int r = 0;
-  for (int r0 = 0; r0 < a.requests; r0 += 64)
-    r += __popcll(__ballot(r0 + lane < a.requests && a.starts[r0 + lane + 1] <= token));
-  int tiles = 0;
-  Request req{};
-  if (r < a.requests) {
-    req = request_of(a, r);
-    if (token >= req.first && token < req.first + req.n) tiles = req.tiles;
+    for (int e = 0; e < PER; ++e) a.out[at * D + PER * lane + e] = (uint16_t)narrow<BF16>(x[e] * inverse);
   }
-  float x[PER], l = 0.0f;
-#pragma unroll
-  for (int e = 0; e < PER; ++e) x[e] = 0.0f;
-  if (tiles == 0) {
-    if (wave % SPREAD == 0) write(x, l);
-    return;
-  }
-  const int head = qh / a.group, of = (int)(token - req.first) * a.group + qh % a.group;
-  const int blocks = (req.n * a.group + ROWS - 1) / ROWS, row = of % ROWS;
-  const int64_t share = share_of(a, a.shares[a.requests]);
-  const int64_t seg0 = a.shares[r] + ((int64_t)head * blocks + of / ROWS) * (tiles + SEGMENT_COST) + SEGMENT_COST;
-  const int64_t seg1 = seg0 + tiles;
-  const int w0 = (int)(seg0 / share), w1 = (int)((seg1 - 1) / share);
-  if (w0 == w1) return;
-  // The first owner's share ends in this segment (slot 1), the others' begin
-  // in it (slot 0).
-  auto slot = [&](int w) { return a.partials + (2 * (int64_t)w + (w == w0)) * STRIDE; };
-  float top = NONE;
-  for (int w = w0 + lane; w <= w1; w += 64) top = fmaxf(top, slot(w)[ROWS * D + 2 * row]);
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
-#pragma unroll 4
-  for (int w = w0 + wave % SPREAD; w <= w1; w += SPREAD) {
-    const float* part = slot(w);
-    const float peak = part[ROWS * D + 2 * row];
-    const float weight = peak == NONE ? 1.0f : __builtin_amdgcn_exp2f(peak - top);
-    const values v = *reinterpret_cast<const values*>(part + row * D + PER * lane);
-    l += part[ROWS * D + 2 * row + 1] * weight;
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      if constexpr (PER == 1) x[e] += v[0] * weight;
-      else x[e] += v[e] * weight;
-    }
-  }
-  if constexpr (SPREAD > 1) {
-    static_assert(SPREAD == 1 || SPREAD == WAVES, "a row or a workgroup's rows");
-#pragma unroll
-    for (int e = 0; e < PER; ++e) held[wave][PER * lane + e] = x[e];
-    if (lane == 0) sums[wave] = l;
-    __syncthreads();
-    if (wave != 0) return;
-    l = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const int d = PER * lane + e;
-      x[e] = (held[0][d] + held[1][d]) + (held[2][d] + held[3][d]);
-    }
-  }
-  write(x, l);
 }
 
 constexpr int CUS = 256;
 
-struct Plan {
-  int64_t partials, shares;      // bytes
-};
-Plan plan_of(int requests, int head_dim, int ct) {
-  return {(int64_t)2 * CUS * resident(head_dim, ct) * WAVES * 8 * ct * (head_dim + 2) * 4, (8 * ((int64_t)requests + 1) + 15) & ~(int64_t)15};
+// Variants by the query rows that one kv head has of a request (its new tokens
+// times the query heads to a kv head): up to 8 and 16 rows at 22 bits, whose
+// cost is the cache's bytes, then 32 to a wave, then blocks that share the work
+// of unpacking a tile.
+enum Variant { ROWS8, ROWS16, ROWS32, TILES };
+Variant variant_of(int64_t rows, int head_dim) {
+  return rows <= 8 ? ROWS8 : rows <= 16 ? ROWS16 : rows <= 32 && head_dim != 256 ? ROWS32 : TILES;
+}
+int rows_of(Variant v, int head_dim) { return v == TILES ? 32 * tile_waves(head_dim) : 8 << v; }
+// Owners that fill the chip: waves of attend_rows_kernel, workgroups of
+// attend_tiles_kernel.
+int owners_of(Variant v, int head_dim) {
+  if (v == TILES) return tile_groups(head_dim) * CUS;
+  return CUS * WAVES * resident(head_dim, v == ROWS32, v == ROWS8 ? 1 : 2);
+}
+int64_t shares_bytes(int requests) { return (8 * ((int64_t)requests + 1) + 15) & ~(int64_t)15; }
+int64_t partials_bytes(Variant v, int head_dim) {
+  return (int64_t)2 * owners_of(v, head_dim) * rows_of(v, head_dim) * (head_dim + 2) * 4;
 }
 
-template <int D, int CT, bool BF16>
-int launch_attend(AttendArgs args, hipStream_t stream) {
-  args.waves = CUS * resident(D, CT) * WAVES;
+template <int D, bool BF16>
+int launch_variant(Variant v, const AttendArgs& args, int index, unsigned grid, hipStream_t stream) {
   const size_t lds = 8 * ((size_t)args.requests + 1);
+  if (v == ROWS8)
+    attend_rows_kernel<D, false, 1, BF16><<<grid, THREADS, lds, stream>>>(args, index);
+  else if (v == ROWS16)
+    attend_rows_kernel<D, false, 2, BF16><<<grid, THREADS, lds, stream>>>(args, index);
+  else if (v == TILES)
+    attend_tiles_kernel<D, BF16><<<grid, 64 * tile_waves(D), lds, stream>>>(args, index);
+  else if constexpr (D != 256)
+    attend_rows_kernel<D, true, 2, BF16><<<grid, THREADS, lds, stream>>>(args, index);
+  return check_launch("exl3_cache_attention");
+}
+
+template <int D, bool BF16>
+int launch_attend(AttendArgs args, int64_t max_new, char* workspace, hipStream_t stream) {
+  const int64_t most = std::min(max_new, args.tokens) * args.group;
+  const Variant variants[2] = {variant_of(most, D), ROWS8};
+  // Single tokens beside longer requests keep the variant made for them, and
+  // rows of up to 16 their precision.
+  args.classes = args.requests > 1 && variants[0] != ROWS8 ? 2 : 1;
+  const int few = variants[0] == ROWS16 ? 8 : 16;
+  for (int i = 0; i < args.classes; ++i) {
+    Class& c = args.of[i];
+    const Variant v = variants[i];
+    c.rows = rows_of(v, D);
+    c.low = args.classes == 2 && i == 0 ? few + 1 : 1;
+    c.high = args.classes == 2 && i == 1 ? few : INT32_MAX;
+    c.owners = owners_of(v, D);
+    // At most so many segments: whole where they fill the chip twice.
+    const int64_t segments = ((args.tokens * args.group + c.rows - 1) / c.rows + args.requests) * args.cache.kv_heads;
+    c.whole = v == TILES && segments >= 2 * c.owners;
+    c.shares = reinterpret_cast<int64_t*>(workspace);
+    workspace += shares_bytes(args.requests);
+    c.partials = reinterpret_cast<float*>(workspace);
+    workspace += partials_bytes(v, D);
+    const int64_t grid = c.whole ? segments : v == TILES ? c.owners : c.owners / WAVES;
+    if (grid > INT32_MAX) return set_error("exl3_cache_attention: too many tokens");
+    if (launch_variant<D, BF16>(v, args, i, (unsigned)grid, stream)) return 1;
+  }
   const int64_t rows = args.tokens * args.q_heads;
-  attend_rows_kernel<D, CT, BF16><<<CUS * resident(D, CT), THREADS, lds, stream>>>(args);
-  if (check_launch("exl3_cache_attention")) return 1;
-  if (rows <= 4 * CUS)
-    attend_join_kernel<D, CT, BF16, WAVES><<<(unsigned)rows, THREADS, 0, stream>>>(args);
-  else
-    attend_join_kernel<D, CT, BF16, 1><<<(unsigned)((rows + WAVES - 1) / WAVES), THREADS, 0, stream>>>(args);
+  if (rows <= CUS) {
+    attend_join_kernel<D, BF16, 16><<<(unsigned)rows, 64 * 16, 0, stream>>>(args, 1);
+  } else {
+    // Rows to a wave: its token's lookups are for all of them.
+    const int64_t run = std::min<int64_t>(std::max<int64_t>(1, rows / (16 * CUS * WAVES)), 64);
+    const int64_t waves = (rows + run - 1) / run;
+    attend_join_kernel<D, BF16, 1><<<(unsigned)((waves + WAVES - 1) / WAVES), THREADS, 0, stream>>>(args, (int)run);
+  }
   return check_launch("exl3_cache_attention");
 }
 
@@ -711,8 +1250,9 @@ extern "C" {
 int64_t exl3_cache_attention_workspace(int requests, int head_dim) {
   if (requests < 1 || requests > CACHE_MAX_REQUESTS || (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return -1;
-  const Plan one = plan_of(requests, head_dim, 1), two = plan_of(requests, head_dim, 2);
-  return std::max(one.partials, two.partials) + one.shares;
+  int64_t most = 0;
+  for (Variant v : {ROWS16, ROWS32, TILES}) most = std::max(most, partials_bytes(v, head_dim));
+  return 2 * shares_bytes(requests) + partials_bytes(ROWS8, head_dim) + most;
 }
 
 int exl3_cache_attention(const void* q, int64_t q_token, int64_t q_head, void* out, int64_t tokens,
@@ -735,6 +1275,7 @@ int exl3_cache_attention(const void* q, int64_t q_token, int64_t q_head, void* o
   if (tokens < 0 || tokens * q_heads > INT32_MAX) return set_error("exl3_cache_attention: too many tokens");
   if (type < 1 || type > 2) return set_error("exl3_cache_attention: queries are float16 or bfloat16");
   if (window < 1) return set_error("exl3_cache_attention: window must be positive");
+  if (!std::isfinite(scale)) return set_error("exl3_cache_attention: scale must be finite");
   if ((reinterpret_cast<uintptr_t>(q) & 15) || q_token % 8 || q_head % 8)
     return set_error("exl3_cache_attention: query rows must be 16-byte aligned");
   if (((reinterpret_cast<uintptr_t>(pages) | reinterpret_cast<uintptr_t>(workspace)) & 15) ||
@@ -754,15 +1295,10 @@ int exl3_cache_attention(const void* q, int64_t q_token, int64_t q_head, void* o
   a.cache = CacheShape{num_pages, kv_heads, head_dim, shift};
   a.requests = requests, a.width = width, a.q_heads = q_heads, a.group = q_heads / kv_heads;
   a.scale = scale;
-  const bool two = std::min<int64_t>(max_new, tokens) * a.group > 8;
-  const Plan p = plan_of(requests, head_dim, two ? 2 : 1);
-  a.shares = static_cast<int64_t*>(workspace);
-  a.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.shares);
   auto launch = [&](auto dim) {
     constexpr int D = decltype(dim)::value;
-    hipStream_t s = (hipStream_t)stream;
-    if (type == 2) return two ? launch_attend<D, 2, true>(a, s) : launch_attend<D, 1, true>(a, s);
-    return two ? launch_attend<D, 2, false>(a, s) : launch_attend<D, 1, false>(a, s);
+    auto call = type == 2 ? launch_attend<D, true> : launch_attend<D, false>;
+    return call(a, max_new, static_cast<char*>(workspace), (hipStream_t)stream);
   };
   if (head_dim == 64) return launch(std::integral_constant<int, 64>{});
   if (head_dim == 128) return launch(std::integral_constant<int, 128>{});

@@ -136,6 +136,6 @@ def cache_attention(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor,
     ``tables`` does not name are not attended; rows that attend nothing, and
     rows of no request, are 0. ``scale`` defaults to head_dim ** -0.5.
     ``max_new``, the most new tokens of any request where the caller knows it,
-    chooses kernels; results do not depend on its truth."""
+    chooses kernels; results depend on it in rounding at most."""
     _unrecorded("cache_attention", q)
     return _native.cache_attention(q, pages, tables, starts, lengths, scale, window, max_new)

@@ -283,7 +283,7 @@ int64_t exl3_cache_attention_workspace(int requests, int head_dim);
  * contiguous. Query head h reads kv head h / (q_heads / kv_heads). Rows that
  * attend nothing and rows of no request are 0; positions whose table entry
  * names no page of the cache are not attended. max_new, the most new tokens of
- * a request, only chooses kernels: results do not depend on it. */
+ * a request, only chooses kernels: results depend on it in rounding at most. */
 int exl3_cache_attention(const void* q, int64_t q_token, int64_t q_head, void* out, int64_t tokens,
                          int q_heads, int type, const void* pages, int64_t num_pages, int page_size,
                          int kv_heads, int head_dim, const int32_t* tables, int width,
