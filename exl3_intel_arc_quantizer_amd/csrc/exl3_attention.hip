@@ -692,10 +692,15 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
     attend_tiles_kernel(AttendArgs a, int index) {
   constexpr int NW = tile_waves(D), NT = 64 * NW, ROWS = 32 * NW, GROUPS = D / 32, STEPS = D / 16;
   constexpr bool REST = !BF16;
-  // Parts of a step's two tiles: a dword of key codes, and two dims (a byte) of
-  // four tokens' values. A thread takes KN of them, a wave's always of one tile.
+  // Parts of a tile: a dword of key codes, and two dims (a byte) of four tokens'
+  // values. A thread takes KN of them.
   constexpr int AHEAD = 2;
-  constexpr int PARTS = 4 * D, KN = 2 * PARTS / NT, INNER = PARTS > NT ? PARTS / NT : 1;
+  constexpr int KN = 4 * D / NT;
+  // Tiles whose codes a thread holds at a time: one, for fewer registers, or
+  // both of a step, where only one wave fits a SIMD and nothing else hides the
+  // shorter way from load to use (chunks of head dimension 256: 284 us, with
+  // one 427).
+  constexpr int HELD = D == 256 ? 2 : 1;
   constexpr int SPAN = D == 64 ? 7 : 15;                 // vectors of a key row that are permuted, less one
   constexpr uint32_t TILE = 64 * D;                      // bytes of a tile's keys, and of its values
   extern __shared__ int64_t prefix[];                    // [requests + 1]
@@ -720,10 +725,9 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
   // A thread's places in a tile (byte, half of the octet, dword column and
   // octet of a value part) and its operands' in shared memory, opaque so that
   // they stay one register each.
-  const uint32_t part0 = tid % PARTS;
-  uint32_t key_at = 4 * part0, key_scale_at = 32 * D + (part0 / (D / 8) * GROUPS + part0 % GROUPS) * 2;
-  uint32_t value_at = 16 * D + part0 / 4 * 16;
-  uint32_t value_scale_at = 34 * D + ((part0 / D * GROUPS + part0 / 8 % (D / 8) / 4) * 2 + (part0 / 4 & 1)) * 8;
+  uint32_t key_at = 4 * tid, key_scale_at = 32 * D + (tid / (D / 8) * GROUPS + tid % GROUPS) * 2;
+  uint32_t value_at = 16 * D + tid / 4 * 16;
+  uint32_t value_scale_at = 34 * D + ((tid / D * GROUPS + tid / 8 % (D / 8) / 4) * 2 + (tid / 4 & 1)) * 8;
   uint32_t key_row = n * (2 * D) + (h ^ (n & SPAN)) * 16, value_row = n * 64 + (h ^ (n >> 2 & 3)) * 16;
   asm volatile("" : "+v"(key_at), "+v"(key_scale_at), "+v"(value_at), "+v"(value_scale_at), "+v"(key_row), "+v"(value_row));
   if (tid < 2) poison[tid] = -1;
@@ -781,26 +785,28 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
     auto bytes_of = [&](int t, int page) {
       return a.pages + exl3::cache_tile_at(a.cache, max(page, 0), head, min(t, t1 - 1) & ((1 << a.cache.tile_shift) - 1));
     };
-    // The codes and scales of this thread's parts of a step.
-    uint32_t kc[KN], ks[KN];
-    u32x4 vc[KN];
-    u32x2 vs[KN];
-    auto tile_of = [&](int u) { return (u * NT + 64 * wave) / PARTS; };
-    auto fetch = [&](int t, int page0, int page1) __attribute__((always_inline)) {
+    // The codes and scales of this thread's parts of HELD tiles.
+    uint32_t kc[HELD * KN], ks[HELD * KN];
+    u32x4 vc[HELD * KN];
+    u32x2 vs[HELD * KN];
+    auto fetch = [&](int t, int page, int next) __attribute__((always_inline)) {
 #pragma unroll
-      for (int u = 0; u < KN; ++u) {
-        const auto tile = tile_resource<D>(bytes_of(t + tile_of(u), tile_of(u) ? page1 : page0));
-        const int i = u % INNER;
-        kc[u] = __builtin_amdgcn_raw_buffer_load_b32(tile, key_at + i * (4 * NT), 0, 0);
-        ks[u] = __builtin_amdgcn_raw_buffer_load_b16(tile, key_scale_at + i * (NT / (D / 8) * GROUPS * 2), 0, 0);
-        vc[u] = __builtin_amdgcn_raw_buffer_load_b128(tile, value_at + i * (4 * NT), 0, 0);
-        vs[u] = __builtin_amdgcn_raw_buffer_load_b64(tile, value_scale_at + i * (NT / D * GROUPS * 16), 0, 0);
+      for (int w = 0; w < HELD; ++w) {
+        const auto tile = tile_resource<D>(bytes_of(t + w, w ? next : page));
+#pragma unroll
+        for (int u = 0; u < KN; ++u) {
+          kc[w * KN + u] = __builtin_amdgcn_raw_buffer_load_b32(tile, key_at + u * (4 * NT), 0, 0);
+          ks[w * KN + u] = __builtin_amdgcn_raw_buffer_load_b16(tile, key_scale_at + u * (NT / (D / 8) * GROUPS * 2), 0, 0);
+          vc[w * KN + u] = __builtin_amdgcn_raw_buffer_load_b128(tile, value_at + u * (4 * NT), 0, 0);
+          vs[w * KN + u] = __builtin_amdgcn_raw_buffer_load_b64(tile, value_scale_at + u * (NT / D * GROUPS * 16), 0, 0);
+        }
       }
     };
-    auto unpack = [&](int buffer) __attribute__((always_inline)) {
+    // Unpacked to tile `which` of a buffer, and the next.
+    auto unpack = [&](int buffer, int which) __attribute__((always_inline)) {
 #pragma unroll
-      for (int u = 0; u < KN; ++u) {
-        const uint32_t d = part0 + u % INNER * NT, base = (2 * buffer + tile_of(u)) * (TILE / 16);
+      for (int u = 0; u < HELD * KN; ++u) {
+        const uint32_t d = tid + u % KN * NT, base = (2 * buffer + which + u / KN) * (TILE / 16);
         {
           const uint32_t token = d / (D / 8), inside = d % (D / 8);
           const uint32_t vector = 4 * (inside % GROUPS) + inside / GROUPS;
@@ -837,7 +843,7 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
     };
     auto clean = [&](int buffer, int name) {
 #pragma unroll
-      for (int u = 0; u < KN; ++u) {
+      for (int u = 0; u < HELD * KN; ++u) {
         bool bad = false;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -914,15 +920,28 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
       return *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(values) + ((value_row + place) ^ (v & 1) << 5) + (v >> 1) * 2048);
     };
     if (t0 < t1) {
-      if (partial(t0, page0[0], page1[0])) clean(count & 1, count);
-      unpack(count & 1);
+      const bool dirty = partial(t0, page0[0], page1[0]);
+      if (dirty) clean(count & 1, count);
+      unpack(count & 1, 0);
+      if constexpr (HELD == 1) {
+        fetch(t0 + 1, page1[0], -1);
+        if (dirty) clean(count & 1, count);
+        unpack(count & 1, 1);
+      }
       fetch(t0 + 2, page0[1], page1[1]);
       __syncthreads();
     }
     for (int t = t0; t < t1; t += 2) {
       const int now = count & 1, then = now ^ 1, pos = t * CACHE_TILE;
       const int page0_after = page_of(t + 6), page1_after = page_of(t + 7);
-      if (partial(t + 2, page0[1], page1[1])) clean(then, count + 1);
+      // The next step's tiles are unpacked after this one's scores are
+      // multiplied; of two whose codes came one by one, the first before.
+      const bool dirty = partial(t + 2, page0[1], page1[1]);
+      if (dirty) clean(then, count + 1);
+      if constexpr (HELD == 1) {
+        unpack(then, 0);
+        fetch(t + 3, page1[1], -1);
+      }
       const uint32_t place = now * (2 * TILE);
       // Operands are read from shared memory AHEAD products before their use.
       // The barriers to the scheduler keep that: left alone it reads each right
@@ -975,7 +994,8 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
 #pragma unroll
       for (int v = 0; v < 2 * AHEAD; ++v) f[v & 1][v / 2] = operand(v);
       __builtin_amdgcn_sched_barrier(0);
-      unpack(then);
+      if (HELD == 1 && dirty) clean(then, count + 1);
+      unpack(then, HELD == 1);
       fetch(t + 4, page0[2], page1[2]);
       u32x4 p[4];
 #pragma unroll
@@ -1232,8 +1252,10 @@ int launch_attend(AttendArgs args, int64_t max_new, char* workspace, hipStream_t
     if (launch_variant<D, BF16>(v, args, i, (unsigned)grid, stream)) return 1;
   }
   const int64_t rows = args.tokens * args.q_heads;
-  if (rows <= CUS) {
+  if (rows <= 2 * CUS) {
     attend_join_kernel<D, BF16, 16><<<(unsigned)rows, 64 * 16, 0, stream>>>(args, 1);
+  } else if (rows <= 8 * CUS) {
+    attend_join_kernel<D, BF16, 4><<<(unsigned)rows, 64 * 4, 0, stream>>>(args, 1);
   } else {
     // Rows to a wave: its token's lookups are for all of them.
     const int64_t run = std::min<int64_t>(std::max<int64_t>(1, rows / (16 * CUS * WAVES)), 64);
