@@ -908,32 +908,43 @@ def extension() -> QuantizeExtension:
 
 # ------------------------------------------------- the 4-bit attention cache
 
+_TYPES = None
+
+
 def _types() -> dict:
-    torch = _torch()
-    return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    """C codes of the element types that rows may have."""
+    global _TYPES
+    if _TYPES is None:
+        torch = _torch()
+        _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    return _TYPES
 
 
-def _rows(t, name: str, like=None, heads=None, dim=None) -> None:
-    """A (tokens, heads, head_dim) GPU tensor whose last axis is contiguous."""
+def _rows(t, name: str, like=None, heads=None, dim=None) -> tuple:
+    """The shape and strides of a (tokens, heads, head_dim) GPU tensor whose
+    last axis is contiguous."""
     torch = _torch()
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.dim() != 3:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != 3:
         raise RuntimeError(f"{name} must be a 3-D GPU (cuda) tensor (tokens, heads, head_dim)")
     if t.dtype not in _types():
         raise RuntimeError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
-    if t.size(2) > 1 and t.stride(2) != 1:
+    shape, strides = t.shape, t.stride()
+    if strides[2] != 1 and shape[2] > 1:
         raise RuntimeError(f"the last axis of {name} must be contiguous")
-    if like is not None and (t.device != like.device or t.dtype != like.dtype
-                             or t.size(0) != like.size(0)):
+    if like is not None and (t.dtype != like.dtype or shape[0] != like.shape[0]
+                             or t.device != like.device):
         raise RuntimeError(f"{name} must have the device, type and tokens of the other rows")
-    if (heads is not None and t.size(1) != heads) or (dim is not None and t.size(2) != dim):
+    if (heads is not None and shape[1] != heads) or (dim is not None and shape[2] != dim):
         raise RuntimeError(f"{name} must have {heads if heads is not None else 'any'} heads of "
-                           f"{dim} values, got {tuple(t.shape)}")
+                           f"{dim} values, got {tuple(shape)}")
+    return shape, strides
 
 
 def _vector(t, name: str, dtypes: tuple, numel, device) -> None:
     torch = _torch()
-    if (not isinstance(t, torch.Tensor) or t.device != device or t.dtype not in dtypes
-            or t.dim() != 1 or not t.is_contiguous() or (numel is not None and t.numel() != numel)):
+    if (not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.dim() != 1
+            or (numel is not None and t.numel() != numel) or not t.is_contiguous()
+            or t.device != device):
         raise RuntimeError(f"{name} must be a contiguous vector of "
                            f"{'any length' if numel is None else numel}, "
                            f"{' or '.join(map(str, dtypes))}, on {device}")
@@ -954,46 +965,46 @@ def _pages(pages) -> tuple:
 
 
 def _run(device, what: str, call, *args) -> None:
-    """One C call on the current stream of ``device``."""
+    """One C call on the current stream of ``device``. A small call is bound by
+    the host: the stream is read without the Stream object that
+    torch.cuda.current_stream makes (1.9 us), and the device switched only where
+    it is not the current one."""
     torch = _torch()
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
-            _check(call(*args, torch.cuda.current_stream(device).cuda_stream), what)
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        status = call(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        _check(call(*args, torch.cuda.current_stream(device).cuda_stream), what)
+        with torch.cuda.device(device):
+            status = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _check(status, what)
 
 
 def rotary(q, k, positions, frequencies, layout: int, magnitude: float, inverse: bool,
            out=None) -> tuple:
     """q and k turned by their positions (exl3_rotary); k may be None."""
     torch = _torch()
-    _rows(q, "q")
-    tokens, heads, dim = q.shape
-    if k is not None:
-        _rows(k, "k", q, None, dim)
-    _vector(positions, "positions", (torch.int32, torch.int64), tokens, q.device)
-    _vector(frequencies, "frequencies", (torch.float64,), None, q.device)
+    (tokens, heads, dim), sq = _rows(q, "q")
+    device = q.device
+    _vector(positions, "positions", (torch.int32, torch.int64), tokens, device)
+    _vector(frequencies, "frequencies", (torch.float64,), None, device)
     pairs = frequencies.numel()
     if not 1 <= pairs <= dim // 2:
         raise RuntimeError(f"frequencies must hold 1 to {dim // 2} pairs, got {pairs}")
-    if out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    else:
-        q_out, k_out = out
-        _rows(q_out, "out[0]", q, heads, dim)
-        if k is not None:
-            _rows(k_out, "out[1]", q, k.size(1), dim)
-    sq, so = q.stride(), q_out.stride()
-    if k is None:
-        k_args = (None, 0, 0, None, 0, 0, 0)
-    else:
-        sk, sp = k.stride(), k_out.stride()
-        k_args = (k.data_ptr(), sk[0], sk[1], k_out.data_ptr(), sp[0], sp[1], k.size(1))
-    _run(q.device, "apply_rotary", load_library().exl3_rotary, q.data_ptr(), sq[0], sq[1],
+    dense = torch.contiguous_format
+    q_out, k_out = out or (torch.empty_like(q, memory_format=dense), None)
+    so = _rows(q_out, "out[0]", q, heads, dim)[1] if out else (heads * dim, dim)
+    k_args = (None, 0, 0, None, 0, 0, 0)
+    if k is not None:
+        (_, k_heads, _), sk = _rows(k, "k", q, None, dim)
+        if not out:
+            k_out = torch.empty_like(k, memory_format=dense)
+        sp = _rows(k_out, "out[1]", q, k_heads, dim)[1] if out else (k_heads * dim, dim)
+        k_args = (k.data_ptr(), sk[0], sk[1], k_out.data_ptr(), sp[0], sp[1], k_heads)
+    _run(device, "apply_rotary", load_library().exl3_rotary, q.data_ptr(), sq[0], sq[1],
          q_out.data_ptr(), so[0], so[1], heads, *k_args, tokens, dim, _types()[q.dtype],
-         positions.data_ptr(), int(positions.dtype == torch.int64), frequencies.data_ptr(), pairs,
-         layout, float(magnitude), int(inverse))
+         positions.data_ptr(), positions.dtype == torch.int64, frequencies.data_ptr(), pairs,
+         layout, magnitude, inverse)
     return q_out, k_out if k is not None else None
 
 
@@ -1011,10 +1022,9 @@ def plan_step(cached, new, tables, free_pages, taken, page_size: int, max_tokens
     _vector(taken, "taken", (torch.int32,), 1, dev)
     if not 0 <= max_tokens < 2 ** 31:
         raise RuntimeError(f"max_tokens must be in 0..2^31 - 1, got {max_tokens}")
-    slots = torch.empty(max_tokens, dtype=torch.int64, device=dev)
-    ints = torch.empty(max_tokens + 2 * requests + 3, dtype=torch.int32, device=dev)
-    positions, starts, lengths, taken_out, status = ints.split(
-        [max_tokens, requests + 1, requests, 1, 1])
+    slots = tables.new_empty(max_tokens, dtype=torch.int64)
+    positions, starts, lengths, taken_out, status = tables.new_empty(
+        max_tokens + 2 * requests + 3).split([max_tokens, requests + 1, requests, 1, 1])
     _run(dev, "plan_step", load_library().exl3_plan_step, cached.data_ptr(), new.data_ptr(),
          requests, tables.data_ptr(), width, free_pages.data_ptr(), free_pages.numel(),
          taken.data_ptr(), page_size, max_tokens, slots.data_ptr(), positions.data_ptr(),
@@ -1027,43 +1037,46 @@ def cache_append(pages, k, v, slots, q, positions, frequencies, layout: int, mag
     returns the turned q."""
     torch = _torch()
     n, page_size, heads, dim = _pages(pages)
-    _rows(k, "k", None, heads, dim)
-    _rows(v, "v", k, heads, dim)
-    tokens = k.size(0)
-    if k.device != pages.device:
-        raise RuntimeError("k and v must be on the cache's device")
-    _vector(slots, "slots", (torch.int64,), tokens, pages.device)
+    device = pages.device
     # The kernel reads 16 bytes at a time; rows that start elsewhere are copied.
     k, v = _wide(k), _wide(v)
+    (tokens, _, _), sk = _rows(k, "k", None, heads, dim)
+    sv = _rows(v, "v", k, heads, dim)[1]
+    if k.device != device:
+        raise RuntimeError("k and v must be on the cache's device")
+    _vector(slots, "slots", (torch.int64,), tokens, device)
     pairs, wide, freq, at = 0, 0, None, None
     q_out, q_args = None, (None, 0, 0, None, 0)
     if frequencies is not None:
-        _vector(frequencies, "frequencies", (torch.float64,), None, pages.device)
+        _vector(frequencies, "frequencies", (torch.float64,), None, device)
         pairs = frequencies.numel()
         if pairs % 8 or not 8 <= pairs <= dim // 2:
             raise RuntimeError(f"frequencies must hold a multiple of 8 pairs up to {dim // 2}, got "
                                f"{pairs}: turn with apply_rotary first")
-        _vector(positions, "positions", (torch.int32, torch.int64), tokens, pages.device)
-        wide, freq, at = int(positions.dtype == torch.int64), frequencies.data_ptr(), positions.data_ptr()
+        _vector(positions, "positions", (torch.int32, torch.int64), tokens, device)
+        wide, freq, at = positions.dtype == torch.int64, frequencies.data_ptr(), positions.data_ptr()
         if q is not None:
-            _rows(q, "q", k, None, dim)
             q = _wide(q)
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            q_args = (q.data_ptr(), q.stride(0), q.stride(1), q_out.data_ptr(), q.size(1))
+            (_, q_heads, _), sq = _rows(q, "q", k, None, dim)
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            q_args = (q.data_ptr(), sq[0], sq[1], q_out.data_ptr(), q_heads)
     elif q is not None or positions is not None:
         raise RuntimeError("q and positions are only taken with frequencies")
-    _run(pages.device, "append_tokens", load_library().exl3_cache_append, *q_args,
-         k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), tokens,
-         _types()[k.dtype], slots.data_ptr(), at, wide, freq, pairs, layout, float(magnitude),
+    _run(device, "append_tokens", load_library().exl3_cache_append, *q_args,
+         k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1], tokens,
+         _types()[k.dtype], slots.data_ptr(), at, wide, freq, pairs, layout, magnitude,
          pages.data_ptr(), n, page_size, heads, dim)
     return q_out
 
 
 def _wide(t):
-    """``t``, or a copy of it, with every row 16-byte aligned."""
-    size = t.element_size()
-    if t.data_ptr() % 16 or t.stride(0) * size % 16 or t.stride(1) * size % 16:
-        return t.clone(memory_format=_torch().contiguous_format)
+    """A 3-D tensor, or a copy of it, with every row 16-byte aligned; anything
+    else as it is, for the checks to refuse."""
+    torch = _torch()
+    if isinstance(t, torch.Tensor) and t.dim() == 3:
+        size, strides = t.element_size(), t.stride()
+        if t.data_ptr() % 16 or strides[0] * size % 16 or strides[1] * size % 16:
+            return t.clone(memory_format=torch.contiguous_format)
     return t
 
 
@@ -1075,7 +1088,7 @@ def cache_read(pages, slots, dtype) -> tuple:
     if dtype not in _types():
         raise RuntimeError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
     tokens = slots.numel()
-    k = torch.empty((tokens, heads, dim), dtype=dtype, device=pages.device)
+    k = slots.new_empty((tokens, heads, dim), dtype=dtype)
     v = torch.empty_like(k)
     _run(pages.device, "read_tokens", load_library().exl3_cache_read, pages.data_ptr(), n,
          page_size, heads, dim, slots.data_ptr(), tokens, _types()[dtype], k.data_ptr(),
@@ -1088,10 +1101,10 @@ def cache_attention(q, pages, tables, starts, lengths, scale, window, max_new):
     torch = _torch()
     n, page_size, heads, dim = _pages(pages)
     dev = pages.device
-    _rows(q, "q", None, None, dim)
+    q = _wide(q)
+    (tokens, q_heads, _), sq = _rows(q, "q", None, None, dim)
     if q.dtype == torch.float32 or q.device != dev:
         raise RuntimeError("q must be float16 or bfloat16, on the cache's device")
-    tokens, q_heads, _ = q.shape
     if q_heads < 1 or q_heads % heads:
         raise RuntimeError(f"q must have a multiple of the cache's {heads} heads, got {q_heads}")
     if (not isinstance(tables, torch.Tensor) or tables.device != dev or tables.dim() != 2
@@ -1104,12 +1117,11 @@ def cache_attention(q, pages, tables, starts, lengths, scale, window, max_new):
         raise RuntimeError(f"window must be positive, got {window}")
     if max_new is not None and max_new < 0:
         raise RuntimeError(f"max_new must not be negative, got {max_new}")
-    q = _wide(q)
     lib = load_library()
-    out = torch.empty((tokens, q_heads, dim), dtype=q.dtype, device=dev)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     size = lib.exl3_cache_attention_workspace(requests, dim)
-    workspace = torch.empty(max(size, 0), dtype=torch.uint8, device=dev)
-    _run(dev, "cache_attention", lib.exl3_cache_attention, q.data_ptr(), q.stride(0), q.stride(1),
+    workspace = pages.new_empty(max(size, 0))
+    _run(dev, "cache_attention", lib.exl3_cache_attention, q.data_ptr(), sq[0], sq[1],
          out.data_ptr(), tokens, q_heads, _types()[q.dtype], pages.data_ptr(), n, page_size, heads,
          dim, tables.data_ptr(), width, starts.data_ptr(), lengths.data_ptr(), requests,
          dim ** -0.5 if scale is None else float(scale), 2 ** 31 - 1 if window is None else
