@@ -15,6 +15,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/exl3_layer.h"
 #include "exl3_cache_layout.h"
@@ -91,10 +92,11 @@ struct Rows {
 };
 
 // Cosines and sines of one block's tokens, [token][pair], in shared memory:
-// every head of a token turns by the same angles. The angle position *
-// frequency is taken in turns and in 64 bits: a float32 product at position
-// 10^6 would be off by 0.06 radians. Only the fraction of a turn goes on in
-// 32 bits.
+// every head of a token turns by the same angles. Angles and their functions
+// are taken in 64 bits and rounded once: a float32 product at position 10^6
+// would be off by 0.06 radians, and float32 functions of the exact fraction of
+// a turn (1.2e-7) put three times as many rotated keys over the edge to the
+// next code as rounding does.
 __device__ __forceinline__ void turn_table(const void* positions, bool wide, const double* freq,
                                            int pairs, float magnitude, float sign, int64_t t0,
                                            int tokens, float* cosines, float* sines) {
@@ -103,10 +105,10 @@ __device__ __forceinline__ void turn_table(const void* positions, bool wide, con
     const double at = wide ? (double)static_cast<const int64_t*>(positions)[t0 + t]
                            : (double)static_cast<const int32_t*>(positions)[t0 + t];
     const double turns = at * (freq[p] * 0.15915494309189535);
-    float s, c;
-    sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-    cosines[i] = c * magnitude;
-    sines[i] = s * magnitude * sign;
+    double s, c;
+    sincospi(2.0 * (turns - rint(turns)), &s, &c);
+    cosines[i] = (float)(c * magnitude);
+    sines[i] = (float)(s * magnitude) * sign;
   }
 }
 
@@ -373,7 +375,7 @@ struct CellArgs {
   const void* positions;
   const double* freq;
   int64_t tokens;
-  int q_heads, pairs, per_block, wide, half;
+  int q_heads, pairs, wide, half, oct_shift;
   float magnitude;
 };
 
@@ -395,43 +397,62 @@ __device__ __forceinline__ Cell cell_of(const CacheShape& c, int64_t slot, int h
           tile + 34 * d + 2 * (((t >> 3) * groups + group) * 8 + (t & 7))};
 }
 
+// Units of eight values of a block's tokens, four lanes (a quad) to a group of
+// 32. With TOK = 8, the quads of eight tokens lie next to each other: one
+// octet's value dwords, when their slots follow each other, are then whole
+// 32-byte sectors of the cache instead of single dwords of eight (8191 tokens
+// of 16 heads of 64: append 22.4 us, with TOK = 1 24.3; read 13.8 and 15.8).
+// TOK = 1 spreads a few tokens over the chip (64 tokens of 32 + 16 heads of 128:
+// append 4.0 us, with TOK = 8 4.9).
+template <int TOK>
+struct Units {
+  int all, at;                   // units of the block, this thread's
+  __device__ __forceinline__ explicit Units(int units)
+      : all(TOK == 1 ? units : units * TOK), at(blockIdx.y * 256 + threadIdx.x) {}
+  __device__ __forceinline__ bool more() const { return at < all; }
+  __device__ __forceinline__ void next() { at += gridDim.y * 256; }
+  __device__ __forceinline__ int token() const { return TOK == 1 ? 0 : at / 4 % TOK; }
+  __device__ __forceinline__ int unit() const { return TOK == 1 ? at : at / (4 * TOK) * 4 + at % 4; }
+};
+
 // A quad of lanes takes one group of 32 values of a key or value, eight each:
 // three butterfly levels in a lane, two by quad permutation, then the group's
 // largest magnitude, scale and codes. Keys turn by their position on the way,
 // in 32 bits, and queries beside them, so a decode step is one launch and one
 // read of the projection. Bound by reading the rows.
-template <typename E, bool TURN>
+template <typename E, bool TURN, int TOK>
 __global__ void __launch_bounds__(256)
     append_kernel(Rows<const typename E::type> q, Rows<const typename E::type> k,
                   Rows<const typename E::type> v, Rows<typename E::type> q_out,
                   uint8_t* __restrict__ pages, CellArgs a) {
   extern __shared__ float table[];
-  const int64_t t0 = (int64_t)blockIdx.x * a.per_block;
-  const int tokens = (int)min((int64_t)a.per_block, a.tokens - t0);
-  float *cosines = table, *sines = table + a.per_block * a.pairs;
+  const int64_t t0 = (int64_t)blockIdx.x * TOK;
+  const int tokens = (int)min((int64_t)TOK, a.tokens - t0);
+  float *cosines = table, *sines = table + TOK * a.pairs;
   if constexpr (TURN) {
     turn_table(a.positions, a.wide, a.freq, a.pairs, a.magnitude, 1.0f, t0, tokens, cosines, sines);
     __syncthreads();
   }
-  const int lane = threadIdx.x & 63, octs = a.cache.head_dim / 8;
+  const int lane = threadIdx.x & 63, oct_shift = a.oct_shift, octs = 1 << oct_shift;
   const int64_t capacity = a.cache.pages << (a.cache.tile_shift + 5);
   // Units of a token: keys, values, then queries; a multiple of four each, so
   // a quad's lanes always work on the same group.
-  const int kv = a.cache.kv_heads * octs, units = 2 * kv + a.q_heads * octs;
-  for (int i = threadIdx.x; i < tokens * units; i += blockDim.x) {
-    const int t = i / units, u = i - t * units;
+  const int kv = a.cache.kv_heads * octs;
+  for (Units<TOK> i(2 * kv + a.q_heads * octs); i.more(); i.next()) {
+    const int t = i.token(), u = i.unit();
+    if (t >= tokens) continue;                           // a whole quad
     const float *c = cosines + t * a.pairs, *s = sines + t * a.pairs;
     float x[8];
     if (u >= 2 * kv) {
       if constexpr (TURN) {
-        const int h = (u - 2 * kv) / octs, d0 = 8 * ((u - 2 * kv) - h * octs);
+        const int h = (u - 2 * kv) >> oct_shift, d0 = 8 * ((u - 2 * kv) & (octs - 1));
         turned8<E>(q.at(t0 + t, h), d0, a.pairs, a.half, c, s, x);
         E::store8(q_out.at(t0 + t, h) + d0, x);
       }
       continue;
     }
     const bool value = u >= kv;
-    const int h = (value ? u - kv : u) / octs, d0 = 8 * ((value ? u - kv : u) - h * octs);
+    const int h = (value ? u - kv : u) >> oct_shift, d0 = 8 * ((value ? u - kv : u) & (octs - 1));
     if (value)
       E::load8(v.at(t0 + t, h) + d0, x);
     else if constexpr (TURN)
@@ -478,20 +499,21 @@ __global__ void __launch_bounds__(256)
 
 // The values that entries stand for: H ((c - 8) s) / 4, a quad a group; zeros
 // for slots outside the cache.
-template <typename E>
+template <typename E, int TOK>
 __global__ void __launch_bounds__(256)
     read_kernel(const uint8_t* __restrict__ pages, Rows<typename E::type> k, Rows<typename E::type> v,
                 CellArgs a) {
-  const int lane = threadIdx.x & 63, octs = a.cache.head_dim / 8;
+  const int64_t t0 = (int64_t)blockIdx.x * TOK;
+  const int tokens = (int)min((int64_t)TOK, a.tokens - t0);
+  const int lane = threadIdx.x & 63, oct_shift = a.oct_shift, octs = 1 << oct_shift;
   const int64_t capacity = a.cache.pages << (a.cache.tile_shift + 5);
   const int kv = a.cache.kv_heads * octs;
-  const int64_t all = a.tokens * 2 * kv;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-    const int64_t t = i / (2 * kv);
-    const int u = (int)(i - t * 2 * kv);
+  for (Units<TOK> i(2 * kv); i.more(); i.next()) {
+    const int t = i.token(), u = i.unit();
+    if (t >= tokens) continue;
     const bool value = u >= kv;
-    const int h = (value ? u - kv : u) / octs, d0 = 8 * ((value ? u - kv : u) - h * octs);
-    const int64_t slot = a.slots[t];
+    const int h = (value ? u - kv : u) >> oct_shift, d0 = 8 * ((value ? u - kv : u) & (octs - 1));
+    const int64_t slot = a.slots[t0 + t];
     float x[8];
     if (slot >= 0 && slot < capacity) {
       const Cell cell = cell_of(a.cache, slot, h, d0, value);
@@ -509,8 +531,19 @@ __global__ void __launch_bounds__(256)
     exl3::quad_transform(x, lane);
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] *= 0.25f;
-    E::store8((value ? v : k).at(t, h) + d0, x);
+    E::store8((value ? v : k).at(t0 + t, h) + d0, x);
   }
+}
+
+// Tokens next to each other in a block: eight once the blocks fill the chip.
+constexpr int64_t MANY_TOKENS = 2048;
+// Blocks for `tokens` of `units` values, `passes` of each at most: what a thread
+// does in turn waits in turn, but a block's angles are made once (8191 tokens:
+// append 22.4 us with 4 passes, 23.7 with 2, 28.2 with 1; read 15.0, 13.8, 13.9).
+template <int TOK>
+dim3 grid_of(int64_t tokens, int64_t units, int64_t passes) {
+  const int64_t all = (units * TOK + 255) / 256;
+  return dim3((unsigned)((tokens + TOK - 1) / TOK), (unsigned)((all + passes - 1) / passes));
 }
 
 template <typename E>
@@ -522,16 +555,38 @@ int launch_append(const void* q, int64_t q_token, int64_t q_head, void* q_out, c
   Rows<const T> rq{static_cast<const T*>(q), q_token, q_head}, rk{static_cast<const T*>(k), k_token, k_head},
       rv{static_cast<const T*>(v), v_token, v_head};
   Rows<T> oq{static_cast<T*>(q_out), args.q_heads * d, d};
-  const unsigned blocks = (unsigned)((args.tokens + args.per_block - 1) / args.per_block);
-  const size_t lds = 2 * sizeof(float) * args.per_block * args.pairs;
-  if (args.pairs)
-    append_kernel<E, true><<<blocks, 256, lds, stream>>>(rq, rk, rv, oq, pages, args);
+  auto launch = [&](auto tok) {
+    constexpr int TOK = decltype(tok)::value;
+    const int64_t units = (2 * (int64_t)args.cache.kv_heads + args.q_heads) * (d / 8);
+    const dim3 blocks = grid_of<TOK>(args.tokens, units, TOK == 1 ? 1 : 4);
+    const size_t lds = 2 * sizeof(float) * TOK * args.pairs;
+    if (args.pairs)
+      append_kernel<E, true, TOK><<<blocks, 256, lds, stream>>>(rq, rk, rv, oq, pages, args);
+    else
+      append_kernel<E, false, TOK><<<blocks, 256, 0, stream>>>(rq, rk, rv, oq, pages, args);
+    return check_launch("exl3_cache_append");
+  };
+  if (args.tokens >= MANY_TOKENS) return launch(std::integral_constant<int, 8>{});
+  return launch(std::integral_constant<int, 1>{});
+}
+
+template <typename E>
+int launch_read(const uint8_t* pages, void* k, void* v, const CellArgs& args, hipStream_t stream) {
+  typedef typename E::type T;
+  const int64_t token = (int64_t)args.cache.kv_heads * args.cache.head_dim, head = args.cache.head_dim;
+  const Rows<T> rk{static_cast<T*>(k), token, head}, rv{static_cast<T*>(v), token, head};
+  const int64_t units = 2 * (int64_t)args.cache.kv_heads * (head / 8);
+  if (args.tokens >= MANY_TOKENS)
+    read_kernel<E, 8><<<grid_of<8>(args.tokens, units, 2), 256, 0, stream>>>(pages, rk, rv, args);
   else
-    append_kernel<E, false><<<blocks, 256, 0, stream>>>(rq, rk, rv, oq, pages, args);
-  return check_launch("exl3_cache_append");
+    read_kernel<E, 1><<<grid_of<1>(args.tokens, units, 1), 256, 0, stream>>>(pages, rk, rv, args);
+  return check_launch("exl3_cache_read");
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// log2 of the units of eight values in a head.
+int oct_shift_of(int head_dim) { return head_dim == 64 ? 3 : head_dim == 128 ? 4 : 5; }
 
 // Rows that 16-byte loads may read: `per` elements make 16 bytes.
 bool wide_rows(const void* p, int64_t token, int64_t head, int64_t per) {
@@ -634,7 +689,7 @@ int exl3_cache_append(const void* q, int64_t q_token, int64_t q_head, void* q_ou
   if (!tokens) return 0;
   a.slots = slots, a.positions = positions, a.freq = frequencies, a.tokens = tokens;
   a.q_heads = q_heads, a.pairs = pairs, a.wide = wide_positions, a.half = layout == 0;
-  a.magnitude = magnitude, a.per_block = 1;
+  a.magnitude = magnitude, a.oct_shift = oct_shift_of(head_dim);
   auto launch = type == 0 ? launch_append<F32> : type == 1 ? launch_append<F16> : launch_append<BF16>;
   return launch(q, q_token, q_head, q_out, k, k_token, k_head, v, v_token, v_head,
                 static_cast<uint8_t*>(pages), a, (hipStream_t)stream);
@@ -650,18 +705,10 @@ int exl3_cache_read(const void* pages, int64_t num_pages, int page_size, int kv_
     return set_error("exl3_cache_read: pages, k and v must be 16-byte aligned");
   if (!tokens) return 0;
   a.slots = slots, a.tokens = tokens;
-  const int64_t units = tokens * 2 * kv_heads * (head_dim / 8);
-  const unsigned blocks = (unsigned)std::min<int64_t>((units + 255) / 256, 1 << 20);
-  const int64_t token = (int64_t)kv_heads * head_dim, head = head_dim;
+  a.oct_shift = oct_shift_of(head_dim);
   const uint8_t* p = static_cast<const uint8_t*>(pages);
-  hipStream_t s = (hipStream_t)stream;
-  if (type == 0)
-    read_kernel<F32><<<blocks, 256, 0, s>>>(p, {static_cast<float*>(k), token, head}, {static_cast<float*>(v), token, head}, a);
-  else if (type == 1)
-    read_kernel<F16><<<blocks, 256, 0, s>>>(p, {static_cast<uint16_t*>(k), token, head}, {static_cast<uint16_t*>(v), token, head}, a);
-  else
-    read_kernel<BF16><<<blocks, 256, 0, s>>>(p, {static_cast<uint16_t*>(k), token, head}, {static_cast<uint16_t*>(v), token, head}, a);
-  return check_launch("exl3_cache_read");
+  auto launch = type == 0 ? launch_read<F32> : type == 1 ? launch_read<F16> : launch_read<BF16>;
+  return launch(p, k, v, a, (hipStream_t)stream);
 }
 
 }  // extern "C"
