@@ -669,8 +669,8 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 }
 
 // Many query rows to a kv head (chunks and prompts): a workgroup takes a block
-// of 32 rows a wave, and unpacks two tiles at a time, as float16, into shared
-// memory, where all its waves read them.
+// of 32 rows a wave, and unpacks two tiles at a time (of head dimension 256,
+// one), as float16, into shared memory, where all its waves read them.
 //
 // The same products as above at 32 x 32 x 16: S^T = K Q^T in one accumulator
 // of 32 tokens x 32 rows a tile, O^T += V^T P^T in D / 32. Lane (n, h) of S^T
@@ -684,28 +684,27 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 // multiplied the next is unpacked, and the codes after it are on their way.
 //
 // Weights, and bfloat16 queries, count with 11 bits (errors under 2^-11 of the
-// output's terms); float16 queries keep their rest in products of their own.
+// output's terms); float16 queries keep their rest in products of their own, of
+// head dimension 256 from shared memory: in registers it made the compiler spill,
+// and every reload waits for the codes on their way as well.
 constexpr int tile_waves(int d) { return d == 128 ? 8 : 4; }
 constexpr int tile_groups(int d) { return d == 64 ? 3 : 1; }  // workgroups of a compute unit
 template <int D, bool BF16>
 __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_waves(D) / 4)
     attend_tiles_kernel(AttendArgs a, int index) {
   constexpr int NW = tile_waves(D), NT = 64 * NW, ROWS = 32 * NW, GROUPS = D / 32, STEPS = D / 16;
-  constexpr bool REST = !BF16;
+  constexpr bool REST = !BF16, SHARED_REST = REST && D == 256;
+  constexpr int TT = D == 256 ? 1 : 2;                   // tiles of a step
   // Parts of a tile: a dword of key codes, and two dims (a byte) of four tokens'
   // values. A thread takes KN of them.
   constexpr int AHEAD = 2;
   constexpr int KN = 4 * D / NT;
-  // Tiles whose codes a thread holds at a time: one, for fewer registers, or
-  // both of a step, where only one wave fits a SIMD and nothing else hides the
-  // shorter way from load to use (chunks of head dimension 256: 284 us, with
-  // one 427).
-  constexpr int HELD = D == 256 ? 2 : 1;
   constexpr int SPAN = D == 64 ? 7 : 15;                 // vectors of a key row that are permuted, less one
   constexpr uint32_t TILE = 64 * D;                      // bytes of a tile's keys, and of its values
   extern __shared__ int64_t prefix[];                    // [requests + 1]
   __shared__ int64_t parts[NW];
-  __shared__ u32x4 keys[4 * TILE / 16], values[4 * TILE / 16];  // [buffer][tile]
+  __shared__ u32x4 keys[2 * TT * TILE / 16], values[2 * TT * TILE / 16];  // [buffer][tile]
+  __shared__ u32x4 rests[SHARED_REST ? NW * STEPS * 64 : 1];    // [wave][step][lane]
   __shared__ int poison[2];
 
   const Class& cls = a.of[index];
@@ -785,28 +784,25 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
     auto bytes_of = [&](int t, int page) {
       return a.pages + exl3::cache_tile_at(a.cache, max(page, 0), head, min(t, t1 - 1) & ((1 << a.cache.tile_shift) - 1));
     };
-    // The codes and scales of this thread's parts of HELD tiles.
-    uint32_t kc[HELD * KN], ks[HELD * KN];
-    u32x4 vc[HELD * KN];
-    u32x2 vs[HELD * KN];
-    auto fetch = [&](int t, int page, int next) __attribute__((always_inline)) {
+    // The codes and scales of this thread's parts of one tile.
+    uint32_t kc[KN], ks[KN];
+    u32x4 vc[KN];
+    u32x2 vs[KN];
+    auto fetch = [&](int t, int page) __attribute__((always_inline)) {
+      const auto tile = tile_resource<D>(bytes_of(t, page));
 #pragma unroll
-      for (int w = 0; w < HELD; ++w) {
-        const auto tile = tile_resource<D>(bytes_of(t + w, w ? next : page));
-#pragma unroll
-        for (int u = 0; u < KN; ++u) {
-          kc[w * KN + u] = __builtin_amdgcn_raw_buffer_load_b32(tile, key_at + u * (4 * NT), 0, 0);
-          ks[w * KN + u] = __builtin_amdgcn_raw_buffer_load_b16(tile, key_scale_at + u * (NT / (D / 8) * GROUPS * 2), 0, 0);
-          vc[w * KN + u] = __builtin_amdgcn_raw_buffer_load_b128(tile, value_at + u * (4 * NT), 0, 0);
-          vs[w * KN + u] = __builtin_amdgcn_raw_buffer_load_b64(tile, value_scale_at + u * (NT / D * GROUPS * 16), 0, 0);
-        }
+      for (int u = 0; u < KN; ++u) {
+        kc[u] = __builtin_amdgcn_raw_buffer_load_b32(tile, key_at + u * (4 * NT), 0, 0);
+        ks[u] = __builtin_amdgcn_raw_buffer_load_b16(tile, key_scale_at + u * (NT / (D / 8) * GROUPS * 2), 0, 0);
+        vc[u] = __builtin_amdgcn_raw_buffer_load_b128(tile, value_at + u * (4 * NT), 0, 0);
+        vs[u] = __builtin_amdgcn_raw_buffer_load_b64(tile, value_scale_at + u * (NT / D * GROUPS * 16), 0, 0);
       }
     };
-    // Unpacked to tile `which` of a buffer, and the next.
+    // Unpacked to a tile of a buffer.
     auto unpack = [&](int buffer, int which) __attribute__((always_inline)) {
 #pragma unroll
-      for (int u = 0; u < HELD * KN; ++u) {
-        const uint32_t d = tid + u % KN * NT, base = (2 * buffer + which + u / KN) * (TILE / 16);
+      for (int u = 0; u < KN; ++u) {
+        const uint32_t d = tid + u * NT, base = (TT * buffer + which) * (TILE / 16);
         {
           const uint32_t token = d / (D / 8), inside = d % (D / 8);
           const uint32_t vector = 4 * (inside % GROUPS) + inside / GROUPS;
@@ -838,12 +834,12 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
     // A weight of 0 must not meet a NaN or infinity: in steps that some row
     // does not attend whole, such scales of values count as 0, and the rows
     // that do attend their tokens are seen to after the product.
-    auto partial = [&](int t, int page0, int page1) {
-      return t * CACHE_TILE < most_from || t * CACHE_TILE + 2 * CACHE_TILE - 1 > least_last || (page0 | page1) < 0;
+    auto partial = [&](int t, int missing) {
+      return t * CACHE_TILE < most_from || (t + TT) * CACHE_TILE - 1 > least_last || missing < 0;
     };
     auto clean = [&](int buffer, int name) {
 #pragma unroll
-      for (int u = 0; u < HELD * KN; ++u) {
+      for (int u = 0; u < KN; ++u) {
         bool bad = false;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -859,15 +855,16 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
     };
 
     // Pages of this step's tiles and of the next two steps'.
-    int page0[3], page1[3];
+    int page[3 * TT];
+    auto missing = [&](int i) { return TT == 1 ? page[i] : page[TT * i] | page[TT * i + TT - 1]; };  // < 0 if one is
     if (t0 < t1) {
 #pragma unroll
-      for (int i = 0; i < 3; ++i) page0[i] = page_of(t0 + 2 * i), page1[i] = page_of(t0 + 2 * i + 1);
-      fetch(t0, page0[0], page1[0]);
+      for (int i = 0; i < 3 * TT; ++i) page[i] = page_of(t0 + i);
+      fetch(t0, page[0]);
     }
 
     // Queries, scaled by a power of two so that float16 holds them.
-    u32x4 qf[STEPS], ql[REST ? STEPS : 1];
+    u32x4 qf[STEPS], ql[REST && !SHARED_REST ? STEPS : 1];
     float qs, rise;
     {
       const uint16_t* src = a.q + (int64_t)(req.first + token) * a.q_token + (int64_t)(head * a.group + of_group) * a.q_head;
@@ -900,7 +897,11 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
           const float y0 = flip * ldexpf(x[k][2 * e], -power), y1 = flip * ldexpf(x[k][2 * e + 1], -power);
           const f16x2 hi = {(_Float16)y0, (_Float16)y1};
           qf[k][e] = bits_of(hi);
-          if constexpr (REST) ql[k][e] = bits_of(f16x2{(_Float16)(y0 - (float)hi[0]), (_Float16)(y1 - (float)hi[1])});
+          const uint32_t low = bits_of(f16x2{(_Float16)(y0 - (float)hi[0]), (_Float16)(y1 - (float)hi[1])});
+          if constexpr (SHARED_REST)
+            reinterpret_cast<uint32_t*>(&rests[(wave * STEPS + k) * 64 + lane])[e] = low;
+          else if constexpr (REST)
+            ql[k][e] = low;
         }
       qs = fmaxf(ldexpf(fabsf(a.scale) * 0.25f * 1.4426950408889634f, power), 0x1p-120f);
       rise = 8.0f / qs;
@@ -920,65 +921,77 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
       return *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(values) + ((value_row + place) ^ (v & 1) << 5) + (v >> 1) * 2048);
     };
     if (t0 < t1) {
-      const bool dirty = partial(t0, page0[0], page1[0]);
-      if (dirty) clean(count & 1, count);
-      unpack(count & 1, 0);
-      if constexpr (HELD == 1) {
-        fetch(t0 + 1, page1[0], -1);
+      const bool dirty = partial(t0, missing(0));
+#pragma unroll
+      for (int u = 0; u < TT; ++u) {
         if (dirty) clean(count & 1, count);
-        unpack(count & 1, 1);
+        unpack(count & 1, u);
+        fetch(t0 + u + 1, page[u + 1]);
       }
-      fetch(t0 + 2, page0[1], page1[1]);
       __syncthreads();
     }
-    for (int t = t0; t < t1; t += 2) {
+    for (int t = t0; t < t1; t += TT) {
       const int now = count & 1, then = now ^ 1, pos = t * CACHE_TILE;
-      const int page0_after = page_of(t + 6), page1_after = page_of(t + 7);
+      int after[TT];
+#pragma unroll
+      for (int u = 0; u < TT; ++u) after[u] = page_of(t + 3 * TT + u);
       // The next step's tiles are unpacked after this one's scores are
-      // multiplied; of two whose codes came one by one, the first before.
-      const bool dirty = partial(t + 2, page0[1], page1[1]);
+      // multiplied; of two, whose codes come one by one, the first before.
+      const bool dirty = partial(t + TT, missing(1));
       if (dirty) clean(then, count + 1);
-      if constexpr (HELD == 1) {
+      if constexpr (TT == 2) {
         unpack(then, 0);
-        fetch(t + 3, page1[1], -1);
+        fetch(t + 3, page[3]);
       }
-      const uint32_t place = now * (2 * TILE);
+      const uint32_t place = now * (TT * TILE);
       // Operands are read from shared memory AHEAD products before their use.
       // The barriers to the scheduler keep that: left alone it reads each right
       // before its product, to save registers, and every product waits for the
-      // whole latency (a prompt of 8192 tokens: 647 us).
-      f32x16 s[2] = {};
+      // whole latency (a prompt of 8192 tokens: 647 us, with them 582).
+      f32x16 s[2] = {};                                  // of two tiles, or of queries and their rest
       u32x4 f[2][AHEAD];
+      auto second = [&](int k) { return TT == 2 ? key(k, place + TILE) : SHARED_REST ? rests[(wave * STEPS + k) * 64 + lane] : u32x4{}; };
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) f[0][k] = key(k, place), f[1][k] = key(k, place + TILE);
+      for (int k = 0; k < AHEAD; ++k) f[0][k] = key(k, place), f[1][k] = second(k);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int k = 0; k < STEPS; ++k) {
-        s[0] = mfma32(f[0][k % AHEAD], qf[k], s[0]);
-        s[1] = mfma32(f[1][k % AHEAD], qf[k], s[1]);
-        if constexpr (REST) {
-          s[0] = mfma32(f[0][k % AHEAD], ql[k], s[0]);
-          s[1] = mfma32(f[1][k % AHEAD], ql[k], s[1]);
+        const u32x4 w0 = f[0][k % AHEAD], w1 = f[1][k % AHEAD];
+        if constexpr (TT == 2) {
+          s[0] = mfma32(w0, qf[k], s[0]);
+          s[1] = mfma32(w1, qf[k], s[1]);
+          if constexpr (REST) {
+            s[0] = mfma32(w0, ql[k], s[0]);
+            s[1] = mfma32(w1, ql[k], s[1]);
+          }
+        } else {
+          // Two sums in turn, as the products of one wait for each other.
+          if constexpr (SHARED_REST) {
+            s[0] = mfma32(w0, qf[k], s[0]);
+            s[1] = mfma32(w0, w1, s[1]);
+          } else {
+            s[k & 1] = mfma32(w0, qf[k], s[k & 1]);
+          }
         }
         if (k + AHEAD < STEPS) {
-          f[0][k % AHEAD] = key(k + AHEAD, place), f[1][k % AHEAD] = key(k + AHEAD, place + TILE);
+          f[0][k % AHEAD] = key(k + AHEAD, place), f[1][k % AHEAD] = second(k + AHEAD);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
-      float x[32];
+      float x[16 * TT];
 #pragma unroll
-      for (int e = 0; e < 32; ++e) x[e] = s[e >> 4][e & 15];
-      if (pos < wave_from || pos + 2 * CACHE_TILE - 1 > wave_least || (page0[0] | page1[0]) < 0) {
+      for (int e = 0; e < 16 * TT; ++e) x[e] = TT == 2 ? s[e >> 4][e & 15] : s[0][e & 15] + s[1][e & 15];
+      if (pos < wave_from || pos + TT * CACHE_TILE - 1 > wave_least || missing(0) < 0) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
+        for (int e = 0; e < 16 * TT; ++e) {
           const int p = pos + 16 * (e >> 3) + 8 * h + (e & 7);
-          x[e] = p >= from && p <= last && (e < 16 ? page0[0] : page1[0]) >= 0 ? x[e] : NONE;
+          x[e] = p >= from && p <= last && page[e >> 4] >= 0 ? x[e] : NONE;
           asm volatile("" : "+v"(x[e]));
         }
       }
       float top = x[0];
 #pragma unroll
-      for (int e = 1; e < 32; ++e) top = fmaxf(top, x[e]);
+      for (int e = 1; e < 16 * TT; ++e) top = fmaxf(top, x[e]);
       if (__any(top > run + rise)) {
         top = fmaxf(top, run);
         top = fmaxf(top, __shfl_xor(top, 32));
@@ -994,22 +1007,22 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
 #pragma unroll
       for (int v = 0; v < 2 * AHEAD; ++v) f[v & 1][v / 2] = operand(v);
       __builtin_amdgcn_sched_barrier(0);
-      if (HELD == 1 && dirty) clean(then, count + 1);
-      unpack(then, HELD == 1);
-      fetch(t + 4, page0[2], page1[2]);
-      u32x4 p[4];
+      if (TT == 2 && dirty) clean(then, count + 1);
+      unpack(then, TT - 1);
+      fetch(t + 2 * TT, page[2 * TT]);
+      u32x4 p[2 * TT];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
+      for (int e = 0; e < 8 * TT; ++e) {
         const f16x2 w = {(_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * e], qs, ref)),
                          (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * e + 1], qs, ref))};
         sum = __builtin_amdgcn_fdot2(w, f16x2{1, 1}, sum, false);
         p[e >> 2][e & 3] = bits_of(w);
       }
 #pragma unroll
-      for (int v = 0; v < 4 * GROUPS; ++v) {
+      for (int v = 0; v < 2 * TT * GROUPS; ++v) {
         u32x4& w = f[v & 1][v / 2 % AHEAD];
         o[v % GROUPS] = mfma32(w, p[v / GROUPS], o[v % GROUPS]);
-        if (v + 2 * AHEAD < 4 * GROUPS) {
+        if (v + 2 * AHEAD < 2 * TT * GROUPS) {
           w = operand(v + 2 * AHEAD);
           if (v & 1) __builtin_amdgcn_sched_barrier(0);
         }
@@ -1018,10 +1031,10 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
       if (poison[now] == count) {
         // Rows that attend a token whose values of a group are NaN.
 #pragma unroll 1
-        for (int k = 0; k < 2 * CACHE_TILE; ++k) {
-          const int page = k < CACHE_TILE ? page0[0] : page1[0];
-          if (page < 0) continue;
-          const uint8_t* scales = bytes_of(t + k / CACHE_TILE, page) + 34 * D;
+        for (int k = 0; k < TT * CACHE_TILE; ++k) {
+          const int id = k < CACHE_TILE ? page[0] : page[TT - 1];
+          if (id < 0) continue;
+          const uint8_t* scales = bytes_of(t + k / CACHE_TILE, id) + 34 * D;
           const bool in = pos + k >= from && pos + k <= last;
 #pragma unroll
           for (int d = 0; d < GROUPS; ++d) {
@@ -1030,8 +1043,8 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
           }
         }
       }
-      page0[0] = page0[1], page0[1] = page0[2], page0[2] = page0_after;
-      page1[0] = page1[1], page1[1] = page1[2], page1[2] = page1_after;
+#pragma unroll
+      for (int i = 0; i < 3 * TT; ++i) page[i] = i < 2 * TT ? page[i + TT] : after[i - 2 * TT];
       ++count;
       __syncthreads();
     }
