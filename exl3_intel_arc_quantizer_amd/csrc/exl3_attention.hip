@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <limits>
 #include <type_traits>
 
 #include "../../include/exl3_layer.h"
@@ -46,10 +47,13 @@ constexpr int THREADS = 256, WAVES = THREADS / 64;
 // a kv head, in blocks of `rows`.
 struct Class {
   int low, high, rows;
+  int by_block;                  // attend_tiles_kernel: the work is a list of blocks,
+  int blocks;                    // of which it has at most so many if they may be cut
   int whole;                     // every owner takes one segment, none is cut
   int owners;                    // else: shares that the work is cut into
   float* partials;               // [2 owners][rows][D + 2]: values, then maximum and sum
-  int64_t* shares;               // [requests + 1] prefix of the work, for the join
+  int64_t* shares;               // [requests + 1] prefix of the work, for the join; by
+                                 // block, of the blocks, and after it that of the blocks' work
 };
 
 struct AttendArgs {
@@ -88,8 +92,7 @@ __device__ __forceinline__ Request request_of(const AttendArgs& a, int r) {
 // A segment is one kv head and block of query rows of a request. Its work is
 // its tiles, and before them what beginning and ending it costs, as tiles: a
 // share of many short segments would end late without. (A ragged batch of 128
-// requests: 107 us at 8, 115 at 4, 130 at 2, 108 at 12.) Where segments are
-// taken whole the work is their number.
+// requests: 107 us at 8, 115 at 4, 130 at 2, 108 at 12.)
 constexpr int SEGMENT_COST = 8;
 __device__ __forceinline__ int blocks_of(const AttendArgs& a, const Class& c, const Request& q) {
   return (int)(((int64_t)q.n * a.group + c.rows - 1) / c.rows);
@@ -101,12 +104,28 @@ __device__ __forceinline__ bool takes(const AttendArgs& a, const Class& c, const
 __device__ __forceinline__ int64_t work_of(const AttendArgs& a, const Class& c, const Request& q) {
   if (!takes(a, c, q)) return 0;
   const int64_t blocks = blocks_of(a, c, q);
-  return a.cache.kv_heads * blocks * (c.whole ? 1 : q.tiles + SEGMENT_COST);
+  return c.by_block ? blocks : a.cache.kv_heads * blocks * (q.tiles + SEGMENT_COST);
+}
+
+// What a block of rows attends: positions from `low` on, tiles [t0, t1), and
+// the last positions of its first and last row.
+struct Block {
+  int row0, row1, least_last, most_last, low, t0, t1;
+};
+__device__ __forceinline__ Block block_of(const AttendArgs& a, const Class& c, const Request& q, int block) {
+  const int rows = q.n * a.group, offset = q.length - q.n;
+  Block b;
+  b.row0 = block * c.rows, b.row1 = min(b.row0 + c.rows, rows) - 1;
+  b.least_last = offset + b.row0 / a.group, b.most_last = offset + b.row1 / a.group;
+  b.low = (int)max((int64_t)b.least_last - a.window + 1, (int64_t)0);
+  b.t0 = b.low / CACHE_TILE;
+  b.t1 = max(b.most_last < 0 ? 0 : b.most_last / CACHE_TILE + 1, b.t0);
+  return b;
 }
 
 // prefix[r] = work before request r, prefix[requests] = all of it.
-template <int NTHREADS>
-__device__ __forceinline__ void sum_work(const AttendArgs& a, const Class& c, int64_t* prefix, int64_t* parts) {
+template <int NTHREADS, typename T>
+__device__ __forceinline__ void sum_work(const AttendArgs& a, const Class& c, T* prefix, int64_t* parts) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int64_t base = 0;
   for (int r0 = 0; r0 < a.requests; r0 += NTHREADS) {
@@ -126,7 +145,7 @@ __device__ __forceinline__ void sum_work(const AttendArgs& a, const Class& c, in
       if (i < wave) before += parts[i];
       base += parts[i];
     }
-    if (r < a.requests) prefix[r + 1] = before + v;
+    if (r < a.requests) prefix[r + 1] = (T)min(before + v, (int64_t)std::numeric_limits<T>::max());
   }
   if (tid == 0) prefix[0] = 0;
   __syncthreads();
@@ -143,6 +162,11 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
 constexpr int LEAST = 2;
 __device__ __forceinline__ int64_t share_of(const Class& c, int64_t all) {
   return max((all + c.owners - 1) / c.owners, (int64_t)LEAST);
+}
+
+// x / d, which nearly always fits 32 bits.
+__device__ __forceinline__ int quotient(int64_t x, int64_t d) {
+  return (x | d) >> 32 ? (int)(x / d) : (int)((uint32_t)x / (uint32_t)d);
 }
 
 // Last index i of [0, n) with at[i] <= x; at[0] <= x.
@@ -332,7 +356,7 @@ __global__ void __launch_bounds__(THREADS, resident(D, WIDE, CT)) attend_rows_ke
     const Request req = request_of(a, r);
     const int blocks = blocks_of(a, cls, req), rows = req.n * a.group;
     const int64_t before = uniform(prefix[r]);
-    const int segment = (int)((uint32_t)(at - before) / (uint32_t)(req.tiles + SEGMENT_COST));
+    const int segment = quotient(at - before, req.tiles + SEGMENT_COST);
     const int head = segment / blocks, block = segment - head * blocks;
     const int64_t seg0 = before + (int64_t)segment * (req.tiles + SEGMENT_COST) + SEGMENT_COST;
     const int64_t seg1 = seg0 + req.tiles;
@@ -341,14 +365,12 @@ __global__ void __launch_bounds__(THREADS, resident(D, WIDE, CT)) attend_rows_ke
     if (past <= first) continue;
     const bool whole = past - first == req.tiles;
     float* part = cls.partials + ((int64_t)owner * 2 + (first == 0)) * (ROWS * (D + 2));
-    // The block's rows attend positions low .. last; what all of them attend,
-    // most_from .. least_last, needs no mask.
-    const int row0 = block * ROWS, row1 = min(row0 + ROWS, rows) - 1;
-    const int least_last = req.length - req.n + row0 / a.group, most_last = req.length - req.n + row1 / a.group;
-    const int low = (int)max((int64_t)least_last - a.window + 1, (int64_t)0);
-    const int most_from = (int)max((int64_t)most_last - a.window + 1, (int64_t)0);
-    const int t0 = max(req.tile0 + first, low / CACHE_TILE);
-    const int t1 = min(req.tile0 + past, most_last < 0 ? 0 : most_last / CACHE_TILE + 1);
+    // What all of the block's rows attend, most_from .. least_last, needs no
+    // mask.
+    const Block b = block_of(a, cls, req, block);
+    const int row0 = b.row0, row1 = b.row1, least_last = b.least_last;
+    const int most_from = (int)max((int64_t)b.most_last - a.window + 1, (int64_t)0);
+    const int t0 = max(req.tile0 + first, b.t0), t1 = min(req.tile0 + past, b.t1);
     if (t1 <= t0) {
       // Nothing to attend in this share.
       for (int i = lane; i <= row1 - row0; i += 64) {
@@ -701,7 +723,7 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
   constexpr int KN = 4 * D / NT;
   constexpr int SPAN = D == 64 ? 7 : 15;                 // vectors of a key row that are permuted, less one
   constexpr uint32_t TILE = 64 * D;                      // bytes of a tile's keys, and of its values
-  extern __shared__ int64_t prefix[];                    // [requests + 1]
+  extern __shared__ int64_t dynamic[];                   // costs, then prefix
   __shared__ int64_t parts[NW];
   __shared__ u32x4 keys[2 * TT * TILE / 16], values[2 * TT * TILE / 16];  // [buffer][tile]
   __shared__ u32x4 rests[SHARED_REST ? NW * STEPS * 64 : 1];    // [wave][step][lane]
@@ -711,14 +733,49 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 31, h = lane >> 5;
   const Magic magic;
+  int64_t* costs = dynamic;                              // [blocks + 1], if blocks may be cut
+  int32_t* prefix = reinterpret_cast<int32_t*>(dynamic + (cls.whole ? 0 : cls.blocks + 1));  // [requests + 1]
   sum_work<NT>(a, cls, prefix, parts);
-  const int64_t all = uniform(prefix[a.requests]);
-  const int owner = blockIdx.x;
-  int64_t begin = owner, end = min(begin + 1, all);
+  const int owner = blockIdx.x, heads = a.cache.kv_heads;
+  int listed = __builtin_amdgcn_readfirstlane(prefix[a.requests]);
+  // (More are asked for only if the requests' rows overlap.)
+  if (!cls.whole) listed = min(listed, cls.blocks);
+  int64_t begin = owner, end = min(begin + 1, (int64_t)listed * heads);
   if (!cls.whole) {
-    if (owner == 0)
-      for (int r = tid; r <= a.requests; r += NT) cls.shares[r] = prefix[r];
-    const int64_t share = share_of(cls, all);
+    // Blocks of a prompt attend more and more tiles, within a window as many:
+    // shares are cut by what each block really attends.
+    int64_t sum = 0;
+    for (int i0 = 0; i0 < listed; i0 += NT) {
+      const int i = i0 + tid;
+      int64_t v = 0;
+      if (i < listed) {
+        const int r = last_at_most(prefix, a.requests + 1, i);
+        const Block b = block_of(a, cls, request_of(a, r), i - prefix[r]);
+        v = b.t1 - b.t0 + SEGMENT_COST;
+      }
+#pragma unroll
+      for (int o = 1; o < 64; o *= 2) {
+        const int64_t w = __shfl_up(v, o);
+        if (lane >= o) v += w;
+      }
+      __syncthreads();
+      if (lane == 63) parts[wave] = v;
+      __syncthreads();
+      int64_t before = sum;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        if (w < wave) before += parts[w];
+        sum += parts[w];
+      }
+      if (i < listed) costs[i + 1] = before + v;
+    }
+    if (tid == 0) costs[0] = 0;
+    __syncthreads();
+    if (owner == 0) {
+      for (int r = tid; r <= a.requests; r += NT) cls.shares[r] = min(prefix[r], listed);
+      for (int i = tid; i <= listed; i += NT) cls.shares[a.requests + 1 + i] = costs[i];
+    }
+    const int64_t all = uniform(costs[listed]) * heads, share = share_of(cls, all);
     begin = owner * share, end = min(begin + share, all);
   }
   // A thread's places in a tile (byte, half of the octet, dword column and
@@ -733,36 +790,36 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
   int count = 0;                                         // steps so far; names a buffer's content
 
   for (int64_t at = begin; at < end;) {
-    const int r = __builtin_amdgcn_readfirstlane(last_at_most(prefix, a.requests + 1, at));
-    const Request req = request_of(a, r);
-    const int blocks = blocks_of(a, cls, req), rows = req.n * a.group;
-    const int64_t before = uniform(prefix[r]);
-    int head, block, first = 0, past = req.tiles;
+    int r, head, block, first = 0, past = INT32_MAX;
     if (cls.whole) {
-      // The longest blocks first, heads next to each other: workgroups are
-      // dealt to the chip's eight dies in turn, so that 8 kv heads' keys and
-      // values lie in one die's cache each.
-      const uint32_t unit = (uint32_t)(at - before), heads = (uint32_t)a.cache.kv_heads;
-      block = blocks - 1 - (int)(unit / heads), head = (int)(unit % heads);
+      // The longest blocks of a request first, heads next to each other:
+      // workgroups are dealt to the chip's eight dies in turn, so that 8 kv
+      // heads' keys and values lie in one die's cache each.
+      r = __builtin_amdgcn_readfirstlane(last_at_most(prefix, a.requests + 1, at / heads));
+      const int before = __builtin_amdgcn_readfirstlane(prefix[r]);
+      const uint32_t unit = (uint32_t)(at - (int64_t)before * heads);
+      block = __builtin_amdgcn_readfirstlane(prefix[r + 1]) - before - 1 - (int)(unit / (uint32_t)heads);
+      head = (int)(unit % (uint32_t)heads);
       at = end;
     } else {
-      const int segment = (int)((uint32_t)(at - before) / (uint32_t)(req.tiles + SEGMENT_COST));
-      head = segment / blocks, block = segment - head * blocks;
-      const int64_t seg0 = before + (int64_t)segment * (req.tiles + SEGMENT_COST) + SEGMENT_COST;
-      const int64_t seg1 = seg0 + req.tiles;
+      const int i = __builtin_amdgcn_readfirstlane(last_at_most(costs, listed + 1, at / heads));
+      const int64_t cost0 = uniform(costs[i]), cost = uniform(costs[i + 1]) - cost0;
+      r = __builtin_amdgcn_readfirstlane(last_at_most(prefix, a.requests + 1, i));
+      block = i - __builtin_amdgcn_readfirstlane(prefix[r]);
+      head = quotient(at - cost0 * heads, cost);
+      const int64_t seg0 = cost0 * heads + head * cost + SEGMENT_COST, seg1 = seg0 - SEGMENT_COST + cost;
       first = (int)max(at - seg0, (int64_t)0), past = (int)(min(end, seg1) - seg0);
       at = min(end, seg1);
       if (past <= first) continue;
     }
-    const bool whole = past - first == req.tiles;
+    const Request req = request_of(a, r);
+    const Block b = block_of(a, cls, req, block);
+    const int row0 = b.row0, row1 = b.row1, rows = req.n * a.group, offset = req.length - req.n;
+    const int least_last = b.least_last;
+    const int most_from = (int)max((int64_t)b.most_last - a.window + 1, (int64_t)0);
+    const int t0 = b.t0 + first, t1 = min(b.t0 + min(past, b.t1 - b.t0), b.t1);
+    const bool whole = t0 == b.t0 && t1 == b.t1;
     float* part = cls.partials + ((int64_t)owner * 2 + (first == 0)) * (ROWS * (D + 2));
-    const int row0 = block * ROWS, row1 = min(row0 + ROWS, rows) - 1;
-    const int offset = req.length - req.n;
-    const int least_last = offset + row0 / a.group, most_last = offset + row1 / a.group;
-    const int low = (int)max((int64_t)least_last - a.window + 1, (int64_t)0);
-    const int most_from = (int)max((int64_t)most_last - a.window + 1, (int64_t)0);
-    const int t0 = max(req.tile0 + first, low / CACHE_TILE);
-    const int t1 = min(req.tile0 + past, most_last < 0 ? 0 : most_last / CACHE_TILE + 1);
 
     // This wave's rows and what they attend.
     const int row = 32 * wave + n;
@@ -1138,11 +1195,21 @@ __global__ void __launch_bounds__(SPREAD > 1 ? 64 * SPREAD : THREADS) attend_joi
       }
       const int head = qh / a.group, of = (int)(token - req.first) * a.group + qh % a.group;
       const int blocks = blocks_of(a, cls, req), row = of % cls.rows, stride = cls.rows * (D + 2);
-      const int64_t share = share_of(cls, cls.shares[a.requests]);
-      const int64_t seg0 = cls.shares[r] + ((int64_t)head * blocks + of / cls.rows) * (req.tiles + SEGMENT_COST) + SEGMENT_COST;
-      const int64_t seg1 = seg0 + req.tiles;
+      int64_t seg0, seg1, all;
+      if (cls.by_block) {
+        const int64_t* costs = cls.shares + a.requests + 1;
+        const int64_t i = min(cls.shares[r] + of / cls.rows, cls.shares[a.requests] - 1), cost = costs[i + 1] - costs[i];
+        all = costs[cls.shares[a.requests]] * a.cache.kv_heads;
+        seg1 = costs[i] * a.cache.kv_heads + (head + 1) * cost;
+        seg0 = seg1 - cost + SEGMENT_COST;
+      } else {
+        all = cls.shares[a.requests];
+        seg0 = cls.shares[r] + ((int64_t)head * blocks + of / cls.rows) * (req.tiles + SEGMENT_COST) + SEGMENT_COST;
+        seg1 = seg0 + req.tiles;
+      }
+      const int64_t share = share_of(cls, all);
       const int w0 = __builtin_amdgcn_readfirstlane((int)(seg0 / share));
-      const int w1 = __builtin_amdgcn_readfirstlane((int)((seg1 - 1) / share));
+      const int w1 = seg1 > seg0 ? __builtin_amdgcn_readfirstlane((int)((seg1 - 1) / share)) : w0 - 1;
       if (w0 == w1) continue;
       const int stats = cls.rows * D + 2 * row;           // a row's maximum and sum in a slot
       for (int w = w0 + wave % SPREAD; w <= w1; w += BATCH * SPREAD) {
@@ -1219,14 +1286,21 @@ int owners_of(Variant v, int head_dim) {
   if (v == TILES) return tile_groups(head_dim) * CUS;
   return CUS * WAVES * resident(head_dim, v == ROWS32, v == ROWS8 ? 1 : 2);
 }
-int64_t shares_bytes(int requests) { return (8 * ((int64_t)requests + 1) + 15) & ~(int64_t)15; }
+// Blocks that a launch which may cut them has at most: fewer than its owners
+// take whole, over one kv head.
+int64_t blocks_bound(Variant v, int head_dim) { return v == TILES ? 2 * owners_of(v, head_dim) : 0; }
+int64_t shares_bytes(Variant v, int requests, int head_dim) {
+  return (8 * ((int64_t)requests + 2 + blocks_bound(v, head_dim)) + 15) & ~(int64_t)15;
+}
 int64_t partials_bytes(Variant v, int head_dim) {
   return (int64_t)2 * owners_of(v, head_dim) * rows_of(v, head_dim) * (head_dim + 2) * 4;
 }
 
 template <int D, bool BF16>
 int launch_variant(Variant v, const AttendArgs& args, int index, unsigned grid, hipStream_t stream) {
-  const size_t lds = 8 * ((size_t)args.requests + 1);
+  const Class& c = args.of[index];
+  const size_t requests = (size_t)args.requests + 1;
+  const size_t lds = v != TILES ? 8 * requests : 4 * requests + (c.whole ? 0 : 8 * ((size_t)c.blocks + 1));
   if (v == ROWS8)
     attend_rows_kernel<D, false, 1, BF16><<<grid, THREADS, lds, stream>>>(args, index);
   else if (v == ROWS16)
@@ -1255,9 +1329,10 @@ int launch_attend(AttendArgs args, int64_t max_new, char* workspace, hipStream_t
     c.owners = owners_of(v, D);
     // At most so many segments: whole where they fill the chip twice.
     const int64_t segments = ((args.tokens * args.group + c.rows - 1) / c.rows + args.requests) * args.cache.kv_heads;
+    c.by_block = v == TILES, c.blocks = (int)blocks_bound(v, D);
     c.whole = v == TILES && segments >= 2 * c.owners;
     c.shares = reinterpret_cast<int64_t*>(workspace);
-    workspace += shares_bytes(args.requests);
+    workspace += shares_bytes(v, args.requests, D);
     c.partials = reinterpret_cast<float*>(workspace);
     workspace += partials_bytes(v, D);
     const int64_t grid = c.whole ? segments : v == TILES ? c.owners : c.owners / WAVES;
@@ -1286,8 +1361,9 @@ int64_t exl3_cache_attention_workspace(int requests, int head_dim) {
   if (requests < 1 || requests > CACHE_MAX_REQUESTS || (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return -1;
   int64_t most = 0;
-  for (Variant v : {ROWS16, ROWS32, TILES}) most = std::max(most, partials_bytes(v, head_dim));
-  return 2 * shares_bytes(requests) + partials_bytes(ROWS8, head_dim) + most;
+  for (Variant v : {ROWS16, ROWS32, TILES})
+    most = std::max(most, shares_bytes(v, requests, head_dim) + partials_bytes(v, head_dim));
+  return shares_bytes(ROWS8, requests, head_dim) + partials_bytes(ROWS8, head_dim) + most;
 }
 
 int exl3_cache_attention(const void* q, int64_t q_token, int64_t q_head, void* out, int64_t tokens,
