@@ -1274,10 +1274,14 @@ constexpr int CUS = 256;
 // Variants by the query rows that one kv head has of a request (its new tokens
 // times the query heads to a kv head): up to 8 and 16 rows at 22 bits, whose
 // cost is the cache's bytes, then 32 to a wave, then blocks that share the work
-// of unpacking a tile.
+// of unpacking a tile. Waves of 32 rows are kept for a few blocks' worth, each
+// of which reads the cache again: 64 requests of 2048 positions, 8 kv heads,
+// float16: head dimension 128, 64 rows 99 us and in blocks 182, 128 rows 160 and
+// 189; head dimension 64, 64 rows 75 and 92, 96 rows 108 and 105.
 enum Variant { ROWS8, ROWS16, ROWS32, TILES };
 Variant variant_of(int64_t rows, int head_dim) {
-  return rows <= 8 ? ROWS8 : rows <= 16 ? ROWS16 : rows <= 32 && head_dim != 256 ? ROWS32 : TILES;
+  const int64_t most = head_dim == 128 ? 128 : head_dim == 64 ? 64 : 16;
+  return rows <= 8 ? ROWS8 : rows <= 16 ? ROWS16 : rows <= most ? ROWS32 : TILES;
 }
 int rows_of(Variant v, int head_dim) { return v == TILES ? 32 * tile_waves(head_dim) : 8 << v; }
 // Owners that fill the chip: waves of attend_rows_kernel, workgroups of

@@ -172,3 +172,29 @@ def plan(cached, new, tables, free, taken, page, max_tokens):
         status |= 4
     lengths = [max(c, 0) + max(n, 0) for c, n in zip(cached, new)]
     return slots, positions, np.array(starts), np.array(lengths), min(at, max(len(free), taken)), status, tables
+
+
+def attention_dense(q, keys, values, page, tables, starts, lengths, scale, window):
+    """As `attention`, in float64 products over whole requests (on the tensors'
+    device), for sizes that row by row would take too long."""
+    tokens, heads, dim = q.shape
+    kv_heads, dev = keys.shape[1], q.device
+    outs = [torch.zeros(tokens, heads, dim, dtype=torch.float64, device=dev) for _ in range(3)]
+    reach = torch.zeros(tokens, heads, 1, dtype=torch.float64, device=dev)
+    turn = torch.from_numpy(sylvester()).to(dev)
+    for r in range(len(lengths)):
+        a, b, n = starts[r], starts[r + 1], lengths[r]
+        t = torch.arange(n, device=dev)
+        slots = torch.as_tensor(tables[r], device=dev).long()[t // page] * page + t % page
+        at = torch.arange(n - (b - a), n, device=dev)[:, None]
+        seen = (t[None] <= at) & (t[None] > at - (window or 1 << 40))
+        for h in range(heads):
+            k, v = keys[slots, h * kv_heads // heads], values[slots, h * kv_heads // heads]
+            row = q[a:b, h].double()
+            x = (row @ k.T * scale).masked_fill(~seen, float("-inf"))
+            w = torch.softmax(x, 1)
+            outs[0][a:b, h], outs[1][a:b, h] = w @ v, w @ v.abs()
+            held = (v.reshape(n, dim // GROUP, GROUP) @ turn).abs().sum(2) / 32
+            outs[2][a:b, h] = (w @ held).repeat_interleave(GROUP, 1)
+            reach[a:b, h, 0] = scale * row.norm(dim=1) * k.norm(dim=1).max()
+    return (*(o.cpu().numpy() for o in outs), reach.cpu().numpy())

@@ -269,6 +269,72 @@ def test_long_context_is_split(new):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads, group, dim, page, new, context, window", [
+    (1, 4, 128, 64, [400, 33, 129], [700, 200, 129], None),     # cut into shares
+    (2, 5, 128, 32, [200, 77], [333, 1500], 250),               # rows of a token in two blocks
+    (1, 2, 256, 128, [301, 65], [301, 900], None),
+    (1, 8, 256, 32, [100], [2000], 600),
+    (3, 3, 64, 64, [150, 1, 260], [2100, 40, 260], 1000),
+    (16, 4, 64, 256, [3100], [3100], None),                     # enough blocks to be dealt whole
+    (16, 2, 128, 64, [2300, 1900], [2350, 1900], 700)])         # and here
+def test_many_rows(heads, group, dim, page, new, context, window, dtype):
+    """Chunks and prompts whose rows fill workgroups, with ragged ends, rows
+    that straddle blocks, windows and the first positions of a context."""
+    rng = np.random.default_rng(dim + heads)
+    starts = np.concatenate([[0], np.cumsum(new)])
+    pages = sum(-(-n // page) for n in context) + 1
+    cache = ref.Cache(pages, page, heads, dim, rng)
+    tables = _tables(context, page, -(-max(context) // page), pages, rng)
+    q = torch.from_numpy(rng.normal(size=(starts[-1], heads * group, dim)) * 2).to(dtype)
+    got = cache_attention(q.cuda(), torch.from_numpy(cache.bytes()).cuda(), _ints(tables), _ints(starts), _ints(context),
+                          window=window, max_new=max(new))
+    keys, values = (torch.from_numpy(x).cuda() for x in cache.values())
+    want, spread, basis, reach = ref.attention_dense(q.cuda(), keys, values, page, tables, starts, context, dim ** -0.5, window)
+    off = np.abs(got.cpu().double().numpy() - want)
+    few = np.repeat(np.asarray(new) * group <= 16, new)[:, None, None]
+    tolerance = np.where(few, _tolerance(want, spread, basis, reach, dtype, True), _tolerance(want, spread, basis, reach, dtype, False))
+    assert (off <= tolerance).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_many_rows_with_holes(dim):
+    """NaN in unattended positions and missing pages under blocks of rows."""
+    rng = np.random.default_rng(dim)
+    page, group, lengths, new = 32, 4, [500, 260], [300, 260]
+    starts = np.concatenate([[0], np.cumsum(new)])
+    cache = ref.Cache(30, page, 1, dim, rng)
+    tables = _tables(lengths, page, 17, 30, rng)
+    clean = torch.from_numpy(cache.bytes()).cuda()
+    q = torch.from_numpy(rng.normal(size=(starts[-1], group, dim))).half().cuda()
+    args = _ints(starts), _ints(lengths)
+    want = cache_attention(q, clean, _ints(tables), *args, window=128)
+    used = [tables[r][t // page] * page + t % page for r in range(2) for t in range(lengths[r])]
+    unused = np.setdiff1d(np.arange(30 * page), used)
+    # The first request's window begins at 200 - 127.
+    unused = np.concatenate([unused, tables[0][np.arange(64) // page] * page + np.arange(64) % page])
+    cache.scales[0][unused], cache.scales[1][unused] = np.nan, np.inf
+    dirty = torch.from_numpy(cache.bytes()).cuda()
+    assert torch.equal(cache_attention(q, dirty, _ints(tables), *args, window=128), want)
+    # One NaN value group, attended by 128 rows of a token; one page missing.
+    slot = tables[0][300 // page] * page + 300 % page
+    cache.scales[1][slot, 0, 1] = np.nan
+    holes = tables.copy()
+    holes[1, 2] = -1
+    got = cache_attention(q, torch.from_numpy(cache.bytes()).cuda(), _ints(holes), *args, window=128).cpu()
+    nan = torch.isnan(got)
+    assert nan[100:228, :, 32:64].all() and nan.sum() == 128 * group * 32
+    keys, values = cache.values()
+    sample = [300, 300 + 64, 300 + 100, 300 + 200, 559]
+    for i in sample:
+        p = i - 300
+        one, *_ = ref.attention(q[i:i + 1].cpu().double().numpy(), keys, values, page, holes[1:], [0, 1], [p + 1], dim ** -0.5, 128)
+        # Weights in 11 bits and the result's own rounding.
+        assert np.abs(got[i].double().numpy() - one[0]).max() <= 2.0 ** -9 * (np.abs(one).max() + 1)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new", [1, 6, 80])
 @pytest.mark.parametrize("dim", [64, 128, 256])
 def test_masked_positions_may_hold_anything(new, dim):
@@ -335,6 +401,11 @@ def test_table_values_out_of_range_are_harmless():
     want = cache_attention(q, pages, tables, _ints([0, 1, 2, 4]), _ints([64, 32, 0]))
     got = cache_attention(q, pages, tables, _ints([-7, 1, 2, 400]), _ints([1 << 30, 40, -5]))
     assert torch.isfinite(got).all() and torch.equal(got[0], want[0]) and not got[2:].any()
+    # Requests that claim the same rows, many and few to a kv head.
+    for rows in (4, 300):
+        many = torch.randn(rows, 2, 64, device="cuda", dtype=torch.float16)
+        over = cache_attention(many, pages, tables, _ints([0, rows, 0, rows]), _ints([64, 32, 60]))
+        assert over.shape == many.shape
     none = cache_attention(q[:0], pages, tables, _ints([0, 0, 0, 0]), _ints([64, 32, 0]))
     assert none.shape == (0, 2, 64)
     empty = cache_attention(q, pages[:0], tables, _ints([0, 1, 2, 4]), _ints([64, 32, 0]))
@@ -444,3 +515,17 @@ def test_refusals():
         plan_step(big, big, torch.zeros(4097, 1, dtype=torch.int32, device="cuda"), big, big[:1], page_size=32, max_tokens=1)
     with pytest.raises(RuntimeError, match="page_size"):
         plan_step(at, at, torch.zeros(3, 1, dtype=torch.int32, device="cuda"), at, at[:1], page_size=33, max_tokens=1)
+
+
+@pytest.mark.gpu
+def test_example_serves_quantized_block():
+    """Group maxima of 32 normal values are about 2.2 sigma, so codes are 0.31
+    sigma apart and off by 0.09 sigma in keys and values both; weights move by
+    about as much for scores of order one: 0.13 together."""
+    import importlib.util
+    from .conftest import REPO_ROOT
+    spec = importlib.util.spec_from_file_location("serve_quantized", REPO_ROOT / "examples" / "serve_quantized.py")
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    error = example.serve(tokens=3)
+    assert 0.01 < error < 0.2
