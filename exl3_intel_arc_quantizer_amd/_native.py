@@ -91,7 +91,7 @@ _SIGNATURES = {
                                    _c_int, _c_vp]),
     "exl3_cache_read": (_c_int, [_c_vp, _c_i64, _c_int, _c_int, _c_int, _c_vp, _c_i64, _c_int,
                                  _c_vp, _c_vp, _c_vp]),
-    "exl3_cache_attention_workspace": (_c_i64, [_c_int, _c_int]),
+    "exl3_cache_attention_workspace": (_c_i64, [_c_i64, _c_int, _c_int, _c_int, _c_int, _c_i64]),
     "exl3_cache_attention": (_c_int, [_c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_int, _c_int, _c_vp,
                                       _c_i64, _c_int, _c_int, _c_int, _c_vp, _c_int, _c_vp, _c_vp,
                                       _c_int, _c_float, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp]),
@@ -1024,7 +1024,7 @@ def plan_step(cached, new, tables, free_pages, taken, page_size: int, max_tokens
         raise RuntimeError(f"max_tokens must be in 0..2^31 - 1, got {max_tokens}")
     slots = tables.new_empty(max_tokens, dtype=torch.int64)
     positions, starts, lengths, taken_out, status = tables.new_empty(
-        max_tokens + 2 * requests + 3).split([max_tokens, requests + 1, requests, 1, 1])
+        max_tokens + 2 * requests + 3).split_with_sizes([max_tokens, requests + 1, requests, 1, 1])
     _run(dev, "plan_step", load_library().exl3_plan_step, cached.data_ptr(), new.data_ptr(),
          requests, tables.data_ptr(), width, free_pages.data_ptr(), free_pages.numel(),
          taken.data_ptr(), page_size, max_tokens, slots.data_ptr(), positions.data_ptr(),
@@ -1119,11 +1119,12 @@ def cache_attention(q, pages, tables, starts, lengths, scale, window, max_new):
         raise RuntimeError(f"max_new must not be negative, got {max_new}")
     lib = load_library()
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    size = lib.exl3_cache_attention_workspace(requests, dim)
+    most = tokens if max_new is None else int(max_new)
+    size = lib.exl3_cache_attention_workspace(tokens, q_heads, heads, dim, requests, most)
     workspace = pages.new_empty(max(size, 0))
     _run(dev, "cache_attention", lib.exl3_cache_attention, q.data_ptr(), sq[0], sq[1],
          out.data_ptr(), tokens, q_heads, _types()[q.dtype], pages.data_ptr(), n, page_size, heads,
          dim, tables.data_ptr(), width, starts.data_ptr(), lengths.data_ptr(), requests,
          dim ** -0.5 if scale is None else float(scale), 2 ** 31 - 1 if window is None else
-         int(window), tokens if max_new is None else int(max_new), workspace.data_ptr(), size)
+         int(window), most, workspace.data_ptr(), size)
     return out

@@ -1300,6 +1300,18 @@ int64_t partials_bytes(Variant v, int head_dim) {
   return (int64_t)2 * owners_of(v, head_dim) * rows_of(v, head_dim) * (head_dim + 2) * 4;
 }
 
+// The launches of a call: the variant for its longest requests, and beside it,
+// so that single tokens keep the variant made for them and up to 16 rows their
+// precision, that of 8 rows for requests of up to `few`.
+struct Launches {
+  int count, few;
+  Variant of[2];
+};
+Launches launches_of(int64_t tokens, int group, int requests, int head_dim, int64_t max_new) {
+  const Variant v = variant_of(std::min(max_new, tokens) * group, head_dim);
+  return {requests > 1 && v != ROWS8 ? 2 : 1, v == ROWS16 ? 8 : 16, {v, ROWS8}};
+}
+
 template <int D, bool BF16>
 int launch_variant(Variant v, const AttendArgs& args, int index, unsigned grid, hipStream_t stream) {
   const Class& c = args.of[index];
@@ -1318,18 +1330,14 @@ int launch_variant(Variant v, const AttendArgs& args, int index, unsigned grid, 
 
 template <int D, bool BF16>
 int launch_attend(AttendArgs args, int64_t max_new, char* workspace, hipStream_t stream) {
-  const int64_t most = std::min(max_new, args.tokens) * args.group;
-  const Variant variants[2] = {variant_of(most, D), ROWS8};
-  // Single tokens beside longer requests keep the variant made for them, and
-  // rows of up to 16 their precision.
-  args.classes = args.requests > 1 && variants[0] != ROWS8 ? 2 : 1;
-  const int few = variants[0] == ROWS16 ? 8 : 16;
+  const Launches launches = launches_of(args.tokens, args.group, args.requests, D, max_new);
+  args.classes = launches.count;
   for (int i = 0; i < args.classes; ++i) {
     Class& c = args.of[i];
-    const Variant v = variants[i];
+    const Variant v = launches.of[i];
     c.rows = rows_of(v, D);
-    c.low = args.classes == 2 && i == 0 ? few + 1 : 1;
-    c.high = args.classes == 2 && i == 1 ? few : INT32_MAX;
+    c.low = args.classes == 2 && i == 0 ? launches.few + 1 : 1;
+    c.high = args.classes == 2 && i == 1 ? launches.few : INT32_MAX;
     c.owners = owners_of(v, D);
     // At most so many segments: whole where they fill the chip twice.
     const int64_t segments = ((args.tokens * args.group + c.rows - 1) / c.rows + args.requests) * args.cache.kv_heads;
@@ -1361,13 +1369,16 @@ int launch_attend(AttendArgs args, int64_t max_new, char* workspace, hipStream_t
 
 extern "C" {
 
-int64_t exl3_cache_attention_workspace(int requests, int head_dim) {
-  if (requests < 1 || requests > CACHE_MAX_REQUESTS || (head_dim != 64 && head_dim != 128 && head_dim != 256))
+int64_t exl3_cache_attention_workspace(int64_t tokens, int q_heads, int kv_heads, int head_dim,
+                                       int requests, int64_t max_new) {
+  if (requests < 1 || requests > CACHE_MAX_REQUESTS || (head_dim != 64 && head_dim != 128 && head_dim != 256) ||
+      tokens < 0 || kv_heads < 1 || q_heads < kv_heads || max_new < 0)
     return -1;
-  int64_t most = 0;
-  for (Variant v : {ROWS16, ROWS32, TILES})
-    most = std::max(most, shares_bytes(v, requests, head_dim) + partials_bytes(v, head_dim));
-  return shares_bytes(ROWS8, requests, head_dim) + partials_bytes(ROWS8, head_dim) + most;
+  const Launches launches = launches_of(tokens, q_heads / kv_heads, requests, head_dim, max_new);
+  int64_t bytes = 0;
+  for (int i = 0; i < launches.count; ++i)
+    bytes += shares_bytes(launches.of[i], requests, head_dim) + partials_bytes(launches.of[i], head_dim);
+  return bytes;
 }
 
 int exl3_cache_attention(const void* q, int64_t q_token, int64_t q_head, void* out, int64_t tokens,
@@ -1396,7 +1407,8 @@ int exl3_cache_attention(const void* q, int64_t q_token, int64_t q_head, void* o
   if (((reinterpret_cast<uintptr_t>(pages) | reinterpret_cast<uintptr_t>(workspace)) & 15) ||
       (reinterpret_cast<uintptr_t>(out) & 7))
     return set_error("exl3_cache_attention: pages, out and workspace must be aligned");
-  if (workspace_bytes < exl3_cache_attention_workspace(requests, head_dim))
+  if (max_new < 0) return set_error("exl3_cache_attention: max_new %lld is negative", (long long)max_new);
+  if (workspace_bytes < exl3_cache_attention_workspace(tokens, q_heads, kv_heads, head_dim, requests, max_new))
     return set_error("exl3_cache_attention: workspace of %lld bytes is too small", (long long)workspace_bytes);
   if (!tokens) return 0;
   AttendArgs a{};

@@ -273,8 +273,10 @@ int exl3_cache_append(const void* q, int64_t q_token, int64_t q_head, void* q_ou
 int exl3_cache_read(const void* pages, int64_t num_pages, int page_size, int kv_heads, int head_dim,
                     const int64_t* slots, int64_t tokens, int type, void* k, void* v, void* stream);
 
-/* Bytes of workspace that exl3_cache_attention needs, or -1. */
-int64_t exl3_cache_attention_workspace(int requests, int head_dim);
+/* Bytes of workspace that exl3_cache_attention needs with these arguments, or
+ * -1. */
+int64_t exl3_cache_attention_workspace(int64_t tokens, int q_heads, int kv_heads, int head_dim,
+                                       int requests, int64_t max_new);
 
 /* Attention of new tokens over the cache. Request r's queries are rows
  * starts[r] .. starts[r + 1] - 1 of q (float16 or bfloat16), its last of
