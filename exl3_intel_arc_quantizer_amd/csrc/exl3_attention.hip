@@ -151,22 +151,22 @@ __device__ __forceinline__ void sum_work(const AttendArgs& a, const Class& c, T*
   __syncthreads();
 }
 
-// A value that all lanes of the wave hold, kept in scalar registers.
-__device__ __forceinline__ int64_t uniform(int64_t v) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
-  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)v >> 32));
+// A value that all lanes of the wave hold, or that of one, in scalar registers.
+__device__ __forceinline__ int64_t uniform(int64_t v, int lane = 0) {
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, lane);
+  const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)((uint64_t)v >> 32), lane);
   return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// x / d, which nearly always fits 32 bits.
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t d) {
+  return (x | d) >> 32 ? x / d : (int64_t)((uint32_t)x / (uint32_t)d);
 }
 
 // The work is cut into equal shares, one an owner, of LEAST at least.
 constexpr int LEAST = 2;
 __device__ __forceinline__ int64_t share_of(const Class& c, int64_t all) {
-  return max((all + c.owners - 1) / c.owners, (int64_t)LEAST);
-}
-
-// x / d, which nearly always fits 32 bits.
-__device__ __forceinline__ int quotient(int64_t x, int64_t d) {
-  return (x | d) >> 32 ? (int)(x / d) : (int)((uint32_t)x / (uint32_t)d);
+  return max(quotient(all + c.owners - 1, c.owners), (int64_t)LEAST);
 }
 
 // Last index i of [0, n) with at[i] <= x; at[0] <= x.
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(THREADS, resident(D, WIDE, CT)) attend_rows_ke
     const Request req = request_of(a, r);
     const int blocks = blocks_of(a, cls, req), rows = req.n * a.group;
     const int64_t before = uniform(prefix[r]);
-    const int segment = quotient(at - before, req.tiles + SEGMENT_COST);
+    const int segment = (int)quotient(at - before, req.tiles + SEGMENT_COST);
     const int head = segment / blocks, block = segment - head * blocks;
     const int64_t seg0 = before + (int64_t)segment * (req.tiles + SEGMENT_COST) + SEGMENT_COST;
     const int64_t seg1 = seg0 + req.tiles;
@@ -400,7 +400,6 @@ __global__ void __launch_bounds__(THREADS, resident(D, WIDE, CT)) attend_rows_ke
     Tile<D> even, odd;
     int page_even = page_of(t0), page_odd = page_of(t0 + 1);
     even.load(tile_at(t0, page_even), lane);
-
     // Queries, scaled by a power of two so that float16 holds them whatever
     // the type's range; hi in columns 0..7 and lo in 8..15 of narrow blocks.
     u32x4 qf[CT][GROUPS], ql[REST ? CT : 1][REST ? GROUPS : 1];
@@ -919,7 +918,6 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
       for (int i = 0; i < 3 * TT; ++i) page[i] = page_of(t0 + i);
       fetch(t0, page[0]);
     }
-
     // Queries, scaled by a power of two so that float16 holds them.
     u32x4 qf[STEPS], ql[REST && !SHARED_REST ? STEPS : 1];
     float qs, rise;
@@ -1152,99 +1150,118 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
 }
 
 // The partial results of an output row (token, query head) that more than one
-// owner has taken, joined; rows of no work are 0; whole ones are left. Partials
-// are taken four at a time with a running maximum, so that a row of few waits
-// for memory once. SPREAD waves share one row's partials where there are few
-// rows, each with many; otherwise a wave takes `run` rows one after another
-// (a prompt's are all whole: it only has to see that).
+// owner has taken, joined; rows of no work are 0; whole ones are left. Its time
+// is that of lookups and loads that wait for each other, so partials are taken
+// BATCH at a time with a running maximum. SPREAD waves share one row's partials
+// where there are few rows, each with many (384 rows of 85: 14 us with 8 waves,
+// 15 with 16 or 4); otherwise a wave takes four rows at once, sixteen lanes
+// each, and `run` one after another (51 MB of partials for 88000 rows of head
+// dimension 256: 17 us, row by row 28). A prompt's rows are all whole: there it
+// only has to see that (6 us for 8192 tokens).
 template <int D, bool BF16, int SPREAD>
 __global__ void __launch_bounds__(SPREAD > 1 ? 64 * SPREAD : THREADS) attend_join_kernel(AttendArgs a, int run) {
-  constexpr int PER = D / 64, BATCH = 4;
+  constexpr int LANES = SPREAD > 1 ? 64 : 16, ROWS = 64 / LANES, PER = D / LANES, VEC = PER < 4 ? PER : 4;
+  constexpr int BATCH = SPREAD > 1 || D < 256 ? 4 : 2;  // by the registers they take
+  typedef float values __attribute__((ext_vector_type(VEC)));
+  typedef uint16_t narrows __attribute__((ext_vector_type(VEC)));
   __shared__ float held[SPREAD][SPREAD > 1 ? D : 1], tops[SPREAD], sums[SPREAD];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t first = SPREAD > 1 ? (int64_t)blockIdx.x : ((int64_t)blockIdx.x * WAVES + wave) * run;
   const int64_t past = min(first + run, a.tokens * a.q_heads);
-  int64_t token = -1;
-  int r = 0;
-  Request req{};
-  bool work = false;
-  for (int64_t at = first; at < past; ++at) {
-    const int64_t of_token = at / a.q_heads;
-    const int qh = (int)(at - of_token * a.q_heads);
-    if (of_token != token) {
-      // The request: as many starts after the first as are not past the token.
-      token = of_token;
-      r = 0;
-      for (int r0 = 0; r0 < a.requests; r0 += 64)
-        r += __popcll(__ballot(r0 + lane < a.requests && a.starts[r0 + lane + 1] <= token));
-      work = false;
-      if (r < a.requests) {
-        req = request_of(a, r);
-        work = req.tiles && token >= req.first && token < req.first + req.n;
+  int64_t found = -1;                                    // the token that `request` is of
+  int request = 0;
+  for (int64_t at = first; at < past; at += ROWS) {
+    const int64_t row = min(at + lane / LANES, past - 1);
+    const int64_t token = quotient(row, a.q_heads);
+    int r = 0;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int64_t of = uniform(token, i * LANES);
+      if (of != found) {
+        // The request: as many starts after the first as are not past the token.
+        found = of, request = 0;
+        for (int r0 = 0; r0 < a.requests; r0 += 64)
+          request += __popcll(__ballot(r0 + lane < a.requests && a.starts[r0 + lane + 1] <= of));
       }
+      r = lane / LANES == i ? request : r;
     }
     float x[PER], top = NONE, l = 0.0f;
 #pragma unroll
     for (int e = 0; e < PER; ++e) x[e] = 0.0f;
-    if (work) {
-      const Class& cls = a.of[a.classes == 1 || takes(a, a.of[0], req) ? 0 : 1];
-      if (cls.whole) {
-        // Nor are the token's other rows: on to the next token's first.
-        at = (token + 1) * a.q_heads - 1;
-        continue;
-      }
-      const int head = qh / a.group, of = (int)(token - req.first) * a.group + qh % a.group;
-      const int blocks = blocks_of(a, cls, req), row = of % cls.rows, stride = cls.rows * (D + 2);
-      int64_t seg0, seg1, all;
-      if (cls.by_block) {
-        const int64_t* costs = cls.shares + a.requests + 1;
-        const int64_t i = min(cls.shares[r] + of / cls.rows, cls.shares[a.requests] - 1), cost = costs[i + 1] - costs[i];
-        all = costs[cls.shares[a.requests]] * a.cache.kv_heads;
-        seg1 = costs[i] * a.cache.kv_heads + (head + 1) * cost;
-        seg0 = seg1 - cost + SEGMENT_COST;
-      } else {
-        all = cls.shares[a.requests];
-        seg0 = cls.shares[r] + ((int64_t)head * blocks + of / cls.rows) * (req.tiles + SEGMENT_COST) + SEGMENT_COST;
-        seg1 = seg0 + req.tiles;
-      }
-      const int64_t share = share_of(cls, all);
-      const int w0 = __builtin_amdgcn_readfirstlane((int)(seg0 / share));
-      const int w1 = seg1 > seg0 ? __builtin_amdgcn_readfirstlane((int)((seg1 - 1) / share)) : w0 - 1;
-      if (w0 == w1) continue;
-      const int stats = cls.rows * D + 2 * row;           // a row's maximum and sum in a slot
-      for (int w = w0 + wave % SPREAD; w <= w1; w += BATCH * SPREAD) {
-        float peak[BATCH], sum[BATCH], v[BATCH][PER];
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-          // The first owner's share ends in this segment (slot 1), the others'
-          // begin in it (slot 0).
-          const int own = min(w + i * SPREAD, w1);
-          const float* part = cls.partials + (2 * (int64_t)own + (own == w0)) * stride;
-          peak[i] = part[stats], sum[i] = part[stats + 1];
-#pragma unroll
-          for (int e = 0; e < PER; ++e) v[i][e] = part[row * D + PER * lane + e];
+    bool writes = at + lane / LANES < past, skip = false;
+    if (r < a.requests) {
+      const Request req = request_of(a, r);
+      if (req.tiles && token >= req.first && token < req.first + req.n) {
+        // Field by field, so that the choice is not a load.
+        const bool main = a.classes == 1 || takes(a, a.of[0], req);
+        auto either = [&](auto Class::*field) { return main ? a.of[0].*field : a.of[1].*field; };
+        Class cls;
+        cls.rows = either(&Class::rows), cls.owners = either(&Class::owners);
+        cls.by_block = either(&Class::by_block), cls.whole = either(&Class::whole);
+        cls.shares = either(&Class::shares), cls.partials = either(&Class::partials);
+        const int qh = (int)(row - token * a.q_heads), head = qh / a.group;
+        const int of = (int)(token - req.first) * a.group + qh - head * a.group;
+        const int block = of / cls.rows, line = of - block * cls.rows, stride = cls.rows * (D + 2);
+        int64_t w0 = 0, w1 = 0;
+        if (cls.whole) {
+          skip = true;
+        } else {
+          int64_t seg0, seg1, all;
+          if (cls.by_block) {
+            const int64_t* costs = cls.shares + a.requests + 1;
+            const int64_t listed = cls.shares[a.requests];
+            const int64_t i = min(cls.shares[r] + block, listed - 1), before = costs[i], cost = costs[i + 1] - before;
+            all = costs[listed] * a.cache.kv_heads;
+            seg1 = before * a.cache.kv_heads + (head + 1) * cost;
+            seg0 = seg1 - cost + SEGMENT_COST;
+          } else {
+            all = cls.shares[a.requests];
+            seg0 = cls.shares[r] + ((int64_t)head * blocks_of(a, cls, req) + block) * (req.tiles + SEGMENT_COST) + SEGMENT_COST;
+            seg1 = seg0 + req.tiles;
+          }
+          const int64_t share = share_of(cls, all);
+          w0 = quotient(seg0, share);
+          w1 = seg1 > seg0 ? quotient(seg1 - 1, share) : w0 - 1;
         }
-        float newer = top;
+        if (w0 == w1) writes = false, w1 = w0 - 1;
+        const int stats = cls.rows * D + 2 * line;       // a row's maximum and sum in a slot
+        for (int64_t w = w0 + wave % SPREAD; w <= w1; w += BATCH * SPREAD) {
+          float peak[BATCH], sum[BATCH];
+          values v[BATCH][PER / VEC];
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) newer = fmaxf(newer, peak[i]);
-        const float keep = top == newer ? 1.0f : __builtin_amdgcn_exp2f(top - newer);
-        top = newer;
-        l *= keep;
+          for (int i = 0; i < BATCH; ++i) {
+            // The first owner's share ends in this segment (slot 1), the others'
+            // begin in it (slot 0).
+            const int64_t own = min(w + i * SPREAD, w1);
+            const float* part = cls.partials + (2 * own + (own == w0)) * stride;
+            peak[i] = part[stats], sum[i] = part[stats + 1];
 #pragma unroll
-        for (int e = 0; e < PER; ++e) x[e] *= keep;
+            for (int e = 0; e < PER / VEC; ++e)
+              v[i][e] = *reinterpret_cast<const values*>(part + line * D + VEC * (e * LANES + lane % LANES));
+          }
+          float newer = top;
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-          // A share without an attended position leaves its values unwritten.
-          const bool holds = w + i * SPREAD <= w1 && (peak[i] != NONE || sum[i] != 0.0f);
-          const float weight = peak[i] == NONE ? 1.0f : __builtin_amdgcn_exp2f(peak[i] - newer);
-          l += holds ? sum[i] * weight : 0.0f;
+          for (int i = 0; i < BATCH; ++i) newer = fmaxf(newer, peak[i]);
+          const float keep = top == newer ? 1.0f : __builtin_amdgcn_exp2f(top - newer);
+          top = newer;
+          l *= keep;
 #pragma unroll
-          for (int e = 0; e < PER; ++e) x[e] += holds ? v[i][e] * weight : 0.0f;
+          for (int e = 0; e < PER; ++e) x[e] *= keep;
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i) {
+            // A share without an attended position leaves its values unwritten.
+            const bool holds = w + i * SPREAD <= w1 && (peak[i] != NONE || sum[i] != 0.0f);
+            const float weight = peak[i] == NONE ? 1.0f : __builtin_amdgcn_exp2f(peak[i] - newer);
+            l += holds ? sum[i] * weight : 0.0f;
+#pragma unroll
+            for (int e = 0; e < PER; ++e) x[e] += holds ? v[i][e / VEC][e % VEC] * weight : 0.0f;
+          }
         }
       }
     }
     if constexpr (SPREAD > 1) {
-      // One row a workgroup: all its waves are here together.
+      // One row a workgroup, whose waves agree on what it is.
+      if (!writes) return;
 #pragma unroll
       for (int e = 0; e < PER; ++e) held[wave][PER * lane + e] = x[e];
       if (lane == 0) tops[wave] = top, sums[wave] = l;
@@ -1263,9 +1280,19 @@ __global__ void __launch_bounds__(SPREAD > 1 ? 64 * SPREAD : THREADS) attend_joi
         for (int e = 0; e < PER; ++e) x[e] += held[i][PER * lane + e] * weight;
       }
     }
-    const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+    if (writes) {
+      const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-    for (int e = 0; e < PER; ++e) a.out[at * D + PER * lane + e] = (uint16_t)narrow<BF16>(x[e] * inverse);
+      for (int e = 0; e < PER / VEC; ++e) {
+        narrows w;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) w[i] = (uint16_t)narrow<BF16>(x[VEC * e + i] * inverse);
+        *reinterpret_cast<narrows*>(a.out + row * D + VEC * (e * LANES + lane % LANES)) = w;
+      }
+    }
+    // Where the last row's request is whole, so are the token's other rows: on
+    // to the next token's first.
+    if (__builtin_amdgcn_readlane(skip, 63)) at = (found + 1) * a.q_heads - ROWS;
   }
 }
 
@@ -1353,12 +1380,12 @@ int launch_attend(AttendArgs args, int64_t max_new, char* workspace, hipStream_t
   }
   const int64_t rows = args.tokens * args.q_heads;
   if (rows <= 2 * CUS) {
-    attend_join_kernel<D, BF16, 16><<<(unsigned)rows, 64 * 16, 0, stream>>>(args, 1);
+    attend_join_kernel<D, BF16, 8><<<(unsigned)rows, 64 * 8, 0, stream>>>(args, 1);
   } else if (rows <= 8 * CUS) {
     attend_join_kernel<D, BF16, 4><<<(unsigned)rows, 64 * 4, 0, stream>>>(args, 1);
   } else {
-    // Rows to a wave: its token's lookups are for all of them.
-    const int64_t run = std::min<int64_t>(std::max<int64_t>(1, rows / (16 * CUS * WAVES)), 64);
+    // Rows to a wave, by fours; as many as a token or more where all are whole.
+    const int64_t run = std::min<int64_t>(std::max<int64_t>(args.of[0].whole ? 64 : 4, rows / (16 * CUS * WAVES) / 4 * 4), 64);
     const int64_t waves = (rows + run - 1) / run;
     attend_join_kernel<D, BF16, 1><<<(unsigned)((waves + WAVES - 1) / WAVES), THREADS, 0, stream>>>(args, (int)run);
   }
