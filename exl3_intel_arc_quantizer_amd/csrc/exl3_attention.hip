@@ -325,6 +325,12 @@ constexpr int resident(int d, bool wide, int ct) {
 //
 // Two tiles' registers take turns: one is loaded while the other is
 // multiplied, and table entries are read a tile further ahead.
+//
+// Bound by reading the cache where there are few rows: 128 requests of up to
+// 8192 positions, 8 kv heads of 128, one token: 504 MB in 107 us, 4.7 TB/s of the
+// 5.0 a large copy reaches, vector instructions on 0.58 of the cycles. With 32
+// rows a tile they and the products get as long as the reading: 157 MB in
+// 51 us, of which about 10 are the waves' start and end.
 template <int D, bool WIDE, int CT, bool BF16>
 __global__ void __launch_bounds__(THREADS, resident(D, WIDE, CT)) attend_rows_kernel(AttendArgs a, int index) {
   constexpr int PER = WIDE ? 16 : 8, ROWS = PER * CT, GROUPS = D / 32, SETS = Tile<D>::SETS, NIB = D == 64 ? 4 : 8;
@@ -693,6 +699,13 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 // of 32 rows a wave, and unpacks two tiles at a time (of head dimension 256,
 // one), as float16, into shared memory, where all its waves read them.
 //
+// Of head dimension 256 two waves share 32 rows, as one has no registers for
+// their outputs beside a second wave on its SIMD: each multiplies half the dims
+// of queries and keys, the parts of the scores are exchanged through shared
+// memory, and each weighs its half of the values (a wave for all dims, one a
+// SIMD: prompts of 8192 tokens in bfloat16 549 TFLOP/s, float16 490; so 655 and
+// 556).
+//
 // The same products as above at 32 x 32 x 16: S^T = K Q^T in one accumulator
 // of 32 tokens x 32 rows a tile, O^T += V^T P^T in D / 32. Lane (n, h) of S^T
 // holds row n's scores of positions 8 b + 4 h + x of the product's rows; keys
@@ -700,21 +713,29 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 // these are tokens 16 c + 8 h .. + 7, the eight that the lane's operand of P^T
 // wants. Sixteen-byte vectors of a key row (of a value dim) are permuted by the
 // low bits of the row (the dim), so that the sixteen lanes that read in one
-// cycle read different banks. Two tiles a step, because the products of one tile's scores
-// wait for each other. Two buffers and one barrier a step: while one is
-// multiplied the next is unpacked, and the codes after it are on their way.
+// cycle read different banks. Two tiles a step, because the products of one
+// tile's scores wait for each other. Two buffers and one barrier a step: while
+// one is multiplied the next is unpacked, and the codes after it are on their
+// way.
+//
+// Bound by issue: matrix instructions take 0.43 of the cycles, vector ones (the
+// softmax above all) 0.5, and two waves a SIMD overlap them little. A prompt of
+// 8192 tokens, 32 heads of 128 over 8, bfloat16: 550 GFLOP in 0.60 ms, 917
+// TFLOP/s (a library product of 8192 a side: 1113).
 //
 // Weights, and bfloat16 queries, count with 11 bits (errors under 2^-11 of the
-// output's terms); float16 queries keep their rest in products of their own, of
-// head dimension 256 from shared memory: in registers it made the compiler spill,
-// and every reload waits for the codes on their way as well.
-constexpr int tile_waves(int d) { return d == 128 ? 8 : 4; }
+// output's terms); float16 queries keep their rest in products of their own.
+constexpr int tile_waves(int d) { return d == 64 ? 4 : 8; }
+constexpr int tile_halves(int d) { return d == 256 ? 2 : 1; }  // waves that share 32 rows, each with a part of the dims
+constexpr int tile_rows(int d) { return 32 * tile_waves(d) / tile_halves(d); }
 constexpr int tile_groups(int d) { return d == 64 ? 3 : 1; }  // workgroups of a compute unit
 template <int D, bool BF16>
 __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_waves(D) / 4)
     attend_tiles_kernel(AttendArgs a, int index) {
-  constexpr int NW = tile_waves(D), NT = 64 * NW, ROWS = 32 * NW, GROUPS = D / 32, STEPS = D / 16;
-  constexpr bool REST = !BF16, SHARED_REST = REST && D == 256;
+  constexpr int NW = tile_waves(D), NT = 64 * NW, ROWS = tile_rows(D), STEPS = D / 16;
+  constexpr int HALVES = tile_halves(D), GROUPS = D / 32, OWN = GROUPS / HALVES, TAKES = STEPS / HALVES;  // a wave's own
+
+  constexpr bool REST = !BF16;
   constexpr int TT = D == 256 ? 1 : 2;                   // tiles of a step
   // Parts of a tile: a dword of key codes, and two dims (a byte) of four tokens'
   // values. A thread takes KN of them.
@@ -725,11 +746,12 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
   extern __shared__ int64_t dynamic[];                   // costs, then prefix
   __shared__ int64_t parts[NW];
   __shared__ u32x4 keys[2 * TT * TILE / 16], values[2 * TT * TILE / 16];  // [buffer][tile]
-  __shared__ u32x4 rests[SHARED_REST ? NW * STEPS * 64 : 1];    // [wave][step][lane]
+  __shared__ f32x4 scores[HALVES == 2 ? NW * 4 * 64 : 1];  // [wave][vector][lane], a wave's part of them
   __shared__ int poison[2];
 
   const Class& cls = a.of[index];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rows32 = wave / HALVES, half = wave % HALVES;
   const int n = lane & 31, h = lane >> 5;
   const Magic magic;
   int64_t* costs = dynamic;                              // [blocks + 1], if blocks may be cut
@@ -783,7 +805,7 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
   uint32_t key_at = 4 * tid, key_scale_at = 32 * D + (tid / (D / 8) * GROUPS + tid % GROUPS) * 2;
   uint32_t value_at = 16 * D + tid / 4 * 16;
   uint32_t value_scale_at = 34 * D + ((tid / D * GROUPS + tid / 8 % (D / 8) / 4) * 2 + (tid / 4 & 1)) * 8;
-  uint32_t key_row = n * (2 * D) + (h ^ (n & SPAN)) * 16, value_row = n * 64 + (h ^ (n >> 2 & 3)) * 16;
+  uint32_t key_row = half * D + n * (2 * D) + (h ^ (n & SPAN)) * 16, value_row = half * (OWN * 2048) + n * 64 + (h ^ (n >> 2 & 3)) * 16;
   asm volatile("" : "+v"(key_at), "+v"(key_scale_at), "+v"(value_at), "+v"(value_scale_at), "+v"(key_row), "+v"(value_row));
   if (tid < 2) poison[tid] = -1;
   int count = 0;                                         // steps so far; names a buffer's content
@@ -821,12 +843,12 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
     float* part = cls.partials + ((int64_t)owner * 2 + (first == 0)) * (ROWS * (D + 2));
 
     // This wave's rows and what they attend.
-    const int row = 32 * wave + n;
+    const int row = 32 * rows32 + n;
     const bool there = row0 + row < rows;
     const int token = there ? (row0 + row) / a.group : 0, of_group = there ? row0 + row - token * a.group : 0;
     const int last = there ? offset + token : -1;
     const int from = there ? (int)max((int64_t)last - a.window + 1, (int64_t)0) : 0;
-    const int wave0 = min(row0 + 32 * wave, row1), wave1 = min(row0 + 32 * wave + 31, row1);
+    const int wave0 = min(row0 + 32 * rows32, row1), wave1 = min(row0 + 32 * rows32 + 31, row1);
     const int wave_least = offset + wave0 / a.group, wave_most = offset + wave1 / a.group;
     const int wave_from = (int)max((int64_t)wave_most - a.window + 1, (int64_t)0);
 
@@ -854,38 +876,39 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
         vs[u] = __builtin_amdgcn_raw_buffer_load_b64(tile, value_scale_at + u * (NT / D * GROUPS * 16), 0, 0);
       }
     };
-    // Unpacked to a tile of a buffer.
+    // Unpacked to a tile of a buffer; of this thread's parts, one.
+    auto unpack_part = [&](int buffer, int which, int u) __attribute__((always_inline)) {
+      const uint32_t d = tid + u * NT, base = (TT * buffer + which) * (TILE / 16);
+      {
+        const uint32_t token = d / (D / 8), inside = d % (D / 8);
+        const uint32_t vector = 4 * (inside % GROUPS) + inside / GROUPS;
+        // Bits 2 and 3 of the token exchanged.
+        const uint32_t to = (token & 0x13) | (token & 4) << 1 | (token & 8) >> 1;
+        const f16x2 scale = halves_of(ks[u] | ks[u] << 16);
+        u32x4 f;
+        f[0] = values_of<true>(kc[u], scale, magic);
+        f[1] = values_of<false>(kc[u], scale, magic);
+        f[2] = values_of<true>(kc[u] >> 8, scale, magic);
+        f[3] = values_of<false>(kc[u] >> 8, scale, magic);
+        keys[base + to * (D / 8) + (vector ^ (to & SPAN))] = f;
+      }
+      const uint32_t byte = d & 3, four = d / 4, octet = d / D, column = d / 8 % (D / 8);
+      const uint32_t pick = 0x0c000c04u | byte << 16 | byte;
+      u32x2 lo, hi;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t w = __builtin_amdgcn_perm(vc[u][2 * e], vc[u][2 * e + 1], pick);
+        const f16x2 scale = halves_of(vs[u][e]);
+        lo[e] = values_of<true>(w, scale, magic);
+        hi[e] = values_of<false>(w, scale, magic);
+      }
+      const uint32_t dim = 8 * column + 2 * byte;      // dims 4 x .. 4 x + 3 permute alike
+      u32x2* to = reinterpret_cast<u32x2*>(&values[base + dim * 4 + (octet ^ (dim >> 2 & 3))]) + (four & 1);
+      to[0] = lo, to[8] = hi;
+    };
     auto unpack = [&](int buffer, int which) __attribute__((always_inline)) {
 #pragma unroll
-      for (int u = 0; u < KN; ++u) {
-        const uint32_t d = tid + u * NT, base = (TT * buffer + which) * (TILE / 16);
-        {
-          const uint32_t token = d / (D / 8), inside = d % (D / 8);
-          const uint32_t vector = 4 * (inside % GROUPS) + inside / GROUPS;
-          // Bits 2 and 3 of the token exchanged.
-          const uint32_t to = (token & 0x13) | (token & 4) << 1 | (token & 8) >> 1;
-          const f16x2 scale = halves_of(ks[u] | ks[u] << 16);
-          u32x4 f;
-          f[0] = values_of<true>(kc[u], scale, magic);
-          f[1] = values_of<false>(kc[u], scale, magic);
-          f[2] = values_of<true>(kc[u] >> 8, scale, magic);
-          f[3] = values_of<false>(kc[u] >> 8, scale, magic);
-          keys[base + to * (D / 8) + (vector ^ (to & SPAN))] = f;
-        }
-        const uint32_t byte = d & 3, four = d / 4, octet = d / D, column = d / 8 % (D / 8);
-        const uint32_t pick = 0x0c000c04u | byte << 16 | byte;
-        u32x2 lo, hi;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint32_t w = __builtin_amdgcn_perm(vc[u][2 * e], vc[u][2 * e + 1], pick);
-          const f16x2 scale = halves_of(vs[u][e]);
-          lo[e] = values_of<true>(w, scale, magic);
-          hi[e] = values_of<false>(w, scale, magic);
-        }
-        const uint32_t dim = 8 * column + 2 * byte;      // dims 4 x .. 4 x + 3 permute alike
-        u32x2* to = reinterpret_cast<u32x2*>(&values[base + dim * 4 + (octet ^ (dim >> 2 & 3))]) + (four & 1);
-        to[0] = lo, to[8] = hi;
-      }
+      for (int u = 0; u < KN; ++u) unpack_part(buffer, which, u);
     };
     // A weight of 0 must not meet a NaN or infinity: in steps that some row
     // does not attend whole, such scales of values count as 0, and the rows
@@ -919,7 +942,7 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
       fetch(t0, page[0]);
     }
     // Queries, scaled by a power of two so that float16 holds them.
-    u32x4 qf[STEPS], ql[REST && !SHARED_REST ? STEPS : 1];
+    u32x4 qf[TAKES], ql[REST ? TAKES : 1];
     float qs, rise;
     {
       const uint16_t* src = a.q + (int64_t)(req.first + token) * a.q_token + (int64_t)(head * a.group + of_group) * a.q_head;
@@ -946,26 +969,24 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
       if (top > 0.0f && top < __builtin_inff()) frexpf(top, &power);
       const float flip = a.scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
-      for (int k = 0; k < STEPS; ++k)
+      for (int k = 0; k < TAKES; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float y0 = flip * ldexpf(x[k][2 * e], -power), y1 = flip * ldexpf(x[k][2 * e + 1], -power);
+          const float z0 = half ? x[STEPS - TAKES + k][2 * e] : x[k][2 * e];
+          const float z1 = half ? x[STEPS - TAKES + k][2 * e + 1] : x[k][2 * e + 1];
+          const float y0 = flip * ldexpf(z0, -power), y1 = flip * ldexpf(z1, -power);
           const f16x2 hi = {(_Float16)y0, (_Float16)y1};
           qf[k][e] = bits_of(hi);
-          const uint32_t low = bits_of(f16x2{(_Float16)(y0 - (float)hi[0]), (_Float16)(y1 - (float)hi[1])});
-          if constexpr (SHARED_REST)
-            reinterpret_cast<uint32_t*>(&rests[(wave * STEPS + k) * 64 + lane])[e] = low;
-          else if constexpr (REST)
-            ql[k][e] = low;
+          if constexpr (REST) ql[k][e] = bits_of(f16x2{(_Float16)(y0 - (float)hi[0]), (_Float16)(y1 - (float)hi[1])});
         }
       qs = fmaxf(ldexpf(fabsf(a.scale) * 0.25f * 1.4426950408889634f, power), 0x1p-120f);
       rise = 8.0f / qs;
     }
 
     float run = NONE, sum = 0.0f;
-    f32x16 o[GROUPS];
+    f32x16 o[OWN];
 #pragma unroll
-    for (int d = 0; d < GROUPS; ++d) o[d] = f32x16{};
+    for (int d = 0; d < OWN; ++d) o[d] = f32x16{};
 
     // This lane's vectors of a key row and a value dim: the permutation is an
     // exclusive or of address bits, so one address serves all of a buffer.
@@ -991,7 +1012,10 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
 #pragma unroll
       for (int u = 0; u < TT; ++u) after[u] = page_of(t + 3 * TT + u);
       // The next step's tiles are unpacked after this one's scores are
-      // multiplied; of two, whose codes come one by one, the first before.
+      // multiplied; of two, whose codes come one by one, the first before. A
+      // single one beside the products of the scores, but not where the
+      // queries' rest needs the registers (head dimension 256, TFLOP/s of a
+      // prompt of 8192: bfloat16 655, after them 617; float16 545 and 556).
       const bool dirty = partial(t + TT, missing(1));
       if (dirty) clean(then, count + 1);
       if constexpr (TT == 2) {
@@ -1005,12 +1029,14 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
       // whole latency (a prompt of 8192 tokens: 647 us, with them 582).
       f32x16 s[2] = {};                                  // of two tiles, or of queries and their rest
       u32x4 f[2][AHEAD];
-      auto second = [&](int k) { return TT == 2 ? key(k, place + TILE) : SHARED_REST ? rests[(wave * STEPS + k) * 64 + lane] : u32x4{}; };
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) f[0][k] = key(k, place), f[1][k] = second(k);
+      for (int k = 0; k < AHEAD; ++k) {
+        f[0][k] = key(k, place);
+        if constexpr (TT == 2) f[1][k] = key(k, place + TILE);
+      }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int k = 0; k < STEPS; ++k) {
+      for (int k = 0; k < TAKES; ++k) {
         const u32x4 w0 = f[0][k % AHEAD], w1 = f[1][k % AHEAD];
         if constexpr (TT == 2) {
           s[0] = mfma32(w0, qf[k], s[0]);
@@ -1019,19 +1045,33 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
             s[0] = mfma32(w0, ql[k], s[0]);
             s[1] = mfma32(w1, ql[k], s[1]);
           }
-        } else {
+        } else if constexpr (REST) {
           // Two sums in turn, as the products of one wait for each other.
-          if constexpr (SHARED_REST) {
-            s[0] = mfma32(w0, qf[k], s[0]);
-            s[1] = mfma32(w0, w1, s[1]);
-          } else {
-            s[k & 1] = mfma32(w0, qf[k], s[k & 1]);
-          }
+          s[0] = mfma32(w0, qf[k], s[0]);
+          s[1] = mfma32(w0, ql[k], s[1]);
+        } else {
+          s[k & 1] = mfma32(w0, qf[k], s[k & 1]);
         }
-        if (k + AHEAD < STEPS) {
-          f[0][k % AHEAD] = key(k + AHEAD, place), f[1][k % AHEAD] = second(k + AHEAD);
+        if constexpr (TT == 1 && !REST) {
+          if (k % (TAKES / KN) == TAKES / KN - 1) unpack_part(then, 0, k / (TAKES / KN));
+        }
+        if (k + AHEAD < TAKES) {
+          f[0][k % AHEAD] = key(k + AHEAD, place);
+          if constexpr (TT == 2) f[1][k % AHEAD] = key(k + AHEAD, place + TILE);
           __builtin_amdgcn_sched_barrier(0);
         }
+      }
+      if constexpr (HALVES == 2) {
+        // Both halves add the same two parts, so they agree on every score.
+        s[0] += s[1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          scores[(wave * 4 + e) * 64 + lane] = f32x4{s[0][4 * e], s[0][4 * e + 1], s[0][4 * e + 2], s[0][4 * e + 3]};
+        if constexpr (REST) unpack(then, 0);
+        fetch(t + 2, page[2]);
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[1][e] = scores[((wave ^ 1) * 4 + (e >> 2)) * 64 + lane][e & 3];
       }
       float x[16 * TT];
 #pragma unroll
@@ -1054,17 +1094,19 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
         run = top;
         sum *= shrink;
 #pragma unroll
-        for (int d = 0; d < GROUPS; ++d) o[d] *= shrink;
+        for (int d = 0; d < OWN; ++d) o[d] *= shrink;
       }
       const float ref = run == NONE ? 0.0f : -run * qs;
-      // Product v of the output: 16 tokens v / GROUPS, dims of group v % GROUPS.
-      auto operand = [&](int v) { return value(2 * (v % GROUPS) + (v / GROUPS & 1), place + v / GROUPS / 2 * TILE); };
+      // Product v of the output: 16 tokens v / OWN, dims of group v % OWN.
+      auto operand = [&](int v) { return value(2 * (v % OWN) + (v / OWN & 1), place + v / OWN / 2 * TILE); };
 #pragma unroll
       for (int v = 0; v < 2 * AHEAD; ++v) f[v & 1][v / 2] = operand(v);
       __builtin_amdgcn_sched_barrier(0);
       if (TT == 2 && dirty) clean(then, count + 1);
-      unpack(then, TT - 1);
-      fetch(t + 2 * TT, page[2 * TT]);
+      if constexpr (TT == 2) {
+        unpack(then, 1);
+        fetch(t + 4, page[4]);
+      }
       u32x4 p[2 * TT];
 #pragma unroll
       for (int e = 0; e < 8 * TT; ++e) {
@@ -1074,10 +1116,10 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
         p[e >> 2][e & 3] = bits_of(w);
       }
 #pragma unroll
-      for (int v = 0; v < 2 * TT * GROUPS; ++v) {
+      for (int v = 0; v < 2 * TT * OWN; ++v) {
         u32x4& w = f[v & 1][v / 2 % AHEAD];
-        o[v % GROUPS] = mfma32(w, p[v / GROUPS], o[v % GROUPS]);
-        if (v + 2 * AHEAD < 2 * TT * GROUPS) {
+        o[v % OWN] = mfma32(w, p[v / OWN], o[v % OWN]);
+        if (v + 2 * AHEAD < 2 * TT * OWN) {
           w = operand(v + 2 * AHEAD);
           if (v & 1) __builtin_amdgcn_sched_barrier(0);
         }
@@ -1092,8 +1134,8 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
           const uint8_t* scales = bytes_of(t + k / CACHE_TILE, id) + 34 * D;
           const bool in = pos + k >= from && pos + k <= last;
 #pragma unroll
-          for (int d = 0; d < GROUPS; ++d) {
-            const uint32_t bits = reinterpret_cast<const uint16_t*>(scales)[((k % CACHE_TILE >> 3) * GROUPS + d) * 8 + (k & 7)];
+          for (int d = 0; d < OWN; ++d) {
+            const uint32_t bits = reinterpret_cast<const uint16_t*>(scales)[((k % CACHE_TILE >> 3) * GROUPS + half * OWN + d) * 8 + (k & 7)];
             if (in && (bits & 0x7fffu) >= 0x7c00u) o[d] = f32x16{} + __builtin_nanf("");
           }
         }
@@ -1107,7 +1149,7 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
     // Taken back from the transformed basis: a lane holds dims 32 d + 8 b +
     // 4 h + x of its row.
     sum += __shfl_xor(sum, 32);
-    if (there && !whole && h == 0) {
+    if (there && !whole && h == 0 && half == 0) {
       part[ROWS * D + 2 * row] = run == NONE ? NONE : run * qs;
       part[ROWS * D + 2 * row + 1] = sum;
     }
@@ -1117,7 +1159,7 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
     asm volatile("" : "+v"(of));
     uint16_t* out = a.out + ((int64_t)(req.first + of / a.group) * a.q_heads + head * a.group + of % a.group) * D;
 #pragma unroll
-    for (int d = 0; d < GROUPS; ++d) {
+    for (int d = 0; d < OWN; ++d) {
       float v[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e) v[e] = o[d][e];
@@ -1135,7 +1177,7 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const f32x4 y = 0.25f * f32x4{v[4 * b], v[4 * b + 1], v[4 * b + 2], v[4 * b + 3]};
-        const int dim = 32 * d + 8 * b + 4 * h;
+        const int dim = 32 * (half * OWN + d) + 8 * b + 4 * h;
         if (whole) {
           u32x2 w;
           w[0] = narrow<BF16>(y[0] * inverse) | narrow<BF16>(y[1] * inverse) << 16;
@@ -1310,7 +1352,7 @@ Variant variant_of(int64_t rows, int head_dim) {
   const int64_t most = head_dim == 128 ? 128 : head_dim == 64 ? 64 : 16;
   return rows <= 8 ? ROWS8 : rows <= 16 ? ROWS16 : rows <= most ? ROWS32 : TILES;
 }
-int rows_of(Variant v, int head_dim) { return v == TILES ? 32 * tile_waves(head_dim) : 8 << v; }
+int rows_of(Variant v, int head_dim) { return v == TILES ? tile_rows(head_dim) : 8 << v; }
 // Owners that fill the chip: waves of attend_rows_kernel, workgroups of
 // attend_tiles_kernel.
 int owners_of(Variant v, int head_dim) {

@@ -154,7 +154,9 @@ struct RotaryArgs {
 // y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin of every pair, the other values
 // copied. A block takes `per_block` tokens, makes their angles once and turns
 // all heads of q and k: per pair one 64-bit product and one sincospi for all
-// heads, so the pass is bound by reading and writing the rows.
+// heads, so the pass is bound by reading and writing the rows (8192 tokens of
+// 32 + 8 heads of 128 in bfloat16, 168 MB that the last-level cache holds:
+// 26 us, 6.4 TB/s; one token 3 us, a launch).
 // A thread turns both values of its pairs and writes them where it read them
 // (out may be the input). VEC: rows are 16-byte aligned, pairs a multiple of
 // 8 and D of 16, so a unit is 16 values in two wide loads.
@@ -298,7 +300,7 @@ __device__ __forceinline__ int last_at_most(const int32_t* at, int n, int x) {
 // and fills its share of the new table entries and of the tokens' slots. A
 // slot in a new page takes the page from the free list itself, so no block
 // reads what another writes. Bound by latency: two reads and two dependent
-// look-ups deep.
+// look-ups deep (256 requests of a token 6 us, 1531 of up to 96 tokens 10 us).
 __global__ void __launch_bounds__(STEP_THREADS) step_kernel(StepArgs a) {
   extern __shared__ int32_t prefix[];  // starts [requests + 1], needs [requests + 1]
   __shared__ int64_t parts[STEP_THREADS / 64];
@@ -419,7 +421,8 @@ struct Units {
 // three butterfly levels in a lane, two by quad permutation, then the group's
 // largest magnitude, scale and codes. Keys turn by their position on the way,
 // in 32 bits, and queries beside them, so a decode step is one launch and one
-// read of the projection. Bound by reading the rows.
+// read of the projection. Bound by reading and writing the rows (8191 tokens of
+// 3 x 16 heads of 64, float16, queries turned: 77 MB in 23 us, 3.3 TB/s).
 template <typename E, bool TURN, int TOK>
 __global__ void __launch_bounds__(256)
     append_kernel(Rows<const typename E::type> q, Rows<const typename E::type> k,
@@ -498,7 +501,7 @@ __global__ void __launch_bounds__(256)
 }
 
 // The values that entries stand for: H ((c - 8) s) / 4, a quad a group; zeros
-// for slots outside the cache.
+// for slots outside the cache. Bound by writing them (43 MB in all in 14 us).
 template <typename E, int TOK>
 __global__ void __launch_bounds__(256)
     read_kernel(const uint8_t* __restrict__ pages, Rows<typename E::type> k, Rows<typename E::type> v,
