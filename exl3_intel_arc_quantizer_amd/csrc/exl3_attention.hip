@@ -756,6 +756,7 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
   const Magic magic;
   int64_t* costs = dynamic;                              // [blocks + 1], if blocks may be cut
   int32_t* prefix = reinterpret_cast<int32_t*>(dynamic + (cls.whole ? 0 : cls.blocks + 1));  // [requests + 1]
+  if (tid < 2) poison[tid] = -1;                         // seen by all after the barriers of the sums
   sum_work<NT>(a, cls, prefix, parts);
   const int owner = blockIdx.x, heads = a.cache.kv_heads;
   int listed = __builtin_amdgcn_readfirstlane(prefix[a.requests]);
@@ -807,7 +808,6 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
   uint32_t value_scale_at = 34 * D + ((tid / D * GROUPS + tid / 8 % (D / 8) / 4) * 2 + (tid / 4 & 1)) * 8;
   uint32_t key_row = half * D + n * (2 * D) + (h ^ (n & SPAN)) * 16, value_row = half * (OWN * 2048) + n * 64 + (h ^ (n >> 2 & 3)) * 16;
   asm volatile("" : "+v"(key_at), "+v"(key_scale_at), "+v"(value_at), "+v"(value_scale_at), "+v"(key_row), "+v"(value_row));
-  if (tid < 2) poison[tid] = -1;
   int count = 0;                                         // steps so far; names a buffer's content
 
   for (int64_t at = begin; at < end;) {
