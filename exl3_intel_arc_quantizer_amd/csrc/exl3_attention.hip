@@ -41,6 +41,13 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float NONE = -__builtin_inff();
+// Weights are 2^(score - maximum + LIFT), scores in powers of two: float16 has
+// all its bits down to 2^-14, so those down to 2^-21 of the largest keep them,
+// and a long context's many small weights count beside a dominant one. The
+// maximum is a running one that moves where a score passes it by RISE: weights
+// stay within 2^11, and five more powers of two are left for the rounding of
+// scores, whose last places are whole powers from 2^24 on.
+constexpr float LIFT = 7.0f, RISE = 4.0f;
 constexpr int THREADS = 256, WAVES = THREADS / 64;
 
 // One launch of a kernel over the requests with `low` to `high` query rows to
@@ -320,7 +327,7 @@ constexpr int resident(int d, bool wide, int ct) {
 // of their own (errors under 2^-11 of the output's terms, which its own
 // rounding of 2^-9 covers); float16 queries keep their rest in products of
 // their own. The running maximum moves only where a row's tile maximum passes
-// it by 8 (in powers of two: weights stay under 2^8), one vote a tile; then
+// it by RISE, one vote a tile; then
 // the rows agree across lanes on a new one. Sums and outputs are float32.
 //
 // Two tiles' registers take turns: one is loaded while the other is
@@ -458,7 +465,7 @@ __global__ void __launch_bounds__(THREADS, resident(D, WIDE, CT)) attend_rows_ke
       // of two.
       // (At least 2^-120: a scale of 0 weighs all positions alike.)
       qs[c] = fmaxf(ldexpf(fabsf(a.scale) * 0.25f * 1.4426950408889634f, power), 0x1p-120f);
-      rise[c] = 8.0f / qs[c];
+      rise[c] = RISE / qs[c];
       last[c] = there ? req.length - req.n + i : -1;
       const int64_t from64 = there ? (int64_t)last[c] - a.window + 1 : 0;
       from[c] = (int)max(from64, (int64_t)0);
@@ -535,7 +542,7 @@ __global__ void __launch_bounds__(THREADS, resident(D, WIDE, CT)) attend_rows_ke
 #pragma unroll
           for (int m = 0; m < SETS * NIB; ++m) o[c][m] *= shrink;
         }
-        const float ref = run[c] == NONE ? 0.0f : -run[c] * qs[c];
+        const float ref = run[c] == NONE ? 0.0f : LIFT - run[c] * qs[c];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float w[2];
@@ -980,7 +987,7 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
           if constexpr (REST) ql[k][e] = bits_of(f16x2{(_Float16)(y0 - (float)hi[0]), (_Float16)(y1 - (float)hi[1])});
         }
       qs = fmaxf(ldexpf(fabsf(a.scale) * 0.25f * 1.4426950408889634f, power), 0x1p-120f);
-      rise = 8.0f / qs;
+      rise = RISE / qs;
     }
 
     float run = NONE, sum = 0.0f;
@@ -1096,7 +1103,7 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
 #pragma unroll
         for (int d = 0; d < OWN; ++d) o[d] *= shrink;
       }
-      const float ref = run == NONE ? 0.0f : -run * qs;
+      const float ref = run == NONE ? 0.0f : LIFT - run * qs;
       // Product v of the output: 16 tokens v / OWN, dims of group v % OWN.
       auto operand = [&](int v) { return value(2 * (v % OWN) + (v / OWN & 1), place + v / OWN / 2 * TILE); };
 #pragma unroll

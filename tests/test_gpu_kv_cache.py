@@ -255,6 +255,37 @@ def test_drafts_chunks_and_prompts(heads, group, dim, page, window, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim, new", [(64, 1), (128, 1), (256, 1), (64, 30), (128, 30), (64, 200), (128, 200), (256, 60)])
+def test_small_weights_of_a_long_context(dim, new, dtype):
+    """Every 32nd position has a value of 0 and outweighs each of the others by
+    about 2^20.3: what is left of the output is all theirs, 2^-15 of a value. (In
+    every tile, so that no share of the context is without one.)"""
+    context, page, group = 20000, 256, 4
+    g = torch.Generator().manual_seed(dim + new)
+    u = torch.sign(torch.randn(dim, generator=g))
+    k, v = torch.zeros(context, 1, dim), 64 * torch.randn(context, 1, dim, generator=g).abs()
+    k[::32, 0], v[::32] = u, 0.0
+    pages = cache_pages(-(-context // page), page, 1, dim)
+    slots = torch.arange(context, device="cuda")
+    append_tokens(pages, k.cuda(), v.cuda(), slots)
+    q = (u * (20.3 * np.log(2) / dim)).to(dtype).expand(new, group, dim).contiguous().cuda()
+    got = cache_attention(q, pages, _ints([np.arange(pages.shape[0])]), _ints([0, new]), _ints([context]), scale=1.0)
+    keys, values = (x[:, 0].double() for x in read_tokens(pages, slots, dtype=torch.float32))
+    scores = q[:, 0].double() @ keys.T
+    at = torch.arange(context, device="cuda")
+    scores[at[None] > (context - new + torch.arange(new, device="cuda"))[:, None]] = -torch.inf
+    weights = torch.softmax(scores, 1)
+    want = (weights @ values)[:, None].expand(-1, group, -1)
+    # Weights (and of many rows bfloat16 queries) in 11 bits, scores up to 15 of
+    # 22 bits or, of those queries, 11; float32 sums of 20000 terms in tiles of 32.
+    # Twice the output bounds sum p |v|, whose few negative values are small.
+    scores_off = 15 * (2.0 ** -18 if new * group <= 16 or dtype == torch.float16 else 2.0 ** -11)
+    share = UNIT[dtype] + 2 * scores_off + 2.0 ** -10 + 2.0 ** -12
+    assert (((got.double() - want).abs()) <= share * 2.0 * want.abs().amax(-1, keepdim=True) + 2.0 ** -24).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new", [1, 4, 70])
 def test_long_context_is_split(new):
     rng = np.random.default_rng(new)
