@@ -108,7 +108,7 @@ def append_tokens(pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: 
     (tokens, q_heads, head_dim) if given, which are returned: the cache's side
     of a step is then one launch that reads the projection once. No slot may
     be given twice in a call."""
-    _unrecorded("append_tokens", k, v, q)
+    _unrecorded("append_tokens", k, v, q, frequencies)
     return _native.cache_append(pages, k, v, slots, q, positions, frequencies,
                                 layout_code(layout), magnitude)
 

@@ -74,7 +74,10 @@ class _Rotary(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, positions, frequencies, layout, magnitude, inverse):
-        ctx.given = (positions, frequencies, layout, magnitude, inverse)
+        # Saved, so that torch refuses a backward pass after they were written to.
+        ctx.save_for_backward(positions, frequencies)
+        ctx.save_for_forward(positions, frequencies)
+        ctx.given = (layout, magnitude, inverse)
         ctx.two = k is not None
         ctx.set_materialize_grads(False)
         q_out, k_out = _native.rotary(q, k, positions, frequencies, layout, magnitude, inverse)
@@ -82,14 +85,16 @@ class _Rotary(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, *grads):
-        positions, frequencies, layout, magnitude, inverse = ctx.given
+        positions, frequencies = ctx.saved_tensors
+        layout, magnitude, inverse = ctx.given
         out = _turned(grads[0], grads[1] if ctx.two else None, positions, frequencies, layout,
                       magnitude, not inverse)
         return (*out, None, None, None, None, None)
 
     @staticmethod
     def jvp(ctx, *tangents):
-        positions, frequencies, layout, magnitude, inverse = ctx.given
+        positions, frequencies = ctx.saved_tensors
+        layout, magnitude, inverse = ctx.given
         q, k = _turned(tangents[0], tangents[1], positions, frequencies, layout, magnitude, inverse)
         return (q, k) if ctx.two else (q,)
 
@@ -124,9 +129,11 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     None in the result. ``positions`` are int32 or int64 (tokens,),
     ``frequencies`` float64 of up to head_dim / 2 pairs: (i, i + pairs) for
     layout ``"half"``, (2 i, 2 i + 1) for ``"interleaved"``; the values past
-    the pairs are copied. Angles are taken in 64 bits and products in 32, so
+    the pairs are copied; frequencies have no gradient. Angles are taken in 64 bits and products in 32, so
     positions in the millions are as exact as the first ones."""
     code = layout_code(layout)
+    if isinstance(frequencies, torch.Tensor) and records(frequencies):
+        raise RuntimeError("apply_rotary has no gradient of frequencies: detach them")
     if records(q) or (k is not None and records(k)):
         if out is not None:
             raise RuntimeError("apply_rotary: out cannot be given where torch records the inputs")

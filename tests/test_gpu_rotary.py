@@ -141,3 +141,16 @@ def test_refusals():
             apply_rotary(*args)
     with pytest.raises(RuntimeError, match="out"):
         apply_rotary(q.requires_grad_(), k, at, f, out=(torch.empty_like(q), torch.empty_like(k)))
+
+
+@pytest.mark.gpu
+def test_backward_sees_the_positions_of_the_forward_pass():
+    q = torch.ones(4, 2, 16, device="cuda", requires_grad=True)
+    at = torch.arange(4, device="cuda")
+    f = torch.ones(8, dtype=torch.float64, device="cuda")
+    y = apply_rotary(q, None, at, f)[0]
+    at += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with pytest.raises(RuntimeError, match="frequencies"):
+        apply_rotary(q, None, at, f.clone().requires_grad_())
