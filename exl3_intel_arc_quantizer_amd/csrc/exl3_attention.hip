@@ -3,6 +3,8 @@
 //
 //   attend_rows_kernel  a few query rows of one kv head against a share of its
 //                       tiles, as partial or whole results
+//   attend_tiles_kernel many query rows (chunks and prompts), tiles unpacked
+//                       once for all rows of a workgroup
 //   attend_join_kernel  the partial results of a row joined, empty rows zeroed
 //
 // Row i of a request's n new tokens sits at position p = length - n + i and
@@ -335,7 +337,7 @@ constexpr int resident(int d, bool wide, int ct) {
 //
 // Bound by reading the cache where there are few rows: 128 requests of up to
 // 8192 positions, 8 kv heads of 128, one token: 504 MB in 107 us, 4.7 TB/s of the
-// 5.0 a large copy reaches, vector instructions on 0.58 of the cycles. With 32
+// 4.9 a large copy reaches, vector instructions on 0.61 of the cycles. With 32
 // rows a tile they and the products get as long as the reading: 157 MB in
 // 51 us, of which about 10 are the waves' start and end.
 template <int D, bool WIDE, int CT, bool BF16>
@@ -725,10 +727,10 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 // one is multiplied the next is unpacked, and the codes after it are on their
 // way.
 //
-// Bound by issue: matrix instructions take 0.43 of the cycles, vector ones (the
-// softmax above all) 0.5, and two waves a SIMD overlap them little. A prompt of
+// Bound by issue: matrix instructions take 0.39 of the cycles, vector ones (the
+// softmax above all) 0.48, and two waves a SIMD overlap them little. A prompt of
 // 8192 tokens, 32 heads of 128 over 8, bfloat16: 550 GFLOP in 0.60 ms, 917
-// TFLOP/s (a library product of 8192 a side: 1113).
+// TFLOP/s (a library product of 8192 a side: 1208).
 //
 // Weights, and bfloat16 queries, count with 11 bits (errors under 2^-11 of the
 // output's terms); float16 queries keep their rest in products of their own.
