@@ -444,6 +444,38 @@ def test_table_values_out_of_range_are_harmless():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 5, 150])
+def test_places_past_32_bits(new):
+    """The last pages of a cache of 5.4 GB hold the same tokens as a small
+    cache's, and give the same bits; so do queries more than 2^31 bytes in."""
+    heads, dim, page, context = 8, 128, 64, 300
+    many = 73_000                                        # 73728 bytes each
+    g = torch.Generator(device="cuda").manual_seed(new)
+    k, v = (torch.randn(context, heads, dim, device="cuda", generator=g).half() for _ in range(2))
+    q = torch.randn(new, 2 * heads, dim, device="cuda", generator=g).half()
+    order = torch.tensor([2, 4, 0, 3, 1], device="cuda")
+    at = torch.arange(context, device="cuda")
+    results = []
+    for pages in (5, many):
+        cache = torch.empty(pages, heads, page // 32, 36 * dim, dtype=torch.uint8, device="cuda")
+        cache[-5:] = 0
+        table = order + (pages - 5)
+        slots = table[at // page] * page + at % page
+        append_tokens(cache, k, v, slots)
+        rows = q
+        if pages == many:
+            stride = (2 ** 31 // new + 1024) // 8 * 8    # the last row starts past 2^31 bytes
+            wide = torch.empty((new - 1) * stride + 2 * heads * dim + 8, dtype=torch.float16, device="cuda")
+            rows = wide.as_strided((new, 2 * heads, dim), (stride, dim, 1))
+            rows.copy_(q)
+        results.append((*read_tokens(cache, slots), cache_attention(
+            rows, cache, table.int()[None], _ints([0, new]), _ints([context]))))
+        del cache
+    for small, large in zip(*results):
+        assert torch.equal(small, large)
+
+
+@pytest.mark.gpu
 def test_other_streams_and_strides():
     rng = np.random.default_rng(10)
     cache = ref.Cache(8, 64, 2, 128, rng)
