@@ -309,7 +309,7 @@ struct Tile {
 // compute unit that a variant's registers allow:
 constexpr int resident(int d, bool wide, int ct) {
   if (wide) return 2;
-  return d == 64 ? (ct == 1 ? 4 : 3) : d == 128 ? (ct == 1 ? 3 : 2) : (ct == 1 ? 2 : 1);
+  return d == 64 ? (ct == 1 ? 4 : 3) : d == 128 ? (ct == 1 ? 3 : 2) : 2;
 }
 
 // Every wave takes one share of all work, an equal run of tiles that may end
@@ -1356,9 +1356,15 @@ constexpr int CUS = 256;
 // of which reads the cache again: 64 requests of 2048 positions, 8 kv heads,
 // float16: head dimension 128, 64 rows 99 us and in blocks 182, 128 rows 160 and
 // 189; head dimension 64, 64 rows 75 and 92, 96 rows 108 and 105.
+// Head dimension 256 has no variants of 16 and 32 rows, for which a wave lacks
+// registers: up to 32 rows go in blocks of 8, whose later ones find the tiles in
+// the caches (the same requests, float16: 16 rows 120 us, in a variant of 16 with
+// spills 151; 32 rows 175 and in blocks that share the unpacking 260; 48 rows
+// 268 and 264. Bfloat16: 32 rows 170 and 228, 48 rows 270 and 231).
 enum Variant { ROWS8, ROWS16, ROWS32, TILES };
 Variant variant_of(int64_t rows, int head_dim) {
-  const int64_t most = head_dim == 128 ? 128 : head_dim == 64 ? 64 : 16;
+  if (head_dim == 256) return rows <= 32 ? ROWS8 : TILES;
+  const int64_t most = head_dim == 128 ? 128 : 64;
   return rows <= 8 ? ROWS8 : rows <= 16 ? ROWS16 : rows <= most ? ROWS32 : TILES;
 }
 int rows_of(Variant v, int head_dim) { return v == TILES ? tile_rows(head_dim) : 8 << v; }
@@ -1380,14 +1386,15 @@ int64_t partials_bytes(Variant v, int head_dim) {
 
 // The launches of a call: the variant for its longest requests, and beside it,
 // so that single tokens keep the variant made for them and up to 16 rows their
-// precision, that of 8 rows for requests of up to `few`.
+// precision, that of 8 rows for requests of up to `few` (where it takes as many
+// alone, those: see above).
 struct Launches {
   int count, few;
   Variant of[2];
 };
 Launches launches_of(int64_t tokens, int group, int requests, int head_dim, int64_t max_new) {
   const Variant v = variant_of(std::min(max_new, tokens) * group, head_dim);
-  return {requests > 1 && v != ROWS8 ? 2 : 1, v == ROWS16 ? 8 : 16, {v, ROWS8}};
+  return {requests > 1 && v != ROWS8 ? 2 : 1, head_dim == 256 ? 32 : v == ROWS16 ? 8 : 16, {v, ROWS8}};
 }
 
 template <int D, bool BF16>
@@ -1397,12 +1404,14 @@ int launch_variant(Variant v, const AttendArgs& args, int index, unsigned grid, 
   const size_t lds = v != TILES ? 8 * requests : 4 * requests + (c.whole ? 0 : 8 * ((size_t)c.blocks + 1));
   if (v == ROWS8)
     attend_rows_kernel<D, false, 1, BF16><<<grid, THREADS, lds, stream>>>(args, index);
-  else if (v == ROWS16)
-    attend_rows_kernel<D, false, 2, BF16><<<grid, THREADS, lds, stream>>>(args, index);
   else if (v == TILES)
     attend_tiles_kernel<D, BF16><<<grid, 64 * tile_waves(D), lds, stream>>>(args, index);
-  else if constexpr (D != 256)
-    attend_rows_kernel<D, true, 2, BF16><<<grid, THREADS, lds, stream>>>(args, index);
+  else if constexpr (D != 256) {
+    if (v == ROWS16)
+      attend_rows_kernel<D, false, 2, BF16><<<grid, THREADS, lds, stream>>>(args, index);
+    else
+      attend_rows_kernel<D, true, 2, BF16><<<grid, THREADS, lds, stream>>>(args, index);
+  }
   return check_launch("exl3_cache_attention");
 }
 

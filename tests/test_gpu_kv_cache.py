@@ -286,6 +286,22 @@ def test_small_weights_of_a_long_context(dim, new, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("group, new, window", [(3, [3, 1, 4, 2, 0, 5], None), (16, [1, 2, 1, 1, 2, 1], 40), (5, [6, 5, 4, 6, 1, 2], 33),
+                                                (4, [8, 3, 60, 1, 7, 8], None)])
+def test_blocks_of_eight_rows_of_large_heads(group, new, window, dtype):
+    """9 to 32 rows of head dimension 256: tokens whose heads lie in two blocks,
+    contexts of the new tokens alone, and beside a chunk of many rows."""
+    rng = np.random.default_rng(group)
+    lengths = [n + c for n, c in zip(new, (700, 0, 31, 32, 5, 1500))]
+    cache = ref.Cache(sum(-(-n // 32) for n in lengths), 32, 2, 256, rng)
+    tables = _tables(lengths, 32, 48, cache.shape[0], rng)
+    starts = np.concatenate([[0], np.cumsum(new)])
+    q = torch.from_numpy(rng.normal(size=(starts[-1], 2 * group, 256)) * 2).to(dtype)
+    _check(q, cache, 32, tables, starts, lengths, dtype, window=window, max_new=max(new), group=group)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new", [1, 4, 70])
 def test_long_context_is_split(new):
     rng = np.random.default_rng(new)
