@@ -122,7 +122,8 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
                  frequencies: torch.Tensor, *, layout: str = "half", magnitude: float = 1.0,
                  out: Optional[tuple] = None) -> tuple:
     """(q, k) turned by their positions, as new contiguous tensors or into
-    ``out`` (a pair like q and k; the inputs themselves are allowed).
+    ``out`` (a pair like q and k; the inputs themselves are allowed), where
+    torch records neither the inputs nor ``out``.
 
     q and k are (tokens, heads, head_dim) of one type, float32, float16 or
     bfloat16, with any strides of tokens and heads; k may be None, and is then
@@ -134,8 +135,9 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     code = layout_code(layout)
     if isinstance(frequencies, torch.Tensor) and records(frequencies):
         raise RuntimeError("apply_rotary has no gradient of frequencies: detach them")
-    if records(q) or (k is not None and records(k)):
-        if out is not None:
-            raise RuntimeError("apply_rotary: out cannot be given where torch records the inputs")
+    recorded = records(q) or (k is not None and records(k))
+    if out is not None and (recorded or any(t is not None and records(t) for t in out)):
+        raise RuntimeError("apply_rotary: out cannot be given where torch records it or the inputs")
+    if recorded:
         return _turned(q, k, positions, frequencies, code, magnitude, False)
     return _native.rotary(q, k, positions, frequencies, code, magnitude, False, out)
