@@ -980,6 +980,12 @@ def _run(device, what: str, call, *args) -> None:
         _check(status, what)
 
 
+def _written(*tensors) -> None:
+    """Tell torch that a kernel wrote into the caller's tensors: a backward pass
+    that saved one of them then refuses, as after torch's own in-place operations."""
+    _torch().autograd.graph.increment_version(tensors)
+
+
 def rotary(q, k, positions, frequencies, layout: int, magnitude: float, inverse: bool,
            out=None) -> tuple:
     """q and k turned by their positions (exl3_rotary); k may be None."""
@@ -1005,7 +1011,10 @@ def rotary(q, k, positions, frequencies, layout: int, magnitude: float, inverse:
          q_out.data_ptr(), so[0], so[1], heads, *k_args, tokens, dim, _types()[q.dtype],
          positions.data_ptr(), positions.dtype == torch.int64, frequencies.data_ptr(), pairs,
          layout, magnitude, inverse)
-    return q_out, k_out if k is not None else None
+    k_out = k_out if k is not None else None
+    if out:
+        _written(*(t for t in (q_out, k_out) if t is not None))
+    return q_out, k_out
 
 
 def plan_step(cached, new, tables, free_pages, taken, page_size: int, max_tokens: int) -> tuple:
@@ -1029,6 +1038,7 @@ def plan_step(cached, new, tables, free_pages, taken, page_size: int, max_tokens
          requests, tables.data_ptr(), width, free_pages.data_ptr(), free_pages.numel(),
          taken.data_ptr(), page_size, max_tokens, slots.data_ptr(), positions.data_ptr(),
          starts.data_ptr(), lengths.data_ptr(), taken_out.data_ptr(), status.data_ptr())
+    _written(tables)
     return slots, positions, starts, lengths, taken_out, status
 
 
@@ -1066,6 +1076,7 @@ def cache_append(pages, k, v, slots, q, positions, frequencies, layout: int, mag
          k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1], tokens,
          _types()[k.dtype], slots.data_ptr(), at, wide, freq, pairs, layout, magnitude,
          pages.data_ptr(), n, page_size, heads, dim)
+    _written(pages)
     return q_out
 
 

@@ -6,6 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from exl3_intel_arc_quantizer_amd.kv_cache import append_tokens, cache_attention, cache_pages, plan_step, read_tokens
 from exl3_intel_arc_quantizer_amd.rotary import apply_rotary
 
 
@@ -45,3 +46,48 @@ def test_recorded_out_is_refused():
     with torch.no_grad():  # as torch's own in-place operations
         apply_rotary(q, None, at, freq, out=(leaf, None))
     assert torch.equal(leaf, apply_rotary(q, None, at, freq)[0])
+
+
+@pytest.mark.gpu
+def test_backward_refuses_tensors_that_were_turned_in_place():
+    q, at, freq = _given()
+    k = torch.randn(6, 1, 32, device="cuda")
+    w = torch.ones_like(q, requires_grad=True)
+    u = torch.ones_like(k, requires_grad=True)
+    y, z = (q * w).sum(), (k * u).sum()
+    apply_rotary(q, k, at, freq, out=(q, k))
+    for result in (y, z):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            result.backward()
+    # A view's write counts for what it is a view of.
+    x = torch.randn(6, 5, 32, device="cuda")
+    w = torch.ones_like(x, requires_grad=True)
+    y = (x * w).sum()
+    apply_rotary(x[:, :4], x[:, 4:], at, freq, out=(x[:, :4], x[:, 4:]))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+@pytest.mark.gpu
+def test_written_caches_and_tables_have_new_versions():
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    pages, tables = cache_pages(3, 32, 1, 64), torch.full((1, 2), -1, dtype=torch.int32, device="cuda")
+    versions = pages._version, tables._version
+    plan = plan_step(ints(0), ints(2), tables, ints(2, 0, 1), ints(0), page_size=32, max_tokens=2)
+    k = torch.randn(2, 1, 64, device="cuda")
+    append_tokens(pages, k, k, plan.slots)
+    assert pages._version > versions[0] and tables._version > versions[1]
+    versions = pages._version, tables._version, k._version
+    read_tokens(pages, plan.slots)
+    cache_attention(k.half(), pages, tables, plan.starts, plan.lengths)
+    assert (pages._version, tables._version, k._version) == versions
+    # A server's tensors are made in inference mode, and used in it or out of it.
+    with torch.inference_mode():
+        held, rows, q = pages.clone(), tables.clone(), torch.randn(2, 1, 64, device="cuda")
+        at, freq = ints(4, 5), torch.ones(32, dtype=torch.float64, device="cuda")
+        plan_step(ints(2), ints(2), rows, ints(2, 0, 1), ints(1), page_size=32, max_tokens=2)
+        append_tokens(held, k, k, plan.slots)
+        apply_rotary(q, None, at, freq, out=(q, None))
+    append_tokens(held, k, k, plan.slots)
+    apply_rotary(q, None, at, freq, out=(q, None))
+    assert torch.equal(held, pages)
