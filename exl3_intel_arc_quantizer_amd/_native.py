@@ -986,6 +986,68 @@ def _written(*tensors) -> None:
     _torch().autograd.graph.increment_version(tensors)
 
 
+class _Span:
+    """Rows at an address, as numpy's overlap solver takes them (it reads none)."""
+
+    def __init__(self, address: int, shape, strides):
+        self.__array_interface__ = {"version": 3, "data": (address, False),
+                                    "shape": tuple(shape[:2]),
+                                    "strides": tuple(strides[:2]), "typestr": f"|V{shape[2]}"}
+
+
+def shares_memory(a: tuple, b: tuple) -> bool:
+    """Whether two (address, (tokens, heads, bytes of a row), (token stride, head
+    stride) in bytes) have a byte in common. Rows of one projection lie between
+    each other without sharing any, so the ranges alone do not say; what the
+    solver gives up on counts as shared."""
+    import numpy as np
+    if not all(a[1]) or not all(b[1]):
+        return False
+    try:
+        return np.shares_memory(np.asarray(_Span(*a)), np.asarray(_Span(*b)), max_work=10 ** 6)
+    except np.exceptions.TooHardError:
+        return True
+
+
+def rows_are_apart(shape, strides) -> bool:
+    """Whether no two rows of (tokens, heads, row size) share memory, from the
+    strides of tokens and heads: the shorter one passes a row, the longer all of
+    the other axis."""
+    reach = shape[2]
+    if not all(shape):
+        return True
+    for stride, n in sorted(zip(strides[:2], shape[:2])):
+        if n > 1:
+            if stride < reach:
+                return False
+            reach += (n - 1) * stride
+    return True
+
+
+def _check_outputs(inputs, outputs) -> None:
+    """The kernel's blocks run in any order, each reading and writing whole rows:
+    an output may be its input, and else shares no memory with any tensor of the
+    call."""
+    def span(t):
+        size = t.element_size()
+        return (t.data_ptr(), (*t.shape[:2], t.shape[2] * size), [n * size for n in t.stride()[:2]])
+
+    spans_in, spans_out = ([None if t is None else span(t) for t in ts] for ts in (inputs, outputs))
+    for i, own in enumerate(spans_out):
+        if own is None:
+            continue
+        if not rows_are_apart(own[1], own[2]):
+            raise RuntimeError(f"rows of out[{i}] share memory with each other")
+        for j, other in enumerate(spans_in):
+            same = i == j and own[:2] == other[:2] and all(
+                a == b for a, b, n in zip(own[2], other[2], own[1]) if n > 1)
+            if other is not None and not same and shares_memory(own, other):
+                raise RuntimeError(f"out[{i}] shares memory with {'qk'[j]}: it may be {'qk'[i]} "
+                                   "itself, or apart from both")
+    if None not in spans_out and shares_memory(*spans_out):
+        raise RuntimeError("out[0] and out[1] share memory")
+
+
 def rotary(q, k, positions, frequencies, layout: int, magnitude: float, inverse: bool,
            out=None) -> tuple:
     """q and k turned by their positions (exl3_rotary); k may be None."""
@@ -1007,11 +1069,14 @@ def rotary(q, k, positions, frequencies, layout: int, magnitude: float, inverse:
             k_out = torch.empty_like(k, memory_format=dense)
         sp = _rows(k_out, "out[1]", q, k_heads, dim)[1] if out else (k_heads * dim, dim)
         k_args = (k.data_ptr(), sk[0], sk[1], k_out.data_ptr(), sp[0], sp[1], k_heads)
+    else:
+        k_out = None
+    if out:
+        _check_outputs((q, k), (q_out, k_out))
     _run(device, "apply_rotary", load_library().exl3_rotary, q.data_ptr(), sq[0], sq[1],
          q_out.data_ptr(), so[0], so[1], heads, *k_args, tokens, dim, _types()[q.dtype],
          positions.data_ptr(), positions.dtype == torch.int64, frequencies.data_ptr(), pairs,
          layout, magnitude, inverse)
-    k_out = k_out if k is not None else None
     if out:
         _written(*(t for t in (q_out, k_out) if t is not None))
     return q_out, k_out

@@ -122,8 +122,9 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
                  frequencies: torch.Tensor, *, layout: str = "half", magnitude: float = 1.0,
                  out: Optional[tuple] = None) -> tuple:
     """(q, k) turned by their positions, as new contiguous tensors or into
-    ``out`` (a pair like q and k; the inputs themselves are allowed), where
-    torch records neither the inputs nor ``out``.
+    ``out`` (a pair like q and k: the inputs themselves, or tensors that share no
+    memory with them or each other), where torch records neither the inputs nor
+    ``out``.
 
     q and k are (tokens, heads, head_dim) of one type, float32, float16 or
     bfloat16, with any strides of tokens and heads; k may be None, and is then

@@ -230,7 +230,8 @@ int exl3_ldlq_scatter(const exl3_ldlq_block* blocks, int nblocks, int64_t tiles,
  * a = position * frequencies[i] (`inverse`: -a, which gives the gradient);
  * the other head_dim - 2 pairs values are copied. positions: int32, or int64
  * if wide_positions. Angles are taken in 64 bits, sums in 32. Outputs may be
- * the inputs. q_heads or k_heads may be 0, its pointers NULL. */
+ * the inputs, with their strides, and share no memory otherwise. q_heads or
+ * k_heads may be 0, its pointers NULL. */
 int exl3_rotary(const void* q, int64_t q_token, int64_t q_head, void* q_out, int64_t qo_token,
                 int64_t qo_head, int q_heads, const void* k, int64_t k_token, int64_t k_head,
                 void* k_out, int64_t ko_token, int64_t ko_head, int k_heads, int64_t tokens,
