@@ -79,6 +79,7 @@ class _Rotary(torch.autograd.Function):
         ctx.save_for_forward(positions, frequencies)
         ctx.given = (layout, magnitude, inverse)
         ctx.two = k is not None
+        ctx.shapes = q.shape, k.shape if ctx.two else None
         ctx.set_materialize_grads(False)
         q_out, k_out = _native.rotary(q, k, positions, frequencies, layout, magnitude, inverse)
         return (q_out, k_out) if ctx.two else (q_out,)
@@ -96,7 +97,11 @@ class _Rotary(torch.autograd.Function):
         positions, frequencies = ctx.saved_tensors
         layout, magnitude, inverse = ctx.given
         q, k = _turned(tangents[0], tangents[1], positions, frequencies, layout, magnitude, inverse)
-        return (q, k) if ctx.two else (q,)
+        if not ctx.two:
+            return (q,)
+        # torch asks for a tangent of every output: that of an input without one is 0.
+        return tuple(other.new_zeros(shape) if x is None else x
+                     for x, other, shape in ((q, k, ctx.shapes[0]), (k, q, ctx.shapes[1])))
 
 
 def _turned(q, k, positions, frequencies, layout, magnitude, inverse):
