@@ -325,10 +325,15 @@ constexpr int resident(int d, bool wide, int ct) {
 // the 16 columns; the other half takes what float16 leaves of the same rows:
 // q = hi + lo and p = hi + lo in columns n and n + 8, so queries and weights
 // count with 22 bits at no further product. WIDE blocks have all columns for
-// rows: weights count with 11 bits, and so do bfloat16 queries, which have 8
-// of their own (errors under 2^-11 of the output's terms, which its own
-// rounding of 2^-9 covers); float16 queries keep their rest in products of
-// their own. The running maximum moves only where a row's tile maximum passes
+// rows. There queries keep their 22 bits by products of their own (bfloat16
+// ones too, whose transform sums 32 values of 8 bits: rounded to 11, scores
+// would be off by up to 2^-11 of |q| |k|, a factor of the weight that grows
+// with the score and that no rounding of the output covers). Weights count with
+// 11 bits, each off by up to 2^-11 of itself whatever the score. With values of
+// both signs that adds 0.4 of the mean square error that a float16 output has by
+// its own rounding (windowed chunks: 2.07e-4 to 2.45e-4 of the output's norm),
+// and 0.01 of a bfloat16 one's; a rest of the weights would double the products
+// of the values. The running maximum moves only where a row's tile maximum passes
 // it by RISE, one vote a tile; then
 // the rows agree across lanes on a new one. Sums and outputs are float32.
 //
@@ -343,7 +348,6 @@ constexpr int resident(int d, bool wide, int ct) {
 template <int D, bool WIDE, int CT, bool BF16>
 __global__ void __launch_bounds__(THREADS, resident(D, WIDE, CT)) attend_rows_kernel(AttendArgs a, int index) {
   constexpr int PER = WIDE ? 16 : 8, ROWS = PER * CT, GROUPS = D / 32, SETS = Tile<D>::SETS, NIB = D == 64 ? 4 : 8;
-  constexpr bool REST = WIDE && !BF16;                   // products of the queries' rest
   extern __shared__ int64_t prefix[];                    // [requests + 1]
   __shared__ int64_t parts[WAVES];
 
@@ -417,7 +421,7 @@ __global__ void __launch_bounds__(THREADS, resident(D, WIDE, CT)) attend_rows_ke
     even.load(tile_at(t0, page_even), lane);
     // Queries, scaled by a power of two so that float16 holds them whatever
     // the type's range; hi in columns 0..7 and lo in 8..15 of narrow blocks.
-    u32x4 qf[CT][GROUPS], ql[REST ? CT : 1][REST ? GROUPS : 1];
+    u32x4 qf[CT][GROUPS], ql[WIDE ? CT : 1][WIDE ? GROUPS : 1];
     float qs[CT], rise[CT];
     int last[CT], from[CT];                              // positions this lane's row attends
 #pragma unroll
@@ -460,7 +464,7 @@ __global__ void __launch_bounds__(THREADS, resident(D, WIDE, CT)) attend_rows_ke
           else
             qf[c][k][e] = bits_of(f16x2{(_Float16)__builtin_fmaf((float)hi[0], rest, y0),
                                         (_Float16)__builtin_fmaf((float)hi[1], rest, y1)});
-          if constexpr (REST) ql[c][k][e] = bits_of(f16x2{(_Float16)(y0 - (float)hi[0]), (_Float16)(y1 - (float)hi[1])});
+          if constexpr (WIDE) ql[c][k][e] = bits_of(f16x2{(_Float16)(y0 - (float)hi[0]), (_Float16)(y1 - (float)hi[1])});
         }
       }
       // An eighth from the query's transform, 2 from both; log2(e) for powers
@@ -506,7 +510,7 @@ __global__ void __launch_bounds__(THREADS, resident(D, WIDE, CT)) attend_rows_ke
 #pragma unroll
           for (int c = 0; c < CT; ++c) {
             s[c][u] = mfma(f, qf[c][k], s[c][u]);
-            if constexpr (REST) s[c][u] = mfma(f, ql[c][k], s[c][u]);
+            if constexpr (WIDE) s[c][u] = mfma(f, ql[c][k], s[c][u]);
           }
         }
       }
@@ -712,8 +716,7 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 // their outputs beside a second wave on its SIMD: each multiplies half the dims
 // of queries and keys, the parts of the scores are exchanged through shared
 // memory, and each weighs its half of the values (a wave for all dims, one a
-// SIMD: prompts of 8192 tokens in bfloat16 549 TFLOP/s, float16 490; so 655 and
-// 556).
+// SIMD: a prompt of 8192 tokens at 490 TFLOP/s, so 556).
 //
 // The same products as above at 32 x 32 x 16: S^T = K Q^T in one accumulator
 // of 32 tokens x 32 rows a tile, O^T += V^T P^T in D / 32. Lane (n, h) of S^T
@@ -727,13 +730,16 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 // one is multiplied the next is unpacked, and the codes after it are on their
 // way.
 //
-// Bound by issue: matrix instructions take 0.39 of the cycles, vector ones (the
-// softmax above all) 0.48, and two waves a SIMD overlap them little. A prompt of
-// 8192 tokens, 32 heads of 128 over 8, bfloat16: 550 GFLOP in 0.60 ms, 917
-// TFLOP/s (a library product of 8192 a side: 1208).
+// Bound by issue: matrix instructions take 0.49 of the cycles, vector ones (the
+// softmax above all) 0.42, and two waves a SIMD overlap them little. Head
+// dimension 64: 0.44 and 0.64; 256: 0.34 and 0.43, of which both waves of a pair
+// do all the softmax. A prompt of 8192 tokens, 32 heads over 8, 550 GFLOP of 128
+// dims without the queries' rest: 0.74 ms, 747 TFLOP/s (with it 1.12 of a
+// PFLOP/s; a library product of 8192 a side 1.21). Of 64 dims 0.45 ms, 610, of
+// 256 1.94 ms, 568; float16 and bfloat16 alike.
 //
-// Weights, and bfloat16 queries, count with 11 bits (errors under 2^-11 of the
-// output's terms); float16 queries keep their rest in products of their own.
+// As in WIDE blocks above, queries count with 22 bits, by a second product of the
+// scores (the same prompt without it 0.59 ms), and weights with 11.
 constexpr int tile_waves(int d) { return d == 64 ? 4 : 8; }
 constexpr int tile_halves(int d) { return d == 256 ? 2 : 1; }  // waves that share 32 rows, each with a part of the dims
 constexpr int tile_rows(int d) { return 32 * tile_waves(d) / tile_halves(d); }
@@ -744,7 +750,6 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
   constexpr int NW = tile_waves(D), NT = 64 * NW, ROWS = tile_rows(D), STEPS = D / 16;
   constexpr int HALVES = tile_halves(D), GROUPS = D / 32, OWN = GROUPS / HALVES, TAKES = STEPS / HALVES;  // a wave's own
 
-  constexpr bool REST = !BF16;
   constexpr int TT = D == 256 ? 1 : 2;                   // tiles of a step
   // Parts of a tile: a dword of key codes, and two dims (a byte) of four tokens'
   // values. A thread takes KN of them.
@@ -885,10 +890,11 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
         vs[u] = __builtin_amdgcn_raw_buffer_load_b64(tile, value_scale_at + u * (NT / D * GROUPS * 16), 0, 0);
       }
     };
-    // Unpacked to a tile of a buffer; of this thread's parts, one.
-    auto unpack_part = [&](int buffer, int which, int u) __attribute__((always_inline)) {
-      const uint32_t d = tid + u * NT, base = (TT * buffer + which) * (TILE / 16);
-      {
+    // Unpacked to a tile of a buffer.
+    auto unpack = [&](int buffer, int which) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < KN; ++u) {
+        const uint32_t d = tid + u * NT, base = (TT * buffer + which) * (TILE / 16);
         const uint32_t token = d / (D / 8), inside = d % (D / 8);
         const uint32_t vector = 4 * (inside % GROUPS) + inside / GROUPS;
         // Bits 2 and 3 of the token exchanged.
@@ -900,24 +906,20 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
         f[2] = values_of<true>(kc[u] >> 8, scale, magic);
         f[3] = values_of<false>(kc[u] >> 8, scale, magic);
         keys[base + to * (D / 8) + (vector ^ (to & SPAN))] = f;
-      }
-      const uint32_t byte = d & 3, four = d / 4, octet = d / D, column = d / 8 % (D / 8);
-      const uint32_t pick = 0x0c000c04u | byte << 16 | byte;
-      u32x2 lo, hi;
+        const uint32_t byte = d & 3, four = d / 4, octet = d / D, column = d / 8 % (D / 8);
+        const uint32_t pick = 0x0c000c04u | byte << 16 | byte;
+        u32x2 lo, hi;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint32_t w = __builtin_amdgcn_perm(vc[u][2 * e], vc[u][2 * e + 1], pick);
-        const f16x2 scale = halves_of(vs[u][e]);
-        lo[e] = values_of<true>(w, scale, magic);
-        hi[e] = values_of<false>(w, scale, magic);
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t w = __builtin_amdgcn_perm(vc[u][2 * e], vc[u][2 * e + 1], pick);
+          const f16x2 scale = halves_of(vs[u][e]);
+          lo[e] = values_of<true>(w, scale, magic);
+          hi[e] = values_of<false>(w, scale, magic);
+        }
+        const uint32_t dim = 8 * column + 2 * byte;      // dims 4 x .. 4 x + 3 permute alike
+        u32x2* pair = reinterpret_cast<u32x2*>(&values[base + dim * 4 + (octet ^ (dim >> 2 & 3))]) + (four & 1);
+        pair[0] = lo, pair[8] = hi;
       }
-      const uint32_t dim = 8 * column + 2 * byte;      // dims 4 x .. 4 x + 3 permute alike
-      u32x2* to = reinterpret_cast<u32x2*>(&values[base + dim * 4 + (octet ^ (dim >> 2 & 3))]) + (four & 1);
-      to[0] = lo, to[8] = hi;
-    };
-    auto unpack = [&](int buffer, int which) __attribute__((always_inline)) {
-#pragma unroll
-      for (int u = 0; u < KN; ++u) unpack_part(buffer, which, u);
     };
     // A weight of 0 must not meet a NaN or infinity: in steps that some row
     // does not attend whole, such scales of values count as 0, and the rows
@@ -951,7 +953,7 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
       fetch(t0, page[0]);
     }
     // Queries, scaled by a power of two so that float16 holds them.
-    u32x4 qf[TAKES], ql[REST ? TAKES : 1];
+    u32x4 qf[TAKES], ql[TAKES];                          // and what float16 leaves of them
     float qs, rise;
     {
       const uint16_t* src = a.q + (int64_t)(req.first + token) * a.q_token + (int64_t)(head * a.group + of_group) * a.q_head;
@@ -986,7 +988,7 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
           const float y0 = flip * ldexpf(z0, -power), y1 = flip * ldexpf(z1, -power);
           const f16x2 hi = {(_Float16)y0, (_Float16)y1};
           qf[k][e] = bits_of(hi);
-          if constexpr (REST) ql[k][e] = bits_of(f16x2{(_Float16)(y0 - (float)hi[0]), (_Float16)(y1 - (float)hi[1])});
+          ql[k][e] = bits_of(f16x2{(_Float16)(y0 - (float)hi[0]), (_Float16)(y1 - (float)hi[1])});
         }
       qs = fmaxf(ldexpf(fabsf(a.scale) * 0.25f * 1.4426950408889634f, power), 0x1p-120f);
       rise = RISE / qs;
@@ -1021,10 +1023,7 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
 #pragma unroll
       for (int u = 0; u < TT; ++u) after[u] = page_of(t + 3 * TT + u);
       // The next step's tiles are unpacked after this one's scores are
-      // multiplied; of two, whose codes come one by one, the first before. A
-      // single one beside the products of the scores, but not where the
-      // queries' rest needs the registers (head dimension 256, TFLOP/s of a
-      // prompt of 8192: bfloat16 655, after them 617; float16 545 and 556).
+      // multiplied; of two, whose codes come one by one, the first before.
       const bool dirty = partial(t + TT, missing(1));
       if (dirty) clean(then, count + 1);
       if constexpr (TT == 2) {
@@ -1035,7 +1034,8 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
       // Operands are read from shared memory AHEAD products before their use.
       // The barriers to the scheduler keep that: left alone it reads each right
       // before its product, to save registers, and every product waits for the
-      // whole latency (a prompt of 8192 tokens: 647 us, with them 582).
+      // whole latency (a prompt of 8192 tokens, without the queries' rest: 647 us,
+      // with them 582).
       f32x16 s[2] = {};                                  // of two tiles, or of queries and their rest
       u32x4 f[2][AHEAD];
 #pragma unroll
@@ -1050,19 +1050,12 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
         if constexpr (TT == 2) {
           s[0] = mfma32(w0, qf[k], s[0]);
           s[1] = mfma32(w1, qf[k], s[1]);
-          if constexpr (REST) {
-            s[0] = mfma32(w0, ql[k], s[0]);
-            s[1] = mfma32(w1, ql[k], s[1]);
-          }
-        } else if constexpr (REST) {
+          s[0] = mfma32(w0, ql[k], s[0]);
+          s[1] = mfma32(w1, ql[k], s[1]);
+        } else {
           // Two sums in turn, as the products of one wait for each other.
           s[0] = mfma32(w0, qf[k], s[0]);
           s[1] = mfma32(w0, ql[k], s[1]);
-        } else {
-          s[k & 1] = mfma32(w0, qf[k], s[k & 1]);
-        }
-        if constexpr (TT == 1 && !REST) {
-          if (k % (TAKES / KN) == TAKES / KN - 1) unpack_part(then, 0, k / (TAKES / KN));
         }
         if (k + AHEAD < TAKES) {
           f[0][k % AHEAD] = key(k + AHEAD, place);
@@ -1076,7 +1069,7 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           scores[(wave * 4 + e) * 64 + lane] = f32x4{s[0][4 * e], s[0][4 * e + 1], s[0][4 * e + 2], s[0][4 * e + 3]};
-        if constexpr (REST) unpack(then, 0);
+        unpack(then, 0);
         fetch(t + 2, page[2]);
         __syncthreads();
 #pragma unroll

@@ -1,0 +1,74 @@
+"""What attention's results may be off, request by request, where scores are
+large and where calls choose different kernels for the same rows."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from exl3_intel_arc_quantizer_amd.kv_cache import cache_attention
+
+from . import cache_ref as ref
+
+UNIT = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+
+
+def _ints(values):
+    return torch.tensor(np.asarray(values), dtype=torch.int32, device="cuda")
+
+
+def _tables(lengths, page, width, pages, rng):
+    ids, at = rng.permutation(pages), 0
+    tables = np.full((len(lengths), width), -1)
+    for r, n in enumerate(lengths):
+        used = -(-n // page)
+        tables[r, :used] = ids[at:at + used]
+        at += used
+    return tables
+
+
+def _tolerance(want, spread, basis, reach, dtype, few):
+    """Queries count with 22 bits whatever their type, so scores (sums of up to
+    256 products in float32) are off by at most 2^-18 of |q| |k| scale and move
+    a weight by that share, numerator and sum. Weights count with 22 bits in
+    requests of few rows to a kv head, with 11 beyond (2^-11 in numerator and
+    sum each); float32 sums 2^-17. Then the output's own rounding."""
+    weights = 2.0 ** -17 + np.where(few, 0.0, 2.0 ** -10)
+    return UNIT[dtype] * np.abs(want) + (2 * 2.0 ** -18 * reach + weights) * spread + 2.0 ** -17 * basis + 2.0 ** -24
+
+
+def _few(new, group, dim):
+    """By row: whether its request has few rows to a kv head."""
+    return np.repeat(np.asarray(new) * group <= (32 if dim == 256 else 16), new)[:, None, None]
+
+
+def _within(got, exact, dtype, few):
+    want, spread, basis, reach = exact
+    got = got.double().cpu().numpy()
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    off = np.abs(got - want) - _tolerance(want, spread, basis, reach, dtype, few)
+    assert not (off > 0).any(), f"{np.nanmax(off)} too far, of {np.nanmax(np.abs(want))}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("strength", [8, 16])
+@pytest.mark.parametrize("dim, group, new, context", [
+    (64, 4, [12, 16], [700, 300]), (64, 4, [130], [2000]), (128, 8, [4, 9], [900, 1500]), (128, 4, [300], [1700]),
+    (256, 4, [20, 70], [300, 1200]), (128, 4, [1100], [1100])])
+def test_sharp_scores_of_many_rows(dim, group, new, context, strength, dtype):
+    """Scores of tens: an error of a score is one of its weight, many times the
+    output's own rounding if queries have fewer bits than their type's sums."""
+    rng = np.random.default_rng(dim + strength)
+    page, heads = 64, 2
+    pages = sum(-(-n // page) for n in context) + 1
+    cache = ref.Cache(pages, page, heads, dim, rng)
+    tables = _tables(context, page, -(-max(context) // page), pages, rng)
+    starts = np.concatenate([[0], np.cumsum(new)])
+    q = torch.from_numpy(rng.normal(size=(starts[-1], heads * group, dim)) * strength).to(dtype).cuda()
+    args = torch.from_numpy(cache.bytes()).cuda(), _ints(tables), _ints(starts), _ints(context)
+    keys, values = (torch.from_numpy(x).cuda() for x in cache.values())
+    exact = ref.attention_dense(q, keys, values, page, tables, starts, context, dim ** -0.5, None)
+    for hint in (None, max(new), 1):
+        _within(cache_attention(q, *args, max_new=hint), exact, dtype, hint == 1 or _few(new, group, dim))
