@@ -1380,14 +1380,17 @@ int64_t partials_bytes(Variant v, int head_dim) {
 // The launches of a call: the variant for its longest requests, and beside it,
 // so that single tokens keep the variant made for them and up to 16 rows their
 // precision, that of 8 rows for requests of up to `few` (where it takes as many
-// alone, those: see above).
+// alone, those: see above). Also where there is one request: how many of the
+// tokens are its own, beside padding or under a bound, the GPU alone knows
+// (a launch that finds none, as beside a whole prompt, takes 3 to 4 us). A single
+// request keeps its bits in blocks of 16 rows.
 struct Launches {
   int count, few;
   Variant of[2];
 };
 Launches launches_of(int64_t tokens, int group, int requests, int head_dim, int64_t max_new) {
   const Variant v = variant_of(std::min(max_new, tokens) * group, head_dim);
-  return {requests > 1 && v != ROWS8 ? 2 : 1, head_dim == 256 ? 32 : v == ROWS16 ? 8 : 16, {v, ROWS8}};
+  return {v == ROWS8 || (v == ROWS16 && requests == 1) ? 1 : 2, head_dim == 256 ? 32 : v == ROWS16 ? 8 : 16, {v, ROWS8}};
 }
 
 template <int D, bool BF16>

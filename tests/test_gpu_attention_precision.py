@@ -72,3 +72,31 @@ def test_sharp_scores_of_many_rows(dim, group, new, context, strength, dtype):
     exact = ref.attention_dense(q, keys, values, page, tables, starts, context, dim ** -0.5, None)
     for hint in (None, max(new), 1):
         _within(cache_attention(q, *args, max_new=hint), exact, dtype, hint == 1 or _few(new, group, dim))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim, group, length", [
+    (128, 4, 2), (64, 4, 6), (256, 2, 10), (64, 8, 2), (128, 4, 400), (64, 8, 2500)])
+def test_a_single_request_of_few_rows_among_padding(dim, group, length, dtype):
+    """One token of one request, in a step padded to 64 rows or with a bound of
+    64 new tokens: the rows that it has, not those it might have, say how many
+    bits its weights count with. Values of neighbouring positions are opposite
+    and their weights nearly equal, so that an output is small beside its terms
+    and their errors stand out."""
+    rng = np.random.default_rng(dim + length)
+    page = 32
+    pages = -(-length // page) + 1
+    cache = ref.Cache(pages, page, 1, dim, rng)
+    cache.codes = np.maximum(cache.codes, -7)
+    cache.codes[1, 1::2], cache.scales[1, 1::2] = -cache.codes[1, ::2], cache.scales[1, ::2]
+    tables = _tables([length], page, pages, pages, rng)
+    q = torch.from_numpy(rng.normal(size=(64, group, dim)) * 0.3).to(dtype)
+    exact = ref.attention(q[:1].double().numpy(), *cache.values(), page, tables, [0, 1], [length], dim ** -0.5, None)
+    held = torch.from_numpy(cache.bytes()).cuda(), _ints(tables)
+    alone = cache_attention(q[:1].cuda(), *held, _ints([0, 1]), _ints([length]), max_new=1)
+    _within(alone, exact, dtype, True)
+    for rows, hint in ((64, None), (64, 64), (64, 1), (1, 64), (2, 2)):
+        got = cache_attention(q[:rows].cuda(), *held, _ints([0, 1]), _ints([length]), max_new=hint)
+        _within(got[:1], exact, dtype, True)
+        assert not got[1:].any()
