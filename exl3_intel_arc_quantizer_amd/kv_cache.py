@@ -85,8 +85,8 @@ def plan_step(cached: torch.Tensor, new: torch.Tensor, tables: torch.Tensor,
     the new tokens need, taken from ``free_pages`` (int32) in order from entry
     ``taken`` (int32, (1,)) on. ``taken`` itself is not changed: the next step
     passes the plan's, so that a step can be planned again. Slots past the last
-    new token are -1, and so are those of tokens that get no page (``status``,
-    ``StepPlan.check``)."""
+    new token are -1, and so are those of tokens that have no page, in this step
+    or because an earlier one ran out of them (``status``, ``StepPlan.check``)."""
     return StepPlan(*_native.plan_step(cached, new, tables, free_pages, taken, page_size,
                                        max_tokens))
 

@@ -248,8 +248,9 @@ int exl3_rotary(const void* q, int64_t q_token, int64_t q_head, void* q_out, int
  * order, slots[t] and positions[t] (its place in the request); -1 and 0 past
  * the last, slot -1 where no page is; starts [requests + 1], the prefix sums
  * of fresh; lengths [requests] = cached + fresh; taken_out = *taken plus the
- * pages used; status: 1 pages ran out, 2 a request outgrew its row, 4 more
- * tokens than max_tokens, added up. */
+ * pages used; status: 1 tokens without a page (the free ones ran out, in this
+ * step or in the one that should have given a page held in part), 2 a request
+ * outgrew its row, 4 more tokens than max_tokens, added up. */
 int exl3_plan_step(const int32_t* cached, const int32_t* fresh, int requests, int32_t* tables,
                    int width, const int32_t* free_pages, int free_count, const int32_t* taken,
                    int page_size, int64_t max_tokens, int64_t* slots, int32_t* positions,
