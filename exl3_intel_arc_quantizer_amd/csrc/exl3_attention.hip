@@ -1431,7 +1431,8 @@ int launch_attend(AttendArgs args, int64_t max_new, char* workspace, hipStream_t
     c.partials = reinterpret_cast<float*>(workspace);
     workspace += partials_bytes(v, D);
     const int64_t grid = c.whole ? segments : v == TILES ? c.owners : c.owners / WAVES;
-    if (grid > INT32_MAX) return set_error("exl3_cache_attention: too many tokens");
+    // A launch has fewer than 2^32 threads.
+    if (grid > UINT32_MAX / (64 * tile_waves(D))) return set_error("exl3_cache_attention: too many tokens and heads");
     if (launch_variant<D, BF16>(v, args, i, (unsigned)grid, stream)) return 1;
   }
   const int64_t rows = args.tokens * args.q_heads;

@@ -89,7 +89,24 @@ struct Rows {
   __device__ __forceinline__ T* at(int64_t t, int h) const {
     return data + t * token + (int64_t)h * head;
   }
+  Rows from(int64_t t) const { return {data ? data + t * token : data, token, head}; }
 };
+
+// Positions, int64 if wide, from token t on.
+const void* positions_from(const void* positions, bool wide, int64_t t) {
+  return positions ? static_cast<const char*>(positions) + t * (wide ? 8 : 4) : positions;
+}
+
+// A launch has fewer than 2^32 threads along an axis: more tokens than so many
+// blocks of 256 take go in several.
+constexpr int64_t MOST_BLOCKS = 1 << 23;
+// launch(first token, tokens), by parts of MOST_BLOCKS blocks of `per_block`.
+template <typename F>
+int in_parts(int64_t tokens, int64_t per_block, F launch) {
+  for (int64_t t = 0; t < tokens; t += MOST_BLOCKS * per_block)
+    if (const int status = launch(t, std::min(tokens - t, MOST_BLOCKS * per_block))) return status;
+  return 0;
+}
 
 // Cosines and sines of one block's tokens, [token][pair], in shared memory:
 // every head of a token turns by the same angles. Angles and their functions
@@ -146,15 +163,13 @@ __device__ __forceinline__ void turned8(const typename E::type* row, int d0, int
 struct RotaryArgs {
   const void* positions;
   const double* freq;
-  int64_t tokens;
-  int q_heads, heads, d, pairs, per_block, wide, half;
+  int q_heads, heads, d, pairs, wide, half;
   float magnitude, sign;
 };
 
 // y1 = x1 cos - x2 sin, y2 = x2 cos + x1 sin of every pair, the other values
-// copied. A block takes `per_block` tokens, makes their angles once and turns
-// all heads of q and k: per pair one 64-bit product and one sincospi for all
-// heads, so the pass is bound by reading and writing the rows (8192 tokens of
+// copied. A block takes a token, makes its angles once and turns all heads of
+// q and k: per pair one 64-bit product and one sincospi for all heads, so the pass is bound by reading and writing the rows (8192 tokens of
 // 32 + 8 heads of 128 in bfloat16, 168 MB that the last-level cache holds:
 // 26 us, 6.4 TB/s; one token 3 us, a launch).
 // A thread turns both values of its pairs and writes them where it read them
@@ -165,20 +180,17 @@ __global__ void __launch_bounds__(256)
     rotary_kernel(Rows<const typename E::type> q, Rows<const typename E::type> k,
                   Rows<typename E::type> q_out, Rows<typename E::type> k_out, RotaryArgs a) {
   extern __shared__ float table[];
-  const int64_t t0 = (int64_t)blockIdx.x * a.per_block;
-  const int tokens = (int)min((int64_t)a.per_block, a.tokens - t0);
-  float *cosines = table, *sines = table + a.per_block * a.pairs;
-  turn_table(a.positions, a.wide, a.freq, a.pairs, a.magnitude, a.sign, t0, tokens, cosines, sines);
+  const int64_t t = blockIdx.x;
+  float *c = table, *s = table + a.pairs;
+  turn_table(a.positions, a.wide, a.freq, a.pairs, a.magnitude, a.sign, t, 1, c, s);
   __syncthreads();
   const int units = VEC ? a.d / 16 : (a.d + 1) / 2;
-  const int all = tokens * a.heads * units;
+  const int all = a.heads * units;
   for (int i = threadIdx.x; i < all; i += blockDim.x) {
-    const int row = i / units, u = i - row * units;
-    const int t = row / a.heads, h = row - t * a.heads;
+    const int h = i / units, u = i - h * units;
     const bool is_k = h >= a.q_heads;
-    const typename E::type* in = is_k ? k.at(t0 + t, h - a.q_heads) : q.at(t0 + t, h);
-    typename E::type* out = is_k ? k_out.at(t0 + t, h - a.q_heads) : q_out.at(t0 + t, h);
-    const float *c = cosines + t * a.pairs, *s = sines + t * a.pairs;
+    const typename E::type* in = is_k ? k.at(t, h - a.q_heads) : q.at(t, h);
+    typename E::type* out = is_k ? k_out.at(t, h - a.q_heads) : q_out.at(t, h);
     if constexpr (VEC) {
       // Turned units first (8 pairs each), copied ones of 16 after them.
       const int turned = a.pairs / 8;
@@ -233,18 +245,19 @@ __global__ void __launch_bounds__(256)
 template <typename E>
 int launch_rotary(const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token,
                   int64_t k_head, void* q_out, int64_t qo_token, int64_t qo_head, void* k_out,
-                  int64_t ko_token, int64_t ko_head, const RotaryArgs& args, bool vec,
-                  hipStream_t stream) {
+                  int64_t ko_token, int64_t ko_head, const RotaryArgs& args, int64_t tokens,
+                  bool vec, hipStream_t stream) {
   typedef typename E::type T;
   Rows<const T> rq{static_cast<const T*>(q), q_token, q_head}, rk{static_cast<const T*>(k), k_token, k_head};
   Rows<T> oq{static_cast<T*>(q_out), qo_token, qo_head}, ok{static_cast<T*>(k_out), ko_token, ko_head};
-  const unsigned blocks = (unsigned)((args.tokens + args.per_block - 1) / args.per_block);
-  const size_t lds = 2 * sizeof(float) * args.per_block * args.pairs;
-  if (vec)
-    rotary_kernel<E, true><<<blocks, 256, lds, stream>>>(rq, rk, oq, ok, args);
-  else
-    rotary_kernel<E, false><<<blocks, 256, lds, stream>>>(rq, rk, oq, ok, args);
-  return check_launch("exl3_rotary");
+  const size_t lds = 2 * sizeof(float) * args.pairs;
+  return in_parts(tokens, 1, [&](int64_t t, int64_t n) {
+    RotaryArgs part = args;
+    part.positions = positions_from(args.positions, args.wide, t);
+    auto kernel = vec ? rotary_kernel<E, true> : rotary_kernel<E, false>;
+    kernel<<<(unsigned)n, 256, lds, stream>>>(rq.from(t), rk.from(t), oq.from(t), ok.from(t), part);
+    return check_launch("exl3_rotary");
+  });
 }
 
 // ------------------------------------------------------------ step plan
@@ -567,13 +580,16 @@ int launch_append(const void* q, int64_t q_token, int64_t q_head, void* q_out, c
   auto launch = [&](auto tok) {
     constexpr int TOK = decltype(tok)::value;
     const int64_t units = (2 * (int64_t)args.cache.kv_heads + args.q_heads) * (d / 8);
-    const dim3 blocks = grid_of<TOK>(args.tokens, units, TOK == 1 ? 1 : 4);
     const size_t lds = 2 * sizeof(float) * TOK * args.pairs;
-    if (args.pairs)
-      append_kernel<E, true, TOK><<<blocks, 256, lds, stream>>>(rq, rk, rv, oq, pages, args);
-    else
-      append_kernel<E, false, TOK><<<blocks, 256, 0, stream>>>(rq, rk, rv, oq, pages, args);
-    return check_launch("exl3_cache_append");
+    auto kernel = args.pairs ? append_kernel<E, true, TOK> : append_kernel<E, false, TOK>;
+    return in_parts(args.tokens, TOK, [&](int64_t t, int64_t n) {
+      CellArgs part = args;
+      part.slots = args.slots + t, part.positions = positions_from(args.positions, args.wide, t);
+      part.tokens = n;
+      kernel<<<grid_of<TOK>(n, units, TOK == 1 ? 1 : 4), 256, lds, stream>>>(
+          rq.from(t), rk.from(t), rv.from(t), oq.from(t), pages, part);
+      return check_launch("exl3_cache_append");
+    });
   };
   if (args.tokens >= MANY_TOKENS) return launch(std::integral_constant<int, 8>{});
   return launch(std::integral_constant<int, 1>{});
@@ -585,11 +601,17 @@ int launch_read(const uint8_t* pages, void* k, void* v, const CellArgs& args, hi
   const int64_t token = (int64_t)args.cache.kv_heads * args.cache.head_dim, head = args.cache.head_dim;
   const Rows<T> rk{static_cast<T*>(k), token, head}, rv{static_cast<T*>(v), token, head};
   const int64_t units = 2 * (int64_t)args.cache.kv_heads * (head / 8);
-  if (args.tokens >= MANY_TOKENS)
-    read_kernel<E, 8><<<grid_of<8>(args.tokens, units, 2), 256, 0, stream>>>(pages, rk, rv, args);
-  else
-    read_kernel<E, 1><<<grid_of<1>(args.tokens, units, 1), 256, 0, stream>>>(pages, rk, rv, args);
-  return check_launch("exl3_cache_read");
+  auto launch = [&](auto tok, int64_t passes) {
+    constexpr int TOK = decltype(tok)::value;
+    return in_parts(args.tokens, TOK, [&](int64_t t, int64_t n) {
+      CellArgs part = args;
+      part.slots = args.slots + t, part.tokens = n;
+      read_kernel<E, TOK><<<grid_of<TOK>(n, units, passes), 256, 0, stream>>>(pages, rk.from(t), rv.from(t), part);
+      return check_launch("exl3_cache_read");
+    });
+  };
+  if (args.tokens >= MANY_TOKENS) return launch(std::integral_constant<int, 8>{}, 2);
+  return launch(std::integral_constant<int, 1>{}, 1);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -635,11 +657,10 @@ int exl3_rotary(const void* q, int64_t q_token, int64_t q_head, void* q_out, int
     return set_error("exl3_rotary: bad type or layout");
   if (!tokens) return 0;
   RotaryArgs args{};
-  args.positions = positions, args.freq = frequencies, args.tokens = tokens;
+  args.positions = positions, args.freq = frequencies;
   args.q_heads = q_heads, args.heads = q_heads + k_heads, args.d = head_dim, args.pairs = pairs;
   args.wide = wide_positions, args.half = layout == 0;
   args.magnitude = magnitude, args.sign = inverse ? -1.0f : 1.0f;
-  args.per_block = 1;
   const int64_t per = type == 0 ? 4 : 8;
   const bool vec = pairs % 8 == 0 && head_dim % 16 == 0 && wide_rows(q, q_token, q_head, per) &&
                    wide_rows(k, k_token, k_head, per) && wide_rows(q_out, qo_token, qo_head, per) &&
@@ -647,7 +668,7 @@ int exl3_rotary(const void* q, int64_t q_token, int64_t q_head, void* q_out, int
   hipStream_t s = (hipStream_t)stream;
   auto launch = type == 0 ? launch_rotary<F32> : type == 1 ? launch_rotary<F16> : launch_rotary<BF16>;
   return launch(q, q_token, q_head, k, k_token, k_head, q_out, qo_token, qo_head, k_out, ko_token,
-                ko_head, args, vec, s);
+                ko_head, args, tokens, vec, s);
 }
 
 int exl3_plan_step(const int32_t* cached, const int32_t* fresh, int requests, int32_t* tables,

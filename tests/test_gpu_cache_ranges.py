@@ -1,0 +1,54 @@
+"""Arguments at the ends of their ranges."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from exl3_intel_arc_quantizer_amd.kv_cache import append_tokens, cache_pages, read_tokens
+from exl3_intel_arc_quantizer_amd.rotary import apply_rotary
+
+
+@pytest.fixture
+def much_memory():
+    """Frees what a test of many tokens takes."""
+    torch.cuda.empty_cache()
+    yield
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pairs, dtype", [(8, torch.float16), (3, torch.bfloat16)])
+def test_rotary_of_more_tokens_than_a_launch_has_blocks(pairs, dtype, much_memory):
+    tokens = 2 ** 24 + 5
+    at = torch.arange(tokens, device="cuda", dtype=torch.int32) % 97
+    freq = torch.linspace(0.1, 1.0, pairs, dtype=torch.float64, device="cuda")
+    row = torch.randn(1, 1, 16, device="cuda", dtype=dtype)
+    few, _ = apply_rotary(row.expand(97, 1, 16), None, at[:97], freq)
+    got, more = apply_rotary(row.expand(tokens, 1, 16), row.expand(tokens, 1, 16), at.long(), freq)
+    assert torch.equal(got, few[at]) and torch.equal(got, more)
+
+
+@pytest.mark.gpu
+def test_append_and_read_of_more_tokens_than_a_launch_has_blocks(much_memory):
+    """All slots but a few lie outside the cache; rows of the others are never
+    looked at and hold what they hold."""
+    tokens = 2 ** 27 + 9
+    some = torch.tensor([0, 2 ** 26 - 1, 2 ** 26, 2 ** 26 + 7, 2 ** 27 - 1, 2 ** 27, 2 ** 27 + 8], device="cuda")
+    x = torch.empty(tokens, 1, 64, device="cuda", dtype=torch.float16)
+    rows = torch.randn(len(some), 1, 64, device="cuda", dtype=torch.float16)
+    x[some] = rows
+    slots = torch.full((tokens,), -1, device="cuda")
+    slots[some] = torch.tensor([5, 70, 3, 127, 64, 0, 31], device="cuda")
+    at = torch.zeros(tokens, device="cuda", dtype=torch.int32)
+    at[some] = torch.arange(len(some), device="cuda", dtype=torch.int32) * 11
+    freq = torch.linspace(0.1, 1.0, 16, dtype=torch.float64, device="cuda")
+    pages, small = cache_pages(2, 64, 1, 64), cache_pages(2, 64, 1, 64)
+    turned = append_tokens(pages, x, x, slots, q=x, positions=at, frequencies=freq)[some]
+    want = append_tokens(small, rows, rows, slots[some], q=rows, positions=at[some], frequencies=freq)
+    assert torch.equal(turned, want) and torch.equal(pages, small)
+    del x, at
+    many, few = read_tokens(pages, slots), read_tokens(pages, slots[some])
+    for a, b in zip(many, few):
+        assert torch.equal(a[some], b)
+        assert not a[[1, 2 ** 26 - 2, 2 ** 26 + 1, 2 ** 27 + 7]].any()
