@@ -100,3 +100,82 @@ def test_a_single_request_of_few_rows_among_padding(dim, group, length, dtype):
         got = cache_attention(q[:rows].cuda(), *held, _ints([0, 1]), _ints([length]), max_new=hint)
         _within(got[:1], exact, dtype, True)
         assert not got[1:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim, group, new, window", [
+    (64, 4, [1, 4, 5, 0, 70], None), (128, 16, [1, 2, 1, 3], 40), (128, 4, [1, 33, 4, 200], None),
+    (256, 16, [1, 2, 3, 2], None), (256, 5, [6, 7, 1, 60], 33), (64, 1, [16, 17, 1, 300], 100)])
+def test_bits_of_each_request(dim, group, new, window, dtype):
+    """Requests of few rows keep the weights' bits beside those of many."""
+    rng = np.random.default_rng(dim + group)
+    page, heads = 32, 2
+    context = [n + c for n, c in zip(new, (3, 700, 0, 90, 400))]
+    pages = sum(-(-n // page) for n in context) + 1
+    cache = ref.Cache(pages, page, heads, dim, rng)
+    tables = _tables(context, page, -(-max(context) // page) + 1, pages, rng)
+    starts = np.concatenate([[0], np.cumsum(new)])
+    q = torch.from_numpy(rng.normal(size=(starts[-1], heads * group, dim)) * 3).to(dtype)
+    args = torch.from_numpy(cache.bytes()).cuda(), _ints(tables), _ints(starts), _ints(context)
+    exact = ref.attention(q.double().numpy(), *cache.values(), page, tables, starts, context, dim ** -0.5, window)
+    for hint in (None, max(new)):
+        _within(cache_attention(q.cuda(), *args, window=window, max_new=hint), exact, dtype, _few(new, group, dim))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_nan_reaches_exactly_its_rows(dim, new):
+    """A finite number where a NaN is due is as wrong as the reverse."""
+    rng = np.random.default_rng(dim)
+    page, context = 32, [90, 130]
+    cache = ref.Cache(9, page, 1, dim, rng)
+    tables = _tables(context, page, 5, 9, rng)
+    for r, at, which, part in ((0, 89, 1, 1), (1, 120, 0, 0), (1, 127, 1, 0)):
+        cache.scales[which][tables[r][at // page] * page + at % page, 0, part] = np.nan
+    starts = np.array([0, new, 2 * new])
+    q = torch.from_numpy(rng.normal(size=(2 * new, 2, dim))).half()
+    for window in (None, 3):
+        exact = ref.attention(q.double().numpy(), *cache.values(), page, tables, starts, context, dim ** -0.5, window)
+        got = cache_attention(q.cuda(), torch.from_numpy(cache.bytes()).cuda(), _ints(tables), _ints(starts),
+                              _ints(context), window=window)
+        assert np.isnan(exact[0]).any()
+        _within(got, exact, torch.float16, _few([new, new], 2, dim))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [4, 300])
+def test_requests_that_claim_the_same_rows(rows):
+    """Starts that are no prefix sums: each row is one claimant's result, or 0."""
+    rng = np.random.default_rng(rows)
+    cache = ref.Cache(3, 32, 1, 64, rng)
+    pages, tables = torch.from_numpy(cache.bytes()).cuda(), _ints([[0, 1], [2, 5], [1, -3]])
+    q = torch.from_numpy(rng.normal(size=(rows, 2, 64))).half().cuda()
+    got = cache_attention(q, pages, tables, _ints([0, rows, 0, rows]), _ints([64, 32, 60]))
+    assert torch.isfinite(got).all()
+    most = cache.values()[1]
+    assert got.abs().max() <= np.abs(most).max() * (1 + 2.0 ** -9)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("most", [1, 3, 40])
+def test_as_many_requests_as_a_call_takes(dim, most):
+    """4096 requests, some empty, of up to `most` tokens of up to 70 positions."""
+    rng = np.random.default_rng(most)
+    page, requests = 32, 4096
+    new = rng.integers(0, most + 1, requests)
+    if most > 3:
+        new[rng.random(requests) < 0.9] = 0
+    context = new + rng.integers(0, 30, requests)
+    pages = int((-(-context // page)).sum()) + 1
+    cache = ref.Cache(pages, page, 1, dim, rng)
+    tables = _tables(context, page, 3, pages, rng)
+    starts = np.concatenate([[0], np.cumsum(new)])
+    q = torch.from_numpy(rng.normal(size=(starts[-1] + 2, 2, dim)) * 2).to(torch.bfloat16)
+    got = cache_attention(q.cuda(), torch.from_numpy(cache.bytes()).cuda(), _ints(tables), _ints(starts), _ints(context))
+    exact = ref.attention(q.double().numpy(), *cache.values(), page, tables, starts, context, dim ** -0.5, None)
+    few = np.concatenate([_few(new, 2, dim), np.ones((2, 1, 1), bool)])
+    _within(got, exact, torch.bfloat16, few)
+    assert not got[starts[-1]:].any()
