@@ -1195,12 +1195,13 @@ def cache_attention(q, pages, tables, starts, lengths, scale, window, max_new):
         raise RuntimeError(f"max_new must not be negative, got {max_new}")
     lib = load_library()
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    most = tokens if max_new is None else int(max_new)
+    # Python's integers end nowhere, the C arguments at 64 bits.
+    most = tokens if max_new is None else min(int(max_new), tokens)
+    window = 2 ** 31 - 1 if window is None else min(int(window), 2 ** 31 - 1)
     size = lib.exl3_cache_attention_workspace(tokens, q_heads, heads, dim, requests, most)
     workspace = pages.new_empty(max(size, 0))
     _run(dev, "cache_attention", lib.exl3_cache_attention, q.data_ptr(), sq[0], sq[1],
          out.data_ptr(), tokens, q_heads, _types()[q.dtype], pages.data_ptr(), n, page_size, heads,
          dim, tables.data_ptr(), width, starts.data_ptr(), lengths.data_ptr(), requests,
-         dim ** -0.5 if scale is None else float(scale), 2 ** 31 - 1 if window is None else
-         int(window), most, workspace.data_ptr(), size)
+         dim ** -0.5 if scale is None else float(scale), window, most, workspace.data_ptr(), size)
     return out

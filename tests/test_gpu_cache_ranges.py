@@ -2,11 +2,18 @@
 
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
-from exl3_intel_arc_quantizer_amd.kv_cache import append_tokens, cache_pages, read_tokens
+from exl3_intel_arc_quantizer_amd.kv_cache import append_tokens, cache_attention, cache_pages, read_tokens
 from exl3_intel_arc_quantizer_amd.rotary import apply_rotary
+
+from . import cache_ref as ref
+
+
+def _ints(values):
+    return torch.tensor(np.asarray(values), dtype=torch.int32, device="cuda")
 
 
 @pytest.fixture
@@ -52,3 +59,17 @@ def test_append_and_read_of_more_tokens_than_a_launch_has_blocks(much_memory):
     for a, b in zip(many, few):
         assert torch.equal(a[some], b)
         assert not a[[1, 2 ** 26 - 2, 2 ** 26 + 1, 2 ** 27 + 7]].any()
+
+
+@pytest.mark.gpu
+def test_windows_and_hints_past_64_bits():
+    """A window no context reaches is no window, however it is written."""
+    rng = np.random.default_rng(2)
+    cache = ref.Cache(4, 32, 1, 64, rng)
+    args = (torch.from_numpy(cache.bytes()).cuda(), _ints([[3, 0, 1]]), _ints([0, 5]), _ints([90]))
+    q = torch.randn(5, 2, 64, device="cuda", dtype=torch.float16)
+    want = cache_attention(q, *args)
+    for window in (90, 2 ** 31, 2 ** 32 + 1, 2 ** 63, 2 ** 64 + 1, 2 ** 70):
+        assert torch.equal(cache_attention(q, *args, window=window), want), window
+    for hint in (5, 2 ** 31, 2 ** 32, 2 ** 63, 2 ** 64 + 1):
+        assert torch.equal(cache_attention(q, *args, max_new=hint), want), hint
