@@ -1373,6 +1373,16 @@ int64_t blocks_bound(Variant v, int head_dim) { return v == TILES ? 2 * owners_o
 int64_t shares_bytes(Variant v, int requests, int head_dim) {
   return (8 * ((int64_t)requests + 2 + blocks_bound(v, head_dim)) + 15) & ~(int64_t)15;
 }
+// At most so many segments.
+int64_t segments_of(Variant v, int head_dim, int64_t tokens, int group, int requests, int kv_heads) {
+  const int rows = rows_of(v, head_dim);
+  return ((tokens * group + rows - 1) / rows + requests) * kv_heads;
+}
+// Blocks of attend_tiles_kernel are dealt whole, and leave no partials, where
+// they fill the chip twice.
+bool whole_of(Variant v, int head_dim, int64_t segments) {
+  return v == TILES && segments >= 2 * owners_of(v, head_dim);
+}
 int64_t partials_bytes(Variant v, int head_dim) {
   return (int64_t)2 * owners_of(v, head_dim) * rows_of(v, head_dim) * (head_dim + 2) * 4;
 }
@@ -1422,14 +1432,13 @@ int launch_attend(AttendArgs args, int64_t max_new, char* workspace, hipStream_t
     c.low = args.classes == 2 && i == 0 ? launches.few + 1 : 1;
     c.high = args.classes == 2 && i == 1 ? launches.few : INT32_MAX;
     c.owners = owners_of(v, D);
-    // At most so many segments: whole where they fill the chip twice.
-    const int64_t segments = ((args.tokens * args.group + c.rows - 1) / c.rows + args.requests) * args.cache.kv_heads;
+    const int64_t segments = segments_of(v, D, args.tokens, args.group, args.requests, args.cache.kv_heads);
     c.by_block = v == TILES, c.blocks = (int)blocks_bound(v, D);
-    c.whole = v == TILES && segments >= 2 * c.owners;
+    c.whole = whole_of(v, D, segments);
     c.shares = reinterpret_cast<int64_t*>(workspace);
     workspace += shares_bytes(v, args.requests, D);
     c.partials = reinterpret_cast<float*>(workspace);
-    workspace += partials_bytes(v, D);
+    if (!c.whole) workspace += partials_bytes(v, D);
     const int64_t grid = c.whole ? segments : v == TILES ? c.owners : c.owners / WAVES;
     // A launch has fewer than 2^32 threads.
     if (grid > UINT32_MAX / (64 * tile_waves(D))) return set_error("exl3_cache_attention: too many tokens and heads");
@@ -1458,10 +1467,15 @@ int64_t exl3_cache_attention_workspace(int64_t tokens, int q_heads, int kv_heads
   if (requests < 1 || requests > CACHE_MAX_REQUESTS || (head_dim != 64 && head_dim != 128 && head_dim != 256) ||
       tokens < 0 || kv_heads < 1 || q_heads < kv_heads || max_new < 0)
     return -1;
-  const Launches launches = launches_of(tokens, q_heads / kv_heads, requests, head_dim, max_new);
+  const int group = q_heads / kv_heads;
+  const Launches launches = launches_of(tokens, group, requests, head_dim, max_new);
   int64_t bytes = 0;
-  for (int i = 0; i < launches.count; ++i)
-    bytes += shares_bytes(launches.of[i], requests, head_dim) + partials_bytes(launches.of[i], head_dim);
+  for (int i = 0; i < launches.count; ++i) {
+    const Variant v = launches.of[i];
+    bytes += shares_bytes(v, requests, head_dim);
+    if (!whole_of(v, head_dim, segments_of(v, head_dim, tokens, group, requests, kv_heads)))
+      bytes += partials_bytes(v, head_dim);
+  }
   return bytes;
 }
 

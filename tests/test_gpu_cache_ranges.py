@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+from exl3_intel_arc_quantizer_amd import _native
 from exl3_intel_arc_quantizer_amd.kv_cache import append_tokens, cache_attention, cache_pages, read_tokens
 from exl3_intel_arc_quantizer_amd.rotary import apply_rotary
 
@@ -73,3 +74,37 @@ def test_windows_and_hints_past_64_bits():
         assert torch.equal(cache_attention(q, *args, window=window), want), window
     for hint in (5, 2 ** 31, 2 ** 32, 2 ** 63, 2 ** 64 + 1):
         assert torch.equal(cache_attention(q, *args, max_new=hint), want), hint
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim, requests, tokens, hint, heads", [
+    (128, 1, 3000, 3000, 16), (64, 1, 1, 1, 2), (128, 40, 40, 40, 16), (128, 1, 8192, 8192, 16), (128, 70, 70, 70, 16),
+    (256, 5, 600, 200, 2), (64, 300, 900, 60, 4)])
+def test_calls_stay_within_their_workspace(dim, requests, tokens, hint, heads, dtype):
+    """Bytes past the asked size keep what they hold; a step whose blocks are all
+    dealt whole has partial results of its few-row requests at most."""
+    lib = _native.load_library()
+    new = tokens // requests
+    context, page, group = new + 40, 64, 2
+    width = -(-context // page)
+    pages = torch.zeros(requests * width, heads, 2, 36 * dim, dtype=torch.uint8, device="cuda")
+    tables = torch.arange(requests * width, dtype=torch.int32, device="cuda").view(requests, width)
+    starts = torch.arange(requests + 1, dtype=torch.int32, device="cuda") * new
+    lengths = torch.full((requests,), context, dtype=torch.int32, device="cuda")
+    q = torch.randn(tokens, group * heads, dim, device="cuda").to(dtype)
+    size = lib.exl3_cache_attention_workspace(tokens, group * heads, heads, dim, requests, hint)
+    if (tokens, hint) in ((8192, 8192), (70, 70)):  # up to (64 + 1) 16 and (1 + 70) 16 blocks of 256 rows
+        assert size <= lib.exl3_cache_attention_workspace(1, group * heads, heads, dim, 1, 1) + 16 * (requests + 2048)
+    held = torch.full((size + (1 << 20),), 173, dtype=torch.uint8, device="cuda")
+    out = torch.full_like(q, 3.0)
+    status = lib.exl3_cache_attention(
+        q.data_ptr(), q.stride(0), dim, out.data_ptr(), tokens, group * heads, 1 if dtype == torch.float16 else 2,
+        pages.data_ptr(), pages.shape[0], page, heads, dim, tables.data_ptr(), width, starts.data_ptr(),
+        lengths.data_ptr(), requests, 1.0, 2 ** 31 - 1, hint, held.data_ptr(), size, torch.cuda.current_stream().cuda_stream)
+    assert status == 0 and (held[size:] == 173).all()
+    assert not out.any()  # a cache of zeros
+    assert lib.exl3_cache_attention(
+        q.data_ptr(), q.stride(0), dim, out.data_ptr(), tokens, group * heads, 1, pages.data_ptr(), pages.shape[0], page,
+        heads, dim, tables.data_ptr(), width, starts.data_ptr(), lengths.data_ptr(), requests, 1.0, 2 ** 31 - 1, hint,
+        held.data_ptr(), size - 1, torch.cuda.current_stream().cuda_stream) != 0
