@@ -179,3 +179,21 @@ def test_as_many_requests_as_a_call_takes(dim, most):
     few = np.concatenate([_few(new, 2, dim), np.ones((2, 1, 1), bool)])
     _within(got, exact, torch.bfloat16, few)
     assert not got[starts[-1]:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim, new", [(64, 1), (64, 100), (128, 1), (128, 12), (256, 1), (256, 30)])
+def test_scales_of_zero_and_below(dim, new, dtype):
+    """A scale of 0 is the mean of what is attended, a negative one prefers the
+    smallest products."""
+    rng = np.random.default_rng(dim + new)
+    page, context = 32, 150
+    cache = ref.Cache(6, page, 1, dim, rng)
+    tables = _tables([context], page, 5, 6, rng)
+    q = torch.from_numpy(rng.normal(size=(new, 2, dim)) * 2).to(dtype)
+    args = torch.from_numpy(cache.bytes()).cuda(), _ints(tables), _ints([0, new]), _ints([context])
+    for scale in (0.0, -0.0, -0.1):
+        *exact, reach = ref.attention(q.double().numpy(), *cache.values(), page, tables, [0, new], [context], scale, None)
+        got = cache_attention(q.cuda(), *args, scale=scale)
+        _within(got, (*exact, np.abs(reach)), dtype, _few([new], 2, dim))
