@@ -334,13 +334,7 @@ __global__ void __launch_bounds__(STEP_THREADS) step_kernel(StepArgs a) {
       const int64_t length = cached + fresh;
       outgrown |= length > room;
       need = min((length + page - 1) >> a.page_shift, (int64_t)a.width) - have_of(r);
-      if (blockIdx.x == 0) {
-        a.lengths[r] = (int32_t)min(length, (int64_t)INT32_MAX);
-        // New tokens begin in a page that is held in part: without one (of a
-        // step that ran out) they have no slot, though this step needs no page.
-        if (fresh && (cached & (page - 1)) && cached < room)
-          missing |= a.tables[(int64_t)r * a.width + (cached >> a.page_shift)] < 0;
-      }
+      if (blockIdx.x == 0) a.lengths[r] = (int32_t)min(length, (int64_t)INT32_MAX);
     }
     int64_t sum_tokens, sum_pages;
     const int64_t end_tokens = tokens + block_sum(fresh, parts, &sum_tokens);
@@ -357,11 +351,13 @@ __global__ void __launch_bounds__(STEP_THREADS) step_kernel(StepArgs a) {
   const int64_t taken = max(a.taken[0], 0);
   if (blockIdx.x == 0) {
     for (int r = tid; r <= a.requests; r += STEP_THREADS) a.starts[r] = starts[r];
-    outgrown = __syncthreads_or(outgrown), missing = __syncthreads_or(missing);
-    if (tid == 0) {
-      a.taken_out[0] = (int32_t)min(taken + pages, (int64_t)max((int64_t)a.free_count, taken));
-      a.status[0] = (taken + pages > a.free_count || missing ? 1 : 0) | (outgrown ? 2 : 0) |
-                    (tokens > a.max_tokens ? 4 : 0);
+    // New tokens begin in a page that is held in part: without one (of a step
+    // that ran out) they have no slot, though this step needs no page. (Looked
+    // up here and asked for at the end, so that nothing waits for it.)
+    for (int r = tid; r < a.requests; r += STEP_THREADS) {
+      const int64_t cached = max(a.cached[r], 0);
+      if (starts[r + 1] > starts[r] && (cached & (page - 1)) && cached < room)
+        missing |= a.tables[(int64_t)r * a.width + (cached >> a.page_shift)] < 0;
     }
   }
   auto new_page = [&](int64_t i) { return taken + i < a.free_count ? a.free_pages[taken + i] : -1; };
@@ -385,6 +381,14 @@ __global__ void __launch_bounds__(STEP_THREADS) step_kernel(StepArgs a) {
     }
     a.slots[t] = slot;
     a.positions[t] = position;
+  }
+  if (blockIdx.x == 0) {
+    outgrown = __syncthreads_or(outgrown), missing = __syncthreads_or(missing);
+    if (tid == 0) {
+      a.taken_out[0] = (int32_t)min(taken + pages, (int64_t)max((int64_t)a.free_count, taken));
+      a.status[0] = (taken + pages > a.free_count || missing ? 1 : 0) | (outgrown ? 2 : 0) |
+                    (tokens > a.max_tokens ? 4 : 0);
+    }
   }
 }
 
