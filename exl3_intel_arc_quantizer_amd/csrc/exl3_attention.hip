@@ -342,9 +342,9 @@ constexpr int resident(int d, bool wide, int ct) {
 //
 // Bound by reading the cache where there are few rows: 128 requests of up to
 // 8192 positions, 8 kv heads of 128, one token: 504 MB in 107 us, 4.7 TB/s of the
-// 4.9 a large copy reaches, vector instructions on 0.61 of the cycles. With 32
-// rows a tile they and the products get as long as the reading: 157 MB in
-// 51 us, of which about 10 are the waves' start and end.
+// 4.9 a large copy reaches, vector instructions on 0.60 of the cycles. With 32
+// rows a tile they (0.50) and the products (0.18) get as long as the reading: 157
+// MB in 55 us, of which about 10 are the waves' start and end.
 template <int D, bool WIDE, int CT, bool BF16>
 __global__ void __launch_bounds__(THREADS, resident(D, WIDE, CT)) attend_rows_kernel(AttendArgs a, int index) {
   constexpr int PER = WIDE ? 16 : 8, ROWS = PER * CT, GROUPS = D / 32, SETS = Tile<D>::SETS, NIB = D == 64 ? 4 : 8;
@@ -734,9 +734,9 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 // softmax above all) 0.42, and two waves a SIMD overlap them little. Head
 // dimension 64: 0.44 and 0.64; 256: 0.34 and 0.43, of which both waves of a pair
 // do all the softmax. A prompt of 8192 tokens, 32 heads over 8, 550 GFLOP of 128
-// dims without the queries' rest: 0.74 ms, 747 TFLOP/s (with it 1.12 of a
-// PFLOP/s; a library product of 8192 a side 1.21). Of 64 dims 0.45 ms, 610, of
-// 256 1.94 ms, 568; float16 and bfloat16 alike.
+// dims without the queries' rest: 0.74 to 0.77 ms, 711 to 747 TFLOP/s (with it
+// 1.07 to 1.12 PFLOP/s; a library product of 8192 a side 1.21). Of 64 dims 0.45
+// ms, 610, of 256 1.94 ms, 568; float16 and bfloat16 alike.
 //
 // As in WIDE blocks above, queries count with 22 bits, by a second product of the
 // scores (the same prompt without it 0.59 ms), and weights with 11.
@@ -1346,14 +1346,19 @@ constexpr int CUS = 256;
 // times the query heads to a kv head): up to 8 and 16 rows at 22 bits, whose
 // cost is the cache's bytes, then 32 to a wave, then blocks that share the work
 // of unpacking a tile. Waves of 32 rows are kept for a few blocks' worth, each
-// of which reads the cache again: 64 requests of 2048 positions, 8 kv heads,
-// float16: head dimension 128, 64 rows 99 us and in blocks 182, 128 rows 160 and
-// 189; head dimension 64, 64 rows 75 and 92, 96 rows 108 and 105.
+// of which reads the cache again. In us, 8 kv heads, both types alike, rows of
+// 32 to a wave and blocks that share the unpacking:
+//                            64 requests of 2048      one of 131072 positions
+//   128 dims, 64 rows            88  175                    90  171
+//             128               143  179                   147  176
+//             160               194  185                   174  181
+//   64 dims,  64 rows            62   79                    60   73
+//             96                 88   86                    78   78
 // Head dimension 256 has no variants of 16 and 32 rows, for which a wave lacks
 // registers: up to 32 rows go in blocks of 8, whose later ones find the tiles in
-// the caches (the same requests, float16: 16 rows 120 us, in a variant of 16 with
-// spills 151; 32 rows 175 and in blocks that share the unpacking 260; 48 rows
-// 268 and 264. Bfloat16: 32 rows 170 and 228, 48 rows 270 and 231).
+// the caches (16 rows 101 us, in a variant of 16 with spills 151; blocks of 8 and
+// blocks that share the unpacking: 32 rows 168 and 258, one request 196 and 249;
+// 48 rows 266 and 260, one request 276 and 253).
 enum Variant { ROWS8, ROWS16, ROWS32, TILES };
 Variant variant_of(int64_t rows, int head_dim) {
   if (head_dim == 256) return rows <= 32 ? ROWS8 : TILES;

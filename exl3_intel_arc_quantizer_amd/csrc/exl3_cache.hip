@@ -313,7 +313,7 @@ __device__ __forceinline__ int last_at_most(const int32_t* at, int n, int x) {
 // and fills its share of the new table entries and of the tokens' slots. A
 // slot in a new page takes the page from the free list itself, so no block
 // reads what another writes. Bound by latency: two reads and two dependent
-// look-ups deep (256 requests of a token 6 us, 1531 of up to 96 tokens 10 us).
+// look-ups deep (256 requests of a token 6 us, 1531 of up to 96 tokens 11 us).
 __global__ void __launch_bounds__(STEP_THREADS) step_kernel(StepArgs a) {
   extern __shared__ int32_t prefix[];  // starts [requests + 1], needs [requests + 1]
   __shared__ int64_t parts[STEP_THREADS / 64];

@@ -287,7 +287,10 @@ int64_t exl3_cache_attention_workspace(int64_t tokens, int q_heads, int kv_heads
  * contiguous. Query head h reads kv head h / (q_heads / kv_heads). Rows that
  * attend nothing and rows of no request are 0; positions whose table entry
  * names no page of the cache are not attended. max_new, the most new tokens of
- * a request, only chooses kernels: results depend on it in rounding at most. */
+ * a request, or a bound, only chooses kernels: results depend on it in rounding
+ * at most. Queries count with 22 bits, scores, maxima and sums are float32;
+ * weights count with 22 bits for requests of up to 16 rows to a kv head (their
+ * tokens times q_heads / kv_heads; 32 rows of head_dim 256), with 11 beyond. */
 int exl3_cache_attention(const void* q, int64_t q_token, int64_t q_head, void* out, int64_t tokens,
                          int q_heads, int type, const void* pages, int64_t num_pages, int page_size,
                          int kv_heads, int head_dim, const int32_t* tables, int width,
