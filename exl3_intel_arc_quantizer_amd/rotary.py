@@ -136,13 +136,15 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     None in the result. ``positions`` are int32 or int64 (tokens,),
     ``frequencies`` float64 of up to head_dim / 2 pairs: (i, i + pairs) for
     layout ``"half"``, (2 i, 2 i + 1) for ``"interleaved"``; the values past
-    the pairs are copied; frequencies have no gradient. Angles are taken in 64 bits and products in 32, so
-    positions in the millions are as exact as the first ones."""
+    the pairs are copied; frequencies have no gradient. Angles are taken in 64
+    bits and products in 32, so positions in the millions are as exact as the
+    first ones."""
     code = layout_code(layout)
     if isinstance(frequencies, torch.Tensor) and records(frequencies):
         raise RuntimeError("apply_rotary has no gradient of frequencies: detach them")
     recorded = records(q) or (k is not None and records(k))
-    if out is not None and (recorded or any(t is not None and records(t) for t in out)):
+    if out is not None and (recorded or any(isinstance(t, torch.Tensor) and records(t)
+                                            for t in out)):
         raise RuntimeError("apply_rotary: out cannot be given where torch records it or the inputs")
     if recorded:
         return _turned(q, k, positions, frequencies, code, magnitude, False)

@@ -42,6 +42,15 @@ def test_recorded_out_is_refused_before_any_device():
 
 
 @pytest.mark.gpu
+def test_out_that_is_no_tensor_is_refused():
+    q, at, freq = _given()
+    with pytest.raises(RuntimeError, match="out"):
+        apply_rotary(q, None, at, freq, out=([0.0], None))
+    with pytest.raises(RuntimeError, match="out"):
+        apply_rotary(q, q[:, :1].clone(), at, freq, out=(torch.empty_like(q), None))
+
+
+@pytest.mark.gpu
 def test_recorded_out_is_refused():
     q, k, at, freq, leaf = _refuses_recorded_out("cuda")
     with torch.no_grad():  # as torch's own in-place operations
