@@ -1000,9 +1000,19 @@ def shares_memory(a: tuple, b: tuple) -> bool:
     stride) in bytes) have a byte in common. Rows of one projection lie between
     each other without sharing any, so the ranges alone do not say; what the
     solver gives up on counts as shared."""
-    import numpy as np
-    if not all(a[1]) or not all(b[1]):
+    (at_a, shape_a, (token, head_a)), (at_b, shape_b, (token_b, head_b)) = a, b
+    if not (all(shape_a) and all(shape_b)):
         return False
+    # What a token's rows reach over: apart where ranges are, or (slices of one
+    # tensor) where the first token's are within a stride of tokens.
+    reach_a = (shape_a[1] - 1) * head_a + shape_a[2]
+    reach_b = (shape_b[1] - 1) * head_b + shape_b[2]
+    if (at_a + (shape_a[0] - 1) * token + reach_a <= at_b
+            or at_b + (shape_b[0] - 1) * token_b + reach_b <= at_a):
+        return False
+    if token and token == token_b and reach_a <= (at_b - at_a) % token <= token - reach_b:
+        return False
+    import numpy as np
     try:
         return np.shares_memory(np.asarray(_Span(*a)), np.asarray(_Span(*b)), max_work=10 ** 6)
     except np.exceptions.TooHardError:
@@ -1016,7 +1026,7 @@ def rows_are_apart(shape, strides) -> bool:
     reach = shape[2]
     if not all(shape):
         return True
-    for stride, n in sorted(zip(strides[:2], shape[:2])):
+    for stride, n in sorted(zip(strides, shape)):
         if n > 1:
             if stride < reach:
                 return False
@@ -1024,27 +1034,31 @@ def rows_are_apart(shape, strides) -> bool:
     return True
 
 
-def _check_outputs(inputs, outputs) -> None:
-    """The kernel's blocks run in any order, each reading and writing whole rows:
-    an output may be its input, and else shares no memory with any tensor of the
-    call."""
-    def span(t):
-        size = t.element_size()
-        return (t.data_ptr(), (*t.shape[:2], t.shape[2] * size), [n * size for n in t.stride()[:2]])
+def _check_outputs(size: int, *rows) -> None:
+    """Of (input, output), each an (address, shape, strides in elements of
+    ``size`` bytes): the kernel's blocks run in any order, each reading and
+    writing whole rows, so an output may be its input, and else shares no memory
+    with any tensor of the call."""
+    def span(address, shape, strides):
+        return (address, (shape[0], shape[1], shape[2] * size),
+                (strides[0] * size, strides[1] * size))
 
-    spans_in, spans_out = ([None if t is None else span(t) for t in ts] for ts in (inputs, outputs))
-    for i, own in enumerate(spans_out):
-        if own is None:
-            continue
-        if not rows_are_apart(own[1], own[2]):
-            raise RuntimeError(f"rows of out[{i}] share memory with each other")
-        for j, other in enumerate(spans_in):
-            same = i == j and own[:2] == other[:2] and all(
-                a == b for a, b, n in zip(own[2], other[2], own[1]) if n > 1)
-            if other is not None and not same and shares_memory(own, other):
-                raise RuntimeError(f"out[{i}] shares memory with {'qk'[j]}: it may be {'qk'[i]} "
-                                   "itself, or apart from both")
-    if None not in spans_out and shares_memory(*spans_out):
+    written, read = [], []
+    for given, out in rows:
+        out = span(*out)
+        if not rows_are_apart(*out[1:]):
+            raise RuntimeError(f"rows of out[{len(written)}] share memory with each other")
+        written.append(out)
+        given = span(*given)
+        (tokens, heads, _), (token, head), (to_token, to_head) = given[1], given[2], out[2]
+        if (given[0] != out[0] or (token != to_token and tokens > 1)
+                or (head != to_head and heads > 1)):
+            read.append(given)
+    for i, out in enumerate(written):
+        if any(shares_memory(out, given) for given in read):
+            raise RuntimeError(f"out[{i}] shares memory with q or k: outputs are the inputs "
+                               "themselves, or apart from both")
+    if len(written) == 2 and shares_memory(*written):
         raise RuntimeError("out[0] and out[1] share memory")
 
 
@@ -1072,7 +1086,10 @@ def rotary(q, k, positions, frequencies, layout: int, magnitude: float, inverse:
     else:
         k_out = None
     if out:
-        _check_outputs((q, k), (q_out, k_out))
+        at, shape = k_args[0], (tokens, heads, dim)
+        more = () if k is None else (((at, k.shape, sk), (k_args[3], k.shape, sp)),)
+        _check_outputs(q.element_size(), ((q.data_ptr(), shape, sq), (q_out.data_ptr(), shape, so)),
+                       *more)
     _run(device, "apply_rotary", load_library().exl3_rotary, q.data_ptr(), sq[0], sq[1],
          q_out.data_ptr(), so[0], so[1], heads, *k_args, tokens, dim, _types()[q.dtype],
          positions.data_ptr(), positions.dtype == torch.int64, frequencies.data_ptr(), pairs,
