@@ -78,6 +78,9 @@ _SIGNATURES = {
     "exl3_block_fold": (_c_int, [_c_vp, _c_vp, _c_vp, _c_i64, _c_vp]),
     "exl3_ldlq_gather": (_c_int, [_c_vp, _c_int, _c_i64, _c_vp, _c_vp]),
     "exl3_ldlq_scatter": (_c_int, [_c_vp, _c_int, _c_i64, _c_vp, _c_vp, _c_vp]),
+    "exl3_linear_workspace": (_c_i64, [_c_i64, _c_i64, _c_i64]),
+    "exl3_linear": (_c_int, [_c_vp, _c_i64, _c_i64, _c_int, _c_vp, _c_vp, _c_vp, _c_int, _c_i64,
+                             _c_i64, _c_int, _c_int, _c_vp, _c_vp, _c_i64, _c_vp]),
     # the attention cache of include/exl3_layer.h
     "exl3_rotary": (_c_int, [_c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_int,
                              _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_int, _c_i64,
@@ -1221,4 +1224,55 @@ def cache_attention(q, pages, tables, starts, lengths, scale, window, max_new):
          out.data_ptr(), tokens, q_heads, _types()[q.dtype], pages.data_ptr(), n, page_size, heads,
          dim, tables.data_ptr(), width, starts.data_ptr(), lengths.data_ptr(), requests,
          dim ** -0.5 if scale is None else float(scale), window, most, workspace.data_ptr(), size)
+    return out
+
+
+# ------------------------------------------------- products with stored weights
+
+def linear(x, trellis, su, sv, K: int, cb: int):
+    """x (..., in) times a stored weight (exl3_linear)."""
+    torch = _torch()
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() < 1:
+        raise RuntimeError("x must be a GPU (cuda) tensor (..., in)")
+    if x.dtype != torch.float16 and x.dtype != torch.bfloat16:
+        raise RuntimeError(f"x must be float16 or bfloat16, got {x.dtype}")
+    device = x.device
+    if not 1 <= K <= 8:
+        raise ValueError(f"K must be in 1..8, got {K}")
+    if cb not in (0, 1, 2):
+        raise ValueError(f"Unknown codebook {cb}")
+    if (not isinstance(trellis, torch.Tensor) or trellis.dtype != torch.int16 or trellis.dim() != 3
+            or not trellis.is_contiguous() or trellis.device != device):
+        raise RuntimeError(f"trellis must be a contiguous 3-D int16 tensor on {device}")
+    tk, tn, words = trellis.shape
+    if words != 16 * K:
+        raise ValueError(f"Trellis last dimension {words} does not match 16 * K = {16 * K}")
+    k, n = 16 * tk, 16 * tn
+    if k % 128 or n % 128 or not k or not n:
+        raise ValueError(f"both dimensions must be divisible by 128, got {(k, n)}")
+    shape = x.shape
+    if shape[-1] != k:
+        raise ValueError(f"x must have {k} input channels, got {tuple(shape)}")
+    scales = (torch.float16, torch.float32)
+    _vector(su, "suh", scales, k, device)
+    _vector(sv, "svh", scales, n, device)
+    # The kernel reads 16 bytes at a time; rows that start elsewhere are copied.
+    rows = x if x.dim() == 2 else x.reshape(-1, k)
+    stride = rows.stride()
+    if stride[1] != 1 or stride[0] % 8 or stride[0] < 0 or rows.data_ptr() % 16:
+        rows = rows.clone(memory_format=torch.contiguous_format)
+        stride = rows.stride()
+    if trellis.data_ptr() % 4:
+        trellis = trellis.clone()
+    count = rows.shape[0]
+    lib = load_library()
+    size = lib.exl3_linear_workspace(count, k, n)
+    if size < 0:
+        raise RuntimeError(f"quantized_linear: {count} rows of {k} by {n} are too many")
+    out = x.new_empty((*shape[:-1], n))
+    workspace = trellis.new_empty(size // 2)
+    _run(device, "quantized_linear", lib.exl3_linear, rows.data_ptr(), stride[0], count,
+         _types()[x.dtype], trellis.data_ptr(), su.data_ptr(), sv.data_ptr(),
+         (su.dtype == torch.float16) + 2 * (sv.dtype == torch.float16), k, n, K, cb,
+         out.data_ptr(), workspace.data_ptr(), size)
     return out

@@ -203,6 +203,24 @@ int exl3_ldlq_gather(const exl3_ldlq_block* blocks, int nblocks, int64_t tiles, 
 int exl3_ldlq_scatter(const exl3_ldlq_block* blocks, int nblocks, int64_t tiles,
                       const float* recon, const int16_t* idx, void* stream);
 
+/* ---- Products with weights as they are stored (no counterpart in the
+ * reference). ---- */
+
+/* Bytes of workspace that exl3_linear needs for `rows` rows of a (k, n) weight,
+ * or -1 where it takes no such sizes. */
+int64_t exl3_linear_workspace(int64_t rows, int64_t k, int64_t n);
+
+/* out (rows, n) = x W, W the (k, n) weight that exl3_decode_weight decodes from
+ * `words` (k / 16 x n / 16 tiles of 16 K) with input scales su and output
+ * scales sv: y = ((x su) H W_tiles) H sv. Rows of x are `stride` elements apart,
+ * type 1 float16 or 2 bfloat16, as is out. half_scales: bit 0 if su, bit 1 if sv
+ * is float16, else float32. Rows are transformed in float32 and count with 22
+ * bits, sums are float32. Rows with a value that is not finite are NaN. k and n
+ * are multiples of 128; x, out and the workspace 16-byte aligned. */
+int exl3_linear(const void* x, int64_t stride, int64_t rows, int type, const uint16_t* words,
+                const void* su, const void* sv, int half_scales, int64_t k, int64_t n, int K,
+                int cb, void* out, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- The 4-bit attention cache of a served model (no counterpart in the
  * reference). Element types: 0 float32, 1 float16, 2 bfloat16. Rows are
  * (tokens, heads, head_dim) tensors whose last axis is contiguous, given by
