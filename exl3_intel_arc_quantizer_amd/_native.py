@@ -78,7 +78,7 @@ _SIGNATURES = {
     "exl3_block_fold": (_c_int, [_c_vp, _c_vp, _c_vp, _c_i64, _c_vp]),
     "exl3_ldlq_gather": (_c_int, [_c_vp, _c_int, _c_i64, _c_vp, _c_vp]),
     "exl3_ldlq_scatter": (_c_int, [_c_vp, _c_int, _c_i64, _c_vp, _c_vp, _c_vp]),
-    "exl3_linear_workspace": (_c_i64, [_c_i64, _c_i64, _c_i64]),
+    "exl3_linear_workspace": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_int]),
     "exl3_linear": (_c_int, [_c_vp, _c_i64, _c_i64, _c_int, _c_vp, _c_vp, _c_vp, _c_int, _c_i64,
                              _c_i64, _c_int, _c_int, _c_vp, _c_vp, _c_i64, _c_vp]),
     # the attention cache of include/exl3_layer.h
@@ -1266,13 +1266,14 @@ def linear(x, trellis, su, sv, K: int, cb: int):
         trellis = trellis.clone()
     count = rows.shape[0]
     lib = load_library()
-    size = lib.exl3_linear_workspace(count, k, n)
+    code = _types()[x.dtype]
+    size = lib.exl3_linear_workspace(count, k, n, code)
     if size < 0:
         raise RuntimeError(f"quantized_linear: {count} rows of {k} by {n} are too many")
     out = x.new_empty((*shape[:-1], n))
     workspace = trellis.new_empty(size // 2)
     _run(device, "quantized_linear", lib.exl3_linear, rows.data_ptr(), stride[0], count,
-         _types()[x.dtype], trellis.data_ptr(), su.data_ptr(), sv.data_ptr(),
+         code, trellis.data_ptr(), su.data_ptr(), sv.data_ptr(),
          (su.dtype == torch.float16) + 2 * (sv.dtype == torch.float16), k, n, K, cb,
          out.data_ptr(), workspace.data_ptr(), size)
     return out

@@ -26,6 +26,7 @@ using exl3::set_error;
 namespace {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -66,56 +67,86 @@ struct Scales {
 // The order of a step of 32 input channels: quarter q of a wave's lanes holds
 // channels 2 q, 2 q + 1, 2 q + 8, 2 q + 9 of both tiles of 16, which are four
 // states next to each other in each tile, a lane's own operand of the decoded
-// weights. So z, the transformed rows, lies as [step][set][q][16 columns][8].
-// Sets are 16 columns: of up to 8 rows one, float16 parts in columns 0..7 and
-// what they leave in 8..15; else two for 16 rows.
+// weights. So z, the transformed rows, lies as [block of rows][step][set][q]
+// [16 columns][8]. A set is 16 columns: of up to 8 rows there is one, float16
+// parts in columns 0..7 and what they leave in 8..15; else one or (with that
+// rest) two for 16 rows.
 struct TurnArgs {
   const uint16_t* x;
   int64_t stride;
-  Scales su;
+  const void* su;
   u32x4* z;
   float* scale;                    // [rows]: what z is multiplied by
-  int rows, k, sets;               // sets of all rows: 1, or 2 for each 16
+  int half, k, sets, block_rows;   // of a block of rows
+  int rest;                        // where the rest lies behind a value, 0 for none
 };
+
+// Channels 2 q, 2 q + 1 of the 16 halves of tiles of a block of 128, times su.
+template <bool BF16>
+__device__ __forceinline__ void load_unit(const TurnArgs& a, const uint16_t* x, int at, float (&v)[32]) {
+  uint32_t w[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) w[i] = *reinterpret_cast<const uint32_t*>(x + at + 8 * i);
+  if (a.half) {
+    uint32_t s[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.su) + at + 8 * i);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      v[2 * i] = widen<BF16>(w[i] & 0xffffu) * widen<false>(s[i] & 0xffffu);
+      v[2 * i + 1] = widen<BF16>(w[i] >> 16) * widen<false>(s[i] >> 16);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const f32x2 s = *reinterpret_cast<const f32x2*>(static_cast<const float*>(a.su) + at + 8 * i);
+      v[2 * i] = widen<BF16>(w[i] & 0xffffu) * s[0];
+      v[2 * i + 1] = widen<BF16>(w[i] >> 16) * s[1];
+    }
+  }
+}
+
+// The largest magnitude as bits: NaN above infinity above all numbers.
+__device__ __forceinline__ uint32_t top_of(const float (&v)[32]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu);
+  return top;
+}
 
 // A row is held as 2^p (hi + lo), both float16, with p from the bound
 // |z| <= sqrt(128) max |x su|: 22 bits of a value, and places down to 2^-39 of
 // the row's largest one, so the products are as exact as float32 makes them.
-// A quad of lanes takes a block of 128: two levels across its lanes, five within
-// one. A row with an infinity or a NaN is all NaN.
+// A workgroup takes a row, a quad of lanes a block of 128: two levels across its
+// lanes, five within one. A row with an infinity or a NaN is all NaN.
 template <bool BF16>
-__global__ void __launch_bounds__(256) linear_turn_kernel(TurnArgs a) {
-  __shared__ uint32_t tops[4];
-  const int row = blockIdx.x, tid = threadIdx.x, q = tid & 3;
+__global__ void __launch_bounds__(1024) linear_turn_kernel(TurnArgs a) {
+  __shared__ uint32_t tops[16];
+  const int row = blockIdx.x, tid = threadIdx.x, q = tid & 3, units = a.k / HAD, step = blockDim.x / 4;
   const uint16_t* x = a.x + row * a.stride;
-  uint32_t top = 0;                // of magnitudes as bits: NaN above infinity above all else
-  for (int i = tid; i < a.k / 8; i += 256) {
-    const u32x4 w = reinterpret_cast<const u32x4*>(x)[i];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float v = widen<BF16>(w[e / 2] >> (16 * (e & 1)) & 0xffffu) * a.su.at(8 * i + e);
-      top = max(top, __builtin_bit_cast(uint32_t, v) & 0x7fffffffu);
-    }
+  float v[32];
+  uint32_t top = 0;
+  int held = tid >> 2;
+  for (int unit = tid >> 2; unit < units; unit += step) {
+    load_unit<BF16>(a, x, HAD * unit + 2 * q, v);
+    top = max(top, top_of(v));
+    held = unit;
   }
 #pragma unroll
   for (int o = 1; o < 64; o *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, o));
   if ((tid & 63) == 0) tops[tid >> 6] = top;
   __syncthreads();
-  top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
-  // 2^11 > sqrt(128) 2^7.5 ... z stays below 2^15.
+  for (int i = 0; i < (int)blockDim.x / 64; ++i) top = max(top, tops[i]);
+  // The row's values are under 2^11, those of z under 2^15.
   const bool finite = top < 0x7f800000u;
   const int power = max((int)(top >> 23), 1) - 126 - 11;
   if (tid == 0) a.scale[row] = finite ? ldexpf(1.0f, power) : __builtin_nanf("");
-  const int m = a.sets == 1 ? row : row & 15, set0 = a.sets == 1 ? 0 : row / 16 * 2;
-  for (int unit = tid >> 2; unit < a.k / HAD; unit += 64) {
-    float v[32];                   // [step 4][tile 2][half 2][2]: channels 32 step + 16 tile + 8 half + 2 q + e
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int at = HAD * unit + 8 * i + 2 * q;
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(x + at);
-      v[2 * i] = widen<BF16>(w & 0xffffu) * a.su.at(at);
-      v[2 * i + 1] = widen<BF16>(w >> 16) * a.su.at(at + 1);
-    }
+  const int block = row / a.block_rows, in_block = row - block * a.block_rows;
+  u32x4* out = a.z + (int64_t)block * (a.k / 32) * a.sets * 64 + q * 16 + (in_block & 15) +
+               (a.rest == 64 ? 128 : 64) * (in_block >> 4);
+  // From the last unit on, which is still held.
+  for (int unit = held; unit >= 0 && unit < units; unit -= step) {
+    if (unit != held) load_unit<BF16>(a, x, HAD * unit + 2 * q, v);
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = ldexpf(v[i], -power);
 #pragma unroll
@@ -138,9 +169,9 @@ __global__ void __launch_bounds__(256) linear_turn_kernel(TurnArgs a) {
         hi[e] = __builtin_bit_cast(uint32_t, f16x2{hy, hw});
         lo[e] = pair_of(y - (float)hy, w - (float)hw);
       }
-      u32x4* z = a.z + ((int64_t)(4 * unit + s) * a.sets + set0) * 64 + q * 16 + m;
+      u32x4* z = out + (int64_t)(4 * unit + s) * a.sets * 64;
       z[0] = hi;
-      z[a.sets == 1 ? 8 : 64] = lo;
+      if (a.rest) z[a.rest] = lo;
     }
   }
 }
@@ -151,8 +182,29 @@ struct LinearArgs {
   const uint32_t* words;
   const u32x4* z;
   float* partials;                 // [split][rows][n]
-  int rows, k, n, bits, splits, sets;
+  const float* scale;              // of the rows
+  Scales sv;
+  uint16_t* out;
+  int rows, k, n, bits, splits;
 };
+
+// One butterfly level between lanes 16 or 32 apart, for two registers at once:
+// the first swap brings the halves of a pair together, the second puts sums
+// and differences back in their lanes.
+template <int APART>
+__device__ __forceinline__ void lane_butterfly(float& x, float& y) {
+  auto swap = [](float& a, float& b) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, a), v = __builtin_bit_cast(uint32_t, b);
+    const auto r = APART == 16 ? __builtin_amdgcn_permlane16_swap(u, v, false, false)
+                               : __builtin_amdgcn_permlane32_swap(u, v, false, false);
+    const uint32_t r0 = r[0], r1 = r[1];
+    a = __builtin_bit_cast(float, r0), b = __builtin_bit_cast(float, r1);
+  };
+  swap(x, y);
+  const float sum = x + y, difference = x - y;
+  x = sum, y = difference;
+  swap(x, y);
+}
 
 // The hash of a state, s M + A. A state has 16 bits: two 24-bit products, which
 // run at full rate where a 32-bit one takes four times as long. (The empty asm
@@ -201,21 +253,41 @@ struct Words {
   uint32_t w[CT][2][WIDE ? 4 : 2];
 };
 
-template <bool WIDE, int CB, int SETS, int CT, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES) linear_kernel(LinearArgs a) {
-  constexpr int ACCS = SETS == 1 ? 1 : SETS / 2;
-  __shared__ f32x4 sums[WAVES][CT * ACCS][64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n = lane & 15, q = lane >> 4;
-  const int tiles_n = a.n / 16, column0 = blockIdx.x * CT, split = blockIdx.y, block = blockIdx.z;
-  const int steps = a.k / 32, parts = a.splits * WAVES, part = split * WAVES + wave;
-  const int begin = (int)((int64_t)steps * part / parts), end = (int)((int64_t)steps * (part + 1) / parts);
-  const int u = 8 * (n & 7) + 2 * q + (n >> 3), bits = a.bits;
-  const Window late = window_of(4 * bits * (u + 1), bits), early = window_of(4 * bits * u + 2 * bits, bits);
+// The four values of a lane's states, of both tiles of a step: its operand.
+template <bool WIDE, int CB>
+__device__ __forceinline__ u32x4 operand_of(const uint32_t (&w)[2][WIDE ? 4 : 2], const Window& late, const Window& early, uint32_t bits) {
+  u32x4 f;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const uint32_t v = __builtin_amdgcn_alignbit(w[t][0], w[t][1], late.shift);
+    const uint32_t s3 = v & 0xffffu, s2 = __builtin_amdgcn_ubfe(v, bits, 16);
+    uint32_t s1, s0;
+    if constexpr (WIDE) {
+      const uint32_t e = __builtin_amdgcn_alignbit(w[t][2], w[t][3], early.shift);
+      s1 = e & 0xffffu, s0 = __builtin_amdgcn_ubfe(e, bits, 16);
+    } else {
+      s1 = __builtin_amdgcn_ubfe(v, 2 * bits, 16), s0 = __builtin_amdgcn_ubfe(v, 3 * bits, 16);
+    }
+    f[2 * t] = values_of<CB>(s0, s1);
+    f[2 * t + 1] = values_of<CB>(s2, s3);
+  }
+  return f;
+}
 
-  const int64_t row_bytes = (int64_t)tiles_n * 32 * bits;
-  const char* next = reinterpret_cast<const char*>(a.words) + 2 * begin * row_bytes + (int64_t)column0 * 32 * bits;
-  auto load = [&]() __attribute__((always_inline)) {
+// A wave's column tiles, read step by step.
+template <bool WIDE, int CT>
+struct Reader {
+  const char* next;                // uniform
+  int64_t row_bytes;
+  Window late, early;
+  uint32_t bits;
+  __device__ __forceinline__ Reader(const LinearArgs& a, int step, int column, int lane) : bits(a.bits) {
+    const int n = lane & 15, q = lane >> 4, u = 8 * (n & 7) + 2 * q + (n >> 3);
+    late = window_of(4 * bits * (u + 1), bits), early = window_of(4 * bits * u + 2 * bits, bits);
+    row_bytes = (int64_t)(a.n / 16) * 32 * bits;
+    next = reinterpret_cast<const char*>(a.words) + 2 * step * row_bytes + (int64_t)column * 32 * bits;
+  }
+  __device__ __forceinline__ Words<WIDE, CT> load() {
     Words<WIDE, CT> r;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -228,67 +300,177 @@ __global__ void __launch_bounds__(64 * WAVES) linear_kernel(LinearArgs a) {
       }
     next += 2 * row_bytes;
     return r;
-  };
-  f32x4 acc[CT][ACCS];
+  }
+};
+
+// Up to 16 rows: every wave takes CT column tiles and its share of the input
+// channels; a workgroup's waves add up in shared memory.
+template <bool WIDE, int CB, int SETS, int CT, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) linear_kernel(LinearArgs a) {
+  __shared__ f32x4 sums[WAVES][CT][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int column0 = blockIdx.x * CT, split = blockIdx.y;
+  const int steps = a.k / 32, parts = a.splits * WAVES, part = split * WAVES + wave;
+  const int begin = (int)((int64_t)steps * part / parts), end = (int)((int64_t)steps * (part + 1) / parts);
+  Reader<WIDE, CT> reader(a, begin, column0, lane);
+  f32x4 acc[CT];
 #pragma unroll
-  for (int c = 0; c < CT; ++c)
-#pragma unroll
-    for (int m = 0; m < ACCS; ++m) acc[c][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int c = 0; c < CT; ++c) acc[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
   auto multiply = [&](const Words<WIDE, CT>& r, int step) __attribute__((always_inline)) {
-    const u32x4* z = a.z + ((int64_t)step * a.sets + block * SETS) * 64 + lane;
+    const u32x4* z = a.z + (int64_t)step * SETS * 64 + lane;
     u32x4 b[SETS];
 #pragma unroll
     for (int s = 0; s < SETS; ++s) b[s] = z[s * 64];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
-      u32x4 f;
+      const u32x4 f = operand_of<WIDE, CB>(r.w[c], reader.late, reader.early, reader.bits);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const uint32_t v = __builtin_amdgcn_alignbit(r.w[c][t][0], r.w[c][t][1], late.shift);
-        const uint32_t s3 = v & 0xffffu, s2 = __builtin_amdgcn_ubfe(v, bits, 16);
-        uint32_t s1, s0;
-        if constexpr (WIDE) {
-          const uint32_t e = __builtin_amdgcn_alignbit(r.w[c][t][2], r.w[c][t][3], early.shift);
-          s1 = e & 0xffffu, s0 = __builtin_amdgcn_ubfe(e, bits, 16);
-        } else {
-          s1 = __builtin_amdgcn_ubfe(v, 2 * bits, 16), s0 = __builtin_amdgcn_ubfe(v, 3 * bits, 16);
-        }
-        f[2 * t] = values_of<CB>(s0, s1);
-        f[2 * t + 1] = values_of<CB>(s2, s3);
-      }
-#pragma unroll
-      for (int s = 0; s < SETS; ++s) acc[c][s / 2] = mfma(f, b[s], acc[c][s / 2]);
+      for (int s = 0; s < SETS; ++s) acc[c] = mfma(f, b[s], acc[c]);
     }
   };
 
   if (begin < end) {
-    Words<WIDE, CT> even = load(), odd = even;
+    Words<WIDE, CT> even = reader.load(), odd = even;
     for (int step = begin; step < end; step += 2) {
-      if (step + 1 < end) odd = load();
+      if (step + 1 < end) odd = reader.load();
       multiply(even, step);
       if (step + 1 == end) break;
-      if (step + 2 < end) even = load();
+      if (step + 2 < end) even = reader.load();
       multiply(odd, step + 1);
     }
   }
 #pragma unroll
-  for (int c = 0; c < CT; ++c)
-#pragma unroll
-    for (int m = 0; m < ACCS; ++m) sums[wave][c * ACCS + m][lane] = acc[c][m];
+  for (int c = 0; c < CT; ++c) sums[wave][c][lane] = acc[c];
   __syncthreads();
-  for (int i = tid; i < CT * ACCS * 64; i += 64 * WAVES) {
-    const int of = i >> 6, l = i & 63, c = of / ACCS, m = of % ACCS;
+  for (int i = tid; i < CT * 64; i += 64 * WAVES) {
+    const int c = i >> 6, l = i & 63;
     if (SETS == 1 && (l & 8)) continue;
-    f32x4 v = sums[0][of][l];
+    f32x4 v = sums[0][c][l];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) v += sums[w][of][l];
+    for (int w = 1; w < WAVES; ++w) v += sums[w][c][l];
     if constexpr (SETS == 1)
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) v += sums[w][of][l + 8];
-    const int row = block * 16 * ACCS + 16 * m + (l & 15), column = 16 * (column0 + c) + 4 * (l >> 4);
-    if (row < a.rows && column < a.n)
+      for (int w = 0; w < WAVES; ++w) v += sums[w][c][l + 8];
+    const int row = l & 15, column = 16 * (column0 + c) + 4 * (l >> 4);
+    if (row < a.rows)
       *reinterpret_cast<f32x4*>(a.partials + ((int64_t)split * a.rows + row) * a.n + column) = v;
+  }
+}
+
+// More rows: a workgroup takes a block of 16 MT rows and, four waves, 64 CT
+// columns of a share of the input channels. The rows come through shared memory,
+// two buffers of STEPS steps, for all waves; each decodes its own columns. Blocks
+// with all channels (splits == 1) are finished here: a lane holds channels 4 (lane
+// / 16) .. + 3 of its tiles, so of the output's transform two levels lie in a
+// lane's registers, two across lanes, two across its CT = 4 tiles, and one across
+// two waves.
+template <bool WIDE, int CB, bool BF16, int MT, int PARTS, int CT>
+__global__ void __launch_bounds__(256, 2) linear_tiles_kernel(LinearArgs a) {
+  constexpr int SETS = MT * PARTS, STEPS = SETS > 8 ? 2 : 4, STAGE = STEPS * SETS * 64;  // vectors of a buffer
+  __shared__ u32x4 held[2 * STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int column0 = (blockIdx.x * 4 + wave) * CT, split = blockIdx.y, block = blockIdx.z;
+  const int stages = a.k / (32 * STEPS);
+  const int begin = (int)((int64_t)stages * split / a.splits), end = (int)((int64_t)stages * (split + 1) / a.splits);
+  const bool there = column0 < a.n / 16;                 // (a wave past the columns reads the first ones)
+  Reader<WIDE, CT> reader(a, begin * STEPS, there ? column0 : 0, lane);
+  const u32x4* z = a.z + ((int64_t)block * (a.k / 32) + begin * STEPS) * SETS * 64;
+  f32x4 acc[CT][MT];
+#pragma unroll
+  for (int c = 0; c < CT; ++c)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[c][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  auto fetch = [&](int buffer) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < STAGE / 256; ++i)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(z + i * 256 + tid),
+                                       (__attribute__((address_space(3))) void*)(held + buffer * STAGE + i * 256 + wave * 64), 16, 0, 0);
+    z += STAGE;
+  };
+  if (begin < end) {
+    fetch(0);
+    Words<WIDE, CT> words = reader.load();
+    for (int stage = begin; stage < end; ++stage) {
+      const int now = (stage - begin) & 1;
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // of the rows that this wave fetched
+      __syncthreads();
+      if (stage + 1 < end) fetch(now ^ 1);
+#pragma unroll
+      for (int step = 0; step < STEPS; ++step) {
+        const Words<WIDE, CT> these = words;
+        if (step + 1 < STEPS || stage + 1 < end) words = reader.load();
+        u32x4 f[CT];
+#pragma unroll
+        for (int c = 0; c < CT; ++c) f[c] = operand_of<WIDE, CB>(these.w[c], reader.late, reader.early, reader.bits);
+#pragma unroll
+        for (int s = 0; s < SETS; ++s) {
+          const u32x4 b = held[now * STAGE + (step * SETS + s) * 64 + lane];
+#pragma unroll
+          for (int c = 0; c < CT; ++c) acc[c][s / PARTS] = mfma(f[c], b, acc[c][s / PARTS]);
+        }
+      }
+    }
+  }
+  const int row0 = block * 16 * MT + (lane & 15);
+  if (CT != 4 || a.splits > 1) {
+    if (!there) return;
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const int row = row0 + 16 * m, column = 16 * (column0 + c) + 4 * (lane >> 4);
+        if (row < a.rows) *reinterpret_cast<f32x4*>(a.partials + ((int64_t)split * a.rows + row) * a.n + column) = acc[c][m];
+      }
+    return;
+  }
+  if constexpr (CT == 4) {
+    f32x4* exchange = reinterpret_cast<f32x4*>(held);
+    constexpr int AT_ONCE = 2 * STAGE / (4 * CT * 64) < MT ? 2 * STAGE / (4 * CT * 64) : MT;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        f32x4& v = acc[c][m];
+        const float s0 = v[0] + v[1], s1 = v[0] - v[1], s2 = v[2] + v[3], s3 = v[2] - v[3];
+        float y[4] = {s0 + s2, s1 + s3, s0 - s2, s1 - s3};
+        lane_butterfly<16>(y[0], y[1]);
+        lane_butterfly<16>(y[2], y[3]);
+        lane_butterfly<32>(y[0], y[1]);
+        lane_butterfly<32>(y[2], y[3]);
+        v = f32x4{y[0], y[1], y[2], y[3]};
+      }
+      f32x4 s0 = acc[0][m] + acc[1][m], s1 = acc[0][m] - acc[1][m], s2 = acc[2][m] + acc[3][m], s3 = acc[2][m] - acc[3][m];
+      acc[0][m] = s0 + s2, acc[1][m] = s1 + s3, acc[2][m] = s0 - s2, acc[3][m] = s1 - s3;
+    }
+#pragma unroll
+    for (int m0 = 0; m0 < MT; m0 += AT_ONCE) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) exchange[((wave * AT_ONCE + i) * CT + c) * 64 + lane] = acc[c][m0 + i];
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const int row = row0 + 16 * (m0 + i);
+        const bool writes = there && row < a.rows;
+        const float scale = writes ? a.scale[row] * ROOT : 0.0f;
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          const int column = 16 * (column0 + c) + 4 * (lane >> 4);
+          const f32x4 other = exchange[(((wave ^ 1) * AT_ONCE + i) * CT + c) * 64 + lane];
+          const f32x4 v = wave & 1 ? other - acc[c][m0 + i] : acc[c][m0 + i] + other;
+          if (writes) {
+            u32x2 w;
+            w[0] = narrow<BF16>(v[0] * scale * a.sv.at(column)) | narrow<BF16>(v[1] * scale * a.sv.at(column + 1)) << 16;
+            w[1] = narrow<BF16>(v[2] * scale * a.sv.at(column + 2)) | narrow<BF16>(v[3] * scale * a.sv.at(column + 3)) << 16;
+            *reinterpret_cast<u32x2*>(a.out + (int64_t)row * a.n + column) = w;
+          }
+        }
+      }
+    }
   }
 }
 
@@ -334,51 +516,81 @@ __global__ void __launch_bounds__(256) linear_join_kernel(JoinArgs a) {
 
 // ------------------------------------------------------------ plan
 
+// Variants by the rows.
+enum Variant { ROWS8, ROWS16, BLOCK32, BLOCK64, BLOCK128 };
+
 // How a call is cut.
 struct Plan {
-  int sets, blocks;                // of columns of z in all; row blocks of a launch
-  int columns, waves, groups;      // column tiles of a wave, waves, column groups
-  int splits;
+  Variant variant;
+  int parts;                       // float16 parts of a value: 2, or 1 in blocks of 128 bfloat16 rows
+  int block_rows, blocks, sets;    // rows of a block, blocks, sets of a block
+  int groups, splits;              // column groups, shares of the input channels
   int64_t z_bytes, scale_bytes, partial_bytes;
 };
 
 constexpr int CUS = 256;
 
-Plan plan_of(int64_t rows, int64_t k, int64_t n) {
+Plan plan_of(int64_t rows, int64_t k, int64_t n, bool bf16) {
   Plan p{};
-  const int sets = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 ? 4 : 8;  // of a row block
-  p.blocks = sets <= 2 ? 1 : (int)((rows + 8 * sets - 1) / (8 * sets));
-  p.sets = sets * p.blocks;
-  p.columns = sets <= 2 ? 2 : 4;
-  p.waves = sets <= 2 ? 8 : 4;
-  p.groups = (int)((n / 16 + p.columns - 1) / p.columns);
-  const int64_t want = (int64_t)2 * CUS * 8 / p.waves;
-  const int64_t most = std::max<int64_t>(1, k / 32 / (2 * p.waves));
-  p.splits = (int)std::min(most, std::max<int64_t>(1, (want + (int64_t)p.groups * p.blocks - 1) / ((int64_t)p.groups * p.blocks)));
-  p.z_bytes = k / 32 * p.sets * 1024;
+  p.variant = rows <= 8 ? ROWS8 : rows <= 16 ? ROWS16 : rows <= 32 ? BLOCK32 : rows <= 64 ? BLOCK64 : BLOCK128;
+  p.parts = p.variant == BLOCK128 && bf16 ? 1 : 2;
+  p.block_rows = 8 << p.variant;
+  p.blocks = (int)((rows + p.block_rows - 1) / p.block_rows);
+  p.sets = p.block_rows * p.parts / 16;
+  int64_t most, want;              // splits: at most, workgroups that fill the chip
+  if (p.variant <= ROWS16) {
+    p.groups = (int)(n / 32);
+    most = std::max<int64_t>(1, k / 512), want = 2 * CUS;
+  } else {
+    const int columns = p.variant == BLOCK128 ? 256 : 128;
+    p.groups = (int)((n + columns - 1) / columns);
+    most = k / HAD, want = 2 * CUS;
+  }
+  p.splits = (int)std::min(most, std::max<int64_t>(1, want / ((int64_t)p.groups * p.blocks)));
+  p.z_bytes = k / 32 * p.sets * 1024 * p.blocks;
   p.scale_bytes = (4 * rows + 15) & ~(int64_t)15;
-  p.partial_bytes = 4 * (int64_t)p.splits * rows * n;
+  const bool direct = p.variant == BLOCK128 && p.splits == 1;
+  p.partial_bytes = direct ? 0 : 4 * (int64_t)p.splits * rows * n;
   return p;
 }
 
-template <bool WIDE, int CB>
+template <bool WIDE, int CB, bool BF16>
 void launch_product(const Plan& p, const LinearArgs& a, hipStream_t stream) {
   const dim3 grid(p.groups, p.splits, p.blocks);
-  switch (p.sets / p.blocks) {
-    case 1: linear_kernel<WIDE, CB, 1, 2, 8><<<grid, 512, 0, stream>>>(a); break;
-    case 2: linear_kernel<WIDE, CB, 2, 2, 8><<<grid, 512, 0, stream>>>(a); break;
-    case 4: linear_kernel<WIDE, CB, 4, 4, 4><<<grid, 256, 0, stream>>>(a); break;
-    default: linear_kernel<WIDE, CB, 8, 4, 4><<<grid, 256, 0, stream>>>(a); break;
+  switch (p.variant) {
+    case ROWS8: linear_kernel<WIDE, CB, 1, 2, 8><<<grid, 512, 0, stream>>>(a); break;
+    case ROWS16: linear_kernel<WIDE, CB, 2, 2, 8><<<grid, 512, 0, stream>>>(a); break;
+    case BLOCK32: linear_tiles_kernel<WIDE, CB, false, 2, 2, 2><<<grid, 256, 0, stream>>>(a); break;
+    case BLOCK64: linear_tiles_kernel<WIDE, CB, false, 4, 2, 2><<<grid, 256, 0, stream>>>(a); break;
+    case BLOCK128: linear_tiles_kernel<WIDE, CB, BF16, 8, BF16 ? 1 : 2, 4><<<grid, 256, 0, stream>>>(a); break;
   }
+}
+
+template <bool BF16>
+int launch_linear(const Plan& p, const TurnArgs& t, const LinearArgs& a, int cb, hipStream_t s) {
+  const int threads = t.k <= 8192 ? 256 : t.k <= 16384 ? 512 : 1024;
+  linear_turn_kernel<BF16><<<(unsigned)a.rows, threads, 0, s>>>(t);
+  if (check_launch("exl3_linear")) return 1;
+  if (a.bits > 5)
+    cb == 0 ? launch_product<true, 0, BF16>(p, a, s) : cb == 1 ? launch_product<true, 1, BF16>(p, a, s) : launch_product<true, 2, BF16>(p, a, s);
+  else
+    cb == 0 ? launch_product<false, 0, BF16>(p, a, s) : cb == 1 ? launch_product<false, 1, BF16>(p, a, s) : launch_product<false, 2, BF16>(p, a, s);
+  if (check_launch("exl3_linear")) return 1;
+  if (!p.partial_bytes) return 0;
+  JoinArgs j{};
+  j.partials = a.partials, j.scale = a.scale, j.sv = a.sv, j.out = a.out, j.rows = a.rows, j.n = a.n, j.splits = p.splits;
+  const int64_t units = (int64_t)a.rows * (a.n / HAD);
+  linear_join_kernel<BF16><<<(unsigned)((units + 15) / 16), 256, 0, s>>>(j);
+  return check_launch("exl3_linear");
 }
 
 }  // namespace
 
 extern "C" {
 
-int64_t exl3_linear_workspace(int64_t rows, int64_t k, int64_t n) {
-  if (rows < 0 || rows > INT32_MAX || k < HAD || n < HAD || k % HAD || n % HAD || k > 1 << 24 || n > 1 << 24) return -1;
-  const Plan p = plan_of(rows, k, n);
+int64_t exl3_linear_workspace(int64_t rows, int64_t k, int64_t n, int type) {
+  if (rows < 0 || rows > 1 << 22 || k < HAD || n < HAD || k % HAD || n % HAD || k > 1 << 24 || n > 1 << 24) return -1;
+  const Plan p = plan_of(rows, k, n, type == 2);
   return p.z_bytes + p.scale_bytes + p.partial_bytes;
 }
 
@@ -388,43 +600,28 @@ int exl3_linear(const void* x, int64_t stride, int64_t rows, int type, const uin
   if (K < 1 || K > 8) return set_error("exl3_linear: K must be in 1..8, got %d", K);
   if (cb < 0 || cb > 2) return set_error("exl3_linear: cb must be 0, 1, or 2, got %d", cb);
   if (type < 1 || type > 2) return set_error("exl3_linear: rows are float16 or bfloat16");
-  const int64_t need = exl3_linear_workspace(rows, k, n);
+  const int64_t need = exl3_linear_workspace(rows, k, n, type);
   if (need < 0) return set_error("exl3_linear: bad sizes: %lld rows of %lld by %lld", (long long)rows, (long long)k, (long long)n);
   if (!rows) return 0;
   if ((reinterpret_cast<uintptr_t>(x) & 15) || stride % 8 || (reinterpret_cast<uintptr_t>(out) & 15) ||
       (reinterpret_cast<uintptr_t>(workspace) & 15) || (reinterpret_cast<uintptr_t>(words) & 3))
     return set_error("exl3_linear: rows, out and workspace must be 16-byte aligned, words 4-byte");
+  if (((reinterpret_cast<uintptr_t>(su) | reinterpret_cast<uintptr_t>(sv)) & 7))
+    return set_error("exl3_linear: su and sv must be 8-byte aligned");
   if (workspace_bytes < need) return set_error("exl3_linear: workspace of %lld bytes is too small", (long long)workspace_bytes);
-  const Plan p = plan_of(rows, k, n);
-  hipStream_t s = (hipStream_t)stream;
+  const Plan p = plan_of(rows, k, n, type == 2);
   char* w = static_cast<char*>(workspace);
   TurnArgs t{};
-  t.x = static_cast<const uint16_t*>(x), t.stride = stride, t.su = {su, half_scales & 1};
+  t.x = static_cast<const uint16_t*>(x), t.stride = stride, t.su = su, t.half = half_scales & 1;
   t.z = reinterpret_cast<u32x4*>(w), t.scale = reinterpret_cast<float*>(w + p.z_bytes);
-  t.rows = (int)rows, t.k = (int)k, t.sets = p.sets;
-  if (type == 2)
-    linear_turn_kernel<true><<<(unsigned)rows, 256, 0, s>>>(t);
-  else
-    linear_turn_kernel<false><<<(unsigned)rows, 256, 0, s>>>(t);
-  if (check_launch("exl3_linear")) return 1;
+  t.k = (int)k, t.sets = p.sets, t.block_rows = p.block_rows;
+  t.rest = p.variant == ROWS8 ? 8 : p.parts == 2 ? 64 : 0;
   LinearArgs a{};
-  a.words = reinterpret_cast<const uint32_t*>(words), a.z = t.z;
-  a.partials = reinterpret_cast<float*>(w + p.z_bytes + p.scale_bytes);
-  a.rows = (int)rows, a.k = (int)k, a.n = (int)n, a.bits = K, a.splits = p.splits, a.sets = p.sets;
-  if (K > 5)
-    cb == 0 ? launch_product<true, 0>(p, a, s) : cb == 1 ? launch_product<true, 1>(p, a, s) : launch_product<true, 2>(p, a, s);
-  else
-    cb == 0 ? launch_product<false, 0>(p, a, s) : cb == 1 ? launch_product<false, 1>(p, a, s) : launch_product<false, 2>(p, a, s);
-  if (check_launch("exl3_linear")) return 1;
-  JoinArgs j{};
-  j.partials = a.partials, j.scale = t.scale, j.sv = {sv, half_scales >> 1 & 1};
-  j.out = static_cast<uint16_t*>(out), j.rows = (int)rows, j.n = (int)n, j.splits = p.splits;
-  const int64_t units = rows * (n / HAD);
-  if (type == 2)
-    linear_join_kernel<true><<<(unsigned)((units + 15) / 16), 256, 0, s>>>(j);
-  else
-    linear_join_kernel<false><<<(unsigned)((units + 15) / 16), 256, 0, s>>>(j);
-  return check_launch("exl3_linear");
+  a.words = reinterpret_cast<const uint32_t*>(words), a.z = t.z, a.scale = t.scale, a.sv = {sv, half_scales >> 1 & 1};
+  a.out = static_cast<uint16_t*>(out), a.partials = reinterpret_cast<float*>(w + p.z_bytes + p.scale_bytes);
+  a.rows = (int)rows, a.k = (int)k, a.n = (int)n, a.bits = K, a.splits = p.splits;
+  auto launch = type == 2 ? launch_linear<true> : launch_linear<false>;
+  return launch(p, t, a, cb, (hipStream_t)stream);
 }
 
 }  // extern "C"

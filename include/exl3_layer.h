@@ -206,9 +206,9 @@ int exl3_ldlq_scatter(const exl3_ldlq_block* blocks, int nblocks, int64_t tiles,
 /* ---- Products with weights as they are stored (no counterpart in the
  * reference). ---- */
 
-/* Bytes of workspace that exl3_linear needs for `rows` rows of a (k, n) weight,
+/* Bytes of workspace that exl3_linear needs for `rows` rows and a (k, n) weight,
  * or -1 where it takes no such sizes. */
-int64_t exl3_linear_workspace(int64_t rows, int64_t k, int64_t n);
+int64_t exl3_linear_workspace(int64_t rows, int64_t k, int64_t n, int type);
 
 /* out (rows, n) = x W, W the (k, n) weight that exl3_decode_weight decodes from
  * `words` (k / 16 x n / 16 tiles of 16 K) with input scales su and output
