@@ -86,18 +86,37 @@ _SIGNATURES = {
                              _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_int, _c_i64,
                              _c_int, _c_int, _c_vp, _c_int, _c_vp, _c_int, _c_int, _c_float,
                              _c_int, _c_vp]),
+    "exl3_rotary_axes": (_c_int, [_c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_int,
+                                  _c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_i64, _c_int, _c_i64,
+                                  _c_int, _c_int, _c_vp, _c_int, _c_vp, _c_int, _c_vp, _c_int,
+                                  _c_int, _c_float, _c_int, _c_vp]),
     "exl3_plan_step": (_c_int, [_c_vp, _c_vp, _c_int, _c_vp, _c_int, _c_vp, _c_int, _c_vp, _c_int,
                                 _c_i64, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp]),
     "exl3_cache_append": (_c_int, [_c_vp, _c_i64, _c_i64, _c_vp, _c_int, _c_vp, _c_i64, _c_i64,
                                    _c_vp, _c_i64, _c_i64, _c_i64, _c_int, _c_vp, _c_vp, _c_int,
                                    _c_vp, _c_int, _c_int, _c_float, _c_vp, _c_i64, _c_int, _c_int,
                                    _c_int, _c_vp]),
+    "exl3_cache_append_axes": (_c_int, [_c_vp, _c_i64, _c_i64, _c_vp, _c_int, _c_vp, _c_i64,
+                                        _c_i64, _c_vp, _c_i64, _c_i64, _c_i64, _c_int, _c_vp,
+                                        _c_vp, _c_int, _c_vp, _c_int, _c_vp, _c_int, _c_int,
+                                        _c_float, _c_vp, _c_i64, _c_int, _c_int, _c_int, _c_vp]),
     "exl3_cache_read": (_c_int, [_c_vp, _c_i64, _c_int, _c_int, _c_int, _c_vp, _c_i64, _c_int,
                                  _c_vp, _c_vp, _c_vp]),
     "exl3_cache_attention_workspace": (_c_i64, [_c_i64, _c_int, _c_int, _c_int, _c_int, _c_i64]),
     "exl3_cache_attention": (_c_int, [_c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_int, _c_int, _c_vp,
                                       _c_i64, _c_int, _c_int, _c_int, _c_vp, _c_int, _c_vp, _c_vp,
                                       _c_int, _c_float, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp]),
+    "exl3_cache_attention_trees": (_c_int, [_c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_int, _c_int,
+                                            _c_vp, _c_i64, _c_int, _c_int, _c_int, _c_vp, _c_int,
+                                            _c_vp, _c_vp, _c_int, _c_vp, _c_int, _c_float, _c_i64,
+                                            _c_i64, _c_vp, _c_i64, _c_vp]),
+    "exl3_plan_tree": (_c_int, [_c_vp, _c_vp, _c_vp, _c_int, _c_i64, _c_int, _c_vp, _c_vp, _c_vp]),
+    "exl3_accept_drafts": (_c_int, [_c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_int,
+                                    _c_i64, _c_vp, _c_vp, _c_vp, _c_vp]),
+    "exl3_cache_keep": (_c_int, [_c_vp, _c_i64, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_vp, _c_int,
+                                 _c_i64, _c_vp]),
+    "exl3_release_pages": (_c_int, [_c_vp, _c_vp, _c_int, _c_vp, _c_int, _c_int, _c_vp, _c_int,
+                                    _c_vp, _c_vp, _c_vp]),
 }
 
 
@@ -953,6 +972,24 @@ def _vector(t, name: str, dtypes: tuple, numel, device) -> None:
                            f"{' or '.join(map(str, dtypes))}, on {device}")
 
 
+def _positions(positions, axes, tokens: int, pairs: int, device) -> tuple:
+    """The arguments of the tokens' positions: a vector, or one of each axis with
+    the axis of every pair."""
+    torch = _torch()
+    if axes is None:
+        _vector(positions, "positions", (torch.int32, torch.int64), tokens, device)
+        return positions.data_ptr(), positions.dtype == torch.int64, None, 1
+    _vector(axes, "axes", (torch.int32,), pairs, device)
+    if (not isinstance(positions, torch.Tensor) or positions.dim() != 2
+            or positions.dtype not in (torch.int32, torch.int64) or positions.shape[0] < 1
+            or positions.shape[1] != tokens or not positions.is_contiguous()
+            or positions.device != device):
+        raise RuntimeError(f"positions must be a contiguous (axes, {tokens}) tensor, int32 or int64, "
+                           f"on {device}")
+    return (positions.data_ptr(), positions.dtype == torch.int64, axes.data_ptr(),
+            positions.shape[0])
+
+
 def _pages(pages) -> tuple:
     """(pages, page size, kv heads, head dim) of a cache."""
     torch = _torch()
@@ -1066,16 +1103,16 @@ def _check_outputs(size: int, *rows) -> None:
 
 
 def rotary(q, k, positions, frequencies, layout: int, magnitude: float, inverse: bool,
-           out=None) -> tuple:
-    """q and k turned by their positions (exl3_rotary); k may be None."""
+           out=None, axes=None) -> tuple:
+    """q and k turned by their positions (exl3_rotary_axes); k may be None."""
     torch = _torch()
     (tokens, heads, dim), sq = _rows(q, "q")
     device = q.device
-    _vector(positions, "positions", (torch.int32, torch.int64), tokens, device)
     _vector(frequencies, "frequencies", (torch.float64,), None, device)
     pairs = frequencies.numel()
     if not 1 <= pairs <= dim // 2:
         raise RuntimeError(f"frequencies must hold 1 to {dim // 2} pairs, got {pairs}")
+    places = _positions(positions, axes, tokens, pairs, device)
     dense = torch.contiguous_format
     q_out, k_out = out or (torch.empty_like(q, memory_format=dense), None)
     so = _rows(q_out, "out[0]", q, heads, dim)[1] if out else (heads * dim, dim)
@@ -1093,10 +1130,9 @@ def rotary(q, k, positions, frequencies, layout: int, magnitude: float, inverse:
         more = () if k is None else (((at, k.shape, sk), (k_args[3], k.shape, sp)),)
         _check_outputs(q.element_size(), ((q.data_ptr(), shape, sq), (q_out.data_ptr(), shape, so)),
                        *more)
-    _run(device, "apply_rotary", load_library().exl3_rotary, q.data_ptr(), sq[0], sq[1],
+    _run(device, "apply_rotary", load_library().exl3_rotary_axes, q.data_ptr(), sq[0], sq[1],
          q_out.data_ptr(), so[0], so[1], heads, *k_args, tokens, dim, _types()[q.dtype],
-         positions.data_ptr(), positions.dtype == torch.int64, frequencies.data_ptr(), pairs,
-         layout, magnitude, inverse)
+         *places, frequencies.data_ptr(), pairs, layout, magnitude, inverse)
     if out:
         _written(*(t for t in (q_out, k_out) if t is not None))
     return q_out, k_out
@@ -1127,8 +1163,9 @@ def plan_step(cached, new, tables, free_pages, taken, page_size: int, max_tokens
     return slots, positions, starts, lengths, taken_out, status
 
 
-def cache_append(pages, k, v, slots, q, positions, frequencies, layout: int, magnitude: float):
-    """k and v into the cache, k (and q) turned first (exl3_cache_append);
+def cache_append(pages, k, v, slots, q, positions, frequencies, layout: int, magnitude: float,
+                 axes=None):
+    """k and v into the cache, k (and q) turned first (exl3_cache_append_axes);
     returns the turned q."""
     torch = _torch()
     n, page_size, heads, dim = _pages(pages)
@@ -1140,7 +1177,7 @@ def cache_append(pages, k, v, slots, q, positions, frequencies, layout: int, mag
     if k.device != device:
         raise RuntimeError("k and v must be on the cache's device")
     _vector(slots, "slots", (torch.int64,), tokens, device)
-    pairs, wide, freq, at = 0, 0, None, None
+    pairs, freq, at = 0, None, (None, 0, None, 1)
     q_out, q_args = None, (None, 0, 0, None, 0)
     if frequencies is not None:
         _vector(frequencies, "frequencies", (torch.float64,), None, device)
@@ -1148,18 +1185,17 @@ def cache_append(pages, k, v, slots, q, positions, frequencies, layout: int, mag
         if pairs % 8 or not 8 <= pairs <= dim // 2:
             raise RuntimeError(f"frequencies must hold a multiple of 8 pairs up to {dim // 2}, got "
                                f"{pairs}: turn with apply_rotary first")
-        _vector(positions, "positions", (torch.int32, torch.int64), tokens, device)
-        wide, freq, at = positions.dtype == torch.int64, frequencies.data_ptr(), positions.data_ptr()
+        at, freq = _positions(positions, axes, tokens, pairs, device), frequencies.data_ptr()
         if q is not None:
             q = _wide(q)
             (_, q_heads, _), sq = _rows(q, "q", k, None, dim)
             q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
             q_args = (q.data_ptr(), sq[0], sq[1], q_out.data_ptr(), q_heads)
-    elif q is not None or positions is not None:
-        raise RuntimeError("q and positions are only taken with frequencies")
-    _run(device, "append_tokens", load_library().exl3_cache_append, *q_args,
+    elif q is not None or positions is not None or axes is not None:
+        raise RuntimeError("q, positions and axes are only taken with frequencies")
+    _run(device, "append_tokens", load_library().exl3_cache_append_axes, *q_args,
          k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1], tokens,
-         _types()[k.dtype], slots.data_ptr(), at, wide, freq, pairs, layout, magnitude,
+         _types()[k.dtype], slots.data_ptr(), *at, freq, pairs, layout, magnitude,
          pages.data_ptr(), n, page_size, heads, dim)
     _written(pages)
     return q_out
@@ -1192,8 +1228,8 @@ def cache_read(pages, slots, dtype) -> tuple:
     return k, v
 
 
-def cache_attention(q, pages, tables, starts, lengths, scale, window, max_new):
-    """Attention over the cache (exl3_cache_attention)."""
+def cache_attention(q, pages, tables, starts, lengths, scale, window, max_new, trees=None):
+    """Attention over the cache (exl3_cache_attention_trees)."""
     torch = _torch()
     n, page_size, heads, dim = _pages(pages)
     dev = pages.device
@@ -1213,6 +1249,14 @@ def cache_attention(q, pages, tables, starts, lengths, scale, window, max_new):
         raise RuntimeError(f"window must be positive, got {window}")
     if max_new is not None and max_new < 0:
         raise RuntimeError(f"max_new must not be negative, got {max_new}")
+    masks, words = None, 0
+    if trees is not None:
+        if (not isinstance(trees, torch.Tensor) or trees.device != dev or trees.dim() != 2
+                or trees.dtype != torch.int64 or not trees.is_contiguous()
+                or trees.shape[0] < tokens or not 1 <= trees.shape[1] <= MAX_TREE_WORDS):
+            raise RuntimeError(f"trees must be a contiguous int64 tensor of at least {tokens} rows of "
+                               f"1 to {MAX_TREE_WORDS} words on {dev}")
+        masks, words = trees.data_ptr(), trees.shape[1]
     lib = load_library()
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     # Python's integers end nowhere, the C arguments at 64 bits.
@@ -1220,10 +1264,93 @@ def cache_attention(q, pages, tables, starts, lengths, scale, window, max_new):
     window = 2 ** 31 - 1 if window is None else min(int(window), 2 ** 31 - 1)
     size = lib.exl3_cache_attention_workspace(tokens, q_heads, heads, dim, requests, most)
     workspace = pages.new_empty(max(size, 0))
-    _run(dev, "cache_attention", lib.exl3_cache_attention, q.data_ptr(), sq[0], sq[1],
+    _run(dev, "cache_attention", lib.exl3_cache_attention_trees, q.data_ptr(), sq[0], sq[1],
          out.data_ptr(), tokens, q_heads, _types()[q.dtype], pages.data_ptr(), n, page_size, heads,
          dim, tables.data_ptr(), width, starts.data_ptr(), lengths.data_ptr(), requests,
-         dim ** -0.5 if scale is None else float(scale), window, most, workspace.data_ptr(), size)
+         masks, words, dim ** -0.5 if scale is None else float(scale), window, most, workspace.data_ptr(), size)
+    return out
+
+
+# ------------------------------------------------- drafted tokens
+
+MAX_TREE_WORDS = 16
+
+
+def _ranges(starts, lengths=None) -> int:
+    """Requests of the starts of their tokens (and of their lengths)."""
+    torch = _torch()
+    if not isinstance(starts, torch.Tensor) or not starts.is_cuda or starts.dim() != 1:
+        raise RuntimeError("starts must be a 1-D GPU (cuda) tensor")
+    _vector(starts, "starts", (torch.int32,), None, starts.device)
+    requests = starts.numel() - 1
+    if lengths is not None:
+        _vector(lengths, "lengths", (torch.int32,), requests, starts.device)
+    return requests
+
+
+def plan_tree(parents, starts, lengths, words: int) -> tuple:
+    """Masks and positions of drafted tokens (exl3_plan_tree)."""
+    torch = _torch()
+    requests, device = _ranges(starts, lengths), starts.device
+    _vector(parents, "parents", (torch.int32,), None, device)
+    tokens = parents.numel()
+    masks = parents.new_empty((tokens, words), dtype=torch.int64)
+    positions = torch.empty_like(parents)
+    _run(device, "plan_tree", load_library().exl3_plan_tree, parents.data_ptr(), starts.data_ptr(),
+         lengths.data_ptr(), requests, tokens, words, masks.data_ptr(), positions.data_ptr())
+    return masks, positions
+
+
+def accept_drafts(tokens, choices, parents, starts, lengths, certain) -> tuple:
+    """Places, lengths and next tokens (exl3_accept_drafts)."""
+    torch = _torch()
+    requests, device = _ranges(starts, lengths), starts.device
+    _vector(parents, "parents", (torch.int32,), None, device)
+    count = parents.numel()
+    _vector(tokens, "tokens", (torch.int32, torch.int64), count, device)
+    _vector(choices, "choices", (tokens.dtype,), count, device)
+    if certain is not None:
+        _vector(certain, "certain", (torch.int32,), requests, device)
+    places, kept = torch.empty_like(parents), torch.empty_like(lengths)
+    following = lengths.new_empty(requests, dtype=tokens.dtype)
+    _run(device, "accept_drafts", load_library().exl3_accept_drafts, tokens.data_ptr(),
+         choices.data_ptr(), tokens.dtype == torch.int64, parents.data_ptr(), starts.data_ptr(),
+         lengths.data_ptr(), None if certain is None else certain.data_ptr(), requests, count,
+         places.data_ptr(), kept.data_ptr(), following.data_ptr())
+    return places, kept, following
+
+
+def cache_keep(pages, slots, starts, places) -> None:
+    """Entries of kept tokens moved together (exl3_cache_keep)."""
+    torch = _torch()
+    n, page_size, heads, dim = _pages(pages)
+    device = pages.device
+    requests = _ranges(starts)
+    _vector(starts, "starts", (torch.int32,), None, device)
+    _vector(slots, "slots", (torch.int64,), None, device)
+    _vector(places, "places", (torch.int32,), slots.numel(), device)
+    _run(device, "keep_tokens", load_library().exl3_cache_keep, pages.data_ptr(), n, page_size, heads,
+         dim, slots.data_ptr(), starts.data_ptr(), places.data_ptr(), requests, slots.numel())
+    _written(pages)
+
+
+def release_pages(before, after, tables, free_pages, taken, page_size: int):
+    """The new ``taken`` (exl3_release_pages)."""
+    torch = _torch()
+    dev = tables.device if isinstance(tables, torch.Tensor) else None
+    if (dev is None or dev.type != "cuda" or tables.dim() != 2 or tables.dtype != torch.int32
+            or not tables.is_contiguous()):
+        raise RuntimeError("tables must be a contiguous 2-D int32 GPU (cuda) tensor")
+    requests, width = tables.shape
+    _vector(before, "before", (torch.int32,), requests, dev)
+    _vector(after, "after", (torch.int32,), requests, dev)
+    _vector(free_pages, "free_pages", (torch.int32,), None, dev)
+    _vector(taken, "taken", (torch.int32,), 1, dev)
+    out = torch.empty_like(taken)
+    _run(dev, "release_pages", load_library().exl3_release_pages, before.data_ptr(), after.data_ptr(),
+         requests, tables.data_ptr(), width, page_size, free_pages.data_ptr(), free_pages.numel(),
+         taken.data_ptr(), out.data_ptr())
+    _written(tables, free_pages)
     return out
 
 

@@ -14,6 +14,12 @@
 // H y / 4, and H H = 32, so q . k = 2 (H q / 8) . (H k / 8): queries are
 // transformed once, keys and values never, and an output row is taken back
 // once.
+//
+// Trees (TREE): the new tokens of a request of up to 64 `words` attend all cached
+// positions, 0 .. length - n - 1, and those new tokens that the row's mask names:
+// a sequence, of which a window leaves the last `window`. Requests of more tokens
+// attend as above. The variants are compiled apart, as masks by bits would cost
+// the others registers.
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
@@ -74,9 +80,17 @@ struct AttendArgs {
   CacheShape cache;
   int requests, width, q_heads, group;
   float scale;
+  const uint32_t* masks;         // (tokens, words) of 32 bits, of trees
+  int words;
   int classes;
   Class of[2];
 };
+
+// Whether a request's new tokens are a tree.
+template <bool TREE>
+__device__ __forceinline__ bool is_tree(const AttendArgs& a, int n) {
+  return TREE && n <= 32 * a.words;
+}
 
 // What a request asks for, every figure bounded by the arrays' sizes whatever
 // the device arrays hold.
@@ -85,12 +99,14 @@ struct Request {
   int length;                    // positions held
   int tile0, tiles;              // tiles that some row attends
 };
+template <bool TREE>
 __device__ __forceinline__ Request request_of(const AttendArgs& a, int r) {
   const int64_t s0 = min(max((int64_t)a.starts[r], (int64_t)0), a.tokens);
   const int64_t s1 = min(max((int64_t)a.starts[r + 1], s0), a.tokens);
   const int64_t room = ((int64_t)a.width << a.cache.tile_shift) * CACHE_TILE;
   const int64_t length = min(max((int64_t)a.lengths[r], (int64_t)0), room);
-  const int64_t low = max(length - (s1 - s0) - a.window + 1, (int64_t)0);
+  // (A row of a tree whose mask is empty attends the last cached positions.)
+  const int64_t low = max(length - (s1 - s0) - a.window + (is_tree<TREE>(a, (int)(s1 - s0)) ? 0 : 1), (int64_t)0);
   Request q;
   q.first = (int)s0, q.n = (int)(s1 - s0), q.length = (int)length;
   q.tile0 = (int)(low / CACHE_TILE);
@@ -117,29 +133,75 @@ __device__ __forceinline__ int64_t work_of(const AttendArgs& a, const Class& c, 
 }
 
 // What a block of rows attends: positions from `low` on, tiles [t0, t1), and
-// the last positions of its first and last row.
+// the last positions of its first and last row (of a tree: the last that all
+// rows attend, and the last that one may).
 struct Block {
   int row0, row1, least_last, most_last, low, t0, t1;
 };
+template <bool TREE>
 __device__ __forceinline__ Block block_of(const AttendArgs& a, const Class& c, const Request& q, int block) {
   const int rows = q.n * a.group, offset = q.length - q.n;
   Block b;
   b.row0 = block * c.rows, b.row1 = min(b.row0 + c.rows, rows) - 1;
-  b.least_last = offset + b.row0 / a.group, b.most_last = offset + b.row1 / a.group;
+  if (is_tree<TREE>(a, q.n))
+    b.least_last = offset - 1, b.most_last = q.length - 1;
+  else
+    b.least_last = offset + b.row0 / a.group, b.most_last = offset + b.row1 / a.group;
   b.low = (int)max((int64_t)b.least_last - a.window + 1, (int64_t)0);
   b.t0 = b.low / CACHE_TILE;
   b.t1 = max(b.most_last < 0 ? 0 : b.most_last / CACHE_TILE + 1, b.t0);
   return b;
 }
 
+// Bits i .. i + 7 of a row's mask, 0 outside it.
+__device__ __forceinline__ uint32_t mask_bits(const uint32_t* mask, int words, int i) {
+  const int w = i >> 5;
+  const uint32_t low = (uint32_t)w < (uint32_t)words ? mask[w] : 0u;
+  const uint32_t high = (uint32_t)(w + 1) < (uint32_t)words ? mask[w + 1] : 0u;
+  return __builtin_amdgcn_alignbit(high, low, i & 31);
+}
+
+// What a row of a tree attends: cached positions from..last, and of the new
+// tokens its mask names those from index `first` on.
+struct Seen {
+  int from, last, first;
+};
+__device__ __forceinline__ Seen seen_of(const AttendArgs& a, const Request& q, const uint32_t* mask) {
+  const int offset = q.length - q.n;
+  Seen s{0, offset - 1, 0};
+  if (a.window >= q.length) return s;
+  const int words = (q.n + 31) / 32;
+  auto word = [&](int w) { return 32 * w + 32 > q.n ? mask[w] & ((1u << (q.n & 31)) - 1u) : mask[w]; };
+  int count = 0;
+  for (int w = 0; w < words; ++w) count += __popc(word(w));
+  const int64_t from = (int64_t)offset + count - a.window;
+  s.from = (int)max(from, (int64_t)0);
+  if (from <= offset) return s;
+  // The window cuts the new tokens: all but their last `window`.
+  int skip = (int)(from - offset);
+  for (int w = 0; w < words; ++w) {
+    uint32_t bits = word(w);
+    const int here = __popc(bits);
+    if (skip >= here) {
+      skip -= here;
+      continue;
+    }
+    for (; skip; --skip) bits &= bits - 1u;
+    s.first = 32 * w + __ffs(bits) - 1;
+    return s;
+  }
+  s.first = q.n;
+  return s;
+}
+
 // prefix[r] = work before request r, prefix[requests] = all of it.
-template <int NTHREADS, typename T>
+template <bool TREE, int NTHREADS, typename T>
 __device__ __forceinline__ void sum_work(const AttendArgs& a, const Class& c, T* prefix, int64_t* parts) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int64_t base = 0;
   for (int r0 = 0; r0 < a.requests; r0 += NTHREADS) {
     const int r = r0 + tid;
-    int64_t v = r < a.requests ? work_of(a, c, request_of(a, r)) : 0;
+    int64_t v = r < a.requests ? work_of(a, c, request_of<TREE>(a, r)) : 0;
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) {
       const int64_t w = __shfl_up(v, o);
@@ -345,7 +407,7 @@ constexpr int resident(int d, bool wide, int ct) {
 // 4.9 a large copy reaches, vector instructions on 0.60 of the cycles. With 32
 // rows a tile they (0.50) and the products (0.18) get as long as the reading: 157
 // MB in 55 us, of which about 10 are the waves' start and end.
-template <int D, bool WIDE, int CT, bool BF16>
+template <int D, bool WIDE, int CT, bool BF16, bool TREE>
 __global__ void __launch_bounds__(THREADS, resident(D, WIDE, CT)) attend_rows_kernel(AttendArgs a, int index) {
   constexpr int PER = WIDE ? 16 : 8, ROWS = PER * CT, GROUPS = D / 32, SETS = Tile<D>::SETS, NIB = D == 64 ? 4 : 8;
   extern __shared__ int64_t prefix[];                    // [requests + 1]
@@ -354,7 +416,7 @@ __global__ void __launch_bounds__(THREADS, resident(D, WIDE, CT)) attend_rows_ke
   const Class& cls = a.of[index];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Magic magic;
-  sum_work<THREADS>(a, cls, prefix, parts);
+  sum_work<TREE, THREADS>(a, cls, prefix, parts);
   if (blockIdx.x == 0)
     for (int r = tid; r <= a.requests; r += THREADS) cls.shares[r] = prefix[r];
   const int64_t all = uniform(prefix[a.requests]), share = share_of(cls, all);
@@ -372,7 +434,8 @@ __global__ void __launch_bounds__(THREADS, resident(D, WIDE, CT)) attend_rows_ke
     // The segment (request, head, block of rows) that `at` lies in, and the
     // tiles of it that are this wave's.
     const int r = __builtin_amdgcn_readfirstlane(last_at_most(prefix, a.requests + 1, at));
-    const Request req = request_of(a, r);
+    const Request req = request_of<TREE>(a, r);
+    const bool tree = is_tree<TREE>(a, req.n);
     const int blocks = blocks_of(a, cls, req), rows = req.n * a.group;
     const int64_t before = uniform(prefix[r]);
     const int segment = (int)quotient(at - before, req.tiles + SEGMENT_COST);
@@ -386,7 +449,7 @@ __global__ void __launch_bounds__(THREADS, resident(D, WIDE, CT)) attend_rows_ke
     float* part = cls.partials + ((int64_t)owner * 2 + (first == 0)) * (ROWS * (D + 2));
     // What all of the block's rows attend, most_from .. least_last, needs no
     // mask.
-    const Block b = block_of(a, cls, req, block);
+    const Block b = block_of<TREE>(a, cls, req, block);
     const int row0 = b.row0, row1 = b.row1, least_last = b.least_last;
     const int most_from = (int)max((int64_t)b.most_last - a.window + 1, (int64_t)0);
     const int t0 = max(req.tile0 + first, b.t0), t1 = min(req.tile0 + past, b.t1);
@@ -424,6 +487,8 @@ __global__ void __launch_bounds__(THREADS, resident(D, WIDE, CT)) attend_rows_ke
     u32x4 qf[CT][GROUPS], ql[WIDE ? CT : 1][WIDE ? GROUPS : 1];
     float qs[CT], rise[CT];
     int last[CT], from[CT];                              // positions this lane's row attends
+    const uint32_t* mask[TREE ? CT : 1];                 // and new tokens, of a tree
+    int first_new[TREE ? CT : 1];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       const int row = row0 + c * PER + (WIDE ? n : n & 7);
@@ -475,6 +540,14 @@ __global__ void __launch_bounds__(THREADS, resident(D, WIDE, CT)) attend_rows_ke
       last[c] = there ? req.length - req.n + i : -1;
       const int64_t from64 = there ? (int64_t)last[c] - a.window + 1 : 0;
       from[c] = (int)max(from64, (int64_t)0);
+      if constexpr (TREE) {
+        mask[c] = nullptr;
+        if (tree && there) {
+          mask[c] = a.masks + (int64_t)(req.first + i) * a.words;
+          const Seen seen = seen_of(a, req, mask[c]);
+          from[c] = seen.from, last[c] = seen.last, first_new[c] = seen.first;
+        }
+      }
     }
 
     float run[CT], sum[CT];                              // run: the maximum before the factor qs
@@ -527,9 +600,14 @@ __global__ void __launch_bounds__(THREADS, resident(D, WIDE, CT)) attend_rows_ke
         }
         if (masked) {
           attended[c] = 0;
+          const int i0 = pos - (req.length - req.n);     // the first of them as a new token
+          uint32_t named = 0;
+          if constexpr (TREE)
+            if (mask[c]) named = mask_bits(mask[c], a.words, i0);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const bool in = pos + e >= from[c] && pos + e <= last[c];
+            bool in = pos + e >= from[c] && pos + e <= last[c];
+            if constexpr (TREE) in |= (named >> e & 1u) && i0 + e >= first_new[c] && i0 + e < req.n;
             x[e] = in ? x[e] : NONE;
             attended[c] |= (uint32_t)in << e;
             asm volatile("" : "+v"(x[e]));
@@ -744,7 +822,7 @@ constexpr int tile_waves(int d) { return d == 64 ? 4 : 8; }
 constexpr int tile_halves(int d) { return d == 256 ? 2 : 1; }  // waves that share 32 rows, each with a part of the dims
 constexpr int tile_rows(int d) { return 32 * tile_waves(d) / tile_halves(d); }
 constexpr int tile_groups(int d) { return d == 64 ? 3 : 1; }  // workgroups of a compute unit
-template <int D, bool BF16>
+template <int D, bool BF16, bool TREE>
 __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_waves(D) / 4)
     attend_tiles_kernel(AttendArgs a, int index) {
   constexpr int NW = tile_waves(D), NT = 64 * NW, ROWS = tile_rows(D), STEPS = D / 16;
@@ -771,7 +849,7 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
   int64_t* costs = dynamic;                              // [blocks + 1], if blocks may be cut
   int32_t* prefix = reinterpret_cast<int32_t*>(dynamic + (cls.whole ? 0 : cls.blocks + 1));  // [requests + 1]
   if (tid < 2) poison[tid] = -1;                         // seen by all after the barriers of the sums
-  sum_work<NT>(a, cls, prefix, parts);
+  sum_work<TREE, NT>(a, cls, prefix, parts);
   const int owner = blockIdx.x, heads = a.cache.kv_heads;
   int listed = __builtin_amdgcn_readfirstlane(prefix[a.requests]);
   // (More are asked for only if the requests' rows overlap.)
@@ -786,7 +864,7 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
       int64_t v = 0;
       if (i < listed) {
         const int r = last_at_most(prefix, a.requests + 1, i);
-        const Block b = block_of(a, cls, request_of(a, r), i - prefix[r]);
+        const Block b = block_of<TREE>(a, cls, request_of<TREE>(a, r), i - prefix[r]);
         v = b.t1 - b.t0 + SEGMENT_COST;
       }
 #pragma unroll
@@ -847,8 +925,9 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
       at = min(end, seg1);
       if (past <= first) continue;
     }
-    const Request req = request_of(a, r);
-    const Block b = block_of(a, cls, req, block);
+    const Request req = request_of<TREE>(a, r);
+    const bool tree = is_tree<TREE>(a, req.n);
+    const Block b = block_of<TREE>(a, cls, req, block);
     const int row0 = b.row0, row1 = b.row1, rows = req.n * a.group, offset = req.length - req.n;
     const int least_last = b.least_last;
     const int most_from = (int)max((int64_t)b.most_last - a.window + 1, (int64_t)0);
@@ -860,10 +939,21 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
     const int row = 32 * rows32 + n;
     const bool there = row0 + row < rows;
     const int token = there ? (row0 + row) / a.group : 0, of_group = there ? row0 + row - token * a.group : 0;
-    const int last = there ? offset + token : -1;
-    const int from = there ? (int)max((int64_t)last - a.window + 1, (int64_t)0) : 0;
+    int last = there ? offset + token : -1;
+    int from = there ? (int)max((int64_t)last - a.window + 1, (int64_t)0) : 0;
+    const uint32_t* mask = nullptr;
+    int first_new = 0;
+    if constexpr (TREE)
+      if (tree && there) {
+        mask = a.masks + (int64_t)(req.first + token) * a.words;
+        const Seen seen = seen_of(a, req, mask);
+        from = seen.from, last = seen.last, first_new = seen.first;
+      }
+    // Whether bit e of `named`, for new tokens from i0 on, is one that the row attends.
+    auto new_in = [&](uint32_t named, int i0, int e) { return (named >> e & 1u) && i0 + e >= first_new && i0 + e < req.n; };
     const int wave0 = min(row0 + 32 * rows32, row1), wave1 = min(row0 + 32 * rows32 + 31, row1);
-    const int wave_least = offset + wave0 / a.group, wave_most = offset + wave1 / a.group;
+    const int wave_least = tree ? offset - 1 : offset + wave0 / a.group;
+    const int wave_most = tree ? req.length - 1 : offset + wave1 / a.group;
     const int wave_from = (int)max((int64_t)wave_most - a.window + 1, (int64_t)0);
 
     const auto* table = (const __attribute__((address_space(4))) int32_t*)(a.tables + (int64_t)r * a.width);
@@ -1079,10 +1169,15 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
 #pragma unroll
       for (int e = 0; e < 16 * TT; ++e) x[e] = TT == 2 ? s[e >> 4][e & 15] : s[0][e & 15] + s[1][e & 15];
       if (pos < wave_from || pos + TT * CACHE_TILE - 1 > wave_least || missing(0) < 0) {
+        uint32_t named = 0;
 #pragma unroll
         for (int e = 0; e < 16 * TT; ++e) {
-          const int p = pos + 16 * (e >> 3) + 8 * h + (e & 7);
-          x[e] = p >= from && p <= last && page[e >> 4] >= 0 ? x[e] : NONE;
+          const int p0 = pos + 16 * (e >> 3) + 8 * h, p = p0 + (e & 7);
+          if constexpr (TREE)
+            if (!(e & 7)) named = mask ? mask_bits(mask, a.words, p0 - offset) : 0u;
+          bool in = p >= from && p <= last;
+          if constexpr (TREE) in |= new_in(named, p0 - offset, e & 7);
+          x[e] = in && page[e >> 4] >= 0 ? x[e] : NONE;
           asm volatile("" : "+v"(x[e]));
         }
       }
@@ -1134,7 +1229,9 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
           const int id = k < CACHE_TILE ? page[0] : page[TT - 1];
           if (id < 0) continue;
           const uint8_t* scales = bytes_of(t + k / CACHE_TILE, id) + 34 * D;
-          const bool in = pos + k >= from && pos + k <= last;
+          bool in = pos + k >= from && pos + k <= last;
+          if constexpr (TREE)
+            if (mask) in |= new_in(mask_bits(mask, a.words, pos + k - offset), pos + k - offset, 0);
 #pragma unroll
           for (int d = 0; d < OWN; ++d) {
             const uint32_t bits = reinterpret_cast<const uint16_t*>(scales)[((k % CACHE_TILE >> 3) * GROUPS + half * OWN + d) * 8 + (k & 7)];
@@ -1202,7 +1299,7 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
 // each, and `run` one after another (51 MB of partials for 88000 rows of head
 // dimension 256: 17 us, row by row 28). A prompt's rows are all whole: there it
 // only has to see that (6 us for 8192 tokens).
-template <int D, bool BF16, int SPREAD>
+template <int D, bool BF16, bool TREE, int SPREAD>
 __global__ void __launch_bounds__(SPREAD > 1 ? 64 * SPREAD : THREADS) attend_join_kernel(AttendArgs a, int run) {
   constexpr int LANES = SPREAD > 1 ? 64 : 16, ROWS = 64 / LANES, PER = D / LANES, VEC = PER < 4 ? PER : 4;
   constexpr int BATCH = SPREAD > 1 || D < 256 ? 4 : 2;  // by the registers they take
@@ -1234,7 +1331,7 @@ __global__ void __launch_bounds__(SPREAD > 1 ? 64 * SPREAD : THREADS) attend_joi
     for (int e = 0; e < PER; ++e) x[e] = 0.0f;
     bool writes = at + lane / LANES < past, skip = false;
     if (r < a.requests) {
-      const Request req = request_of(a, r);
+      const Request req = request_of<TREE>(a, r);
       if (req.tiles && token >= req.first && token < req.first + req.n) {
         // Field by field, so that the choice is not a load.
         const bool main = a.classes == 1 || takes(a, a.of[0], req);
@@ -1341,6 +1438,7 @@ __global__ void __launch_bounds__(SPREAD > 1 ? 64 * SPREAD : THREADS) attend_joi
 }
 
 constexpr int CUS = 256;
+constexpr int MAX_WORDS = 16;                            // of a row's mask, 64 bits each
 
 // Variants by the query rows that one kv head has of a request (its new tokens
 // times the query heads to a kv head): up to 8 and 16 rows at 22 bits, whose
@@ -1408,25 +1506,25 @@ Launches launches_of(int64_t tokens, int group, int requests, int head_dim, int6
   return {v == ROWS8 || (v == ROWS16 && requests == 1) ? 1 : 2, head_dim == 256 ? 32 : v == ROWS16 ? 8 : 16, {v, ROWS8}};
 }
 
-template <int D, bool BF16>
+template <int D, bool BF16, bool TREE>
 int launch_variant(Variant v, const AttendArgs& args, int index, unsigned grid, hipStream_t stream) {
   const Class& c = args.of[index];
   const size_t requests = (size_t)args.requests + 1;
   const size_t lds = v != TILES ? 8 * requests : 4 * requests + (c.whole ? 0 : 8 * ((size_t)c.blocks + 1));
   if (v == ROWS8)
-    attend_rows_kernel<D, false, 1, BF16><<<grid, THREADS, lds, stream>>>(args, index);
+    attend_rows_kernel<D, false, 1, BF16, TREE><<<grid, THREADS, lds, stream>>>(args, index);
   else if (v == TILES)
-    attend_tiles_kernel<D, BF16><<<grid, 64 * tile_waves(D), lds, stream>>>(args, index);
+    attend_tiles_kernel<D, BF16, TREE><<<grid, 64 * tile_waves(D), lds, stream>>>(args, index);
   else if constexpr (D != 256) {
     if (v == ROWS16)
-      attend_rows_kernel<D, false, 2, BF16><<<grid, THREADS, lds, stream>>>(args, index);
+      attend_rows_kernel<D, false, 2, BF16, TREE><<<grid, THREADS, lds, stream>>>(args, index);
     else
-      attend_rows_kernel<D, true, 2, BF16><<<grid, THREADS, lds, stream>>>(args, index);
+      attend_rows_kernel<D, true, 2, BF16, TREE><<<grid, THREADS, lds, stream>>>(args, index);
   }
   return check_launch("exl3_cache_attention");
 }
 
-template <int D, bool BF16>
+template <int D, bool BF16, bool TREE>
 int launch_attend(AttendArgs args, int64_t max_new, char* workspace, hipStream_t stream) {
   const Launches launches = launches_of(args.tokens, args.group, args.requests, D, max_new);
   args.classes = launches.count;
@@ -1447,18 +1545,18 @@ int launch_attend(AttendArgs args, int64_t max_new, char* workspace, hipStream_t
     const int64_t grid = c.whole ? segments : v == TILES ? c.owners : c.owners / WAVES;
     // A launch has fewer than 2^32 threads.
     if (grid > UINT32_MAX / (64 * tile_waves(D))) return set_error("exl3_cache_attention: too many tokens and heads");
-    if (launch_variant<D, BF16>(v, args, i, (unsigned)grid, stream)) return 1;
+    if (launch_variant<D, BF16, TREE>(v, args, i, (unsigned)grid, stream)) return 1;
   }
   const int64_t rows = args.tokens * args.q_heads;
   if (rows <= 2 * CUS) {
-    attend_join_kernel<D, BF16, 8><<<(unsigned)rows, 64 * 8, 0, stream>>>(args, 1);
+    attend_join_kernel<D, BF16, TREE, 8><<<(unsigned)rows, 64 * 8, 0, stream>>>(args, 1);
   } else if (rows <= 8 * CUS) {
-    attend_join_kernel<D, BF16, 4><<<(unsigned)rows, 64 * 4, 0, stream>>>(args, 1);
+    attend_join_kernel<D, BF16, TREE, 4><<<(unsigned)rows, 64 * 4, 0, stream>>>(args, 1);
   } else {
     // Rows to a wave, by fours; as many as a token or more where all are whole.
     const int64_t run = std::min<int64_t>(std::max<int64_t>(args.of[0].whole ? 64 : 4, rows / (16 * CUS * WAVES) / 4 * 4), 64);
     const int64_t waves = (rows + run - 1) / run;
-    attend_join_kernel<D, BF16, 1><<<(unsigned)((waves + WAVES - 1) / WAVES), THREADS, 0, stream>>>(args, (int)run);
+    attend_join_kernel<D, BF16, TREE, 1><<<(unsigned)((waves + WAVES - 1) / WAVES), THREADS, 0, stream>>>(args, (int)run);
   }
   return check_launch("exl3_cache_attention");
 }
@@ -1484,12 +1582,13 @@ int64_t exl3_cache_attention_workspace(int64_t tokens, int q_heads, int kv_heads
   return bytes;
 }
 
-int exl3_cache_attention(const void* q, int64_t q_token, int64_t q_head, void* out, int64_t tokens,
-                         int q_heads, int type, const void* pages, int64_t num_pages, int page_size,
-                         int kv_heads, int head_dim, const int32_t* tables, int width,
-                         const int32_t* starts, const int32_t* lengths, int requests, float scale,
-                         int64_t window, int64_t max_new, void* workspace, int64_t workspace_bytes,
-                         void* stream) {
+int exl3_cache_attention_trees(const void* q, int64_t q_token, int64_t q_head, void* out,
+                               int64_t tokens, int q_heads, int type, const void* pages,
+                               int64_t num_pages, int page_size, int kv_heads, int head_dim,
+                               const int32_t* tables, int width, const int32_t* starts,
+                               const int32_t* lengths, int requests, const int64_t* masks, int words,
+                               float scale, int64_t window, int64_t max_new, void* workspace,
+                               int64_t workspace_bytes, void* stream) {
   if (head_dim != 64 && head_dim != 128 && head_dim != 256)
     return set_error("exl3_cache_attention: head_dim must be 64, 128 or 256, got %d", head_dim);
   if (page_size < 32 || page_size > 256 || (page_size & (page_size - 1)))
@@ -1510,6 +1609,8 @@ int exl3_cache_attention(const void* q, int64_t q_token, int64_t q_head, void* o
   if (((reinterpret_cast<uintptr_t>(pages) | reinterpret_cast<uintptr_t>(workspace)) & 15) ||
       (reinterpret_cast<uintptr_t>(out) & 7))
     return set_error("exl3_cache_attention: pages, out and workspace must be aligned");
+  if (masks && (words < 1 || words > MAX_WORDS))
+    return set_error("exl3_cache_attention: masks must have 1 to %d words, got %d", MAX_WORDS, words);
   if (max_new < 0) return set_error("exl3_cache_attention: max_new %lld is negative", (long long)max_new);
   if (workspace_bytes < exl3_cache_attention_workspace(tokens, q_heads, kv_heads, head_dim, requests, max_new))
     return set_error("exl3_cache_attention: workspace of %lld bytes is too small", (long long)workspace_bytes);
@@ -1525,14 +1626,27 @@ int exl3_cache_attention(const void* q, int64_t q_token, int64_t q_head, void* o
   a.cache = CacheShape{num_pages, kv_heads, head_dim, shift};
   a.requests = requests, a.width = width, a.q_heads = q_heads, a.group = q_heads / kv_heads;
   a.scale = scale;
+  a.masks = reinterpret_cast<const uint32_t*>(masks), a.words = 2 * words;
   auto launch = [&](auto dim) {
     constexpr int D = decltype(dim)::value;
-    auto call = type == 2 ? launch_attend<D, true> : launch_attend<D, false>;
+    auto call = masks ? (type == 2 ? launch_attend<D, true, true> : launch_attend<D, false, true>)
+                      : (type == 2 ? launch_attend<D, true, false> : launch_attend<D, false, false>);
     return call(a, max_new, static_cast<char*>(workspace), (hipStream_t)stream);
   };
   if (head_dim == 64) return launch(std::integral_constant<int, 64>{});
   if (head_dim == 128) return launch(std::integral_constant<int, 128>{});
   return launch(std::integral_constant<int, 256>{});
+}
+
+int exl3_cache_attention(const void* q, int64_t q_token, int64_t q_head, void* out, int64_t tokens,
+                         int q_heads, int type, const void* pages, int64_t num_pages, int page_size,
+                         int kv_heads, int head_dim, const int32_t* tables, int width,
+                         const int32_t* starts, const int32_t* lengths, int requests, float scale,
+                         int64_t window, int64_t max_new, void* workspace, int64_t workspace_bytes,
+                         void* stream) {
+  return exl3_cache_attention_trees(q, q_token, q_head, out, tokens, q_heads, type, pages, num_pages, page_size,
+                                    kv_heads, head_dim, tables, width, starts, lengths, requests, nullptr, 0, scale,
+                                    window, max_new, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

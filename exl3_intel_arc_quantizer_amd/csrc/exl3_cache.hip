@@ -5,6 +5,10 @@
 //   append_kernel   keys and values to 4-bit cache entries, the keys (and
 //                   queries) rotated on the way
 //   read_kernel     cache entries back to keys and values
+//   tree_kernel     masks and positions of drafted tokens from their parents
+//   accept_kernel   the drafted tokens that the model would have chosen
+//   release_kernel  pages past the kept tokens back to the free ones
+//   keep_kernel     entries of kept tokens moved together
 //
 // The cache's layout and group transform: exl3_cache_layout.h; attention over
 // it: exl3_attention.hip.
@@ -92,10 +96,27 @@ struct Rows {
   Rows from(int64_t t) const { return {data ? data + t * token : data, token, head}; }
 };
 
-// Positions, int64 if wide, from token t on.
-const void* positions_from(const void* positions, bool wide, int64_t t) {
-  return positions ? static_cast<const char*>(positions) + t * (wide ? 8 : 4) : positions;
-}
+// Positions of tokens, int64 if wide. With axes they are (num_axes, stride), and
+// a pair's axis is axes[pair]; one of another axis stays at position 0.
+struct Positions {
+  const void* data;
+  const int32_t* axes;
+  int64_t stride;
+  int wide, num_axes;
+  __device__ __forceinline__ double at(int pair, int64_t t) const {
+    if (axes) {
+      const int axis = axes[pair];
+      if ((uint32_t)axis >= (uint32_t)num_axes) return 0.0;
+      t += axis * stride;
+    }
+    return wide ? (double)static_cast<const int64_t*>(data)[t] : (double)static_cast<const int32_t*>(data)[t];
+  }
+  Positions from(int64_t t) const {
+    Positions p = *this;
+    if (p.data) p.data = static_cast<const char*>(data) + t * (wide ? 8 : 4);
+    return p;
+  }
+};
 
 // A launch has fewer than 2^32 threads along an axis: more tokens than so many
 // blocks of 256 take go in several.
@@ -114,14 +135,12 @@ int in_parts(int64_t tokens, int64_t per_block, F launch) {
 // would be off by 0.06 radians, and float32 functions of the exact fraction of
 // a turn (1.2e-7) put three times as many rotated keys over the edge to the
 // next code as rounding does.
-__device__ __forceinline__ void turn_table(const void* positions, bool wide, const double* freq,
-                                           int pairs, float magnitude, float sign, int64_t t0,
-                                           int tokens, float* cosines, float* sines) {
+__device__ __forceinline__ void turn_table(const Positions& positions, const double* freq, int pairs,
+                                           float magnitude, float sign, int64_t t0, int tokens,
+                                           float* cosines, float* sines) {
   for (int i = threadIdx.x; i < tokens * pairs; i += blockDim.x) {
     const int t = i / pairs, p = i - t * pairs;
-    const double at = wide ? (double)static_cast<const int64_t*>(positions)[t0 + t]
-                           : (double)static_cast<const int32_t*>(positions)[t0 + t];
-    const double turns = at * (freq[p] * 0.15915494309189535);
+    const double turns = positions.at(p, t0 + t) * (freq[p] * 0.15915494309189535);
     double s, c;
     sincospi(2.0 * (turns - rint(turns)), &s, &c);
     cosines[i] = (float)(c * magnitude);
@@ -161,9 +180,9 @@ __device__ __forceinline__ void turned8(const typename E::type* row, int d0, int
 // ------------------------------------------------------------ rotary
 
 struct RotaryArgs {
-  const void* positions;
+  Positions positions;
   const double* freq;
-  int q_heads, heads, d, pairs, wide, half;
+  int q_heads, heads, d, pairs, half;
   float magnitude, sign;
 };
 
@@ -182,7 +201,7 @@ __global__ void __launch_bounds__(256)
   extern __shared__ float table[];
   const int64_t t = blockIdx.x;
   float *c = table, *s = table + a.pairs;
-  turn_table(a.positions, a.wide, a.freq, a.pairs, a.magnitude, a.sign, t, 1, c, s);
+  turn_table(a.positions, a.freq, a.pairs, a.magnitude, a.sign, t, 1, c, s);
   __syncthreads();
   const int units = VEC ? a.d / 16 : (a.d + 1) / 2;
   const int all = a.heads * units;
@@ -253,7 +272,7 @@ int launch_rotary(const void* q, int64_t q_token, int64_t q_head, const void* k,
   const size_t lds = 2 * sizeof(float) * args.pairs;
   return in_parts(tokens, 1, [&](int64_t t, int64_t n) {
     RotaryArgs part = args;
-    part.positions = positions_from(args.positions, args.wide, t);
+    part.positions = args.positions.from(t);
     auto kernel = vec ? rotary_kernel<E, true> : rotary_kernel<E, false>;
     kernel<<<(unsigned)n, 256, lds, stream>>>(rq.from(t), rk.from(t), oq.from(t), ok.from(t), part);
     return check_launch("exl3_rotary");
@@ -397,10 +416,10 @@ __global__ void __launch_bounds__(STEP_THREADS) step_kernel(StepArgs a) {
 struct CellArgs {
   CacheShape cache;
   const int64_t* slots;
-  const void* positions;
+  Positions positions;
   const double* freq;
   int64_t tokens;
-  int q_heads, pairs, wide, half, oct_shift;
+  int q_heads, pairs, half, oct_shift;
   float magnitude;
 };
 
@@ -456,7 +475,7 @@ __global__ void __launch_bounds__(256)
   const int tokens = (int)min((int64_t)TOK, a.tokens - t0);
   float *cosines = table, *sines = table + TOK * a.pairs;
   if constexpr (TURN) {
-    turn_table(a.positions, a.wide, a.freq, a.pairs, a.magnitude, 1.0f, t0, tokens, cosines, sines);
+    turn_table(a.positions, a.freq, a.pairs, a.magnitude, 1.0f, t0, tokens, cosines, sines);
     __syncthreads();
   }
   const int lane = threadIdx.x & 63, oct_shift = a.oct_shift, octs = 1 << oct_shift;
@@ -588,7 +607,7 @@ int launch_append(const void* q, int64_t q_token, int64_t q_head, void* q_out, c
     auto kernel = args.pairs ? append_kernel<E, true, TOK> : append_kernel<E, false, TOK>;
     return in_parts(args.tokens, TOK, [&](int64_t t, int64_t n) {
       CellArgs part = args;
-      part.slots = args.slots + t, part.positions = positions_from(args.positions, args.wide, t);
+      part.slots = args.slots + t, part.positions = args.positions.from(t);
       part.tokens = n;
       kernel<<<grid_of<TOK>(n, units, TOK == 1 ? 1 : 4), 256, lds, stream>>>(
           rq.from(t), rk.from(t), rv.from(t), oq.from(t), pages, part);
@@ -616,6 +635,304 @@ int launch_read(const uint8_t* pages, void* k, void* v, const CellArgs& args, hi
   };
   if (args.tokens >= MANY_TOKENS) return launch(std::integral_constant<int, 8>{}, 2);
   return launch(std::integral_constant<int, 1>{}, 1);
+}
+
+// ------------------------------------------------------------ drafted tokens
+
+// Trees of drafted tokens: those of request r are starts[r] .. starts[r + 1] - 1,
+// the last of its lengths[r] positions, and parents[t] is the place among them of
+// the token that t follows, -1 for the cached ones. A place that is not before t
+// counts as -1, so every walk upwards ends.
+struct TreeArgs {
+  const int32_t *parents, *starts, *lengths;
+  int64_t max_tokens;
+  int requests;
+};
+
+// A request's tokens, within the arrays whatever the device arrays hold.
+struct Drafts {
+  int64_t first;
+  int n, cached;
+};
+__device__ __forceinline__ Drafts drafts_of(const TreeArgs& a, int r) {
+  const int64_t s0 = min(max((int64_t)a.starts[r], (int64_t)0), a.max_tokens);
+  const int64_t s1 = min(max((int64_t)a.starts[r + 1], s0), a.max_tokens);
+  return {s0, (int)(s1 - s0), (int)max((int64_t)a.lengths[r] - (s1 - s0), (int64_t)0)};
+}
+
+// The blocks from `requests` on write what belongs to no request.
+template <typename F>
+__device__ __forceinline__ void for_padding(const TreeArgs& a, F write) {
+  const int64_t step = (int64_t)(gridDim.x - a.requests) * blockDim.x;
+  const int64_t s0 = min(max((int64_t)a.starts[0], (int64_t)0), a.max_tokens);
+  const int64_t s1 = min(max((int64_t)a.starts[a.requests], (int64_t)0), a.max_tokens);
+  const int64_t first = (int64_t)(blockIdx.x - a.requests) * blockDim.x + threadIdx.x;
+  for (int64_t t = first; t < s0; t += step) write(t);
+  for (int64_t t = s1 + first; t < a.max_tokens; t += step) write(t);
+}
+
+constexpr int TREE_THREADS = 256, MAX_TREE = 1024;       // tokens of a tree: 16 words of 64
+
+// A thread walks up from its token, from place to lower place, and writes each
+// word of its mask as the walk leaves it: no array of masks, and as many steps as
+// the tree is deep. Requests of more tokens than a mask has bits are no trees:
+// their positions count up, their masks are left 0. Bound by latency (parents
+// once to shared memory, then a look-up a step): 512 trees of up to 48 tokens 4.5
+// us, one of 13 2.2.
+__global__ void __launch_bounds__(TREE_THREADS) tree_kernel(TreeArgs a, int words, uint64_t* masks, int32_t* positions) {
+  __shared__ int16_t up[MAX_TREE];
+  const int r = blockIdx.x, tid = threadIdx.x;
+  if (r >= a.requests) {
+    for_padding(a, [&](int64_t t) {
+      positions[t] = 0;
+      for (int w = 0; w < words; ++w) masks[t * words + w] = 0;
+    });
+    return;
+  }
+  const Drafts d = drafts_of(a, r);
+  if (d.n > 64 * words) {
+    for (int i = tid; i < d.n; i += TREE_THREADS) {
+      positions[d.first + i] = (int32_t)min((int64_t)d.cached + i, (int64_t)INT32_MAX);
+      for (int w = 0; w < words; ++w) masks[(d.first + i) * words + w] = 0;
+    }
+    return;
+  }
+  for (int i = tid; i < d.n; i += TREE_THREADS) {
+    const int p = a.parents[d.first + i];
+    up[i] = (int16_t)(p >= 0 && p < i ? p : -1);
+  }
+  __syncthreads();
+  for (int i = tid; i < d.n; i += TREE_THREADS) {
+    uint64_t* mask = masks + (d.first + i) * words;
+    int word = i >> 6, depth = 0;
+    for (int w = words - 1; w > word; --w) mask[w] = 0;
+    uint64_t bits = 1ull << (i & 63);
+    for (int p = up[i]; p >= 0; p = up[p], ++depth) {
+      if (p >> 6 != word) {
+        mask[word] = bits;
+        for (--word; word > p >> 6; --word) mask[word] = 0;
+        bits = 0;
+      }
+      bits |= 1ull << (p & 63);
+    }
+    mask[word] = bits;
+    for (--word; word >= 0; --word) mask[word] = 0;
+    positions[d.first + i] = (int32_t)min((int64_t)d.cached + depth, (int64_t)INT32_MAX);
+  }
+}
+
+// What the model would have chosen: the request's first `certain` tokens, then
+// from the last of them down, as long as there is one, the first child that is
+// the token chosen after its parent. A wave takes a request; of up to 64 tokens a
+// lane holds one each, and a step is a vote (512 requests of up to 48 tokens 3.6 us,
+// one of 13 1.9: a launch and two loads).
+template <typename ID>
+struct AcceptArgs {
+  TreeArgs tree;
+  const ID *tokens, *choices;
+  const int32_t* certain;
+  int32_t *places, *lengths;
+  ID* next;
+};
+template <typename ID>
+__global__ void __launch_bounds__(64) accept_kernel(AcceptArgs<ID> a) {
+  const int r = blockIdx.x, lane = threadIdx.x;
+  if (r >= a.tree.requests) {
+    for_padding(a.tree, [&](int64_t t) { a.places[t] = -1; });
+    return;
+  }
+  const Drafts d = drafts_of(a.tree, r);
+  const int certain = min(max(a.certain ? a.certain[r] : 1, 1), d.n);
+  const int32_t* parents = a.tree.parents + d.first;
+  const ID *tokens = a.tokens + d.first, *choices = a.choices + d.first;
+  int32_t* places = a.places + d.first;
+  int at = certain - 1, count = certain;
+  if (d.n <= 64) {
+    const bool there = lane < d.n;
+    const int parent = there ? parents[lane] : -1;
+    const ID token = there ? tokens[lane] : 0, choice = there ? choices[lane] : 0;
+    int place = lane < certain ? lane : -1;
+    while (at >= 0) {
+      const ID chosen = __shfl(choice, at);
+      const uint64_t fits = __ballot(there && lane >= certain && lane > at && parent == at && token == chosen);
+      if (!fits) break;
+      at = __ffsll((unsigned long long)fits) - 1;
+      if (lane == at) place = count;
+      ++count;
+    }
+    if (there) places[lane] = place;
+  } else {
+    // Lane i % 64 writes the places of i: first these, then those found.
+    for (int i = lane; i < d.n; i += 64) places[i] = i < certain ? i : -1;
+    for (bool found = true; found;) {
+      const ID chosen = choices[at];
+      found = false;
+      for (int base = (at + 1) & ~63; base < d.n && !found; base += 64) {
+        const int i = base + lane;
+        const bool fits = i < d.n && i >= certain && i > at && parents[i] == at && tokens[i] == chosen;
+        const uint64_t all = __ballot(fits);
+        if (!all) continue;
+        found = true;
+        const int next = base + __ffsll((unsigned long long)all) - 1;
+        if (i == next) places[i] = count;
+        at = next;
+        ++count;
+        break;
+      }
+    }
+  }
+  if (lane == 0) {
+    a.lengths[r] = (int32_t)min((int64_t)d.cached + count, (int64_t)INT32_MAX);
+    a.next[r] = d.n ? choices[at] : (ID)-1;
+  }
+}
+
+// A request that holds `before` tokens and keeps `after` of them gives back the
+// pages from ceil(after / P) to ceil(before / P) of its row, in the order of the
+// requests and their rows, onto the stack of which `taken` is the top. One
+// workgroup: prefix sums over the requests, then the entries as one list, counted
+// and then written (entries without a page are not). Bound by latency (512
+// requests of a page or two each 5.6 us, one 2.3).
+struct ReleaseArgs {
+  const int32_t *before, *after, *taken;
+  int32_t *tables, *free_pages, *taken_out;
+  int requests, width, page_shift, free_count;
+};
+__global__ void __launch_bounds__(STEP_THREADS) release_kernel(ReleaseArgs a) {
+  extern __shared__ int32_t prefix[];                    // [requests + 1], of entries given back
+  __shared__ int64_t parts[STEP_THREADS / 64];
+  const int tid = threadIdx.x;
+  auto pages_of = [&](const int32_t* tokens, int r) {
+    const int64_t page = (int64_t)1 << a.page_shift;
+    return (int)min((max((int64_t)tokens[r], (int64_t)0) + page - 1) >> a.page_shift, (int64_t)a.width);
+  };
+  int64_t entries = 0;
+  for (int r0 = 0; r0 < a.requests; r0 += STEP_THREADS) {
+    const int r = r0 + tid;
+    const int64_t back = r < a.requests ? max(pages_of(a.before, r) - pages_of(a.after, r), 0) : 0;
+    int64_t sum;
+    const int64_t end = entries + block_sum(back, parts, &sum);
+    if (r < a.requests) prefix[r + 1] = (int32_t)end;
+    entries += sum;
+  }
+  if (tid == 0) prefix[0] = 0;
+  __syncthreads();
+  // The place of an entry in the tables.
+  auto entry_of = [&](int64_t i) {
+    const int r = last_at_most(prefix, a.requests + 1, (int)i);
+    return (int64_t)r * a.width + pages_of(a.after, r) + (i - prefix[r]);
+  };
+  int64_t held = 0;
+  int32_t page = -1;
+  int64_t entry = 0;
+  for (int64_t i0 = 0; i0 < entries; i0 += STEP_THREADS) {
+    page = -1;
+    if (i0 + tid < entries) entry = entry_of(i0 + tid), page = a.tables[entry];
+    held += __syncthreads_count(page >= 0);
+  }
+  const int64_t top = max((int64_t)a.taken[0], (int64_t)0) - held;
+  int64_t done = 0;
+  for (int64_t i0 = 0; i0 < entries; i0 += STEP_THREADS) {
+    if (entries > STEP_THREADS) {
+      page = -1;
+      if (i0 + tid < entries) entry = entry_of(i0 + tid), page = a.tables[entry];
+    }
+    int64_t sum;
+    const int64_t rank = done + block_sum(page >= 0, parts, &sum) - 1, to = top + rank;
+    if (page >= 0) {
+      a.tables[entry] = -1;
+      if (to >= 0 && to < a.free_count) a.free_pages[to] = page;
+    }
+    done += sum;
+  }
+  if (tid == 0) a.taken_out[0] = (int32_t)max(top, (int64_t)0);
+}
+
+// A token's entry of one head as dwords (codes) and halves (scales) that are its
+// own. `i` counts D / 8 dwords of key codes, as many of value codes, then D / 32
+// scales of each.
+__device__ __forceinline__ int64_t piece_of(const CacheShape& c, int64_t slot, int head, int i, bool scale) {
+  const int per = scale ? c.head_dim / 32 : c.head_dim / 8;
+  const bool value = i >= per;
+  const int d0 = (value ? i - per : i) * (scale ? 32 : 8);
+  const Cell cell = cell_of(c, slot, head, d0, value);
+  return scale ? cell.scale : cell.code;
+}
+
+// Token i's entry moves to the slot of place places[i] <= i. A workgroup takes a
+// request and a kv head, and its tokens in order, KEPT at a time that are read
+// before one of them is written: later ones come from slots past all of those
+// places, so nothing is read after it was written over. A wave's lanes take the
+// dwords of a token, then the scales. Bound by latency: four reads that wait for each
+// other (256 requests of up to 40 tokens, 4 kv heads of 128: 5.2 us; 4 requests 3.7).
+constexpr int KEPT = 16;
+struct KeepArgs {
+  CacheShape cache;
+  TreeArgs tree;
+  const int64_t* slots;
+  const int32_t* places;
+};
+__global__ void __launch_bounds__(256) keep_kernel(uint8_t* __restrict__ pages, KeepArgs a) {
+  constexpr int WAVES = 4, EACH = KEPT / WAVES;
+  __shared__ int list[256];
+  __shared__ int counts[WAVES];
+  const int r = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t s0 = min(max((int64_t)a.tree.starts[r], (int64_t)0), a.tree.max_tokens);
+  const int64_t s1 = min(max((int64_t)a.tree.starts[r + 1], s0), a.tree.max_tokens);
+  const int n = (int)(s1 - s0), d = a.cache.head_dim;
+  const int64_t capacity = a.cache.pages << (a.cache.tile_shift + 5);
+  for (int i0 = 0; i0 < n; i0 += 256) {
+    const int i = i0 + tid;
+    const int place = i < n ? a.places[s0 + i] : -1;
+    const bool moves = place >= 0 && place < i;
+    const uint64_t all = __ballot(moves);
+    if (lane == 0) counts[wave] = __popcll(all);
+    __syncthreads();
+    int at = __popcll(all & ((1ull << lane) - 1ull)), total = 0;
+    for (int w = 0; w < WAVES; ++w) {
+      if (w < wave) at += counts[w];
+      total += counts[w];
+    }
+    if (moves) list[at] = i;
+    __syncthreads();
+    for (int m0 = 0; m0 < total; m0 += KEPT) {
+      uint32_t words[EACH];
+      uint16_t scales[EACH];
+      int64_t to[EACH];
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const int m = m0 + e * WAVES + wave;
+        to[e] = -1;
+        if (m < total) {
+          const int from = list[m];
+          const int64_t source = a.slots[s0 + from], target = a.slots[s0 + a.places[s0 + from]];
+          if (source >= 0 && source < capacity && target >= 0 && target < capacity) {
+            to[e] = target;
+            if (lane < d / 4)
+              words[e] = *reinterpret_cast<const uint32_t*>(pages + piece_of(a.cache, source, head, lane, false));
+            if (lane < d / 16)
+              scales[e] = *reinterpret_cast<const uint16_t*>(pages + piece_of(a.cache, source, head, lane, true));
+          }
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        if (to[e] < 0) continue;
+        if (lane < d / 4) *reinterpret_cast<uint32_t*>(pages + piece_of(a.cache, to[e], head, lane, false)) = words[e];
+        if (lane < d / 16) *reinterpret_cast<uint16_t*>(pages + piece_of(a.cache, to[e], head, lane, true)) = scales[e];
+      }
+      __syncthreads();
+    }
+    __syncthreads();
+  }
+}
+
+int check_drafts(const char* what, int requests, int64_t max_tokens) {
+  if (requests < 1 || requests > CACHE_MAX_REQUESTS)
+    return set_error("%s: requests must be in 1..%d, got %d", what, CACHE_MAX_REQUESTS, requests);
+  if (max_tokens < 0 || max_tokens > INT32_MAX) return set_error("%s: bad number of tokens", what);
+  return 0;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -646,12 +963,12 @@ int check_cache(const char* what, int64_t pages, int page_size, int kv_heads, in
 
 extern "C" {
 
-int exl3_rotary(const void* q, int64_t q_token, int64_t q_head, void* q_out, int64_t qo_token,
-                int64_t qo_head, int q_heads, const void* k, int64_t k_token, int64_t k_head,
-                void* k_out, int64_t ko_token, int64_t ko_head, int k_heads, int64_t tokens,
-                int head_dim, int type, const void* positions, int wide_positions,
-                const double* frequencies, int pairs, int layout, float magnitude, int inverse,
-                void* stream) {
+int exl3_rotary_axes(const void* q, int64_t q_token, int64_t q_head, void* q_out, int64_t qo_token,
+                     int64_t qo_head, int q_heads, const void* k, int64_t k_token, int64_t k_head,
+                     void* k_out, int64_t ko_token, int64_t ko_head, int k_heads, int64_t tokens,
+                     int head_dim, int type, const void* positions, int wide_positions,
+                     const int32_t* axes, int num_axes, const double* frequencies, int pairs,
+                     int layout, float magnitude, int inverse, void* stream) {
   if (tokens < 0 || tokens > INT32_MAX || q_heads < 0 || k_heads < 0 || q_heads + k_heads < 1 ||
       q_heads + k_heads > 65535)
     return set_error("exl3_rotary: bad sizes");
@@ -659,11 +976,12 @@ int exl3_rotary(const void* q, int64_t q_token, int64_t q_head, void* q_out, int
     return set_error("exl3_rotary: needs 1 <= 2 * pairs <= head_dim <= 4096");
   if (type < 0 || type > 2 || layout < 0 || layout > 1)
     return set_error("exl3_rotary: bad type or layout");
+  if (axes && num_axes < 1) return set_error("exl3_rotary: needs an axis, got %d", num_axes);
   if (!tokens) return 0;
   RotaryArgs args{};
-  args.positions = positions, args.freq = frequencies;
+  args.positions = {positions, axes, tokens, wide_positions, num_axes}, args.freq = frequencies;
   args.q_heads = q_heads, args.heads = q_heads + k_heads, args.d = head_dim, args.pairs = pairs;
-  args.wide = wide_positions, args.half = layout == 0;
+  args.half = layout == 0;
   args.magnitude = magnitude, args.sign = inverse ? -1.0f : 1.0f;
   const int64_t per = type == 0 ? 4 : 8;
   const bool vec = pairs % 8 == 0 && head_dim % 16 == 0 && wide_rows(q, q_token, q_head, per) &&
@@ -673,6 +991,17 @@ int exl3_rotary(const void* q, int64_t q_token, int64_t q_head, void* q_out, int
   auto launch = type == 0 ? launch_rotary<F32> : type == 1 ? launch_rotary<F16> : launch_rotary<BF16>;
   return launch(q, q_token, q_head, k, k_token, k_head, q_out, qo_token, qo_head, k_out, ko_token,
                 ko_head, args, tokens, vec, s);
+}
+
+int exl3_rotary(const void* q, int64_t q_token, int64_t q_head, void* q_out, int64_t qo_token,
+                int64_t qo_head, int q_heads, const void* k, int64_t k_token, int64_t k_head,
+                void* k_out, int64_t ko_token, int64_t ko_head, int k_heads, int64_t tokens,
+                int head_dim, int type, const void* positions, int wide_positions,
+                const double* frequencies, int pairs, int layout, float magnitude, int inverse,
+                void* stream) {
+  return exl3_rotary_axes(q, q_token, q_head, q_out, qo_token, qo_head, q_heads, k, k_token, k_head, k_out, ko_token,
+                          ko_head, k_heads, tokens, head_dim, type, positions, wide_positions, nullptr, 1, frequencies,
+                          pairs, layout, magnitude, inverse, stream);
 }
 
 int exl3_plan_step(const int32_t* cached, const int32_t* fresh, int requests, int32_t* tables,
@@ -699,13 +1028,13 @@ int exl3_plan_step(const int32_t* cached, const int32_t* fresh, int requests, in
   return check_launch("exl3_plan_step");
 }
 
-int exl3_cache_append(const void* q, int64_t q_token, int64_t q_head, void* q_out, int q_heads,
-                      const void* k, int64_t k_token, int64_t k_head, const void* v,
-                      int64_t v_token, int64_t v_head, int64_t tokens, int type,
-                      const int64_t* slots, const void* positions, int wide_positions,
-                      const double* frequencies, int pairs, int layout, float magnitude,
-                      void* pages, int64_t num_pages, int page_size, int kv_heads, int head_dim,
-                      void* stream) {
+int exl3_cache_append_axes(const void* q, int64_t q_token, int64_t q_head, void* q_out, int q_heads,
+                           const void* k, int64_t k_token, int64_t k_head, const void* v,
+                           int64_t v_token, int64_t v_head, int64_t tokens, int type,
+                           const int64_t* slots, const void* positions, int wide_positions,
+                           const int32_t* axes, int num_axes, const double* frequencies, int pairs,
+                           int layout, float magnitude, void* pages, int64_t num_pages,
+                           int page_size, int kv_heads, int head_dim, void* stream) {
   CellArgs a{};
   if (check_cache("exl3_cache_append", num_pages, page_size, kv_heads, head_dim, &a.cache)) return 1;
   if (tokens < 0 || tokens > INT32_MAX || q_heads < 0 || q_heads > 65535 || type < 0 || type > 2 ||
@@ -716,17 +1045,30 @@ int exl3_cache_append(const void* q, int64_t q_token, int64_t q_head, void* q_ou
   if (!aligned16(pages) || (q_heads && !aligned16(q_out)))
     return set_error("exl3_cache_append: pages and q_out must be 16-byte aligned");
   if (q_heads && !pairs) return set_error("exl3_cache_append: queries are only taken to be turned");
+  if (axes && num_axes < 1) return set_error("exl3_cache_append: needs an axis, got %d", num_axes);
   const int64_t per = type == 0 ? 4 : 8;
   if (!wide_rows(q_heads ? q : nullptr, q_token, q_head, per) || !wide_rows(k, k_token, k_head, per) ||
       !wide_rows(v, v_token, v_head, per))
     return set_error("exl3_cache_append: rows must be 16-byte aligned");
   if (!tokens) return 0;
-  a.slots = slots, a.positions = positions, a.freq = frequencies, a.tokens = tokens;
-  a.q_heads = q_heads, a.pairs = pairs, a.wide = wide_positions, a.half = layout == 0;
+  a.slots = slots, a.positions = {positions, axes, tokens, wide_positions, num_axes}, a.freq = frequencies;
+  a.tokens = tokens, a.q_heads = q_heads, a.pairs = pairs, a.half = layout == 0;
   a.magnitude = magnitude, a.oct_shift = oct_shift_of(head_dim);
   auto launch = type == 0 ? launch_append<F32> : type == 1 ? launch_append<F16> : launch_append<BF16>;
   return launch(q, q_token, q_head, q_out, k, k_token, k_head, v, v_token, v_head,
                 static_cast<uint8_t*>(pages), a, (hipStream_t)stream);
+}
+
+int exl3_cache_append(const void* q, int64_t q_token, int64_t q_head, void* q_out, int q_heads,
+                      const void* k, int64_t k_token, int64_t k_head, const void* v,
+                      int64_t v_token, int64_t v_head, int64_t tokens, int type,
+                      const int64_t* slots, const void* positions, int wide_positions,
+                      const double* frequencies, int pairs, int layout, float magnitude,
+                      void* pages, int64_t num_pages, int page_size, int kv_heads, int head_dim,
+                      void* stream) {
+  return exl3_cache_append_axes(q, q_token, q_head, q_out, q_heads, k, k_token, k_head, v, v_token, v_head, tokens, type,
+                                slots, positions, wide_positions, nullptr, 1, frequencies, pairs, layout, magnitude, pages,
+                                num_pages, page_size, kv_heads, head_dim, stream);
 }
 
 int exl3_cache_read(const void* pages, int64_t num_pages, int page_size, int kv_heads, int head_dim,
@@ -743,6 +1085,59 @@ int exl3_cache_read(const void* pages, int64_t num_pages, int page_size, int kv_
   const uint8_t* p = static_cast<const uint8_t*>(pages);
   auto launch = type == 0 ? launch_read<F32> : type == 1 ? launch_read<F16> : launch_read<BF16>;
   return launch(p, k, v, a, (hipStream_t)stream);
+}
+
+int exl3_plan_tree(const int32_t* parents, const int32_t* starts, const int32_t* lengths, int requests,
+                   int64_t max_tokens, int words, int64_t* masks, int32_t* positions, void* stream) {
+  if (check_drafts("exl3_plan_tree", requests, max_tokens)) return 1;
+  if (words < 1 || 64 * words > MAX_TREE)
+    return set_error("exl3_plan_tree: words must be in 1..%d, got %d", MAX_TREE / 64, words);
+  const TreeArgs a{parents, starts, lengths, max_tokens, requests};
+  tree_kernel<<<(unsigned)requests + 8, TREE_THREADS, 0, (hipStream_t)stream>>>(a, words, reinterpret_cast<uint64_t*>(masks),
+                                                                              positions);
+  return check_launch("exl3_plan_tree");
+}
+
+int exl3_accept_drafts(const void* tokens, const void* choices, int wide, const int32_t* parents,
+                       const int32_t* starts, const int32_t* lengths, const int32_t* certain, int requests,
+                       int64_t max_tokens, int32_t* places, int32_t* kept, void* next, void* stream) {
+  if (check_drafts("exl3_accept_drafts", requests, max_tokens)) return 1;
+  const TreeArgs tree{parents, starts, lengths, max_tokens, requests};
+  auto launch = [&](auto id) {
+    typedef decltype(id) ID;
+    const AcceptArgs<ID> a{tree, static_cast<const ID*>(tokens), static_cast<const ID*>(choices), certain, places, kept,
+                           static_cast<ID*>(next)};
+    accept_kernel<ID><<<(unsigned)requests + 8, 64, 0, (hipStream_t)stream>>>(a);
+    return check_launch("exl3_accept_drafts");
+  };
+  return wide ? launch((int64_t)0) : launch((int32_t)0);
+}
+
+int exl3_release_pages(const int32_t* before, const int32_t* after, int requests, int32_t* tables, int width,
+                       int page_size, int32_t* free_pages, int free_count, const int32_t* taken, int32_t* taken_out,
+                       void* stream) {
+  CacheShape cache;
+  if (check_cache("exl3_release_pages", 0, page_size, 1, 64, &cache)) return 1;
+  if (check_drafts("exl3_release_pages", requests, 0)) return 1;
+  if (width < 1 || (int64_t)width * page_size > INT32_MAX || (int64_t)width * requests > INT32_MAX)
+    return set_error("exl3_release_pages: bad table width %d", width);
+  if (free_count < 0) return set_error("exl3_release_pages: bad sizes");
+  const ReleaseArgs a{before, after, taken, tables, free_pages, taken_out, requests, width, cache.tile_shift + 5, free_count};
+  release_kernel<<<1, STEP_THREADS, 4 * (requests + 1), (hipStream_t)stream>>>(a);
+  return check_launch("exl3_release_pages");
+}
+
+int exl3_cache_keep(void* pages, int64_t num_pages, int page_size, int kv_heads, int head_dim, const int64_t* slots,
+                    const int32_t* starts, const int32_t* places, int requests, int64_t max_tokens, void* stream) {
+  KeepArgs a{};
+  if (check_cache("exl3_cache_keep", num_pages, page_size, kv_heads, head_dim, &a.cache)) return 1;
+  if (check_drafts("exl3_cache_keep", requests, max_tokens)) return 1;
+  if (!aligned16(pages)) return set_error("exl3_cache_keep: pages must be 16-byte aligned");
+  if (!max_tokens) return 0;
+  a.tree = TreeArgs{nullptr, starts, nullptr, max_tokens, requests};
+  a.slots = slots, a.places = places;
+  keep_kernel<<<dim3((unsigned)requests, (unsigned)kv_heads), 256, 0, (hipStream_t)stream>>>(static_cast<uint8_t*>(pages), a);
+  return check_launch("exl3_cache_keep");
 }
 
 }  // extern "C"

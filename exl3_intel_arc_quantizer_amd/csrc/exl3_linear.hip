@@ -590,6 +590,7 @@ extern "C" {
 
 int64_t exl3_linear_workspace(int64_t rows, int64_t k, int64_t n, int type) {
   if (rows < 0 || rows > 1 << 22 || k < HAD || n < HAD || k % HAD || n % HAD || k > 1 << 24 || n > 1 << 24) return -1;
+  if (!rows) return 0;
   const Plan p = plan_of(rows, k, n, type == 2);
   return p.z_bytes + p.scale_bytes + p.partial_bytes;
 }

@@ -13,7 +13,19 @@ served model is
     out = cache_attention(q, pages, tables, plan.starts, plan.lengths,
                           max_new=most)               # most new tokens of a request
 
-with no host synchronisation in it. The cache of a layer is one uint8 tensor
+with no host synchronisation in it. Drafted tokens of a request may be a tree:
+
+    tree = plan_tree(parents, plan.starts, plan.lengths, max_new=most)
+    q = append_tokens(..., positions=tree.positions, ...)
+    out = cache_attention(..., trees=tree.masks)
+    ...                                               # the model's choice after every token
+    kept = accept_drafts(tokens, choices, parents, plan.starts, plan.lengths)
+    taken = release_pages(plan.lengths, kept.lengths, tables, free_pages, plan.taken,
+                          page_size=64)
+    keep_tokens(pages, plan.slots, plan.starts, kept.places)     # every layer
+
+after which the requests hold ``kept.lengths`` tokens, and ``kept.next`` follows.
+The cache of a layer is one uint8 tensor
 (``cache_pages``); tables, slots and lengths serve all layers. The functions
 enqueue work on the current stream of the tensors' device and keep nothing
 between calls. None of them has a gradient except the rotary step, which is
@@ -100,18 +112,19 @@ def _unrecorded(what: str, *tensors) -> None:
 def append_tokens(pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, *,
                   q: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
                   frequencies: Optional[torch.Tensor] = None, layout: str = "half",
-                  magnitude: float = 1.0) -> Optional[torch.Tensor]:
+                  magnitude: float = 1.0, axes: Optional[torch.Tensor] = None
+                  ) -> Optional[torch.Tensor]:
     """Write keys and values (tokens, kv_heads, head_dim) to their slots
     (int64), in place; tokens with a slot outside the cache are skipped.
 
     With ``frequencies`` (a multiple of 8 pairs) and ``positions`` the keys
-    first turn as in ``rotary.apply_rotary``, and so do the queries ``q``
+    first turn as in ``rotary.apply_rotary`` (with ``axes`` too), and so do the queries ``q``
     (tokens, q_heads, head_dim) if given, which are returned: the cache's side
     of a step is then one launch that reads the projection once. No slot may
     be given twice in a call."""
     _unrecorded("append_tokens", k, v, q, frequencies)
     return _native.cache_append(pages, k, v, slots, q, positions, frequencies,
-                                layout_code(layout), magnitude)
+                                layout_code(layout), magnitude, axes)
 
 
 def read_tokens(pages: torch.Tensor, slots: torch.Tensor, *,
@@ -124,7 +137,8 @@ def read_tokens(pages: torch.Tensor, slots: torch.Tensor, *,
 def cache_attention(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor,
                     starts: torch.Tensor, lengths: torch.Tensor, *,
                     scale: Optional[float] = None, window: Optional[int] = None,
-                    max_new: Optional[int] = None) -> torch.Tensor:
+                    max_new: Optional[int] = None,
+                    trees: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of a step's new tokens over the cache, with its new tokens
     appended already; (tokens, q_heads, head_dim) like ``q`` (float16 or
     bfloat16), which may have more query heads than the cache has kv heads (a
@@ -142,8 +156,81 @@ def cache_attention(q: torch.Tensor, pages: torch.Tensor, tables: torch.Tensor,
     rows beside its own (128 requests of 4096 positions: 134 us with
     ``max_new=1``, 178 without).
 
+    ``trees`` (int64, (tokens or more, words), ``plan_tree``) are masks of the new
+    tokens: of a request with up to 64 * words of them, row i attends the positions
+    before the request's new tokens and its new token j where bit j of the row's
+    mask is set (bit j % 64 of word j // 64), of this sequence the last ``window``.
+    Any mask may be given; a row that it leaves empty is 0. Requests with more new
+    tokens attend as without.
+
     Queries count with 22 bits, and so do the weights of requests of up to 16
     rows to a kv head (32 of head_dim 256); beyond, weights count with 11 bits, as
     in products of 16-bit operands. Scores, maxima and sums are float32."""
     _unrecorded("cache_attention", q)
-    return _native.cache_attention(q, pages, tables, starts, lengths, scale, window, max_new)
+    return _native.cache_attention(q, pages, tables, starts, lengths, scale, window, max_new, trees)
+
+
+class TreePlan(NamedTuple):
+    """What a step's layers share of the trees of drafted tokens, on the GPU."""
+
+    masks: torch.Tensor      # int64 (tokens, words): a token's ancestors and itself
+    positions: torch.Tensor  # int32 (tokens,): its position, one more than its parent's
+
+
+def plan_tree(parents: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor, *,
+              max_new: int) -> TreePlan:
+    """Masks and positions of a step whose new tokens are trees.
+
+    ``parents`` (int32, (tokens,), as many as the step's slots) gives, for each new
+    token of a request (rows starts[r] .. starts[r + 1] - 1, the last of its
+    lengths[r] tokens), the place among them of the token it follows, counted from
+    0 and less than its own, or -1 if it follows the cached ones; any other number
+    counts as -1. ``max_new`` (at most 1024) bounds the tokens of a tree: masks
+    have ceil(max_new / 64) words, and a request of more tokens than they have bits
+    is no tree but a run: its positions count up. Tokens of no request get 0."""
+    if not 1 <= max_new <= 64 * _native.MAX_TREE_WORDS:
+        raise ValueError(f"max_new must be in 1..{64 * _native.MAX_TREE_WORDS}, got {max_new}")
+    return TreePlan(*_native.plan_tree(parents, starts, lengths, -(-max_new // 64)))
+
+
+class Accepted(NamedTuple):
+    """What a step keeps of its drafted tokens, on the GPU."""
+
+    places: torch.Tensor     # int32 (tokens,): place among the request's kept tokens, or -1
+    lengths: torch.Tensor    # int32 (requests,): tokens held, those kept among them
+    next: torch.Tensor       # (requests,): the token chosen after the last kept one
+
+
+def accept_drafts(tokens: torch.Tensor, choices: torch.Tensor, parents: torch.Tensor,
+                  starts: torch.Tensor, lengths: torch.Tensor, *,
+                  certain: Optional[torch.Tensor] = None) -> Accepted:
+    """The drafted tokens that the model would have chosen itself.
+
+    ``tokens`` are the step's token ids and ``choices`` the model's choice after
+    each of them (int32 or int64, (tokens,)); ``parents``, ``starts`` and
+    ``lengths`` as in ``plan_tree``. Of every request the first ``certain`` tokens
+    (int32, (requests,); at least, and if left out, the first: the one that the
+    last step chose) are kept, then from the last of them down, as long as there is
+    one, the first token after those whose parent is the last kept and which is the
+    choice after it. ``next`` is -1 for requests without new tokens."""
+    return Accepted(*_native.accept_drafts(tokens, choices, parents, starts, lengths, certain))
+
+
+def keep_tokens(pages: torch.Tensor, slots: torch.Tensor, starts: torch.Tensor,
+                places: torch.Tensor) -> None:
+    """Move the entries of kept tokens together, in place: a token goes to the slot
+    of its request's token number ``places`` (int32, as ``accept_drafts`` gives
+    them: growing along a request, -1 for tokens that stay where they are, and no
+    larger than its own number). ``slots`` and ``starts`` are the step's; moves from
+    or to a slot outside the cache are skipped."""
+    _native.cache_keep(pages, slots, starts, places)
+
+
+def release_pages(before: torch.Tensor, after: torch.Tensor, tables: torch.Tensor,
+                  free_pages: torch.Tensor, taken: torch.Tensor, *, page_size: int) -> torch.Tensor:
+    """Give back the pages of requests that held ``before`` tokens and keep
+    ``after`` of them (int32, (requests,); 0 ends a request): their entries of
+    ``tables`` become -1 and the pages, in order, the last of ``free_pages`` before
+    entry ``taken``, both in place. Returns the new ``taken``; the step plans'
+    ``free_pages`` are thus a stack, from which the next ``plan_step`` takes."""
+    return _native.release_pages(before, after, tables, free_pages, taken, page_size)

@@ -10,7 +10,7 @@ same on the way into a cache.
 from __future__ import annotations
 
 import math
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -68,35 +68,50 @@ def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0,
     return freq.to(device), magnitude
 
 
+def rotary_axes(sections: Sequence[int], *, interleaved: bool = False,
+                device="cuda") -> torch.Tensor:
+    """The axis of every pair, int32 on ``device``, for models whose tokens have
+    several positions (time, height and width): ``sections[a]`` pairs of axis a,
+    one axis after the other, or (``interleaved``) in turn, each round a pair of
+    every axis that has some left."""
+    sections = [int(n) for n in sections]
+    if not sections or min(sections) < 0 or not sum(sections):
+        raise ValueError(f"sections must hold pairs of each axis, got {sections}")
+    if interleaved:
+        axes = [a for turn in range(max(sections)) for a, n in enumerate(sections) if turn < n]
+    else:
+        axes = [a for a, n in enumerate(sections) for _ in range(n)]
+    return torch.tensor(axes, dtype=torch.int32, device=device)
+
+
 class _Rotary(torch.autograd.Function):
     """The rotation is linear: its gradient turns back, its tangent turns the
     same way. Both can be differentiated again."""
 
     @staticmethod
-    def forward(ctx, q, k, positions, frequencies, layout, magnitude, inverse):
+    def forward(ctx, q, k, positions, frequencies, axes, layout, magnitude, inverse):
         # Saved, so that torch refuses a backward pass after they were written to.
-        ctx.save_for_backward(positions, frequencies)
-        ctx.save_for_forward(positions, frequencies)
+        ctx.save_for_backward(positions, frequencies, axes)
+        ctx.save_for_forward(positions, frequencies, axes)
         ctx.given = (layout, magnitude, inverse)
         ctx.two = k is not None
         ctx.shapes = q.shape, k.shape if ctx.two else None
         ctx.set_materialize_grads(False)
-        q_out, k_out = _native.rotary(q, k, positions, frequencies, layout, magnitude, inverse)
+        q_out, k_out = _native.rotary(q, k, positions, frequencies, layout, magnitude, inverse,
+                                      axes=axes)
         return (q_out, k_out) if ctx.two else (q_out,)
 
     @staticmethod
     def backward(ctx, *grads):
-        positions, frequencies = ctx.saved_tensors
         layout, magnitude, inverse = ctx.given
-        out = _turned(grads[0], grads[1] if ctx.two else None, positions, frequencies, layout,
+        out = _turned(grads[0], grads[1] if ctx.two else None, *ctx.saved_tensors, layout,
                       magnitude, not inverse)
-        return (*out, None, None, None, None, None)
+        return (*out, None, None, None, None, None, None)
 
     @staticmethod
     def jvp(ctx, *tangents):
-        positions, frequencies = ctx.saved_tensors
         layout, magnitude, inverse = ctx.given
-        q, k = _turned(tangents[0], tangents[1], positions, frequencies, layout, magnitude, inverse)
+        q, k = _turned(tangents[0], tangents[1], *ctx.saved_tensors, layout, magnitude, inverse)
         if not ctx.two:
             return (q,)
         # torch asks for a tangent of every output: that of an input without one is 0.
@@ -104,17 +119,17 @@ class _Rotary(torch.autograd.Function):
                      for x, other, shape in ((q, k, ctx.shapes[0]), (k, q, ctx.shapes[1])))
 
 
-def _turned(q, k, positions, frequencies, layout, magnitude, inverse):
+def _turned(q, k, positions, frequencies, axes, layout, magnitude, inverse):
     """Both turned; either may be None (and stays None)."""
     if q is None:
         return (None, None) if k is None else \
-            (None, _turned(k, None, positions, frequencies, layout, magnitude, inverse)[0])
+            (None, _turned(k, None, positions, frequencies, axes, layout, magnitude, inverse)[0])
     # A gradient may arrive expanded or with any strides.
     q, k = (x if x is None or x.stride(-1) == 1 else x.contiguous() for x in (q, k))
     if records(q) or (k is not None and records(k)):
-        out = _Rotary.apply(q, k, positions, frequencies, layout, magnitude, inverse)
+        out = _Rotary.apply(q, k, positions, frequencies, axes, layout, magnitude, inverse)
         return out if k is not None else (out[0], None)
-    return _native.rotary(q, k, positions, frequencies, layout, magnitude, inverse)
+    return _native.rotary(q, k, positions, frequencies, layout, magnitude, inverse, axes=axes)
 
 
 def layout_code(layout: str) -> int:
@@ -125,7 +140,7 @@ def layout_code(layout: str) -> int:
 
 def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
                  frequencies: torch.Tensor, *, layout: str = "half", magnitude: float = 1.0,
-                 out: Optional[tuple] = None) -> tuple:
+                 out: Optional[tuple] = None, axes: Optional[torch.Tensor] = None) -> tuple:
     """(q, k) turned by their positions, as new contiguous tensors or into
     ``out`` (a pair like q and k: the inputs themselves, or tensors that share no
     memory with them or each other), where torch records neither the inputs nor
@@ -138,7 +153,11 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     layout ``"half"``, (2 i, 2 i + 1) for ``"interleaved"``; the values past
     the pairs are copied; frequencies have no gradient. Angles are taken in 64
     bits and products in 32, so positions in the millions are as exact as the
-    first ones."""
+    first ones.
+
+    With ``axes`` (int32, one of every pair: ``rotary_axes``) ``positions`` are
+    (axes, tokens), and pair i turns by its frequency times the position on axis
+    ``axes[i]``; pairs whose axis is not one of those do not turn."""
     code = layout_code(layout)
     if isinstance(frequencies, torch.Tensor) and records(frequencies):
         raise RuntimeError("apply_rotary has no gradient of frequencies: detach them")
@@ -147,5 +166,5 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
                                             for t in out)):
         raise RuntimeError("apply_rotary: out cannot be given where torch records it or the inputs")
     if recorded:
-        return _turned(q, k, positions, frequencies, code, magnitude, False)
-    return _native.rotary(q, k, positions, frequencies, code, magnitude, False, out)
+        return _turned(q, k, positions, frequencies, axes, code, magnitude, False)
+    return _native.rotary(q, k, positions, frequencies, code, magnitude, False, out, axes)

@@ -257,6 +257,16 @@ int exl3_rotary(const void* q, int64_t q_token, int64_t q_head, void* q_out, int
                 const double* frequencies, int pairs, int layout, float magnitude, int inverse,
                 void* stream);
 
+/* exl3_rotary with positions of several axes (time, height and width):
+ * positions is (num_axes, tokens), and pair i turns by positions[axes[i]]; a
+ * pair whose axis is not one of them turns by 0. axes NULL: as exl3_rotary. */
+int exl3_rotary_axes(const void* q, int64_t q_token, int64_t q_head, void* q_out, int64_t qo_token,
+                     int64_t qo_head, int q_heads, const void* k, int64_t k_token, int64_t k_head,
+                     void* k_out, int64_t ko_token, int64_t ko_head, int k_heads, int64_t tokens,
+                     int head_dim, int type, const void* positions, int wide_positions,
+                     const int32_t* axes, int num_axes, const double* frequencies, int pairs,
+                     int layout, float magnitude, int inverse, void* stream);
+
 /* The tables of one serving step from the requests' lengths (cached: tokens
  * held, fresh: new ones; negative counts as 0; at most 4096 requests). A
  * request holds ceil(cached / page_size) pages in its row of `tables`
@@ -288,6 +298,15 @@ int exl3_cache_append(const void* q, int64_t q_token, int64_t q_head, void* q_ou
                       void* pages, int64_t num_pages, int page_size, int kv_heads, int head_dim,
                       void* stream);
 
+/* exl3_cache_append with positions of several axes, as in exl3_rotary_axes. */
+int exl3_cache_append_axes(const void* q, int64_t q_token, int64_t q_head, void* q_out, int q_heads,
+                           const void* k, int64_t k_token, int64_t k_head, const void* v,
+                           int64_t v_token, int64_t v_head, int64_t tokens, int type,
+                           const int64_t* slots, const void* positions, int wide_positions,
+                           const int32_t* axes, int num_axes, const double* frequencies, int pairs,
+                           int layout, float magnitude, void* pages, int64_t num_pages,
+                           int page_size, int kv_heads, int head_dim, void* stream);
+
 /* The keys and values that the entries at `slots` stand for, contiguous
  * (tokens, kv_heads, head_dim); zeros for slots outside the cache. */
 int exl3_cache_read(const void* pages, int64_t num_pages, int page_size, int kv_heads, int head_dim,
@@ -315,6 +334,62 @@ int exl3_cache_attention(const void* q, int64_t q_token, int64_t q_head, void* o
                          const int32_t* starts, const int32_t* lengths, int requests, float scale,
                          int64_t window, int64_t max_new, void* workspace, int64_t workspace_bytes,
                          void* stream);
+
+/* exl3_cache_attention with trees of drafted tokens. masks is (tokens, words) of
+ * 64 bits (1 to 16 words). Of a request with n <= 64 words new tokens, which are
+ * the last n of its lengths[r] positions, row i attends the positions before them
+ * and new token j where bit j of its mask is set, of this sequence the last
+ * `window` places; a mask may leave a row empty, which is 0 then. Requests with
+ * more new tokens attend as in exl3_cache_attention. The same workspace. masks
+ * NULL: exl3_cache_attention. */
+int exl3_cache_attention_trees(const void* q, int64_t q_token, int64_t q_head, void* out,
+                               int64_t tokens, int q_heads, int type, const void* pages,
+                               int64_t num_pages, int page_size, int kv_heads, int head_dim,
+                               const int32_t* tables, int width, const int32_t* starts,
+                               const int32_t* lengths, int requests, const int64_t* masks, int words,
+                               float scale, int64_t window, int64_t max_new, void* workspace,
+                               int64_t workspace_bytes, void* stream);
+
+/* Masks and positions of trees of drafted tokens. Request r's are tokens
+ * starts[r] .. starts[r + 1] - 1 of max_tokens, the last of lengths[r]
+ * positions; parents[t] is the place among them (0 the first) of the token that t
+ * follows, which is before t, or -1 (as is any other number) for the tokens
+ * cached before. A token's mask, `words` (1 to 16) of 64 bits, names its ancestors
+ * and itself, its position is that of the first new token plus its ancestors'
+ * number. Requests of more than 64 words tokens are no trees: masks 0, positions
+ * counting up. Tokens of no request: 0. */
+int exl3_plan_tree(const int32_t* parents, const int32_t* starts, const int32_t* lengths,
+                   int requests, int64_t max_tokens, int words, int64_t* masks, int32_t* positions,
+                   void* stream);
+
+/* The drafted tokens that the model would have chosen itself. choices[t] is its
+ * choice after token t; both are int64 if `wide`, else int32. A request keeps its
+ * first certain[r] tokens (at least its first; certain NULL: that one), and then
+ * from the last of them down, as long as there is one, the first token past them
+ * whose parent is the last kept and which is the choice after it. places[t] is a
+ * token's place among those kept, -1 if it is not (or of no request); kept[r] the
+ * request's tokens cached before plus those kept, next[r] the choice after the
+ * last kept, -1 where there are no new tokens. */
+int exl3_accept_drafts(const void* tokens, const void* choices, int wide, const int32_t* parents,
+                       const int32_t* starts, const int32_t* lengths, const int32_t* certain,
+                       int requests, int64_t max_tokens, int32_t* places, int32_t* kept, void* next,
+                       void* stream);
+
+/* Moves the entry of every token t with 0 <= places[t] < its place in its request
+ * to the slot of the request's token of that place, keys and values of all heads.
+ * places grow along a request's kept tokens, as exl3_accept_drafts gives them, and
+ * no two slots are alike. Moves from or to a slot outside the cache are skipped. */
+int exl3_cache_keep(void* pages, int64_t num_pages, int page_size, int kv_heads, int head_dim,
+                    const int64_t* slots, const int32_t* starts, const int32_t* places, int requests,
+                    int64_t max_tokens, void* stream);
+
+/* Gives back the pages of requests that held before[r] tokens and keep after[r]
+ * of them (none: all its pages): entries ceil(after / page_size) to ceil(before /
+ * page_size) of its row become -1, and their pages (where there are any) the last
+ * of free_pages before *taken, in order; *taken_out = *taken less their number. */
+int exl3_release_pages(const int32_t* before, const int32_t* after, int requests, int32_t* tables,
+                       int width, int page_size, int32_t* free_pages, int free_count,
+                       const int32_t* taken, int32_t* taken_out, void* stream);
 
 #ifdef __cplusplus
 }
