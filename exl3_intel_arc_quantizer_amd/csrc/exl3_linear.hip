@@ -206,21 +206,11 @@ __device__ __forceinline__ void lane_butterfly(float& x, float& y) {
   swap(x, y);
 }
 
-// The hash of a state, s M + A. A state has 16 bits: two 24-bit products, which
-// run at full rate where a 32-bit one takes four times as long. (The empty asm
-// keeps the compiler from making one 32-bit product of them.)
-template <int CB>
-__device__ __forceinline__ uint32_t hash_of(uint32_t s) {
-  uint32_t high = s * (hash_mult(CB) >> 24);
-  asm("" : "+v"(high));
-  return (high << 24) + (s * (hash_mult(CB) & 0xffffffu) + (CB == 0 ? 64248484u : 0u));
-}
-
 // The values of two states (exl3_codebook.h): the sum of a hash's bytes, scaled,
 // or the sum of its halves.
 template <int CB>
 __device__ __forceinline__ uint32_t values_of(uint32_t s0, uint32_t s1) {
-  const uint32_t x0 = hash_of<CB>(s0), x1 = hash_of<CB>(s1);
+  const uint32_t x0 = hash_state(CB, s0), x1 = hash_state(CB, s1);  // (32-bit products run at full rate)
   if constexpr (CB == 2) {
     const uint32_t sums = __builtin_amdgcn_sad_hi_u8(x1, 0u, __builtin_amdgcn_sad_u8(x0, 0u, 0x64006400u));
     const f16 scale = f16_bits(0x1EEEu), shift = f16_bits(0xC931u);
@@ -253,24 +243,26 @@ struct Words {
   uint32_t w[CT][2][WIDE ? 4 : 2];
 };
 
+// Two of the four values of a lane's states of a tile (the first, or of H = 1 the
+// last), so that decoding can be spread over other work.
+template <bool WIDE, int CB, int H>
+__device__ __forceinline__ uint32_t half_of(const uint32_t (&w)[WIDE ? 4 : 2], const Window& late, const Window& early, uint32_t bits) {
+  if constexpr (WIDE) {
+    const uint32_t v = H ? __builtin_amdgcn_alignbit(w[0], w[1], late.shift) : __builtin_amdgcn_alignbit(w[2], w[3], early.shift);
+    return values_of<CB>(__builtin_amdgcn_ubfe(v, bits, 16), v & 0xffffu);
+  }
+  const uint32_t v = __builtin_amdgcn_alignbit(w[0], w[1], late.shift);
+  if constexpr (H) return values_of<CB>(__builtin_amdgcn_ubfe(v, bits, 16), v & 0xffffu);
+  return values_of<CB>(__builtin_amdgcn_ubfe(v, 3 * bits, 16), __builtin_amdgcn_ubfe(v, 2 * bits, 16));
+}
+
 // The four values of a lane's states, of both tiles of a step: its operand.
 template <bool WIDE, int CB>
 __device__ __forceinline__ u32x4 operand_of(const uint32_t (&w)[2][WIDE ? 4 : 2], const Window& late, const Window& early, uint32_t bits) {
   u32x4 f;
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const uint32_t v = __builtin_amdgcn_alignbit(w[t][0], w[t][1], late.shift);
-    const uint32_t s3 = v & 0xffffu, s2 = __builtin_amdgcn_ubfe(v, bits, 16);
-    uint32_t s1, s0;
-    if constexpr (WIDE) {
-      const uint32_t e = __builtin_amdgcn_alignbit(w[t][2], w[t][3], early.shift);
-      s1 = e & 0xffffu, s0 = __builtin_amdgcn_ubfe(e, bits, 16);
-    } else {
-      s1 = __builtin_amdgcn_ubfe(v, 2 * bits, 16), s0 = __builtin_amdgcn_ubfe(v, 3 * bits, 16);
-    }
-    f[2 * t] = values_of<CB>(s0, s1);
-    f[2 * t + 1] = values_of<CB>(s2, s3);
-  }
+  for (int t = 0; t < 2; ++t)
+    f[2 * t] = half_of<WIDE, CB, 0>(w[t], late, early, bits), f[2 * t + 1] = half_of<WIDE, CB, 1>(w[t], late, early, bits);
   return f;
 }
 
@@ -287,7 +279,7 @@ struct Reader {
     row_bytes = (int64_t)(a.n / 16) * 32 * bits;
     next = reinterpret_cast<const char*>(a.words) + 2 * step * row_bytes + (int64_t)column * 32 * bits;
   }
-  __device__ __forceinline__ Words<WIDE, CT> load() {
+  __device__ __forceinline__ Words<WIDE, CT> load(bool on = true) {
     Words<WIDE, CT> r;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -298,10 +290,16 @@ struct Reader {
         r.w[c][t][0] = word(late.at0), r.w[c][t][1] = word(late.at1);
         if constexpr (WIDE) r.w[c][t][2] = word(early.at0), r.w[c][t][3] = word(early.at1);
       }
-    next += 2 * row_bytes;
+    next += on ? 2 * row_bytes : 0;
     return r;
   }
 };
+
+// Sixteen bytes a lane from memory to shared memory, to `to` and on from there.
+__device__ __forceinline__ void to_shared(const u32x4* from, u32x4* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                   (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
 
 // Up to 16 rows: every wave takes CT column tiles and its share of the input
 // channels; a workgroup's waves add up in shared memory.
@@ -360,21 +358,16 @@ __global__ void __launch_bounds__(64 * WAVES) linear_kernel(LinearArgs a) {
 
 // More rows: a workgroup takes a block of 16 MT rows and, four waves, 64 CT
 // columns of a share of the input channels. The rows come through shared memory,
-// two buffers of STEPS steps, for all waves; each decodes its own columns. Blocks
-// with all channels (splits == 1) are finished here: a lane holds channels 4 (lane
-// / 16) .. + 3 of its tiles, so of the output's transform two levels lie in a
-// lane's registers, two across lanes, two across its CT = 4 tiles, and one across
-// two waves.
-template <bool WIDE, int CB, bool BF16, int MT, int PARTS, int CT>
+// two buffers of STEPS steps, for all waves; each decodes its own columns.
+template <bool WIDE, int CB, int MT, int PARTS, int CT>
 __global__ void __launch_bounds__(256, 2) linear_tiles_kernel(LinearArgs a) {
-  constexpr int SETS = MT * PARTS, STEPS = SETS > 8 ? 2 : 4, STAGE = STEPS * SETS * 64;  // vectors of a buffer
+  constexpr int SETS = MT * PARTS, STEPS = 4, STAGE = STEPS * SETS * 64;  // vectors of a buffer
   __shared__ u32x4 held[2 * STAGE];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int column0 = (blockIdx.x * 4 + wave) * CT, split = blockIdx.y, block = blockIdx.z;
   const int stages = a.k / (32 * STEPS);
   const int begin = (int)((int64_t)stages * split / a.splits), end = (int)((int64_t)stages * (split + 1) / a.splits);
-  const bool there = column0 < a.n / 16;                 // (a wave past the columns reads the first ones)
-  Reader<WIDE, CT> reader(a, begin * STEPS, there ? column0 : 0, lane);
+  Reader<WIDE, CT> reader(a, begin * STEPS, column0, lane);
   const u32x4* z = a.z + ((int64_t)block * (a.k / 32) + begin * STEPS) * SETS * 64;
   f32x4 acc[CT][MT];
 #pragma unroll
@@ -384,9 +377,7 @@ __global__ void __launch_bounds__(256, 2) linear_tiles_kernel(LinearArgs a) {
 
   auto fetch = [&](int buffer) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < STAGE / 256; ++i)
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(z + i * 256 + tid),
-                                       (__attribute__((address_space(3))) void*)(held + buffer * STAGE + i * 256 + wave * 64), 16, 0, 0);
+    for (int i = 0; i < STAGE / 256; ++i) to_shared(z + i * 256 + tid, held + buffer * STAGE + i * 256 + wave * 64);
     z += STAGE;
   };
   if (begin < end) {
@@ -413,8 +404,116 @@ __global__ void __launch_bounds__(256, 2) linear_tiles_kernel(LinearArgs a) {
       }
     }
   }
+#pragma unroll
+  for (int c = 0; c < CT; ++c)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int row = block * 16 * MT + 16 * m + (lane & 15), column = 16 * (column0 + c) + 4 * (lane >> 4);
+      if (row < a.rows) *reinterpret_cast<f32x4*>(a.partials + ((int64_t)split * a.rows + row) * a.n + column) = acc[c][m];
+    }
+}
+
+// Many rows: a workgroup takes 16 MT rows and 256 columns, 64 a wave and one wave
+// a SIMD, whose sums fill half of its registers. A step is then 4 MT PARTS matrix
+// instructions and 16 halves of tiles to decode for the next one; a matrix
+// instruction takes as long as four vector ones and runs beside them, so a step's
+// are dealt out one by three. Rows come through shared memory as above, a part
+// of the next buffer each step, and operands are read from it AHEAD sets before
+// their use.
+//
+// Blocks of all input channels (splits == 1) are finished here: a lane holds
+// channels 4 (lane / 16) .. + 3 of its tiles, so of the output's transform two
+// levels lie in a lane's registers, two across lanes, two across its four tiles,
+// and one across two waves.
+template <bool WIDE, int CB, bool BF16, int MT, int PARTS>
+__global__ void __launch_bounds__(256, 2) linear_blocks_kernel(LinearArgs a) {
+  constexpr int CT = 4, SETS = MT * PARTS, STEPS = SETS > 8 ? 2 : 4, STAGE = STEPS * SETS * 64, AHEAD = 4;
+  constexpr int LOADS = STAGE / 256, HALVES = 4 * CT;    // a lane's of a buffer, and of a step
+  constexpr int RING = 2;                                // steps whose words are on their way
+  __shared__ u32x4 held[2 * STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // Workgroups are dealt to the chip's eight dies in turn: each die takes a run
+  // of them, which share a block of rows in its cache.
+  const int groups = (a.n + 255) / 256, all = gridDim.x, die = blockIdx.x & 7;
+  const int unit = die * (all / 8) + min(die, all % 8) + (int)(blockIdx.x >> 3);
+  const int split = unit % a.splits, group = unit / a.splits % groups, block = unit / a.splits / groups;
+  const int column0 = (group * 4 + wave) * CT;
+  const int stages = a.k / (32 * STEPS);
+  const int begin = (int)((int64_t)stages * split / a.splits), end = (int)((int64_t)stages * (split + 1) / a.splits);
+  const bool there = column0 < a.n / 16;                 // (waves past the columns read the first ones)
+  Reader<WIDE, CT> reader(a, begin * STEPS, there ? column0 : 0, lane);
+  const u32x4* z = a.z + ((int64_t)block * (a.k / 32) + begin * STEPS) * SETS * 64 + tid;
+  f32x4 acc[CT][MT];
+#pragma unroll
+  for (int c = 0; c < CT; ++c)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[c][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  // Part `step` of a buffer's rows, all in the first half of the STEPS.
+  auto fetch = [&](int buffer, int step) __attribute__((always_inline)) {
+    constexpr int EACH = LOADS / (STEPS / 2);
+#pragma unroll
+    for (int i = step * EACH; i < (step + 1) * EACH && i < LOADS; ++i)
+      to_shared(z + i * 256, held + buffer * STAGE + i * 256 + wave * 64);
+  };
+  if (begin < end) {
+    const int last = (end - begin) * STEPS - 1;          // step
+#pragma unroll
+    for (int step = 0; step < STEPS; ++step) fetch(0, step);
+    z += begin + 1 < end ? STAGE : 0;
+    asm volatile("" ::: "memory");                       // words after rows: see the wait below
+    __builtin_amdgcn_sched_barrier(0);
+    Words<WIDE, CT> words[RING];
+#pragma unroll
+    for (int i = 0; i < RING; ++i) words[i] = reader.load(i < last);
+    u32x4 f[2][CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) f[0][c] = operand_of<WIDE, CB>(words[0].w[c], reader.late, reader.early, reader.bits);
+    for (int stage = begin; stage < end; ++stage) {
+      const int now = (stage - begin) & 1;
+      const u32x4* rows = held + now * STAGE + lane;
+      // For the rows that this wave fetched in the first half of the steps: words
+      // were loaded in the others, CT 2 (or, in pairs, CT) loads a step at least,
+      // and stay on their way.
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(CT * STEPS) : "memory");
+      u32x4 b[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) b[i] = rows[i * 64];
+#pragma unroll
+      for (int step = 0; step < STEPS; ++step) {
+        // (Past the last step and stage the last ones again, which nobody uses: a
+        // branch would cut the loop's body, whose registers then do not agree.)
+        words[step % RING] = reader.load((stage - begin) * STEPS + step + RING < last);
+        fetch(now ^ 1, step);
+        u32x4 (&here)[CT] = f[step & 1], (&next)[CT] = f[(step + 1) & 1];
+        const Words<WIDE, CT>& coming = words[(step + 1) % RING];
+#pragma unroll
+        for (int s = 0; s < SETS; ++s) {
+          const int set = step * SETS + s;
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int c = 0; c < CT; ++c) acc[c][s / PARTS] = mfma(here[c], b[set % AHEAD], acc[c][s / PARTS]);
+          if (set + AHEAD < STEPS * SETS) b[set % AHEAD] = rows[(set + AHEAD) * 64];
+          // This set's share of the next step's halves of tiles: (column tile, tile, half).
+#pragma unroll
+          for (int of = s * HALVES / SETS; of < (s + 1) * HALVES / SETS; ++of) {
+            const int c = of >> 2, t = of >> 1 & 1;
+            next[c][of & 3] = of & 1 ? half_of<WIDE, CB, 1>(coming.w[c][t], reader.late, reader.early, reader.bits)
+                                     : half_of<WIDE, CB, 0>(coming.w[c][t], reader.late, reader.early, reader.bits);
+          }
+#pragma unroll
+          for (int c = 0; c < CT; ++c) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      z += stage + 2 < end ? STAGE : 0;
+    }
+  }
   const int row0 = block * 16 * MT + (lane & 15);
-  if (CT != 4 || a.splits > 1) {
+  if (a.splits > 1) {
     if (!there) return;
 #pragma unroll
     for (int c = 0; c < CT; ++c)
@@ -425,49 +524,48 @@ __global__ void __launch_bounds__(256, 2) linear_tiles_kernel(LinearArgs a) {
       }
     return;
   }
-  if constexpr (CT == 4) {
-    f32x4* exchange = reinterpret_cast<f32x4*>(held);
-    constexpr int AT_ONCE = 2 * STAGE / (4 * CT * 64) < MT ? 2 * STAGE / (4 * CT * 64) : MT;
+  f32x4* exchange = reinterpret_cast<f32x4*>(held);
+  constexpr int AT_ONCE = 2;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
+  for (int m = 0; m < MT; ++m) {
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      f32x4& v = acc[c][m];
+      const float s0 = v[0] + v[1], s1 = v[0] - v[1], s2 = v[2] + v[3], s3 = v[2] - v[3];
+      float y[4] = {s0 + s2, s1 + s3, s0 - s2, s1 - s3};
+      lane_butterfly<16>(y[0], y[1]);
+      lane_butterfly<16>(y[2], y[3]);
+      lane_butterfly<32>(y[0], y[1]);
+      lane_butterfly<32>(y[2], y[3]);
+      v = f32x4{y[0], y[1], y[2], y[3]};
+    }
+    const f32x4 s0 = acc[0][m] + acc[1][m], s1 = acc[0][m] - acc[1][m], s2 = acc[2][m] + acc[3][m], s3 = acc[2][m] - acc[3][m];
+    acc[0][m] = s0 + s2, acc[1][m] = s1 + s3, acc[2][m] = s0 - s2, acc[3][m] = s1 - s3;
+    if (m % AT_ONCE != AT_ONCE - 1) continue;
+    // Two buffers take turns: a wave writes one after its partner has read the other.
+    const int m0 = m - AT_ONCE + 1;
+    f32x4* held_now = exchange + (m0 / AT_ONCE & 1) * (4 * AT_ONCE * CT * 64);
+    if (m0 == 0) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i)
+#pragma unroll
+      for (int c = 0; c < CT; ++c) held_now[((wave * AT_ONCE + i) * CT + c) * 64 + lane] = acc[c][m0 + i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const int row = row0 + 16 * (m0 + i);
+      const bool writes = there && row < a.rows;
+      const float scale = writes ? a.scale[row] * ROOT : 0.0f;
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
-        f32x4& v = acc[c][m];
-        const float s0 = v[0] + v[1], s1 = v[0] - v[1], s2 = v[2] + v[3], s3 = v[2] - v[3];
-        float y[4] = {s0 + s2, s1 + s3, s0 - s2, s1 - s3};
-        lane_butterfly<16>(y[0], y[1]);
-        lane_butterfly<16>(y[2], y[3]);
-        lane_butterfly<32>(y[0], y[1]);
-        lane_butterfly<32>(y[2], y[3]);
-        v = f32x4{y[0], y[1], y[2], y[3]};
-      }
-      f32x4 s0 = acc[0][m] + acc[1][m], s1 = acc[0][m] - acc[1][m], s2 = acc[2][m] + acc[3][m], s3 = acc[2][m] - acc[3][m];
-      acc[0][m] = s0 + s2, acc[1][m] = s1 + s3, acc[2][m] = s0 - s2, acc[3][m] = s1 - s3;
-    }
-#pragma unroll
-    for (int m0 = 0; m0 < MT; m0 += AT_ONCE) {
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i)
-#pragma unroll
-        for (int c = 0; c < CT; ++c) exchange[((wave * AT_ONCE + i) * CT + c) * 64 + lane] = acc[c][m0 + i];
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i) {
-        const int row = row0 + 16 * (m0 + i);
-        const bool writes = there && row < a.rows;
-        const float scale = writes ? a.scale[row] * ROOT : 0.0f;
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-          const int column = 16 * (column0 + c) + 4 * (lane >> 4);
-          const f32x4 other = exchange[(((wave ^ 1) * AT_ONCE + i) * CT + c) * 64 + lane];
-          const f32x4 v = wave & 1 ? other - acc[c][m0 + i] : acc[c][m0 + i] + other;
-          if (writes) {
-            u32x2 w;
-            w[0] = narrow<BF16>(v[0] * scale * a.sv.at(column)) | narrow<BF16>(v[1] * scale * a.sv.at(column + 1)) << 16;
-            w[1] = narrow<BF16>(v[2] * scale * a.sv.at(column + 2)) | narrow<BF16>(v[3] * scale * a.sv.at(column + 3)) << 16;
-            *reinterpret_cast<u32x2*>(a.out + (int64_t)row * a.n + column) = w;
-          }
+        const int column = 16 * (column0 + c) + 4 * (lane >> 4);
+        const f32x4 other = held_now[(((wave ^ 1) * AT_ONCE + i) * CT + c) * 64 + lane];
+        const f32x4 v = wave & 1 ? other - acc[c][m0 + i] : acc[c][m0 + i] + other;
+        if (writes) {
+          u32x2 w;
+          w[0] = narrow<BF16>(v[0] * scale * a.sv.at(column)) | narrow<BF16>(v[1] * scale * a.sv.at(column + 1)) << 16;
+          w[1] = narrow<BF16>(v[2] * scale * a.sv.at(column + 2)) | narrow<BF16>(v[3] * scale * a.sv.at(column + 3)) << 16;
+          *reinterpret_cast<u32x2*>(a.out + (int64_t)row * a.n + column) = w;
         }
       }
     }
@@ -517,7 +615,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(JoinArgs a) {
 // ------------------------------------------------------------ plan
 
 // Variants by the rows.
-enum Variant { ROWS8, ROWS16, BLOCK32, BLOCK64, BLOCK128 };
+enum Variant { ROWS8, ROWS16, TILES32, TILES64, BLOCK128, BLOCK256 };
 
 // How a call is cut.
 struct Plan {
@@ -528,13 +626,13 @@ struct Plan {
   int64_t z_bytes, scale_bytes, partial_bytes;
 };
 
-constexpr int CUS = 256;
+constexpr int CUS = 256, MANY = 8;
 
 Plan plan_of(int64_t rows, int64_t k, int64_t n, bool bf16) {
   Plan p{};
-  p.variant = rows <= 8 ? ROWS8 : rows <= 16 ? ROWS16 : rows <= 32 ? BLOCK32 : rows <= 64 ? BLOCK64 : BLOCK128;
-  p.parts = p.variant == BLOCK128 && bf16 ? 1 : 2;
-  p.block_rows = 8 << p.variant;
+  p.variant = rows <= 8 ? ROWS8 : rows <= 16 ? ROWS16 : rows <= 32 ? TILES32 : rows <= 64 ? TILES64 : rows <= 128 && !bf16 ? BLOCK128 : BLOCK256;
+  p.parts = p.variant >= BLOCK128 && bf16 ? 1 : 2;
+  p.block_rows = p.variant == BLOCK256 ? 16 * MANY : 8 << p.variant;
   p.blocks = (int)((rows + p.block_rows - 1) / p.block_rows);
   p.sets = p.block_rows * p.parts / 16;
   int64_t most, want;              // splits: at most, workgroups that fill the chip
@@ -542,27 +640,32 @@ Plan plan_of(int64_t rows, int64_t k, int64_t n, bool bf16) {
     p.groups = (int)(n / 32);
     most = std::max<int64_t>(1, k / 512), want = 2 * CUS;
   } else {
-    const int columns = p.variant == BLOCK128 ? 256 : 128;
+    const int columns = p.variant >= BLOCK128 ? 256 : 128;
     p.groups = (int)((n + columns - 1) / columns);
-    most = k / HAD, want = 2 * CUS;
+    most = k / HAD, want = p.variant >= BLOCK128 ? CUS : 2 * CUS;
   }
   p.splits = (int)std::min(most, std::max<int64_t>(1, want / ((int64_t)p.groups * p.blocks)));
   p.z_bytes = k / 32 * p.sets * 1024 * p.blocks;
   p.scale_bytes = (4 * rows + 15) & ~(int64_t)15;
-  const bool direct = p.variant == BLOCK128 && p.splits == 1;
+  const bool direct = p.variant >= BLOCK128 && p.splits == 1;
   p.partial_bytes = direct ? 0 : 4 * (int64_t)p.splits * rows * n;
   return p;
 }
 
 template <bool WIDE, int CB, bool BF16>
 void launch_product(const Plan& p, const LinearArgs& a, hipStream_t stream) {
+  constexpr int PARTS = BF16 ? 1 : 2;
   const dim3 grid(p.groups, p.splits, p.blocks);
+  const unsigned all = (unsigned)(p.groups * p.splits * p.blocks);
   switch (p.variant) {
     case ROWS8: linear_kernel<WIDE, CB, 1, 2, 8><<<grid, 512, 0, stream>>>(a); break;
     case ROWS16: linear_kernel<WIDE, CB, 2, 2, 8><<<grid, 512, 0, stream>>>(a); break;
-    case BLOCK32: linear_tiles_kernel<WIDE, CB, false, 2, 2, 2><<<grid, 256, 0, stream>>>(a); break;
-    case BLOCK64: linear_tiles_kernel<WIDE, CB, false, 4, 2, 2><<<grid, 256, 0, stream>>>(a); break;
-    case BLOCK128: linear_tiles_kernel<WIDE, CB, BF16, 8, BF16 ? 1 : 2, 4><<<grid, 256, 0, stream>>>(a); break;
+    case TILES32: linear_tiles_kernel<WIDE, CB, 2, 2, 2><<<grid, 256, 0, stream>>>(a); break;
+    case TILES64: linear_tiles_kernel<WIDE, CB, 4, 2, 2><<<grid, 256, 0, stream>>>(a); break;
+    case BLOCK128:
+      if constexpr (!BF16) linear_blocks_kernel<WIDE, CB, false, 8, 2><<<all, 256, 0, stream>>>(a);
+      break;
+    case BLOCK256: linear_blocks_kernel<WIDE, CB, BF16, MANY, PARTS><<<all, 256, 0, stream>>>(a); break;
   }
 }
 
