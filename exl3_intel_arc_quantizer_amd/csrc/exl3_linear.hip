@@ -295,10 +295,14 @@ struct Reader {
   }
 };
 
-// Sixteen bytes a lane from memory to shared memory, to `to` and on from there.
-__device__ __forceinline__ void to_shared(const u32x4* from, u32x4* to) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                   (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+// Sixteen bytes a lane from memory to shared memory, to `to` (of the wave's first
+// lane) and on from there. Written out, as the compiler would wait for all of these
+// before it reads any shared memory; the waits are the caller's (counts of vmcnt,
+// which the compiler's own waits beside them only make stricter).
+__device__ __forceinline__ void to_shared(const void* from, const void* to) {
+  const uint32_t at = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)to;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               ::"s"(__builtin_amdgcn_readfirstlane(at)), "v"(from) : "memory");
 }
 
 // Up to 16 rows: every wave takes CT column tiles and its share of the input
@@ -357,163 +361,150 @@ __global__ void __launch_bounds__(64 * WAVES) linear_kernel(LinearArgs a) {
 }
 
 // More rows: a workgroup takes a block of 16 MT rows and, four waves, 64 CT
-// columns of a share of the input channels. The rows come through shared memory,
-// two buffers of STEPS steps, for all waves; each decodes its own columns.
-template <bool WIDE, int CB, int MT, int PARTS, int CT>
-__global__ void __launch_bounds__(256, 2) linear_tiles_kernel(LinearArgs a) {
-  constexpr int SETS = MT * PARTS, STEPS = 4, STAGE = STEPS * SETS * 64;  // vectors of a buffer
-  __shared__ u32x4 held[2 * STAGE];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int column0 = (blockIdx.x * 4 + wave) * CT, split = blockIdx.y, block = blockIdx.z;
-  const int stages = a.k / (32 * STEPS);
-  const int begin = (int)((int64_t)stages * split / a.splits), end = (int)((int64_t)stages * (split + 1) / a.splits);
-  Reader<WIDE, CT> reader(a, begin * STEPS, column0, lane);
-  const u32x4* z = a.z + ((int64_t)block * (a.k / 32) + begin * STEPS) * SETS * 64;
-  f32x4 acc[CT][MT];
-#pragma unroll
-  for (int c = 0; c < CT; ++c)
-#pragma unroll
-    for (int m = 0; m < MT; ++m) acc[c][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-  auto fetch = [&](int buffer) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < STAGE / 256; ++i) to_shared(z + i * 256 + tid, held + buffer * STAGE + i * 256 + wave * 64);
-    z += STAGE;
-  };
-  if (begin < end) {
-    fetch(0);
-    Words<WIDE, CT> words = reader.load();
-    for (int stage = begin; stage < end; ++stage) {
-      const int now = (stage - begin) & 1;
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // of the rows that this wave fetched
-      __syncthreads();
-      if (stage + 1 < end) fetch(now ^ 1);
-#pragma unroll
-      for (int step = 0; step < STEPS; ++step) {
-        const Words<WIDE, CT> these = words;
-        if (step + 1 < STEPS || stage + 1 < end) words = reader.load();
-        u32x4 f[CT];
-#pragma unroll
-        for (int c = 0; c < CT; ++c) f[c] = operand_of<WIDE, CB>(these.w[c], reader.late, reader.early, reader.bits);
-#pragma unroll
-        for (int s = 0; s < SETS; ++s) {
-          const u32x4 b = held[now * STAGE + (step * SETS + s) * 64 + lane];
-#pragma unroll
-          for (int c = 0; c < CT; ++c) acc[c][s / PARTS] = mfma(f[c], b, acc[c][s / PARTS]);
-        }
-      }
-    }
-  }
-#pragma unroll
-  for (int c = 0; c < CT; ++c)
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int row = block * 16 * MT + 16 * m + (lane & 15), column = 16 * (column0 + c) + 4 * (lane >> 4);
-      if (row < a.rows) *reinterpret_cast<f32x4*>(a.partials + ((int64_t)split * a.rows + row) * a.n + column) = acc[c][m];
-    }
-}
-
-// Many rows: a workgroup takes 16 MT rows and 256 columns, 64 a wave and one wave
-// a SIMD, whose sums fill half of its registers. A step is then 4 MT PARTS matrix
-// instructions and 16 halves of tiles to decode for the next one; a matrix
-// instruction takes as long as four vector ones and runs beside them, so a step's
-// are dealt out one by three. Rows come through shared memory as above, a part
-// of the next buffer each step, and operands are read from it AHEAD sets before
-// their use.
+// columns, of a share of the input channels. Rows come through shared memory for
+// all waves; each wave decodes its own columns, one step ahead of the products,
+// and its words come through shared memory too: a lane's dwords lie 16 bytes from
+// its neighbour's, which the vector cache takes one by four (2055 rows of 4096 by
+// 12288 with words read from memory: L1_US us), shared memory all at once.
 //
-// Blocks of all input channels (splits == 1) are finished here: a lane holds
-// channels 4 (lane / 16) .. + 3 of its tiles, so of the output's transform two
-// levels lie in a lane's registers, two across lanes, two across its four tiles,
-// and one across two waves.
-template <bool WIDE, int CB, bool BF16, int MT, int PARTS>
+// In step s rows s + DEPTH + 1 and words s + DEPTH + 2 are sent for, in as many
+// instructions each step (past the end the last ones again, which nobody uses), so
+// that a step begins when all but those of the last DEPTH steps are there.
+//
+// A step of MT = 8 is 32 matrix instructions (PARTS: 64), and 16 halves of tiles
+// decoded between them. Two workgroups a CU: a wave alone issues one instruction
+// in five cycles, two in two and a half.
+//
+// Blocks of all input channels (splits == 1) of CT = 4 are finished here: a lane
+// holds channels 4 (lane / 16) .. + 3 of its tiles, so of the output's transform
+// two levels lie in a lane's registers, two across lanes, two across its four
+// tiles, and one across two waves.
+constexpr int depth_of(int mt, int parts, int k) {
+  return mt < 8 ? 4 : parts == 2 ? 1 : k <= 6 ? 3 : 2;
+}
+template <int K, int CB, bool BF16, int MT, int PARTS, int CT>
 __global__ void __launch_bounds__(256, 2) linear_blocks_kernel(LinearArgs a) {
-  constexpr int CT = 4, SETS = MT * PARTS, STEPS = SETS > 8 ? 2 : 4, STAGE = STEPS * SETS * 64, AHEAD = 4;
-  constexpr int LOADS = STAGE / 256, HALVES = 4 * CT;    // a lane's of a buffer, and of a step
-  constexpr int RING = 2;                                // steps whose words are on their way
-  __shared__ u32x4 held[2 * STAGE];
+  constexpr int SETS = MT * PARTS, DEPTH = depth_of(MT, PARTS, K), AHEAD = 4, HALVES = 4 * CT;
+  constexpr int ROWS = SETS * 64, ROW_SLOTS = DEPTH + 2;                     // vectors of a step's rows
+  constexpr int SEGMENT = CT * 32 * K, WORDS = 2 * SEGMENT, WORD_SLOTS = DEPTH + 2;  // bytes of a wave's words
+  constexpr int ROW_LOADS = SETS / 4, WORD_LOADS = (WORDS + 1023) / 1024;    // a wave's of a step
+  __shared__ u32x4 rows_held[ROW_SLOTS * ROWS];
+  __shared__ u32x4 words_held[4 * WORD_SLOTS * WORDS / 16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // Workgroups are dealt to the chip's eight dies in turn: each die takes a run
   // of them, which share a block of rows in its cache.
-  const int groups = (a.n + 255) / 256, all = gridDim.x, die = blockIdx.x & 7;
+  const int groups = (a.n + 64 * CT - 1) / (64 * CT), all = gridDim.x, die = blockIdx.x & 7;
   const int unit = die * (all / 8) + min(die, all % 8) + (int)(blockIdx.x >> 3);
   const int split = unit % a.splits, group = unit / a.splits % groups, block = unit / a.splits / groups;
   const int column0 = (group * 4 + wave) * CT;
-  const int stages = a.k / (32 * STEPS);
-  const int begin = (int)((int64_t)stages * split / a.splits), end = (int)((int64_t)stages * (split + 1) / a.splits);
   const bool there = column0 < a.n / 16;                 // (waves past the columns read the first ones)
-  Reader<WIDE, CT> reader(a, begin * STEPS, there ? column0 : 0, lane);
-  const u32x4* z = a.z + ((int64_t)block * (a.k / 32) + begin * STEPS) * SETS * 64 + tid;
+  const int all_steps = a.k / 32;
+  const int begin = (int)((int64_t)all_steps * split / a.splits), steps = (int)((int64_t)all_steps * (split + 1) / a.splits) - begin;
+
+  const int64_t row_bytes = (int64_t)(a.n / 16) * 32 * K;
+  const char* next_words = reinterpret_cast<const char*>(a.words) + 2 * begin * row_bytes + (int64_t)(there ? column0 : 0) * 32 * K;
+  const u32x4* next_rows = a.z + ((int64_t)block * all_steps + begin) * ROWS;
+  u32x4* own_words = words_held + wave * (WORD_SLOTS * WORDS / 16);
+  int64_t word_at[WORD_LOADS];                           // this lane's of a step
+#pragma unroll
+  for (int i = 0; i < WORD_LOADS; ++i) {
+    const int at = 1024 * i + 16 * lane;
+    word_at[i] = at / SEGMENT * row_bytes + at % SEGMENT;
+  }
+  int rows_sent = 0, words_sent = 0, row_slot = 0, word_slot = 0;  // steps and slots sent for
+  auto send_rows = [&](u32x4* to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < ROW_LOADS; ++i) to_shared(next_rows + i * 256 + tid, to + i * 256 + wave * 64);
+    next_rows += ++rows_sent < steps ? ROWS : 0;
+    row_slot = row_slot == ROW_SLOTS - 1 ? 0 : row_slot + 1;
+  };
+  auto send_words = [&](u32x4* to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < WORD_LOADS; ++i)
+      if (1024 * i + 16 * lane < WORDS) to_shared(next_words + word_at[i], to + 64 * i);
+    next_words += ++words_sent < steps ? 2 * row_bytes : 0;
+    word_slot = word_slot == WORD_SLOTS - 1 ? 0 : word_slot + 1;
+  };
+
+  const int n = lane & 15, q = lane >> 4, u = 8 * (n & 7) + 2 * q + (n >> 3);
+  const Window late = window_of(4 * K * (u + 1), K), early = window_of(4 * K * u + 2 * K, K);
+  constexpr bool WIDE = K > 5;
+  int reads = 0;                                         // slot of the words to read next
+  Words<WIDE, CT> words;
+  auto read_words = [&](const u32x4* from) __attribute__((always_inline)) {
+    auto word = [&](uint32_t at, int place) {
+      return *reinterpret_cast<const uint32_t*>(reinterpret_cast<const char*>(from) + at + place);
+    };
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int place = t * SEGMENT + c * 32 * K;
+        words.w[c][t][0] = word(late.at0, place), words.w[c][t][1] = word(late.at1, place);
+        if constexpr (WIDE) words.w[c][t][2] = word(early.at0, place), words.w[c][t][3] = word(early.at1, place);
+      }
+    reads = reads == WORD_SLOTS - 1 ? 0 : reads + 1;
+  };
+
   f32x4 acc[CT][MT];
 #pragma unroll
   for (int c = 0; c < CT; ++c)
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[c][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-  // Part `step` of a buffer's rows, all in the first half of the STEPS.
-  auto fetch = [&](int buffer, int step) __attribute__((always_inline)) {
-    constexpr int EACH = LOADS / (STEPS / 2);
+  send_words(own_words);
 #pragma unroll
-    for (int i = step * EACH; i < (step + 1) * EACH && i < LOADS; ++i)
-      to_shared(z + i * 256, held + buffer * STAGE + i * 256 + wave * 64);
-  };
-  if (begin < end) {
-    const int last = (end - begin) * STEPS - 1;          // step
-#pragma unroll
-    for (int step = 0; step < STEPS; ++step) fetch(0, step);
-    z += begin + 1 < end ? STAGE : 0;
-    asm volatile("" ::: "memory");                       // words after rows: see the wait below
-    __builtin_amdgcn_sched_barrier(0);
-    Words<WIDE, CT> words[RING];
-#pragma unroll
-    for (int i = 0; i < RING; ++i) words[i] = reader.load(i < last);
-    u32x4 f[2][CT];
-#pragma unroll
-    for (int c = 0; c < CT; ++c) f[0][c] = operand_of<WIDE, CB>(words[0].w[c], reader.late, reader.early, reader.bits);
-    for (int stage = begin; stage < end; ++stage) {
-      const int now = (stage - begin) & 1;
-      const u32x4* rows = held + now * STAGE + lane;
-      // For the rows that this wave fetched in the first half of the steps: words
-      // were loaded in the others, CT 2 (or, in pairs, CT) loads a step at least,
-      // and stay on their way.
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(CT * STEPS) : "memory");
-      u32x4 b[AHEAD];
-#pragma unroll
-      for (int i = 0; i < AHEAD; ++i) b[i] = rows[i * 64];
-#pragma unroll
-      for (int step = 0; step < STEPS; ++step) {
-        // (Past the last step and stage the last ones again, which nobody uses: a
-        // branch would cut the loop's body, whose registers then do not agree.)
-        words[step % RING] = reader.load((stage - begin) * STEPS + step + RING < last);
-        fetch(now ^ 1, step);
-        u32x4 (&here)[CT] = f[step & 1], (&next)[CT] = f[(step + 1) & 1];
-        const Words<WIDE, CT>& coming = words[(step + 1) % RING];
-#pragma unroll
-        for (int s = 0; s < SETS; ++s) {
-          const int set = step * SETS + s;
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int c = 0; c < CT; ++c) acc[c][s / PARTS] = mfma(here[c], b[set % AHEAD], acc[c][s / PARTS]);
-          if (set + AHEAD < STEPS * SETS) b[set % AHEAD] = rows[(set + AHEAD) * 64];
-          // This set's share of the next step's halves of tiles: (column tile, tile, half).
-#pragma unroll
-          for (int of = s * HALVES / SETS; of < (s + 1) * HALVES / SETS; ++of) {
-            const int c = of >> 2, t = of >> 1 & 1;
-            next[c][of & 3] = of & 1 ? half_of<WIDE, CB, 1>(coming.w[c][t], reader.late, reader.early, reader.bits)
-                                     : half_of<WIDE, CB, 0>(coming.w[c][t], reader.late, reader.early, reader.bits);
-          }
-#pragma unroll
-          for (int c = 0; c < CT; ++c) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
-          }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      z += stage + 2 < end ? STAGE : 0;
-    }
+  for (int i = 0; i <= DEPTH; ++i) {
+    send_rows(rows_held + i * ROWS);
+    send_words(own_words + (i + 1) % WORD_SLOTS * (WORDS / 16));
   }
+  u32x4 f[2][CT];
+  int slot = 0;                                          // of the rows
+  auto wait = [&]() __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(DEPTH * (ROW_LOADS + WORD_LOADS)) : "memory");
+  };
+  wait();
+  read_words(own_words);
+#pragma unroll
+  for (int c = 0; c < CT; ++c) f[0][c] = operand_of<WIDE, CB>(words.w[c], late, early, K);
+  auto step = [&](u32x4 (&here)[CT], u32x4 (&next)[CT]) __attribute__((always_inline)) {
+    wait();
+    const u32x4* rows = rows_held + slot * ROWS + lane;
+    slot = slot == ROW_SLOTS - 1 ? 0 : slot + 1;
+    u32x4 b[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD && i < SETS; ++i) b[i] = rows[i * 64];
+    read_words(own_words + reads * (WORDS / 16));
+    send_rows(rows_held + row_slot * ROWS);
+    send_words(own_words + word_slot * (WORDS / 16));
+#pragma unroll
+    for (int s = 0; s < SETS; ++s) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int c = 0; c < CT; ++c) acc[c][s / PARTS] = mfma(here[c], b[s % AHEAD], acc[c][s / PARTS]);
+      if (s + AHEAD < SETS) b[s % AHEAD] = rows[(s + AHEAD) * 64];
+      // This set's share of the next step's halves of tiles: (column tile, tile, half).
+#pragma unroll
+      for (int of = s * HALVES / SETS; of < (s + 1) * HALVES / SETS; ++of) {
+        const int c = of >> 2, t = of >> 1 & 1;
+        next[c][of & 3] = of & 1 ? half_of<WIDE, CB, 1>(words.w[c][t], late, early, K)
+                                 : half_of<WIDE, CB, 0>(words.w[c][t], late, early, K);
+      }
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  for (int i = 0; i < steps; i += 2) {
+    step(f[0], f[1]);
+    if (i + 1 < steps) step(f[1], f[0]);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // nothing on its way into memory that is used again below
+
   const int row0 = block * 16 * MT + (lane & 15);
-  if (a.splits > 1) {
+  if (CT != 4 || a.splits > 1) {
     if (!there) return;
 #pragma unroll
     for (int c = 0; c < CT; ++c)
@@ -524,43 +515,39 @@ __global__ void __launch_bounds__(256, 2) linear_blocks_kernel(LinearArgs a) {
       }
     return;
   }
-  f32x4* exchange = reinterpret_cast<f32x4*>(held);
-  constexpr int AT_ONCE = 2;
+  if constexpr (CT == 4) {
+    constexpr int CHUNK = 4 * CT * 64;                   // vectors of the four waves' 16 rows
+    f32x4* exchange = reinterpret_cast<f32x4*>(rows_held);
+    static_assert(ROW_SLOTS * ROWS >= 2 * CHUNK, "two chunks of 16 rows in the rows' memory");
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
+    for (int m = 0; m < MT; ++m) {
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {
-      f32x4& v = acc[c][m];
-      const float s0 = v[0] + v[1], s1 = v[0] - v[1], s2 = v[2] + v[3], s3 = v[2] - v[3];
-      float y[4] = {s0 + s2, s1 + s3, s0 - s2, s1 - s3};
-      lane_butterfly<16>(y[0], y[1]);
-      lane_butterfly<16>(y[2], y[3]);
-      lane_butterfly<32>(y[0], y[1]);
-      lane_butterfly<32>(y[2], y[3]);
-      v = f32x4{y[0], y[1], y[2], y[3]};
-    }
-    const f32x4 s0 = acc[0][m] + acc[1][m], s1 = acc[0][m] - acc[1][m], s2 = acc[2][m] + acc[3][m], s3 = acc[2][m] - acc[3][m];
-    acc[0][m] = s0 + s2, acc[1][m] = s1 + s3, acc[2][m] = s0 - s2, acc[3][m] = s1 - s3;
-    if (m % AT_ONCE != AT_ONCE - 1) continue;
-    // Two buffers take turns: a wave writes one after its partner has read the other.
-    const int m0 = m - AT_ONCE + 1;
-    f32x4* held_now = exchange + (m0 / AT_ONCE & 1) * (4 * AT_ONCE * CT * 64);
-    if (m0 == 0) __syncthreads();
+      for (int c = 0; c < CT; ++c) {
+        f32x4& v = acc[c][m];
+        const float s0 = v[0] + v[1], s1 = v[0] - v[1], s2 = v[2] + v[3], s3 = v[2] - v[3];
+        float y[4] = {s0 + s2, s1 + s3, s0 - s2, s1 - s3};
+        lane_butterfly<16>(y[0], y[1]);
+        lane_butterfly<16>(y[2], y[3]);
+        lane_butterfly<32>(y[0], y[1]);
+        lane_butterfly<32>(y[2], y[3]);
+        v = f32x4{y[0], y[1], y[2], y[3]};
+      }
+      const f32x4 s0 = acc[0][m] + acc[1][m], s1 = acc[0][m] - acc[1][m], s2 = acc[2][m] + acc[3][m], s3 = acc[2][m] - acc[3][m];
+      acc[0][m] = s0 + s2, acc[1][m] = s1 + s3, acc[2][m] = s0 - s2, acc[3][m] = s1 - s3;
+      // Two chunks take turns: a wave writes one after its partner has read the other.
+      f32x4* held = exchange + (m & 1) * CHUNK;
+      if (m == 0) __syncthreads();
 #pragma unroll
-    for (int i = 0; i < AT_ONCE; ++i)
-#pragma unroll
-      for (int c = 0; c < CT; ++c) held_now[((wave * AT_ONCE + i) * CT + c) * 64 + lane] = acc[c][m0 + i];
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < AT_ONCE; ++i) {
-      const int row = row0 + 16 * (m0 + i);
+      for (int c = 0; c < CT; ++c) held[(wave * CT + c) * 64 + lane] = acc[c][m];
+      __syncthreads();
+      const int row = row0 + 16 * m;
       const bool writes = there && row < a.rows;
       const float scale = writes ? a.scale[row] * ROOT : 0.0f;
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
         const int column = 16 * (column0 + c) + 4 * (lane >> 4);
-        const f32x4 other = held_now[(((wave ^ 1) * AT_ONCE + i) * CT + c) * 64 + lane];
-        const f32x4 v = wave & 1 ? other - acc[c][m0 + i] : acc[c][m0 + i] + other;
+        const f32x4 other = held[((wave ^ 1) * CT + c) * 64 + lane];
+        const f32x4 v = wave & 1 ? other - acc[c][m] : acc[c][m] + other;
         if (writes) {
           u32x2 w;
           w[0] = narrow<BF16>(v[0] * scale * a.sv.at(column)) | narrow<BF16>(v[1] * scale * a.sv.at(column + 1)) << 16;
@@ -614,8 +601,8 @@ __global__ void __launch_bounds__(256) linear_join_kernel(JoinArgs a) {
 
 // ------------------------------------------------------------ plan
 
-// Variants by the rows.
-enum Variant { ROWS8, ROWS16, TILES32, TILES64, BLOCK128, BLOCK256 };
+// Variants by the rows: of 8 << variant rows, the last in blocks of 128.
+enum Variant { ROWS8, ROWS16, BLOCK32, BLOCK64, BLOCK128 };
 
 // How a call is cut.
 struct Plan {
@@ -626,46 +613,55 @@ struct Plan {
   int64_t z_bytes, scale_bytes, partial_bytes;
 };
 
-constexpr int CUS = 256, MANY = 8;
+constexpr int CUS = 256;
 
 Plan plan_of(int64_t rows, int64_t k, int64_t n, bool bf16) {
   Plan p{};
-  p.variant = rows <= 8 ? ROWS8 : rows <= 16 ? ROWS16 : rows <= 32 ? TILES32 : rows <= 64 ? TILES64 : rows <= 128 && !bf16 ? BLOCK128 : BLOCK256;
-  p.parts = p.variant >= BLOCK128 && bf16 ? 1 : 2;
-  p.block_rows = p.variant == BLOCK256 ? 16 * MANY : 8 << p.variant;
+  p.variant = rows <= 8 ? ROWS8 : rows <= 16 ? ROWS16 : rows <= 32 ? BLOCK32 : rows <= 64 ? BLOCK64 : BLOCK128;
+  p.parts = p.variant == BLOCK128 && bf16 ? 1 : 2;
+  p.block_rows = 8 << p.variant;
   p.blocks = (int)((rows + p.block_rows - 1) / p.block_rows);
   p.sets = p.block_rows * p.parts / 16;
-  int64_t most, want;              // splits: at most, workgroups that fill the chip
+  int64_t most, want = 2 * CUS;    // splits: at most, workgroups that fill the chip
   if (p.variant <= ROWS16) {
     p.groups = (int)(n / 32);
-    most = std::max<int64_t>(1, k / 512), want = 2 * CUS;
+    most = std::max<int64_t>(1, k / 512);
   } else {
-    const int columns = p.variant >= BLOCK128 ? 256 : 128;
+    const int columns = p.variant == BLOCK128 ? 256 : 128;
     p.groups = (int)((n + columns - 1) / columns);
-    most = k / HAD, want = p.variant >= BLOCK128 ? CUS : 2 * CUS;
+    most = k / HAD;
   }
   p.splits = (int)std::min(most, std::max<int64_t>(1, want / ((int64_t)p.groups * p.blocks)));
   p.z_bytes = k / 32 * p.sets * 1024 * p.blocks;
   p.scale_bytes = (4 * rows + 15) & ~(int64_t)15;
-  const bool direct = p.variant >= BLOCK128 && p.splits == 1;
+  const bool direct = p.variant == BLOCK128 && p.splits == 1;
   p.partial_bytes = direct ? 0 : 4 * (int64_t)p.splits * rows * n;
   return p;
 }
 
-template <bool WIDE, int CB, bool BF16>
+template <int K, int CB, bool BF16>
 void launch_product(const Plan& p, const LinearArgs& a, hipStream_t stream) {
-  constexpr int PARTS = BF16 ? 1 : 2;
-  const dim3 grid(p.groups, p.splits, p.blocks);
+  const dim3 grid(p.groups, p.splits);
   const unsigned all = (unsigned)(p.groups * p.splits * p.blocks);
   switch (p.variant) {
-    case ROWS8: linear_kernel<WIDE, CB, 1, 2, 8><<<grid, 512, 0, stream>>>(a); break;
-    case ROWS16: linear_kernel<WIDE, CB, 2, 2, 8><<<grid, 512, 0, stream>>>(a); break;
-    case TILES32: linear_tiles_kernel<WIDE, CB, 2, 2, 2><<<grid, 256, 0, stream>>>(a); break;
-    case TILES64: linear_tiles_kernel<WIDE, CB, 4, 2, 2><<<grid, 256, 0, stream>>>(a); break;
-    case BLOCK128:
-      if constexpr (!BF16) linear_blocks_kernel<WIDE, CB, false, 8, 2><<<all, 256, 0, stream>>>(a);
-      break;
-    case BLOCK256: linear_blocks_kernel<WIDE, CB, BF16, MANY, PARTS><<<all, 256, 0, stream>>>(a); break;
+    case ROWS8: linear_kernel<(K > 5), CB, 1, 2, 8><<<grid, 512, 0, stream>>>(a); break;
+    case ROWS16: linear_kernel<(K > 5), CB, 2, 2, 8><<<grid, 512, 0, stream>>>(a); break;
+    case BLOCK32: linear_blocks_kernel<K, CB, false, 2, 2, 2><<<all, 256, 0, stream>>>(a); break;
+    case BLOCK64: linear_blocks_kernel<K, CB, false, 4, 2, 2><<<all, 256, 0, stream>>>(a); break;
+    case BLOCK128: linear_blocks_kernel<K, CB, BF16, 8, BF16 ? 1 : 2, 4><<<all, 256, 0, stream>>>(a); break;
+  }
+}
+template <int CB, bool BF16>
+void launch_rate(const Plan& p, const LinearArgs& a, hipStream_t stream) {
+  switch (a.bits) {
+    case 1: launch_product<1, CB, BF16>(p, a, stream); break;
+    case 2: launch_product<2, CB, BF16>(p, a, stream); break;
+    case 3: launch_product<3, CB, BF16>(p, a, stream); break;
+    case 4: launch_product<4, CB, BF16>(p, a, stream); break;
+    case 5: launch_product<5, CB, BF16>(p, a, stream); break;
+    case 6: launch_product<6, CB, BF16>(p, a, stream); break;
+    case 7: launch_product<7, CB, BF16>(p, a, stream); break;
+    default: launch_product<8, CB, BF16>(p, a, stream); break;
   }
 }
 
@@ -674,10 +670,7 @@ int launch_linear(const Plan& p, const TurnArgs& t, const LinearArgs& a, int cb,
   const int threads = t.k <= 8192 ? 256 : t.k <= 16384 ? 512 : 1024;
   linear_turn_kernel<BF16><<<(unsigned)a.rows, threads, 0, s>>>(t);
   if (check_launch("exl3_linear")) return 1;
-  if (a.bits > 5)
-    cb == 0 ? launch_product<true, 0, BF16>(p, a, s) : cb == 1 ? launch_product<true, 1, BF16>(p, a, s) : launch_product<true, 2, BF16>(p, a, s);
-  else
-    cb == 0 ? launch_product<false, 0, BF16>(p, a, s) : cb == 1 ? launch_product<false, 1, BF16>(p, a, s) : launch_product<false, 2, BF16>(p, a, s);
+  cb == 0 ? launch_rate<0, BF16>(p, a, s) : cb == 1 ? launch_rate<1, BF16>(p, a, s) : launch_rate<2, BF16>(p, a, s);
   if (check_launch("exl3_linear")) return 1;
   if (!p.partial_bytes) return 0;
   JoinArgs j{};
