@@ -295,14 +295,16 @@ struct Reader {
   }
 };
 
-// Sixteen bytes a lane from memory to shared memory, to `to` (of the wave's first
-// lane) and on from there. Written out, as the compiler would wait for all of these
-// before it reads any shared memory; the waits are the caller's (counts of vmcnt,
-// which the compiler's own waits beside them only make stricter).
-__device__ __forceinline__ void to_shared(const void* from, const void* to) {
-  const uint32_t at = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)to;
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-               ::"s"(__builtin_amdgcn_readfirstlane(at)), "v"(from) : "memory");
+// Sixteen bytes a lane from memory, `lane_at` bytes past `from`, to shared memory,
+// to byte `to` (of the wave's first lane) and on from there. Written out, as the
+// compiler would wait for all of these before it reads any shared memory; the waits
+// are the caller's (counts of vmcnt, which the compiler's own waits beside them only
+// make stricter).
+__device__ __forceinline__ void to_shared(const void* from, uint32_t lane_at, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(lane_at), "s"(from) : "memory");
+}
+__device__ __forceinline__ uint32_t shared_byte(const void* p) {
+  return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p);
 }
 
 // Up to 16 rows: every wave takes CT column tiles and its share of the input
@@ -374,17 +376,12 @@ __global__ void __launch_bounds__(64 * WAVES) linear_kernel(LinearArgs a) {
 // A step of MT = 8 is 32 matrix instructions (PARTS: 64), and 16 halves of tiles
 // decoded between them. Two workgroups a CU: a wave alone issues one instruction
 // in five cycles, two in two and a half.
-//
-// Blocks of all input channels (splits == 1) of CT = 4 are finished here: a lane
-// holds channels 4 (lane / 16) .. + 3 of its tiles, so of the output's transform
-// two levels lie in a lane's registers, two across lanes, two across its four
-// tiles, and one across two waves.
-constexpr int depth_of(int mt, int parts, int k) {
-  return mt < 8 ? 4 : parts == 2 ? 1 : k <= 6 ? 3 : 2;
+constexpr int depth_of(int mt, int k) {
+  return mt < 8 ? 4 : k <= 6 ? 3 : 2;
 }
-template <int K, int CB, bool BF16, int MT, int PARTS, int CT>
+template <int K, int CB, int MT, int PARTS, int CT>
 __global__ void __launch_bounds__(256, 2) linear_blocks_kernel(LinearArgs a) {
-  constexpr int SETS = MT * PARTS, DEPTH = depth_of(MT, PARTS, K), AHEAD = 4, HALVES = 4 * CT;
+  constexpr int SETS = MT * PARTS, DEPTH = depth_of(MT, K), AHEAD = 4, HALVES = 4 * CT;
   constexpr int ROWS = SETS * 64, ROW_SLOTS = DEPTH + 2;                     // vectors of a step's rows
   constexpr int SEGMENT = CT * 32 * K, WORDS = 2 * SEGMENT, WORD_SLOTS = DEPTH + 2;  // bytes of a wave's words
   constexpr int ROW_LOADS = SETS / 4, WORD_LOADS = (WORDS + 1023) / 1024;    // a wave's of a step
@@ -403,27 +400,29 @@ __global__ void __launch_bounds__(256, 2) linear_blocks_kernel(LinearArgs a) {
 
   const int64_t row_bytes = (int64_t)(a.n / 16) * 32 * K;
   const char* next_words = reinterpret_cast<const char*>(a.words) + 2 * begin * row_bytes + (int64_t)(there ? column0 : 0) * 32 * K;
-  const u32x4* next_rows = a.z + ((int64_t)block * all_steps + begin) * ROWS;
+  const char* next_rows = reinterpret_cast<const char*>(a.z + ((int64_t)block * all_steps + begin) * ROWS);
   u32x4* own_words = words_held + wave * (WORD_SLOTS * WORDS / 16);
-  int64_t word_at[WORD_LOADS];                           // this lane's of a step
+  uint32_t word_at[WORD_LOADS];                          // this lane's of a step (row_bytes is under 2^29)
 #pragma unroll
   for (int i = 0; i < WORD_LOADS; ++i) {
     const int at = 1024 * i + 16 * lane;
-    word_at[i] = at / SEGMENT * row_bytes + at % SEGMENT;
+    word_at[i] = (uint32_t)(at / SEGMENT * row_bytes + at % SEGMENT);
   }
-  int rows_sent = 0, words_sent = 0, row_slot = 0, word_slot = 0;  // steps and slots sent for
-  auto send_rows = [&](u32x4* to) __attribute__((always_inline)) {
+  int rows_sent = 0, words_sent = 0;                     // steps sent for, and places of the next
+  const uint32_t rows0 = shared_byte(rows_held + wave * 64), words0 = shared_byte(own_words);
+  uint32_t rows_to = rows0, words_to = words0;
+  auto send_rows = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < ROW_LOADS; ++i) to_shared(next_rows + i * 256 + tid, to + i * 256 + wave * 64);
-    next_rows += ++rows_sent < steps ? ROWS : 0;
-    row_slot = row_slot == ROW_SLOTS - 1 ? 0 : row_slot + 1;
+    for (int i = 0; i < ROW_LOADS; ++i) to_shared(next_rows + i * 4096, 16 * tid, rows_to + i * 4096);
+    next_rows += ++rows_sent < steps ? 16 * ROWS : 0;
+    rows_to = rows_to == rows0 + (ROW_SLOTS - 1) * (16 * ROWS) ? rows0 : rows_to + 16 * ROWS;
   };
-  auto send_words = [&](u32x4* to) __attribute__((always_inline)) {
+  auto send_words = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < WORD_LOADS; ++i)
-      if (1024 * i + 16 * lane < WORDS) to_shared(next_words + word_at[i], to + 64 * i);
+      if (1024 * i + 16 * lane < WORDS) to_shared(next_words, word_at[i], words_to + 1024 * i);
     next_words += ++words_sent < steps ? 2 * row_bytes : 0;
-    word_slot = word_slot == WORD_SLOTS - 1 ? 0 : word_slot + 1;
+    words_to = words_to == words0 + (WORD_SLOTS - 1) * WORDS ? words0 : words_to + WORDS;
   };
 
   const int n = lane & 15, q = lane >> 4, u = 8 * (n & 7) + 2 * q + (n >> 3);
@@ -451,11 +450,11 @@ __global__ void __launch_bounds__(256, 2) linear_blocks_kernel(LinearArgs a) {
   for (int c = 0; c < CT; ++c)
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[c][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  send_words(own_words);
+  send_words();
 #pragma unroll
   for (int i = 0; i <= DEPTH; ++i) {
-    send_rows(rows_held + i * ROWS);
-    send_words(own_words + (i + 1) % WORD_SLOTS * (WORDS / 16));
+    send_rows();
+    send_words();
   }
   u32x4 f[2][CT];
   int slot = 0;                                          // of the rows
@@ -474,11 +473,11 @@ __global__ void __launch_bounds__(256, 2) linear_blocks_kernel(LinearArgs a) {
 #pragma unroll
     for (int i = 0; i < AHEAD && i < SETS; ++i) b[i] = rows[i * 64];
     read_words(own_words + reads * (WORDS / 16));
-    send_rows(rows_held + row_slot * ROWS);
-    send_words(own_words + word_slot * (WORDS / 16));
 #pragma unroll
     for (int s = 0; s < SETS; ++s) {
       __builtin_amdgcn_sched_barrier(0);
+      if (s == 1) send_rows();
+      if (s == 2) send_words();
 #pragma unroll
       for (int c = 0; c < CT; ++c) acc[c][s / PARTS] = mfma(here[c], b[s % AHEAD], acc[c][s / PARTS]);
       if (s + AHEAD < SETS) b[s % AHEAD] = rows[(s + AHEAD) * 64];
@@ -501,59 +500,202 @@ __global__ void __launch_bounds__(256, 2) linear_blocks_kernel(LinearArgs a) {
     step(f[0], f[1]);
     if (i + 1 < steps) step(f[1], f[0]);
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // nothing on its way into memory that is used again below
-
-  const int row0 = block * 16 * MT + (lane & 15);
-  if (CT != 4 || a.splits > 1) {
-    if (!there) return;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // nothing on its way into memory that others get
+  if (!there) return;
 #pragma unroll
-    for (int c = 0; c < CT; ++c)
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const int row = row0 + 16 * m, column = 16 * (column0 + c) + 4 * (lane >> 4);
-        if (row < a.rows) *reinterpret_cast<f32x4*>(a.partials + ((int64_t)split * a.rows + row) * a.n + column) = acc[c][m];
-      }
-    return;
-  }
-  if constexpr (CT == 4) {
-    constexpr int CHUNK = 4 * CT * 64;                   // vectors of the four waves' 16 rows
-    f32x4* exchange = reinterpret_cast<f32x4*>(rows_held);
-    static_assert(ROW_SLOTS * ROWS >= 2 * CHUNK, "two chunks of 16 rows in the rows' memory");
+  for (int c = 0; c < CT; ++c)
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
+      const int row = block * 16 * MT + 16 * m + (lane & 15), column = 16 * (column0 + c) + 4 * (lane >> 4);
+      if (row < a.rows) *reinterpret_cast<f32x4*>(a.partials + ((int64_t)split * a.rows + row) * a.n + column) = acc[c][m];
+    }
+}
+
+// Many rows: eight waves take 256 rows (128 of two parts) and 256 columns, so two
+// waves share 64 columns, each with half of the rows. Each decodes half of the
+// columns' operands, in a step for the next one, and hands them to the other
+// through shared memory: vector instructions, four cycles each (and eight of a
+// matrix one's sixteen) on a SIMD that two waves share, are then as long as the
+// matrix ones. Products begin with a wave's own operands, and rows are read for the
+// next step as this one's are used up, so nothing is waited for after the barrier.
+template <int K, int CB, bool BF16, int PARTS>
+__global__ void __launch_bounds__(512, 2) linear_wide_kernel(LinearArgs a) {
+  constexpr int MT = 8 / PARTS, SETS = 8, DEPTH = 2;     // of a wave
+  constexpr int ROWS = 2 * SETS * 64, ROW_SLOTS = DEPTH + 3;                 // vectors of a step's rows
+  constexpr int SEGMENT = 2 * 32 * K, WORDS = 2 * SEGMENT, WORD_SLOTS = DEPTH + 2;  // bytes of a wave's words
+  constexpr bool WIDE = K > 5;
+  __shared__ u32x4 rows_held[ROW_SLOTS * ROWS];
+  __shared__ u32x4 words_held[8 * WORD_SLOTS * WORDS / 16];
+  __shared__ u32x4 operands[2][4][4][64];                // [step & 1][column group][column tile]
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int side = wave & 1, quarter = wave >> 1;        // half of the rows, 64 columns
+  // Workgroups are dealt to the chip's eight dies in turn: each die takes a run
+  // of them, which share a block of rows in its cache.
+  const int groups = (a.n + 255) / 256, all = gridDim.x, die = blockIdx.x & 7;
+  const int unit = die * (all / 8) + min(die, all % 8) + (int)(blockIdx.x >> 3);
+  const int split = unit % a.splits, group = unit / a.splits % groups, block = unit / a.splits / groups;
+  const int column0 = (group * 4 + quarter) * 4;
+  const bool there = column0 < a.n / 16;                 // (waves past the columns read the first ones)
+  const int all_steps = a.k / 32;
+  const int begin = (int)((int64_t)all_steps * split / a.splits), steps = (int)((int64_t)all_steps * (split + 1) / a.splits) - begin;
+
+  const int64_t row_bytes = (int64_t)(a.n / 16) * 32 * K;
+  const char* next_words = reinterpret_cast<const char*>(a.words) + 2 * begin * row_bytes + (int64_t)((there ? column0 : 0) + 2 * side) * 32 * K;
+  const uint32_t word_at = (uint32_t)(16 * lane / SEGMENT * row_bytes + 16 * lane % SEGMENT);  // (row_bytes is under 2^29)
+  const char* next_rows = reinterpret_cast<const char*>(a.z + ((int64_t)block * all_steps + begin) * ROWS);
+  u32x4* own_words = words_held + wave * (WORD_SLOTS * WORDS / 16);
+  // What is sent for next, and its places in shared memory.
+  int sent = 0;
+  const uint32_t rows0 = shared_byte(rows_held + wave * 64), words0 = shared_byte(own_words);
+  uint32_t rows_to = rows0, words_to = words0;
+  static_assert(ROWS == 2 * 512, "a step's rows are two of each thread");
+  auto send = [&](int part) __attribute__((always_inline)) {
+    if (part < 2) {
+      to_shared(next_rows + part * 8192, 16 * tid, rows_to + part * 8192);
+      return;
+    }
+    if (16 * lane < WORDS) to_shared(next_words, word_at, words_to);
+    const bool on = ++sent < steps;
+    next_rows += on ? 16 * ROWS : 0, next_words += on ? 2 * row_bytes : 0;
+    rows_to = rows_to == rows0 + (ROW_SLOTS - 1) * (16 * ROWS) ? rows0 : rows_to + 16 * ROWS;
+    words_to = words_to == words0 + (WORD_SLOTS - 1) * WORDS ? words0 : words_to + WORDS;
+  };
+  // All but what the last DEPTH steps sent for.
+  auto wait = [&]() __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(DEPTH * 3) : "memory");
+  };
+
+  const int n = lane & 15, q = lane >> 4, u = 8 * (n & 7) + 2 * q + (n >> 3);
+  const Window late = window_of(4 * K * (u + 1), K), early = window_of(4 * K * u + 2 * K, K);
+  int read_slot = 0, slot = 0;
+  Words<WIDE, 2> words;
+  auto read_words = [&]() __attribute__((always_inline)) {
+    const char* from = reinterpret_cast<const char*>(own_words) + read_slot * WORDS;
+    auto word = [&](uint32_t at, int place) { return *reinterpret_cast<const uint32_t*>(from + at + place); };
 #pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        f32x4& v = acc[c][m];
-        const float s0 = v[0] + v[1], s1 = v[0] - v[1], s2 = v[2] + v[3], s3 = v[2] - v[3];
-        float y[4] = {s0 + s2, s1 + s3, s0 - s2, s1 - s3};
-        lane_butterfly<16>(y[0], y[1]);
-        lane_butterfly<16>(y[2], y[3]);
-        lane_butterfly<32>(y[0], y[1]);
-        lane_butterfly<32>(y[2], y[3]);
-        v = f32x4{y[0], y[1], y[2], y[3]};
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int place = t * SEGMENT + c * 32 * K;
+        words.w[c][t][0] = word(late.at0, place), words.w[c][t][1] = word(late.at1, place);
+        if constexpr (WIDE) words.w[c][t][2] = word(early.at0, place), words.w[c][t][3] = word(early.at1, place);
       }
-      const f32x4 s0 = acc[0][m] + acc[1][m], s1 = acc[0][m] - acc[1][m], s2 = acc[2][m] + acc[3][m], s3 = acc[2][m] - acc[3][m];
-      acc[0][m] = s0 + s2, acc[1][m] = s1 + s3, acc[2][m] = s0 - s2, acc[3][m] = s1 - s3;
-      // Two chunks take turns: a wave writes one after its partner has read the other.
-      f32x4* held = exchange + (m & 1) * CHUNK;
-      if (m == 0) __syncthreads();
+    read_slot = read_slot == WORD_SLOTS - 1 ? 0 : read_slot + 1;
+  };
+
+  f32x4 acc[4][MT];                                      // of this wave's operands, then the other's
 #pragma unroll
-      for (int c = 0; c < CT; ++c) held[(wave * CT + c) * 64 + lane] = acc[c][m];
-      __syncthreads();
-      const int row = row0 + 16 * m;
-      const bool writes = there && row < a.rows;
-      const float scale = writes ? a.scale[row] * ROOT : 0.0f;
+  for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        const int column = 16 * (column0 + c) + 4 * (lane >> 4);
-        const f32x4 other = held[((wave ^ 1) * CT + c) * 64 + lane];
-        const f32x4 v = wave & 1 ? other - acc[c][m] : acc[c][m] + other;
-        if (writes) {
-          u32x2 w;
-          w[0] = narrow<BF16>(v[0] * scale * a.sv.at(column)) | narrow<BF16>(v[1] * scale * a.sv.at(column + 1)) << 16;
-          w[1] = narrow<BF16>(v[2] * scale * a.sv.at(column + 2)) | narrow<BF16>(v[3] * scale * a.sv.at(column + 3)) << 16;
-          *reinterpret_cast<u32x2*>(a.out + (int64_t)row * a.n + column) = w;
-        }
+    for (int m = 0; m < MT; ++m) acc[j][m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < DEPTH + 2; ++i) send(0), send(1), send(2);
+  wait();
+  u32x4 f[2][2], b[SETS];
+  read_words();
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    f[0][c] = operand_of<WIDE, CB>(words.w[c], late, early, K);
+    operands[0][quarter][2 * side + c][lane] = f[0][c];
+  }
+#pragma unroll
+  for (int s = 0; s < SETS; ++s) b[s] = rows_held[(side * SETS + s) * 64 + lane];
+
+  auto step = [&](u32x4 (&here)[2], u32x4 (&next)[2], int parity) __attribute__((always_inline)) {
+    wait();
+    slot = slot == ROW_SLOTS - 1 ? 0 : slot + 1;
+    const u32x4* coming = rows_held + slot * ROWS + side * (SETS * 64) + lane;
+    u32x4 other[2];
+#pragma unroll
+    for (int s = 0; s < 2 * SETS; ++s) {
+      const int set = s % SETS;
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        f32x4& sum = acc[s / SETS * 2 + c][set / PARTS];
+        sum = mfma(s < SETS ? here[c] : other[c], b[set], sum);
+      }
+      if (s == 0) read_words();
+      if (s == 1)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) other[c] = operands[parity][quarter][2 * (side ^ 1) + c][lane];
+      if (s >= 1 && s < 4) send(s - 1);
+      if (s >= SETS) b[set] = coming[set * 64];
+      // The next step's eight halves of tiles, (column tile, tile, half).
+      if (s >= 3 && s < 11) {
+        const int of = s - 3, c = of >> 2, t = of >> 1 & 1;
+        next[c][of & 3] = of & 1 ? half_of<WIDE, CB, 1>(words.w[c][t], late, early, K) : half_of<WIDE, CB, 0>(words.w[c][t], late, early, K);
+      }
+      if (s == 7 || s == 11) operands[parity ^ 1][quarter][2 * side + s / 8][lane] = next[s / 8];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  for (int i = 0; i < steps; i += 2) {
+    step(f[0], f[1], 0);
+    if (i + 1 < steps) step(f[1], f[0], 1);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // nothing on its way into memory that is used again below
+
+  const int row0 = (2 * block + side) * 16 * MT + (lane & 15);
+  auto column_of = [&](int j) { return 16 * (column0 + (j < 2 ? 2 * side + j : 2 * (side ^ 1) + j - 2)) + 4 * (lane >> 4); };
+  if (a.splits > 1) {
+    if (!there) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        if (row0 + 16 * m < a.rows)
+          *reinterpret_cast<f32x4*>(a.partials + ((int64_t)split * a.rows + row0 + 16 * m) * a.n + column_of(j)) = acc[j][m];
+    return;
+  }
+  // The output's transform: a lane holds channels 4 (lane / 16) .. + 3 of its tiles,
+  // so two levels lie in its registers, two across lanes, two across the four tiles,
+  // and one across the waves of 64 columns beside each other.
+  constexpr int CHUNK = 8 * 4 * 64;                      // vectors of the eight waves' 16 rows
+  f32x4* exchange = reinterpret_cast<f32x4*>(rows_held);
+  static_assert(ROW_SLOTS * ROWS >= 2 * CHUNK, "two chunks in the rows' memory");
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      f32x4& v = acc[j][m];
+      const float s0 = v[0] + v[1], s1 = v[0] - v[1], s2 = v[2] + v[3], s3 = v[2] - v[3];
+      float y[4] = {s0 + s2, s1 + s3, s0 - s2, s1 - s3};
+      lane_butterfly<16>(y[0], y[1]);
+      lane_butterfly<16>(y[2], y[3]);
+      lane_butterfly<32>(y[0], y[1]);
+      lane_butterfly<32>(y[2], y[3]);
+      v = f32x4{y[0], y[1], y[2], y[3]};
+    }
+    const f32x4 s0 = acc[0][m] + acc[1][m], s1 = acc[0][m] - acc[1][m], s2 = acc[2][m] + acc[3][m], s3 = acc[2][m] - acc[3][m];
+    // The tiles of side 0 come first.
+    const f32x4 d0 = side ? s2 - s0 : s0 - s2, d1 = side ? s3 - s1 : s1 - s3;
+    acc[0][m] = side ? d0 : s0 + s2, acc[1][m] = side ? d1 : s1 + s3;
+    acc[2][m] = side ? s0 + s2 : d0, acc[3][m] = side ? s1 + s3 : d1;
+    // Two chunks take turns: a wave writes one after its partner has read the other.
+    f32x4* held = exchange + (m & 1) * CHUNK;
+    if (m == 0) __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) held[(wave * 4 + j) * 64 + lane] = acc[j][m];
+    __syncthreads();
+    const int row = row0 + 16 * m;
+    const bool writes = there && row < a.rows;
+    const float scale = writes ? a.scale[row] * ROOT : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int column = column_of(j);
+      const f32x4 other = held[((wave ^ 2) * 4 + j) * 64 + lane];
+      const f32x4 v = quarter & 1 ? other - acc[j][m] : acc[j][m] + other;
+      if (writes) {
+        u32x2 w;
+        w[0] = narrow<BF16>(v[0] * scale * a.sv.at(column)) | narrow<BF16>(v[1] * scale * a.sv.at(column + 1)) << 16;
+        w[1] = narrow<BF16>(v[2] * scale * a.sv.at(column + 2)) | narrow<BF16>(v[3] * scale * a.sv.at(column + 3)) << 16;
+        *reinterpret_cast<u32x2*>(a.out + (int64_t)row * a.n + column) = w;
       }
     }
   }
@@ -601,13 +743,13 @@ __global__ void __launch_bounds__(256) linear_join_kernel(JoinArgs a) {
 
 // ------------------------------------------------------------ plan
 
-// Variants by the rows: of 8 << variant rows, the last in blocks of 128.
-enum Variant { ROWS8, ROWS16, BLOCK32, BLOCK64, BLOCK128 };
+// Variants by the rows.
+enum Variant { ROWS8, ROWS16, BLOCK32, BLOCK64, BLOCK128, BLOCK_WIDE };
 
 // How a call is cut.
 struct Plan {
   Variant variant;
-  int parts;                       // float16 parts of a value: 2, or 1 in blocks of 128 bfloat16 rows
+  int parts;                       // float16 parts of a value: 2, or 1 of more than 64 bfloat16 rows
   int block_rows, blocks, sets;    // rows of a block, blocks, sets of a block
   int groups, splits;              // column groups, shares of the input channels
   int64_t z_bytes, scale_bytes, partial_bytes;
@@ -617,24 +759,24 @@ constexpr int CUS = 256;
 
 Plan plan_of(int64_t rows, int64_t k, int64_t n, bool bf16) {
   Plan p{};
-  p.variant = rows <= 8 ? ROWS8 : rows <= 16 ? ROWS16 : rows <= 32 ? BLOCK32 : rows <= 64 ? BLOCK64 : BLOCK128;
-  p.parts = p.variant == BLOCK128 && bf16 ? 1 : 2;
-  p.block_rows = 8 << p.variant;
+  p.variant = rows <= 8 ? ROWS8 : rows <= 16 ? ROWS16 : rows <= 32 ? BLOCK32 : rows <= 64 ? BLOCK64 : rows <= 128 && bf16 ? BLOCK128 : BLOCK_WIDE;
+  p.parts = p.variant >= BLOCK128 && bf16 ? 1 : 2;
+  p.block_rows = p.variant == BLOCK_WIDE ? 256 / p.parts : 8 << p.variant;
   p.blocks = (int)((rows + p.block_rows - 1) / p.block_rows);
   p.sets = p.block_rows * p.parts / 16;
-  int64_t most, want = 2 * CUS;    // splits: at most, workgroups that fill the chip
+  int64_t most, want;              // splits: at most, workgroups that fill the chip
   if (p.variant <= ROWS16) {
     p.groups = (int)(n / 32);
-    most = std::max<int64_t>(1, k / 512);
+    most = std::max<int64_t>(1, k / 512), want = 2 * CUS;
   } else {
-    const int columns = p.variant == BLOCK128 ? 256 : 128;
+    const int columns = p.variant >= BLOCK128 ? 256 : 128;
     p.groups = (int)((n + columns - 1) / columns);
-    most = k / HAD;
+    most = k / HAD, want = p.variant == BLOCK_WIDE ? CUS : 2 * CUS;
   }
   p.splits = (int)std::min(most, std::max<int64_t>(1, want / ((int64_t)p.groups * p.blocks)));
   p.z_bytes = k / 32 * p.sets * 1024 * p.blocks;
   p.scale_bytes = (4 * rows + 15) & ~(int64_t)15;
-  const bool direct = p.variant == BLOCK128 && p.splits == 1;
+  const bool direct = p.variant == BLOCK_WIDE && p.splits == 1;
   p.partial_bytes = direct ? 0 : 4 * (int64_t)p.splits * rows * n;
   return p;
 }
@@ -646,9 +788,10 @@ void launch_product(const Plan& p, const LinearArgs& a, hipStream_t stream) {
   switch (p.variant) {
     case ROWS8: linear_kernel<(K > 5), CB, 1, 2, 8><<<grid, 512, 0, stream>>>(a); break;
     case ROWS16: linear_kernel<(K > 5), CB, 2, 2, 8><<<grid, 512, 0, stream>>>(a); break;
-    case BLOCK32: linear_blocks_kernel<K, CB, false, 2, 2, 2><<<all, 256, 0, stream>>>(a); break;
-    case BLOCK64: linear_blocks_kernel<K, CB, false, 4, 2, 2><<<all, 256, 0, stream>>>(a); break;
-    case BLOCK128: linear_blocks_kernel<K, CB, BF16, 8, BF16 ? 1 : 2, 4><<<all, 256, 0, stream>>>(a); break;
+    case BLOCK32: linear_blocks_kernel<K, CB, 2, 2, 2><<<all, 256, 0, stream>>>(a); break;
+    case BLOCK64: linear_blocks_kernel<K, CB, 4, 2, 2><<<all, 256, 0, stream>>>(a); break;
+    case BLOCK128: linear_blocks_kernel<K, CB, 8, 1, 4><<<all, 256, 0, stream>>>(a); break;
+    case BLOCK_WIDE: linear_wide_kernel<K, CB, BF16, BF16 ? 1 : 2><<<all, 512, 0, stream>>>(a); break;
   }
 }
 template <int CB, bool BF16>
