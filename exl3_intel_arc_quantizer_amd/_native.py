@@ -1389,8 +1389,12 @@ def linear(x, trellis, su, sv, K: int, cb: int):
     if stride[1] != 1 or stride[0] % 8 or stride[0] < 0 or rows.data_ptr() % 16:
         rows = rows.clone(memory_format=torch.contiguous_format)
         stride = rows.stride()
-    if trellis.data_ptr() % 4:
+    if trellis.data_ptr() % 16:
         trellis = trellis.clone()
+    if su.data_ptr() % 16:
+        su = su.clone()
+    if sv.data_ptr() % 16:
+        sv = sv.clone()
     count = rows.shape[0]
     lib = load_library()
     code = _types()[x.dtype]

@@ -1,9 +1,11 @@
 // MI355X (gfx950) kernels of products with trellis weights as they are stored:
 //
-//   linear_turn_kernel  rows of x scaled, transformed and split in two float16
-//                       parts, in the order of the matrix instructions' operands
-//   linear_kernel       tiles decoded in registers and multiplied
-//   linear_join_kernel  sums of the shares, taken back and scaled
+//   linear_turn_kernel    rows of x scaled, transformed and split in float16 parts,
+//                         in the order of the matrix instructions' operands
+//   linear_rows_kernel    tiles decoded in registers and multiplied, up to 16 rows
+//   linear_blocks_kernel  up to 64 rows, 128 of bfloat16
+//   linear_wide_kernel    more
+//   linear_join_kernel    sums of the shares, transformed and scaled
 //
 // Weights of (in, out) are tiles W of 16 x 16 codebook values, scales su and sv
 // and the orthonormal Sylvester matrix H of order 128, block by block:
@@ -182,7 +184,11 @@ struct LinearArgs {
   const uint32_t* words;
   const u32x4* z;
   float* partials;                 // [split][rows][n]
-  const float* scale;              // of the rows
+  const float* scale;              // of the rows; null where they are done
+  const uint16_t* x;               // the rows themselves, of up to FEW
+  int64_t stride;
+  const void* su;
+  int half_su;
   Scales sv;
   uint16_t* out;
   int rows, k, n, bits, splits;
@@ -266,35 +272,6 @@ __device__ __forceinline__ u32x4 operand_of(const uint32_t (&w)[2][WIDE ? 4 : 2]
   return f;
 }
 
-// A wave's column tiles, read step by step.
-template <bool WIDE, int CT>
-struct Reader {
-  const char* next;                // uniform
-  int64_t row_bytes;
-  Window late, early;
-  uint32_t bits;
-  __device__ __forceinline__ Reader(const LinearArgs& a, int step, int column, int lane) : bits(a.bits) {
-    const int n = lane & 15, q = lane >> 4, u = 8 * (n & 7) + 2 * q + (n >> 3);
-    late = window_of(4 * bits * (u + 1), bits), early = window_of(4 * bits * u + 2 * bits, bits);
-    row_bytes = (int64_t)(a.n / 16) * 32 * bits;
-    next = reinterpret_cast<const char*>(a.words) + 2 * step * row_bytes + (int64_t)column * 32 * bits;
-  }
-  __device__ __forceinline__ Words<WIDE, CT> load(bool on = true) {
-    Words<WIDE, CT> r;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        const char* at = next + t * row_bytes + c * (32 * bits);
-        auto word = [&](uint32_t byte) { return *reinterpret_cast<const uint32_t*>(at + byte); };
-        r.w[c][t][0] = word(late.at0), r.w[c][t][1] = word(late.at1);
-        if constexpr (WIDE) r.w[c][t][2] = word(early.at0), r.w[c][t][3] = word(early.at1);
-      }
-    next += on ? 2 * row_bytes : 0;
-    return r;
-  }
-};
-
 // Sixteen bytes a lane from memory, `lane_at` bytes past `from`, to shared memory,
 // to byte `to` (of the wave's first lane) and on from there. Written out, as the
 // compiler would wait for all of these before it reads any shared memory; the waits
@@ -307,120 +284,234 @@ __device__ __forceinline__ uint32_t shared_byte(const void* p) {
   return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p);
 }
 
-// Up to 16 rows: every wave takes CT column tiles and its share of the input
-// channels; a workgroup's waves add up in shared memory.
-template <bool WIDE, int CB, int SETS, int CT, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES) linear_kernel(LinearArgs a) {
-  __shared__ f32x4 sums[WAVES][CT][64];
+// The value of the lane whose number differs in bit X, of rows of 16 lanes.
+template <int X>
+__device__ __forceinline__ float row_other(float v) {
+  if constexpr (X < 4) return exl3::quad_other<X>(v);
+  int w = __builtin_bit_cast(int, v);
+  if constexpr (X == 4) {                                // 7 - i, then back within quads
+    w = __builtin_amdgcn_update_dpp(0, w, 0x141, 0xF, 0xF, true);
+    w = __builtin_amdgcn_update_dpp(0, w, 0x1B, 0xF, 0xF, true);
+  } else {
+    w = __builtin_amdgcn_update_dpp(0, w, 0x128, 0xF, 0xF, true);
+  }
+  return __builtin_bit_cast(float, w);
+}
+template <int X>
+__device__ __forceinline__ float row_butterfly(float v, int lane) {
+  const float o = row_other<X>(v);
+  return lane & X ? o - v : v + o;
+}
+
+// Up to 16 rows: a wave takes 32 columns and a share of the blocks of 128 input
+// channels; a workgroup's eight waves add up in shared memory. Words come through
+// shared memory, each wave's own, a block ahead (2 KB at 4 bits), as a lane's dwords
+// lie 16 bytes from its neighbour's, and the vector cache then takes four of them at a
+// time. One row of 4096 by 4096, 8.6 MB of words: 6.8 us and 3.2 to join; launches and
+// latency bound it (by 12288, 25 MB: 12.5 us, 2 TB/s).
+//
+// FUSED (up to FEW rows): the wave transforms its blocks of the rows itself, two
+// channels a lane, with a power of two of their own, which saves a launch; each of
+// the n / 32 waves of a block does so, 60 instructions a row where decoding a block
+// of 32 columns takes 300. Parts of a row lie in columns r and r + 4 of 8 (each twice
+// in 16). Else the rows are read as linear_turn_kernel left them: SETS 1, up to 8
+// rows, or 2.
+constexpr int FEW = 4;
+template <int K, int CB, bool BF16, int SETS, bool FUSED>
+__global__ void __launch_bounds__(512) linear_rows_kernel(LinearArgs a) {
+  constexpr int CT = 2, WAVES = 8, SEGMENT = CT * 32 * K, WORDS = 8 * SEGMENT, LOADS = (WORDS + 1023) / 1024;
+  constexpr int OWN = 2 * WORDS > CT * 1024 ? 2 * WORDS : CT * 1024;  // bytes of a wave: two blocks' words, or its sums
+  constexpr bool WIDE = K > 5;
+  __shared__ u32x4 held[WAVES * OWN / 16];
+  __shared__ u32x4 turned[FUSED ? WAVES * 128 : 1];      // [wave][step][q][column 8]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int column0 = blockIdx.x * CT, split = blockIdx.y;
-  const int steps = a.k / 32, parts = a.splits * WAVES, part = split * WAVES + wave;
-  const int begin = (int)((int64_t)steps * part / parts), end = (int)((int64_t)steps * (part + 1) / parts);
-  Reader<WIDE, CT> reader(a, begin, column0, lane);
-  f32x4 acc[CT];
-#pragma unroll
-  for (int c = 0; c < CT; ++c) acc[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const int blocks = a.k / HAD, parts = a.splits * WAVES, part = split * WAVES + wave;
+  const int begin = (int)((int64_t)blocks * part / parts), end = (int)((int64_t)blocks * (part + 1) / parts);
+  const int n = lane & 15, q = lane >> 4, u = 8 * (n & 7) + 2 * q + (n >> 3);
+  const Window late = window_of(4 * K * (u + 1), K), early = window_of(4 * K * u + 2 * K, K);
 
-  auto multiply = [&](const Words<WIDE, CT>& r, int step) __attribute__((always_inline)) {
-    const u32x4* z = a.z + (int64_t)step * SETS * 64 + lane;
-    u32x4 b[SETS];
+  const int64_t row_bytes = (int64_t)(a.n / 16) * 32 * K;
+  const char* next_words = reinterpret_cast<const char*>(a.words) + 8 * begin * row_bytes + (int64_t)column0 * 32 * K;
+  char* own = reinterpret_cast<char*>(held) + wave * OWN;
+  const uint32_t own_byte = shared_byte(own);
+  uint32_t word_at[LOADS];                               // (row_bytes is at most 2^28)
 #pragma unroll
-    for (int s = 0; s < SETS; ++s) b[s] = z[s * 64];
+  for (int i = 0; i < LOADS; ++i) {
+    const int at = 1024 * i + 16 * lane;
+    word_at[i] = (uint32_t)(at / SEGMENT * row_bytes + at % SEGMENT);
+  }
+  auto send = [&](int to) __attribute__((always_inline)) {
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {
-      const u32x4 f = operand_of<WIDE, CB>(r.w[c], reader.late, reader.early, reader.bits);
+    for (int i = 0; i < LOADS; ++i)
+      if (1024 * i + 16 * lane < WORDS) to_shared(next_words, word_at[i], __builtin_amdgcn_readfirstlane(own_byte + to * WORDS + 1024 * i));
+    next_words += 8 * row_bytes;
+  };
+  // A block's rows: two channels a lane (FUSED), or operands.
+  uint32_t xs[FUSED ? FEW : 1];
+  f32x2 su;
+  u32x4 b[FUSED ? 1 : 4 * SETS];
+  auto load = [&](int block) __attribute__((always_inline)) {
+    if constexpr (FUSED) {
+      const int64_t at = (int64_t)block * HAD + 2 * lane;
+      if (a.half_su) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.su) + at);
+        su = f32x2{widen<false>(w & 0xffffu), widen<false>(w >> 16)};
+      } else {
+        su = *reinterpret_cast<const f32x2*>(static_cast<const float*>(a.su) + at);
+      }
 #pragma unroll
-      for (int s = 0; s < SETS; ++s) acc[c] = mfma(f, b[s], acc[c]);
+      for (int r = 0; r < FEW; ++r)
+        if (r < a.rows) xs[r] = *reinterpret_cast<const uint32_t*>(a.x + r * a.stride + at);
+    } else {
+      const u32x4* z = a.z + (int64_t)block * (4 * SETS * 64) + lane;
+#pragma unroll
+      for (int i = 0; i < 4 * SETS; ++i) b[i] = z[i * 64];
     }
   };
-
+  f32x4 total[CT];
+#pragma unroll
+  for (int c = 0; c < CT; ++c) total[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   if (begin < end) {
-    Words<WIDE, CT> even = reader.load(), odd = even;
-    for (int step = begin; step < end; step += 2) {
-      if (step + 1 < end) odd = reader.load();
-      multiply(even, step);
-      if (step + 1 == end) break;
-      if (step + 2 < end) even = reader.load();
-      multiply(odd, step + 1);
-    }
+    load(begin);
+    send(0);
   }
+  for (int block = begin; block < end; ++block) {
+    const int now = (block - begin) & 1;
+    float scale = 0.0f;                                  // of this lane's column
+    u32x4* z = turned + wave * 128;
+    if constexpr (FUSED) {
+      // The dword of a lane's two channels in a column's operand.
+      uint32_t* to = reinterpret_cast<uint32_t*>(z + ((lane >> 4) * 4 + (lane & 3)) * 8) + (lane >> 2 & 3);
 #pragma unroll
-  for (int c = 0; c < CT; ++c) sums[wave][c][lane] = acc[c];
+      for (int r = 0; r < FEW; ++r) {
+        if (r >= a.rows) break;
+        float x = widen<BF16>(xs[r] & 0xffffu) * su[0], y = widen<BF16>(xs[r] >> 16) * su[1];
+        // The largest magnitude as bits: NaN above infinity above all numbers.
+        uint32_t top = max(__builtin_bit_cast(uint32_t, x) & 0x7fffffffu, __builtin_bit_cast(uint32_t, y) & 0x7fffffffu);
+        auto other = [&](float v) { top = max(top, __builtin_bit_cast(uint32_t, v)); };
+        other(row_other<1>(__builtin_bit_cast(float, top)));
+        other(row_other<2>(__builtin_bit_cast(float, top)));
+        other(row_other<4>(__builtin_bit_cast(float, top)));
+        other(row_other<8>(__builtin_bit_cast(float, top)));
+        top = max(max((uint32_t)__builtin_amdgcn_readlane((int)top, 0), (uint32_t)__builtin_amdgcn_readlane((int)top, 16)),
+                  max((uint32_t)__builtin_amdgcn_readlane((int)top, 32), (uint32_t)__builtin_amdgcn_readlane((int)top, 48)));
+        // As in linear_turn_kernel: values under 2^11, those of z under 2^15.
+        const int power = max((int)(top >> 23), 1) - 126 - 11;
+        const float own_scale = top < 0x7f800000u ? ldexpf(1.0f, power) : __builtin_nanf("");
+        if ((n & 3) == r) scale = own_scale;
+        x = ldexpf(x, -power), y = ldexpf(y, -power);
+        const float sum = x + y, difference = x - y;
+        x = row_butterfly<8>(row_butterfly<4>(row_butterfly<2>(row_butterfly<1>(sum, lane), lane), lane), lane);
+        y = row_butterfly<8>(row_butterfly<4>(row_butterfly<2>(row_butterfly<1>(difference, lane), lane), lane), lane);
+        lane_butterfly<16>(x, y);
+        lane_butterfly<32>(x, y);
+        x *= ROOT, y *= ROOT;
+        const _Float16 hx = (_Float16)x, hy = (_Float16)y;
+        to[4 * r] = __builtin_bit_cast(uint32_t, f16x2{hx, hy});
+        to[4 * (r + 4)] = pair_of(x - (float)hx, y - (float)hy);
+      }
+    }
+    // The block's words (and what was loaded before them).
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    u32x4 rows[4 * SETS];
+#pragma unroll
+    for (int i = 0; i < 4 * SETS; ++i) rows[i] = FUSED ? z[(i * 4 + q) * 8 + (n & 7)] : b[i];
+    if (block + 1 < end) {
+      load(block + 1);
+      send(now ^ 1);
+    }
+    f32x4 acc[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) acc[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const char* from = own + now * WORDS;
+#pragma unroll
+    for (int step = 0; step < 4; ++step)
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        uint32_t w[2][WIDE ? 4 : 2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int place = (2 * step + t) * SEGMENT + c * 32 * K;
+          auto word = [&](uint32_t at) { return *reinterpret_cast<const uint32_t*>(from + at + place); };
+          w[t][0] = word(late.at0), w[t][1] = word(late.at1);
+          if constexpr (WIDE) w[t][2] = word(early.at0), w[t][3] = word(early.at1);
+        }
+        const u32x4 f = operand_of<WIDE, CB>(w, late, early, K);
+#pragma unroll
+        for (int s = 0; s < SETS; ++s) acc[c] = mfma(f, rows[step * SETS + s], acc[c]);
+      }
+#pragma unroll
+    for (int c = 0; c < CT; ++c) total[c] += FUSED ? acc[c] * scale : acc[c];
+  }
+  // A wave's words are read; its sums take their place.
+  f32x4* sums = reinterpret_cast<f32x4*>(own);
+#pragma unroll
+  for (int c = 0; c < CT; ++c) sums[c * 64 + lane] = total[c];
   __syncthreads();
+  constexpr int PARTS = FUSED ? 4 : 8;                   // columns between a row's parts
   for (int i = tid; i < CT * 64; i += 64 * WAVES) {
-    const int c = i >> 6, l = i & 63;
-    if (SETS == 1 && (l & 8)) continue;
-    f32x4 v = sums[0][c][l];
+    const int c = i >> 6, l = i & 63, row = l & 15;
+    if (row >= a.rows) continue;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) v += sums[w][c][l];
-    if constexpr (SETS == 1)
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) v += sums[w][c][l + 8];
-    const int row = l & 15, column = 16 * (column0 + c) + 4 * (l >> 4);
-    if (row < a.rows)
-      *reinterpret_cast<f32x4*>(a.partials + ((int64_t)split * a.rows + row) * a.n + column) = v;
+    for (int w = 0; w < WAVES; ++w) {
+      const f32x4* of = reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(held) + w * OWN) + c * 64;
+      v += of[l];
+      if (SETS == 1) v += of[l + PARTS];
+    }
+    *reinterpret_cast<f32x4*>(a.partials + ((int64_t)split * a.rows + row) * a.n + 16 * (column0 + c) + 4 * (l >> 4)) = v;
   }
 }
 
-// More rows: a workgroup takes a block of 16 MT rows and, four waves, 64 CT
-// columns, of a share of the input channels. Rows come through shared memory for
-// all waves; each wave decodes its own columns, one step ahead of the products,
-// and its words come through shared memory too: a lane's dwords lie 16 bytes from
-// its neighbour's, which the vector cache takes one by four (2055 rows of 4096 by
-// 12288 with words read from memory: L1_US us), shared memory all at once.
+// Up to 64 rows, or 128 of one part: a workgroup takes all of them, 16 MT, and, eight
+// waves, 256 columns, of a share of the input channels. Rows come through shared
+// memory for all waves; each wave decodes its own columns, one step ahead of the
+// products, and its words come through shared memory as above. 64 rows of 4096 by
+// 4096, 22 us: 5 to turn the rows, 12 here, 4 to join 16 shares (four waves of twice
+// the columns and 32 shares, which two waves a SIMD hide less of: 30).
 //
 // In step s rows s + DEPTH + 1 and words s + DEPTH + 2 are sent for, in as many
 // instructions each step (past the end the last ones again, which nobody uses), so
 // that a step begins when all but those of the last DEPTH steps are there.
-//
-// A step of MT = 8 is 32 matrix instructions (PARTS: 64), and 16 halves of tiles
-// decoded between them. Two workgroups a CU: a wave alone issues one instruction
-// in five cycles, two in two and a half.
-constexpr int depth_of(int mt, int k) {
-  return mt < 8 ? 4 : k <= 6 ? 3 : 2;
-}
-template <int K, int CB, int MT, int PARTS, int CT>
-__global__ void __launch_bounds__(256, 2) linear_blocks_kernel(LinearArgs a) {
-  constexpr int SETS = MT * PARTS, DEPTH = depth_of(MT, K), AHEAD = 4, HALVES = 4 * CT;
+template <int K, int CB, int MT, int PARTS>
+__global__ void __launch_bounds__(512, 2) linear_blocks_kernel(LinearArgs a) {
+  constexpr int CT = 2, SETS = MT * PARTS, DEPTH = 4, AHEAD = 4, HALVES = 4 * CT;
   constexpr int ROWS = SETS * 64, ROW_SLOTS = DEPTH + 2;                     // vectors of a step's rows
   constexpr int SEGMENT = CT * 32 * K, WORDS = 2 * SEGMENT, WORD_SLOTS = DEPTH + 2;  // bytes of a wave's words
-  constexpr int ROW_LOADS = SETS / 4, WORD_LOADS = (WORDS + 1023) / 1024;    // a wave's of a step
+  static_assert(SETS <= 8 && WORDS <= 1024, "a step's rows, and a wave's words, are one load of a wave each");
   __shared__ u32x4 rows_held[ROW_SLOTS * ROWS];
-  __shared__ u32x4 words_held[4 * WORD_SLOTS * WORDS / 16];
+  __shared__ u32x4 words_held[8 * WORD_SLOTS * WORDS / 16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // Workgroups are dealt to the chip's eight dies in turn: each die takes a run
   // of them, which share a block of rows in its cache.
-  const int groups = (a.n + 64 * CT - 1) / (64 * CT), all = gridDim.x, die = blockIdx.x & 7;
+  const int all = gridDim.x, die = blockIdx.x & 7;
   const int unit = die * (all / 8) + min(die, all % 8) + (int)(blockIdx.x >> 3);
-  const int split = unit % a.splits, group = unit / a.splits % groups, block = unit / a.splits / groups;
-  const int column0 = (group * 4 + wave) * CT;
+  const int split = unit % a.splits, group = unit / a.splits;
+  const int column0 = (group * 8 + wave) * CT;
   const bool there = column0 < a.n / 16;                 // (waves past the columns read the first ones)
   const int all_steps = a.k / 32;
   const int begin = (int)((int64_t)all_steps * split / a.splits), steps = (int)((int64_t)all_steps * (split + 1) / a.splits) - begin;
 
   const int64_t row_bytes = (int64_t)(a.n / 16) * 32 * K;
   const char* next_words = reinterpret_cast<const char*>(a.words) + 2 * begin * row_bytes + (int64_t)(there ? column0 : 0) * 32 * K;
-  const char* next_rows = reinterpret_cast<const char*>(a.z + ((int64_t)block * all_steps + begin) * ROWS);
+  const char* next_rows = reinterpret_cast<const char*>(a.z + (int64_t)begin * ROWS);
   u32x4* own_words = words_held + wave * (WORD_SLOTS * WORDS / 16);
-  uint32_t word_at[WORD_LOADS];                          // this lane's of a step (row_bytes is under 2^29)
-#pragma unroll
-  for (int i = 0; i < WORD_LOADS; ++i) {
-    const int at = 1024 * i + 16 * lane;
-    word_at[i] = (uint32_t)(at / SEGMENT * row_bytes + at % SEGMENT);
-  }
+  const uint32_t word_at = (uint32_t)(16 * lane / SEGMENT * row_bytes + 16 * lane % SEGMENT);  // (row_bytes is at most 2^28)
   int rows_sent = 0, words_sent = 0;                     // steps sent for, and places of the next
   const uint32_t rows0 = shared_byte(rows_held + wave * 64), words0 = shared_byte(own_words);
   uint32_t rows_to = rows0, words_to = words0;
+  // (A wave past the rows' sets sends for its words twice, so that all count alike.)
   auto send_rows = [&]() __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < ROW_LOADS; ++i) to_shared(next_rows + i * 4096, 16 * tid, rows_to + i * 4096);
+    if (wave < SETS)
+      to_shared(next_rows, 16 * tid, rows_to);
+    else if (16 * lane < WORDS)
+      to_shared(next_words, word_at, words_to);
     next_rows += ++rows_sent < steps ? 16 * ROWS : 0;
     rows_to = rows_to == rows0 + (ROW_SLOTS - 1) * (16 * ROWS) ? rows0 : rows_to + 16 * ROWS;
   };
   auto send_words = [&]() __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < WORD_LOADS; ++i)
-      if (1024 * i + 16 * lane < WORDS) to_shared(next_words, word_at[i], words_to + 1024 * i);
+    if (16 * lane < WORDS) to_shared(next_words, word_at, words_to);
     next_words += ++words_sent < steps ? 2 * row_bytes : 0;
     words_to = words_to == words0 + (WORD_SLOTS - 1) * WORDS ? words0 : words_to + WORDS;
   };
@@ -459,7 +550,7 @@ __global__ void __launch_bounds__(256, 2) linear_blocks_kernel(LinearArgs a) {
   u32x4 f[2][CT];
   int slot = 0;                                          // of the rows
   auto wait = [&]() __attribute__((always_inline)) {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(DEPTH * (ROW_LOADS + WORD_LOADS)) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(DEPTH * 2) : "memory");
   };
   wait();
   read_words(own_words);
@@ -506,7 +597,7 @@ __global__ void __launch_bounds__(256, 2) linear_blocks_kernel(LinearArgs a) {
   for (int c = 0; c < CT; ++c)
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      const int row = block * 16 * MT + 16 * m + (lane & 15), column = 16 * (column0 + c) + 4 * (lane >> 4);
+      const int row = 16 * m + (lane & 15), column = 16 * (column0 + c) + 4 * (lane >> 4);
       if (row < a.rows) *reinterpret_cast<f32x4*>(a.partials + ((int64_t)split * a.rows + row) * a.n + column) = acc[c][m];
     }
 }
@@ -710,43 +801,57 @@ struct JoinArgs {
   int rows, n, splits;
 };
 
-// Sixteen lanes take a block of 128 outputs of a row, eight each.
+// A wave takes a block of 128 outputs of a row, eight a lane; its four rows of
+// lanes take shares in turn, as their loads wait for each other.
 template <bool BF16>
 __global__ void __launch_bounds__(256) linear_join_kernel(JoinArgs a) {
-  const int64_t unit = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
   const int lane = threadIdx.x & 63, blocks = a.n / HAD;
-  const bool there = unit < (int64_t)a.rows * blocks;
-  const int row = there ? (int)(unit / blocks) : 0, column = there ? (int)(unit % blocks) * HAD + 8 * (lane & 15) : 8 * (lane & 15);
+  if (unit >= (int64_t)a.rows * blocks) return;
+  const int row = (int)(unit / blocks), column = (int)(unit % blocks) * HAD + 8 * (lane & 15);
   float v[8] = {};
-  for (int s = 0; s < a.splits; ++s) {
-    const f32x4* p = reinterpret_cast<const f32x4*>(a.partials + ((int64_t)s * a.rows + row) * a.n + column);
-    const f32x4 x = p[0], y = p[1];
+  for (int s = lane >> 4; s < a.splits; s += 16) {
+    f32x4 x[4][2];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] += x[e], v[4 + e] += y[e];
+    for (int i = 0; i < 4; ++i) {
+      const f32x4* p = reinterpret_cast<const f32x4*>(a.partials + ((int64_t)min(s + 4 * i, a.splits - 1) * a.rows + row) * a.n + column);
+      x[i][0] = p[0], x[i][1] = p[1];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += s + 4 * i < a.splits ? x[i][e / 4][e % 4] : 0.0f;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    v[e] += __shfl_xor(v[e], 16);
+    v[e] += __shfl_xor(v[e], 32);
   }
   exl3::quad_transform(v, lane);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float o4 = __shfl_xor(v[e], 4);
-    v[e] = lane & 4 ? o4 - v[e] : v[e] + o4;
-    const float o8 = __shfl_xor(v[e], 8);
-    v[e] = lane & 8 ? o8 - v[e] : v[e] + o8;
-  }
-  const float scale = a.scale[row] * ROOT;
+  for (int e = 0; e < 8; ++e) v[e] = row_butterfly<8>(row_butterfly<4>(v[e], lane), lane);
+  if (lane >= 16) return;
+  const float scale = (a.scale ? a.scale[row] : 1.0f) * ROOT;
   u32x4 w;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     w[e] = narrow<BF16>(v[2 * e] * scale * a.sv.at(column + 2 * e)) |
            narrow<BF16>(v[2 * e + 1] * scale * a.sv.at(column + 2 * e + 1)) << 16;
-  if (there) *reinterpret_cast<u32x4*>(a.out + (int64_t)row * a.n + column) = w;
+  *reinterpret_cast<u32x4*>(a.out + (int64_t)row * a.n + column) = w;
 }
 
 // ------------------------------------------------------------ plan
 
 // Variants by the rows.
-enum Variant { ROWS8, ROWS16, BLOCK32, BLOCK64, BLOCK128, BLOCK_WIDE };
+enum Variant { ROWS_FEW, ROWS8, ROWS16, BLOCK32, BLOCK48, BLOCK64, BLOCK128, BLOCK_WIDE };
+constexpr int BLOCK_ROWS[] = {FEW, 8, 16, 32, 48, 64, 128};
 
-// How a call is cut.
+// How a call is cut: the variant of the fewest rows that takes them all (two float16
+// parts). Times in a graph, us, of the one chosen and of the next larger one, at 4
+// bits: 1 row of 4096 by 4096 9.0 and 12.6, 4 rows 10.3 and 13.0; 8 rows of 4096 by
+// 12288 17.7 and 18.7; 16 rows of 12288 by 4096 24.4 and 27.0; 32 rows of 4096 by 4096
+// 16.9 and 18.3; 48 rows of 4096 by 12288 32.1 and 33.1; 128 rows of 4096 by 4096
+// (bfloat16) 28.0 and 30.1.
 struct Plan {
   Variant variant;
   int parts;                       // float16 parts of a value: 2, or 1 of more than 64 bfloat16 rows
@@ -759,23 +864,29 @@ constexpr int CUS = 256;
 
 Plan plan_of(int64_t rows, int64_t k, int64_t n, bool bf16) {
   Plan p{};
-  p.variant = rows <= 8 ? ROWS8 : rows <= 16 ? ROWS16 : rows <= 32 ? BLOCK32 : rows <= 64 ? BLOCK64 : rows <= 128 && bf16 ? BLOCK128 : BLOCK_WIDE;
+  p.variant = ROWS_FEW;
+  while (p.variant < BLOCK_WIDE && rows > BLOCK_ROWS[p.variant]) p.variant = (Variant)(p.variant + 1);
+  if (p.variant == BLOCK128 && !bf16) p.variant = BLOCK_WIDE;
   p.parts = p.variant >= BLOCK128 && bf16 ? 1 : 2;
-  p.block_rows = p.variant == BLOCK_WIDE ? 256 / p.parts : 8 << p.variant;
+  p.block_rows = p.variant == BLOCK_WIDE ? 256 / p.parts : BLOCK_ROWS[p.variant];
   p.blocks = (int)((rows + p.block_rows - 1) / p.block_rows);
-  p.sets = p.block_rows * p.parts / 16;
-  int64_t most, want;              // splits: at most, workgroups that fill the chip
+  p.sets = p.variant == ROWS_FEW ? 0 : p.block_rows * p.parts / 16;
+  // Shares of the input channels that fill the chip: a wave of linear_rows_kernel
+  // takes at least one block of 128, a workgroup of linear_blocks_kernel too; one of
+  // linear_wide_kernel at least 640 channels, as the shares' sums go through memory
+  // (300 rows of 4096 by 4096: 8 shares 58 us, 6 52; 200 rows: 16 45 us, 6 39).
+  int64_t most, want = CUS;
   if (p.variant <= ROWS16) {
     p.groups = (int)(n / 32);
-    most = std::max<int64_t>(1, k / 512), want = 2 * CUS;
+    most = k / (8 * HAD), want = 4 * CUS;
   } else {
-    const int columns = p.variant >= BLOCK128 ? 256 : 128;
-    p.groups = (int)((n + columns - 1) / columns);
-    most = k / HAD, want = p.variant == BLOCK_WIDE ? CUS : 2 * CUS;
+    p.groups = (int)((n + 255) / 256);
+    most = p.variant == BLOCK_WIDE ? k / (5 * HAD) : k / HAD;
   }
+  most = std::max<int64_t>(1, most);
   p.splits = (int)std::min(most, std::max<int64_t>(1, want / ((int64_t)p.groups * p.blocks)));
   p.z_bytes = k / 32 * p.sets * 1024 * p.blocks;
-  p.scale_bytes = (4 * rows + 15) & ~(int64_t)15;
+  p.scale_bytes = p.variant == ROWS_FEW ? 0 : (4 * rows + 15) & ~(int64_t)15;
   const bool direct = p.variant == BLOCK_WIDE && p.splits == 1;
   p.partial_bytes = direct ? 0 : 4 * (int64_t)p.splits * rows * n;
   return p;
@@ -786,11 +897,13 @@ void launch_product(const Plan& p, const LinearArgs& a, hipStream_t stream) {
   const dim3 grid(p.groups, p.splits);
   const unsigned all = (unsigned)(p.groups * p.splits * p.blocks);
   switch (p.variant) {
-    case ROWS8: linear_kernel<(K > 5), CB, 1, 2, 8><<<grid, 512, 0, stream>>>(a); break;
-    case ROWS16: linear_kernel<(K > 5), CB, 2, 2, 8><<<grid, 512, 0, stream>>>(a); break;
-    case BLOCK32: linear_blocks_kernel<K, CB, 2, 2, 2><<<all, 256, 0, stream>>>(a); break;
-    case BLOCK64: linear_blocks_kernel<K, CB, 4, 2, 2><<<all, 256, 0, stream>>>(a); break;
-    case BLOCK128: linear_blocks_kernel<K, CB, 8, 1, 4><<<all, 256, 0, stream>>>(a); break;
+    case ROWS_FEW: linear_rows_kernel<K, CB, BF16, 1, true><<<grid, 512, 0, stream>>>(a); break;
+    case ROWS8: linear_rows_kernel<K, CB, false, 1, false><<<grid, 512, 0, stream>>>(a); break;
+    case ROWS16: linear_rows_kernel<K, CB, false, 2, false><<<grid, 512, 0, stream>>>(a); break;
+    case BLOCK32: linear_blocks_kernel<K, CB, 2, 2><<<all, 512, 0, stream>>>(a); break;
+    case BLOCK48: linear_blocks_kernel<K, CB, 3, 2><<<all, 512, 0, stream>>>(a); break;
+    case BLOCK64: linear_blocks_kernel<K, CB, 4, 2><<<all, 512, 0, stream>>>(a); break;
+    case BLOCK128: linear_blocks_kernel<K, CB, 8, 1><<<all, 512, 0, stream>>>(a); break;
     case BLOCK_WIDE: linear_wide_kernel<K, CB, BF16, BF16 ? 1 : 2><<<all, 512, 0, stream>>>(a); break;
   }
 }
@@ -811,15 +924,17 @@ void launch_rate(const Plan& p, const LinearArgs& a, hipStream_t stream) {
 template <bool BF16>
 int launch_linear(const Plan& p, const TurnArgs& t, const LinearArgs& a, int cb, hipStream_t s) {
   const int threads = t.k <= 8192 ? 256 : t.k <= 16384 ? 512 : 1024;
-  linear_turn_kernel<BF16><<<(unsigned)a.rows, threads, 0, s>>>(t);
-  if (check_launch("exl3_linear")) return 1;
+  if (p.variant != ROWS_FEW) {
+    linear_turn_kernel<BF16><<<(unsigned)a.rows, threads, 0, s>>>(t);
+    if (check_launch("exl3_linear")) return 1;
+  }
   cb == 0 ? launch_rate<0, BF16>(p, a, s) : cb == 1 ? launch_rate<1, BF16>(p, a, s) : launch_rate<2, BF16>(p, a, s);
   if (check_launch("exl3_linear")) return 1;
   if (!p.partial_bytes) return 0;
   JoinArgs j{};
   j.partials = a.partials, j.scale = a.scale, j.sv = a.sv, j.out = a.out, j.rows = a.rows, j.n = a.n, j.splits = p.splits;
   const int64_t units = (int64_t)a.rows * (a.n / HAD);
-  linear_join_kernel<BF16><<<(unsigned)((units + 15) / 16), 256, 0, s>>>(j);
+  linear_join_kernel<BF16><<<(unsigned)((units + 3) / 4), 256, 0, s>>>(j);
   return check_launch("exl3_linear");
 }
 
@@ -844,10 +959,9 @@ int exl3_linear(const void* x, int64_t stride, int64_t rows, int type, const uin
   if (need < 0) return set_error("exl3_linear: bad sizes: %lld rows of %lld by %lld", (long long)rows, (long long)k, (long long)n);
   if (!rows) return 0;
   if ((reinterpret_cast<uintptr_t>(x) & 15) || stride % 8 || (reinterpret_cast<uintptr_t>(out) & 15) ||
-      (reinterpret_cast<uintptr_t>(workspace) & 15) || (reinterpret_cast<uintptr_t>(words) & 3))
-    return set_error("exl3_linear: rows, out and workspace must be 16-byte aligned, words 4-byte");
-  if (((reinterpret_cast<uintptr_t>(su) | reinterpret_cast<uintptr_t>(sv)) & 7))
-    return set_error("exl3_linear: su and sv must be 8-byte aligned");
+      (reinterpret_cast<uintptr_t>(workspace) & 15) || (reinterpret_cast<uintptr_t>(words) & 15) ||
+      (reinterpret_cast<uintptr_t>(su) & 15) || (reinterpret_cast<uintptr_t>(sv) & 15))
+    return set_error("exl3_linear: all memory must be 16-byte aligned");
   if (workspace_bytes < need) return set_error("exl3_linear: workspace of %lld bytes is too small", (long long)workspace_bytes);
   const Plan p = plan_of(rows, k, n, type == 2);
   char* w = static_cast<char*>(workspace);
@@ -857,7 +971,8 @@ int exl3_linear(const void* x, int64_t stride, int64_t rows, int type, const uin
   t.k = (int)k, t.sets = p.sets, t.block_rows = p.block_rows;
   t.rest = p.variant == ROWS8 ? 8 : p.parts == 2 ? 64 : 0;
   LinearArgs a{};
-  a.words = reinterpret_cast<const uint32_t*>(words), a.z = t.z, a.scale = t.scale, a.sv = {sv, half_scales >> 1 & 1};
+  a.words = reinterpret_cast<const uint32_t*>(words), a.z = t.z, a.scale = p.scale_bytes ? t.scale : nullptr;
+  a.x = t.x, a.stride = stride, a.su = su, a.half_su = t.half, a.sv = {sv, half_scales >> 1 & 1};
   a.out = static_cast<uint16_t*>(out), a.partials = reinterpret_cast<float*>(w + p.z_bytes + p.scale_bytes);
   a.rows = (int)rows, a.k = (int)k, a.n = (int)n, a.bits = K, a.splits = p.splits;
   auto launch = type == 2 ? launch_linear<true> : launch_linear<false>;

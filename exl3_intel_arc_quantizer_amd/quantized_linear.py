@@ -21,11 +21,13 @@ def quantized_linear(x: torch.Tensor, trellis: torch.Tensor, suh: torch.Tensor, 
     16, out / 16, 16 K), ``suh`` (in,) and ``svh`` (out,) in float16 or float32,
     ``cb`` its codebook; all on x's device.
 
-    The rows are scaled and transformed in float32 and count with 22 bits, the
+    The rows are scaled and transformed in float32 and count with 22 bits, or,
+    more than 64 of them in bfloat16, with 11 (three more than their own); the
     codebook's values are exact, sums are float32; the result is rounded once. A
-    row with an infinity or a NaN is NaN. The call enqueues work on the current
-    stream of x's device and keeps nothing. It has no gradient: train through
-    ``x @ decode_weight_from_storage(...)``."""
+    row with an infinity or a NaN is NaN. Tensors that do not start at a multiple
+    of 16 bytes, and rows that lie otherwise, are copied first. The call enqueues
+    work on the current stream of x's device and keeps nothing. It has no
+    gradient: train through ``x @ decode_weight_from_storage(...)``."""
     if any(isinstance(t, torch.Tensor) and records(t) for t in (x, suh, svh)):
         raise RuntimeError("quantized_linear has no gradient: detach its inputs")
     return _native.linear(x, trellis, suh, svh, K, cb)

@@ -215,8 +215,9 @@ int64_t exl3_linear_workspace(int64_t rows, int64_t k, int64_t n, int type);
  * scales sv: y = ((x su) H W_tiles) H sv. Rows of x are `stride` elements apart,
  * type 1 float16 or 2 bfloat16, as is out. half_scales: bit 0 if su, bit 1 if sv
  * is float16, else float32. Rows are transformed in float32 and count with 22
- * bits, sums are float32. Rows with a value that is not finite are NaN. k and n
- * are multiples of 128; x, out and the workspace 16-byte aligned. */
+ * bits (11 where there are more than 64 of bfloat16), sums are float32. Rows with a
+ * value that is not finite are NaN. k and n are multiples of 128; all memory is
+ * 16-byte aligned. */
 int exl3_linear(const void* x, int64_t stride, int64_t rows, int type, const uint16_t* words,
                 const void* su, const void* sv, int half_scales, int64_t k, int64_t n, int K,
                 int cb, void* out, void* workspace, int64_t workspace_bytes, void* stream);

@@ -252,3 +252,40 @@ def test_refuses_cpu_tensors_and_sizes():
         assert lib.exl3_linear(None, 128, 4, kind, None, None, None, 0, 128, 128, K, cb, None, None, 1 << 40, None) == 1
     assert lib.exl3_linear(None, 128, 4, 1, None, None, None, 0, 128, 128, 4, 2, None, None, 16, None) == 1
     assert b"too small" in lib.exl3_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [3, 7, 30, 45, 100, 140])
+def test_weights_that_start_anywhere(rows):
+    """Words and scales that begin inside another tensor."""
+    x, words, su, sv = (t.cuda() for t in _given(rows, 256, 384, 3, torch.bfloat16))
+    want = quantized_linear(x, words, su, sv, 3)
+
+    def moved(t, by):
+        return torch.empty(t.numel() + by, dtype=t.dtype, device="cuda")[by:].view(t.shape).copy_(t)
+
+    for by in (1, 2, 4):
+        assert torch.equal(want, quantized_linear(x, moved(words, by), su, sv, 3))
+        assert torch.equal(want, quantized_linear(x, words, moved(su, by), moved(sv, by), 3))
+        assert torch.equal(want, quantized_linear(x, words, moved(su.float(), by), moved(sv.float(), by), 3))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [2, 3, 4, 48, 100])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_a_row_that_is_not_finite_is_alone(rows, dtype):
+    x, words, su, sv = (t.cuda() for t in _given(rows, 640, 256, 5, dtype))
+    want = quantized_linear(x, words, su, sv, 5)
+    for value in (float("nan"), float("inf")):
+        y = x.clone()
+        y[1, 637] = value
+        got = quantized_linear(y, words, su, sv, 5)
+        assert torch.isnan(got[1]).all() and torch.equal(got[0], want[0]) and torch.equal(got[2:], want[2:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows, k, n", [(4, 4096, 1408), (13, 4224, 256), (33, 2176, 768), (48, 1408, 4096), (128, 1152, 640),
+                                        (257, 640, 1280), (1024, 256, 512)])
+def test_more_sizes(rows, k, n):
+    for dtype in (torch.float16, torch.bfloat16):
+        _check(rows, k, n, 1 + rows % 8, rows % 3, dtype)
