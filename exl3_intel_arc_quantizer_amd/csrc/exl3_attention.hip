@@ -234,10 +234,12 @@ __device__ __forceinline__ int64_t quotient(int64_t x, int64_t d) {
   return (x | d) >> 32 ? x / d : (int64_t)((uint32_t)x / (uint32_t)d);
 }
 
-// The work is cut into equal shares, one an owner, of LEAST at least.
-constexpr int LEAST = 2;
+// The work is cut into equal shares, one an owner, of 2 at least; of trees more, as
+// each of their rows joins its shares' partials again (13 tokens of 4 heads over 4097
+// positions: 36 us at 2, 28.5 at 4, 31 at 8; over 1000 positions 24, 25 and 28).
+template <bool TREE>
 __device__ __forceinline__ int64_t share_of(const Class& c, int64_t all) {
-  return max(quotient(all + c.owners - 1, c.owners), (int64_t)LEAST);
+  return max(quotient(all + c.owners - 1, c.owners), (int64_t)(TREE ? 4 : 2));
 }
 
 // Last index i of [0, n) with at[i] <= x; at[0] <= x.
@@ -419,7 +421,7 @@ __global__ void __launch_bounds__(THREADS, resident(D, WIDE, CT)) attend_rows_ke
   sum_work<TREE, THREADS>(a, cls, prefix, parts);
   if (blockIdx.x == 0)
     for (int r = tid; r <= a.requests; r += THREADS) cls.shares[r] = prefix[r];
-  const int64_t all = uniform(prefix[a.requests]), share = share_of(cls, all);
+  const int64_t all = uniform(prefix[a.requests]), share = share_of<TREE>(cls, all);
   const int owner = (int)blockIdx.x * WAVES + wave;
   const int64_t begin = owner * share, end = min(begin + share, all);
 
@@ -889,7 +891,7 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
       for (int r = tid; r <= a.requests; r += NT) cls.shares[r] = min(prefix[r], listed);
       for (int i = tid; i <= listed; i += NT) cls.shares[a.requests + 1 + i] = costs[i];
     }
-    const int64_t all = uniform(costs[listed]) * heads, share = share_of(cls, all);
+    const int64_t all = uniform(costs[listed]) * heads, share = share_of<TREE>(cls, all);
     begin = owner * share, end = min(begin + share, all);
   }
   // A thread's places in a tile (byte, half of the octet, dword column and
@@ -1112,6 +1114,26 @@ __global__ void __launch_bounds__(64 * tile_waves(D), tile_groups(D) * tile_wave
       int after[TT];
 #pragma unroll
       for (int u = 0; u < TT; ++u) after[u] = page_of(t + 3 * TT + u);
+      if (TREE && row0 + 32 * rows32 > row1) {
+        // A wave without rows only unpacks (24 requests of 1..40 tokens and 4 heads to
+        // a kv head, in blocks of 256 rows: 196 us, so 184).
+        if (partial(t + TT, missing(1))) clean(then, count + 1);
+        unpack(then, 0);
+        if constexpr (TT == 2) {
+          fetch(t + 3, page[3]);
+          if (partial(t + TT, missing(1))) clean(then, count + 1);
+          unpack(then, 1);
+          fetch(t + 4, page[4]);
+        } else {
+          fetch(t + 2, page[2]);
+        }
+        if constexpr (HALVES == 2) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 3 * TT; ++i) page[i] = i < 2 * TT ? page[i + TT] : after[i - 2 * TT];
+        ++count;
+        __syncthreads();
+        continue;
+      }
       // The next step's tiles are unpacked after this one's scores are
       // multiplied; of two, whose codes come one by one, the first before.
       const bool dirty = partial(t + TT, missing(1));
@@ -1360,7 +1382,7 @@ __global__ void __launch_bounds__(SPREAD > 1 ? 64 * SPREAD : THREADS) attend_joi
             seg0 = cls.shares[r] + ((int64_t)head * blocks_of(a, cls, req) + block) * (req.tiles + SEGMENT_COST) + SEGMENT_COST;
             seg1 = seg0 + req.tiles;
           }
-          const int64_t share = share_of(cls, all);
+          const int64_t share = share_of<TREE>(cls, all);
           w0 = quotient(seg0, share);
           w1 = seg1 > seg0 ? quotient(seg1 - 1, share) : w0 - 1;
         }
@@ -1457,10 +1479,19 @@ constexpr int MAX_WORDS = 16;                            // of a row's mask, 64 
 // the caches (16 rows 101 us, in a variant of 16 with spills 151; blocks of 8 and
 // blocks that share the unpacking: 32 rows 168 and 258, one request 196 and 249;
 // 48 rows 266 and 260, one request 276 and 253).
+//
+// Trees of several requests differ in size, and a block of 256 rows that has a few
+// takes as long as a full one, so they go in waves of 32 rows somewhat longer; one
+// request, whose waves would have few tiles each, shorter. In us, as above:
+//                            1..40 tokens of 4 heads (160 rows)  40 each   one request of 20 (of 32)
+//   128 dims, 24 requests        157  184                        280  266   39  33 (41  38)
+//             100                376  696
+//   64 dims,  24 (24 each)        79   92  (96 rows)              78   92   32  32
 enum Variant { ROWS8, ROWS16, ROWS32, TILES };
-Variant variant_of(int64_t rows, int head_dim) {
+Variant variant_of(int64_t rows, int head_dim, int requests, bool trees) {
   if (head_dim == 256) return rows <= 32 ? ROWS8 : TILES;
-  const int64_t most = head_dim == 128 ? 128 : 64;
+  int64_t most = head_dim == 128 ? 128 : 64;
+  if (trees) most = requests == 1 ? 64 : head_dim == 128 ? 160 : 96;
   return rows <= 8 ? ROWS8 : rows <= 16 ? ROWS16 : rows <= most ? ROWS32 : TILES;
 }
 int rows_of(Variant v, int head_dim) { return v == TILES ? tile_rows(head_dim) : 8 << v; }
@@ -1501,8 +1532,8 @@ struct Launches {
   int count, few;
   Variant of[2];
 };
-Launches launches_of(int64_t tokens, int group, int requests, int head_dim, int64_t max_new) {
-  const Variant v = variant_of(std::min(max_new, tokens) * group, head_dim);
+Launches launches_of(int64_t tokens, int group, int requests, int head_dim, int64_t max_new, bool trees) {
+  const Variant v = variant_of(std::min(max_new, tokens) * group, head_dim, requests, trees);
   return {v == ROWS8 || (v == ROWS16 && requests == 1) ? 1 : 2, head_dim == 256 ? 32 : v == ROWS16 ? 8 : 16, {v, ROWS8}};
 }
 
@@ -1526,7 +1557,7 @@ int launch_variant(Variant v, const AttendArgs& args, int index, unsigned grid, 
 
 template <int D, bool BF16, bool TREE>
 int launch_attend(AttendArgs args, int64_t max_new, char* workspace, hipStream_t stream) {
-  const Launches launches = launches_of(args.tokens, args.group, args.requests, D, max_new);
+  const Launches launches = launches_of(args.tokens, args.group, args.requests, D, max_new, TREE);
   args.classes = launches.count;
   for (int i = 0; i < args.classes; ++i) {
     Class& c = args.of[i];
@@ -1571,15 +1602,20 @@ int64_t exl3_cache_attention_workspace(int64_t tokens, int q_heads, int kv_heads
       tokens < 0 || kv_heads < 1 || q_heads < kv_heads || max_new < 0)
     return -1;
   const int group = q_heads / kv_heads;
-  const Launches launches = launches_of(tokens, group, requests, head_dim, max_new);
-  int64_t bytes = 0;
-  for (int i = 0; i < launches.count; ++i) {
-    const Variant v = launches.of[i];
-    bytes += shares_bytes(v, requests, head_dim);
-    if (!whole_of(v, head_dim, segments_of(v, head_dim, tokens, group, requests, kv_heads)))
-      bytes += partials_bytes(v, head_dim);
+  // Enough for trees and for sequences.
+  int64_t most = 0;
+  for (const bool trees : {false, true}) {
+    const Launches launches = launches_of(tokens, group, requests, head_dim, max_new, trees);
+    int64_t bytes = 0;
+    for (int i = 0; i < launches.count; ++i) {
+      const Variant v = launches.of[i];
+      bytes += shares_bytes(v, requests, head_dim);
+      if (!whole_of(v, head_dim, segments_of(v, head_dim, tokens, group, requests, kv_heads)))
+        bytes += partials_bytes(v, head_dim);
+    }
+    most = std::max(most, bytes);
   }
-  return bytes;
+  return most;
 }
 
 int exl3_cache_attention_trees(const void* q, int64_t q_token, int64_t q_head, void* out,
