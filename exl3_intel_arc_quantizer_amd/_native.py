@@ -1381,6 +1381,11 @@ def linear(x, trellis, su, sv, K: int, cb: int):
     if shape[-1] != k:
         raise ValueError(f"x must have {k} input channels, got {tuple(shape)}")
     scales = (torch.float16, torch.float32)
+    # As columns and rows too, as quantisation returns them.
+    if isinstance(su, torch.Tensor) and su.dim() == 2:
+        su = su.flatten()
+    if isinstance(sv, torch.Tensor) and sv.dim() == 2:
+        sv = sv.flatten()
     _vector(su, "suh", scales, k, device)
     _vector(sv, "svh", scales, n, device)
     # The kernel reads 16 bytes at a time; rows that start elsewhere are copied.

@@ -64,7 +64,9 @@ def build_native(force: bool = True, verbose: bool = False) -> Path:
     if not force and not needs_rebuild():
         return LIB_PATH
     tmp = LIB_PATH.with_suffix(".so.tmp")
-    cmd = [hipcc_path(), *HIPCC_FLAGS, "-o", str(tmp), *map(str, SOURCES)]
+    # Sources side by side: two minutes one after the other, one like this.
+    jobs = f"-parallel-jobs={min(8, os.cpu_count() or 1)}"
+    cmd = [hipcc_path(), *HIPCC_FLAGS, jobs, "-o", str(tmp), *map(str, SOURCES)]
     t0 = time.perf_counter()
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:

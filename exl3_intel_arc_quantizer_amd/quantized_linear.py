@@ -18,7 +18,8 @@ def quantized_linear(x: torch.Tensor, trellis: torch.Tensor, suh: torch.Tensor, 
                      K: int, cb: int = CB_MUL1) -> torch.Tensor:
     """``x @ W`` (..., out) in x's type, for x (..., in) in float16 or bfloat16
     and W the (in, out) weight of a stored projection: ``trellis`` int16 (in /
-    16, out / 16, 16 K), ``suh`` (in,) and ``svh`` (out,) in float16 or float32,
+    16, out / 16, 16 K), ``suh`` (in,) and ``svh`` (out,) in float16 or float32
+    (or as a column and a row of them, as ``quantize_linear_module`` returns them),
     ``cb`` its codebook; all on x's device.
 
     The rows are scaled and transformed in float32 and count with 22 bits, or,

@@ -145,6 +145,7 @@ def test_shapes_strides_and_scale_types(rows):
     assert torch.equal(want[0], quantized_linear(x[0], words, su, sv, 4)) or rows > 1
     assert torch.equal(want, quantized_linear(x, words, su.float(), sv.float(), 4))
     assert torch.equal(want, quantized_linear(x, words, su.float(), sv, 4))
+    assert torch.equal(want, quantized_linear(x, words, su[:, None], sv[None], 4))
     same = quantized_linear(x[:1].expand(rows, 256), words, su, sv, 4)
     assert torch.equal(same, same[:1].expand(rows, 256))
     assert quantized_linear(x[:0], words, su, sv, 4).shape == (0, 256)

@@ -508,3 +508,39 @@ def test_refusals():
                   torch.zeros(3, 2, dtype=torch.int64, device="cuda")[:, :1], torch.zeros(3, 1, dtype=torch.int32, device="cuda")):
         with pytest.raises(RuntimeError, match="trees"):
             cache_attention(q, pages, tables, starts, lengths, trees=trees)
+
+
+@pytest.mark.gpu
+def test_example_decodes_drafted_trees():
+    """A step keeps one to three of a tree's five tokens."""
+    import importlib.util
+    from .conftest import REPO_ROOT
+    spec = importlib.util.spec_from_file_location("serve_drafts", REPO_ROOT / "examples" / "serve_drafts.py")
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    answers, steps = example.serve(tokens=10)
+    assert len(answers) == 3 and min(map(len, answers)) >= 10
+    for answer in answers:
+        assert steps < len(answer) <= 3 * steps + 1
+        assert all(0 <= token < example.VOCABULARY for token in answer)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim, most, requests", [(64, 25, 9), (64, 40, 5), (128, 40, 7), (128, 45, 9), (128, 17, 1), (256, 12, 6), (256, 70, 2)])
+def test_ragged_batches(dim, most, requests, dtype):
+    """Requests of one token to `most`, four heads to a kv head: waves of 32 rows,
+    blocks of which some waves have no rows, and those of few rows beside them; at
+    last with a NaN in the first request's newest values."""
+    rng = np.random.default_rng(dim + most)
+    new = [most, *rng.integers(1, most + 1, requests - 1).tolist()]
+    lengths = [int(n + rng.integers(0, 400)) for n in new]
+    parents = _forest(new, rng)
+    cache = ref.Cache(sum(-(-n // 64) for n in lengths) + 1, 64, 2, dim, rng)
+    tables = _tables(lengths, 64, 8, cache.shape[0], rng)
+    q = torch.from_numpy(rng.normal(size=(sum(new), 8, dim)) * 2).to(dtype)
+    _check(q, cache, 64, tables, new, lengths, _paths(new, parents), 2, dtype, max_new=most, group=4)
+    _check(q, cache, 64, tables, new, lengths, _paths(new, parents), 2, dtype, window=100, group=4)
+    cache.scales[1][tables[0][(lengths[0] - 1) // 64] * 64 + (lengths[0] - 1) % 64, 1, 0] = np.nan
+    got = _check(q, cache, 64, tables, new, lengths, _paths(new, parents), 2, dtype, max_new=most, group=4)
+    assert torch.isnan(got).any()
