@@ -103,6 +103,7 @@ _SIGNATURES = {
     "exl3_cache_read": (_c_int, [_c_vp, _c_i64, _c_int, _c_int, _c_int, _c_vp, _c_i64, _c_int,
                                  _c_vp, _c_vp, _c_vp]),
     "exl3_cache_attention_workspace": (_c_i64, [_c_i64, _c_int, _c_int, _c_int, _c_int, _c_i64]),
+    "exl3_cache_attention_trees_workspace": (_c_i64, [_c_i64, _c_int, _c_int, _c_int, _c_int, _c_i64]),
     "exl3_cache_attention": (_c_int, [_c_vp, _c_i64, _c_i64, _c_vp, _c_i64, _c_int, _c_int, _c_vp,
                                       _c_i64, _c_int, _c_int, _c_int, _c_vp, _c_int, _c_vp, _c_vp,
                                       _c_int, _c_float, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp]),
@@ -1262,7 +1263,8 @@ def cache_attention(q, pages, tables, starts, lengths, scale, window, max_new, t
     # Python's integers end nowhere, the C arguments at 64 bits.
     most = tokens if max_new is None else min(int(max_new), tokens)
     window = 2 ** 31 - 1 if window is None else min(int(window), 2 ** 31 - 1)
-    size = lib.exl3_cache_attention_workspace(tokens, q_heads, heads, dim, requests, most)
+    asked = lib.exl3_cache_attention_workspace if masks is None else lib.exl3_cache_attention_trees_workspace
+    size = asked(tokens, q_heads, heads, dim, requests, most)
     workspace = pages.new_empty(max(size, 0))
     _run(dev, "cache_attention", lib.exl3_cache_attention_trees, q.data_ptr(), sq[0], sq[1],
          out.data_ptr(), tokens, q_heads, _types()[q.dtype], pages.data_ptr(), n, page_size, heads,

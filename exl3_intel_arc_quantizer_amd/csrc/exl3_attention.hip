@@ -1592,30 +1592,34 @@ int launch_attend(AttendArgs args, int64_t max_new, char* workspace, hipStream_t
   return check_launch("exl3_cache_attention");
 }
 
+int64_t workspace_of(int64_t tokens, int q_heads, int kv_heads, int head_dim, int requests, int64_t max_new, bool trees) {
+  if (requests < 1 || requests > CACHE_MAX_REQUESTS || (head_dim != 64 && head_dim != 128 && head_dim != 256) ||
+      tokens < 0 || kv_heads < 1 || q_heads < kv_heads || max_new < 0)
+    return -1;
+  const int group = q_heads / kv_heads;
+  const Launches launches = launches_of(tokens, group, requests, head_dim, max_new, trees);
+  int64_t bytes = 0;
+  for (int i = 0; i < launches.count; ++i) {
+    const Variant v = launches.of[i];
+    bytes += shares_bytes(v, requests, head_dim);
+    if (!whole_of(v, head_dim, segments_of(v, head_dim, tokens, group, requests, kv_heads)))
+      bytes += partials_bytes(v, head_dim);
+  }
+  return bytes;
+}
+
 }  // namespace
 
 extern "C" {
 
 int64_t exl3_cache_attention_workspace(int64_t tokens, int q_heads, int kv_heads, int head_dim,
                                        int requests, int64_t max_new) {
-  if (requests < 1 || requests > CACHE_MAX_REQUESTS || (head_dim != 64 && head_dim != 128 && head_dim != 256) ||
-      tokens < 0 || kv_heads < 1 || q_heads < kv_heads || max_new < 0)
-    return -1;
-  const int group = q_heads / kv_heads;
-  // Enough for trees and for sequences.
-  int64_t most = 0;
-  for (const bool trees : {false, true}) {
-    const Launches launches = launches_of(tokens, group, requests, head_dim, max_new, trees);
-    int64_t bytes = 0;
-    for (int i = 0; i < launches.count; ++i) {
-      const Variant v = launches.of[i];
-      bytes += shares_bytes(v, requests, head_dim);
-      if (!whole_of(v, head_dim, segments_of(v, head_dim, tokens, group, requests, kv_heads)))
-        bytes += partials_bytes(v, head_dim);
-    }
-    most = std::max(most, bytes);
-  }
-  return most;
+  return workspace_of(tokens, q_heads, kv_heads, head_dim, requests, max_new, false);
+}
+
+int64_t exl3_cache_attention_trees_workspace(int64_t tokens, int q_heads, int kv_heads, int head_dim,
+                                             int requests, int64_t max_new) {
+  return workspace_of(tokens, q_heads, kv_heads, head_dim, requests, max_new, true);
 }
 
 int exl3_cache_attention_trees(const void* q, int64_t q_token, int64_t q_head, void* out,
@@ -1648,7 +1652,7 @@ int exl3_cache_attention_trees(const void* q, int64_t q_token, int64_t q_head, v
   if (masks && (words < 1 || words > MAX_WORDS))
     return set_error("exl3_cache_attention: masks must have 1 to %d words, got %d", MAX_WORDS, words);
   if (max_new < 0) return set_error("exl3_cache_attention: max_new %lld is negative", (long long)max_new);
-  if (workspace_bytes < exl3_cache_attention_workspace(tokens, q_heads, kv_heads, head_dim, requests, max_new))
+  if (workspace_bytes < workspace_of(tokens, q_heads, kv_heads, head_dim, requests, max_new, masks != nullptr))
     return set_error("exl3_cache_attention: workspace of %lld bytes is too small", (long long)workspace_bytes);
   if (!tokens) return 0;
   AttendArgs a{};

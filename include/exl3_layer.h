@@ -341,8 +341,10 @@ int exl3_cache_attention(const void* q, int64_t q_token, int64_t q_head, void* o
  * the last n of its lengths[r] positions, row i attends the positions before them
  * and new token j where bit j of its mask is set, of this sequence the last
  * `window` places; a mask may leave a row empty, which is 0 then. Requests with
- * more new tokens attend as in exl3_cache_attention. The same workspace. masks
- * NULL: exl3_cache_attention. */
+ * more new tokens attend as in exl3_cache_attention. masks NULL:
+ * exl3_cache_attention, with its workspace. */
+int64_t exl3_cache_attention_trees_workspace(int64_t tokens, int q_heads, int kv_heads, int head_dim,
+                                             int requests, int64_t max_new);
 int exl3_cache_attention_trees(const void* q, int64_t q_token, int64_t q_head, void* out,
                                int64_t tokens, int q_heads, int type, const void* pages,
                                int64_t num_pages, int page_size, int kv_heads, int head_dim,

@@ -544,3 +544,32 @@ def test_ragged_batches(dim, most, requests, dtype):
     cache.scales[1][tables[0][(lengths[0] - 1) // 64] * 64 + (lengths[0] - 1) % 64, 1, 0] = np.nan
     got = _check(q, cache, 64, tables, new, lengths, _paths(new, parents), 2, dtype, max_new=most, group=4)
     assert torch.isnan(got).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim, requests, new, hint, heads", [
+    (128, 1, 3, 3, 8), (128, 1, 30, 30, 8), (64, 70, 20, 24, 4), (128, 40, 25, 40, 16), (256, 5, 60, 64, 2), (64, 1, 900, 900, 16)])
+def test_calls_stay_within_their_workspace(dim, requests, new, hint, heads):
+    """Bytes past the asked size keep what they hold, and less is refused."""
+    lib = _native.load_library()
+    tokens, context, group, words = requests * new, new + 700, 4, -(-hint // 64)
+    width = -(-context // 64)
+    pages = torch.zeros(requests * width, heads, 2, 36 * dim, dtype=torch.uint8, device="cuda")
+    tables = torch.arange(requests * width, dtype=torch.int32, device="cuda").view(requests, width)
+    starts = torch.arange(requests + 1, dtype=torch.int32, device="cuda") * new
+    lengths = torch.full((requests,), context, dtype=torch.int32, device="cuda")
+    masks = torch.full((tokens, words), -1, dtype=torch.int64, device="cuda")
+    q = torch.randn(tokens, group * heads, dim, device="cuda").half()
+    size = lib.exl3_cache_attention_trees_workspace(tokens, group * heads, heads, dim, requests, hint)
+    held = torch.full((size + (1 << 20),), 173, dtype=torch.uint8, device="cuda")
+    out = torch.full_like(q, 3.0)
+
+    def call(bytes_):
+        return lib.exl3_cache_attention_trees(
+            q.data_ptr(), q.stride(0), dim, out.data_ptr(), tokens, group * heads, 1, pages.data_ptr(), pages.shape[0], 64, heads,
+            dim, tables.data_ptr(), width, starts.data_ptr(), lengths.data_ptr(), requests, masks.data_ptr(), words, 1.0,
+            2 ** 31 - 1, hint, held.data_ptr(), bytes_, torch.cuda.current_stream().cuda_stream)
+
+    assert call(size) == 0 and (held[size:] == 173).all()
+    assert not out.any()  # a cache of zeros
+    assert call(size - 1) != 0
