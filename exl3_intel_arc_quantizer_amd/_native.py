@@ -182,9 +182,17 @@ def _check(status: int, what: str) -> None:
 
 # ------------------------------------------------------------- validation
 
+_TORCH = None
+
+
 def _torch():
-    import torch
-    return torch
+    """torch, imported on first use and then held: a small call's checks ask for it
+    up to ten times, and the import statement alone takes 0.1 us."""
+    global _TORCH
+    if _TORCH is None:
+        import torch
+        _TORCH = torch
+    return _TORCH
 
 
 def _check_device_tensor(t, name: str, dtype, ndim: int) -> int:
@@ -965,8 +973,8 @@ def _rows(t, name: str, like=None, heads=None, dim=None) -> tuple:
 
 def _vector(t, name: str, dtypes: tuple, numel, device) -> None:
     torch = _torch()
-    if (not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.dim() != 1
-            or (numel is not None and t.numel() != numel) or not t.is_contiguous()
+    if (not isinstance(t, torch.Tensor) or t.dtype not in dtypes
+            or (t.dim() != 1 if numel is None else t.shape != (numel,)) or not t.is_contiguous()
             or t.device != device):
         raise RuntimeError(f"{name} must be a contiguous vector of "
                            f"{'any length' if numel is None else numel}, "
@@ -1283,7 +1291,8 @@ def _ranges(starts, lengths=None) -> int:
     torch = _torch()
     if not isinstance(starts, torch.Tensor) or not starts.is_cuda or starts.dim() != 1:
         raise RuntimeError("starts must be a 1-D GPU (cuda) tensor")
-    _vector(starts, "starts", (torch.int32,), None, starts.device)
+    if starts.dtype != torch.int32 or not starts.is_contiguous():
+        raise RuntimeError(f"starts must be a contiguous int32 vector, got {starts.dtype}")
     requests = starts.numel() - 1
     if lengths is not None:
         _vector(lengths, "lengths", (torch.int32,), requests, starts.device)
@@ -1328,7 +1337,8 @@ def cache_keep(pages, slots, starts, places) -> None:
     n, page_size, heads, dim = _pages(pages)
     device = pages.device
     requests = _ranges(starts)
-    _vector(starts, "starts", (torch.int32,), None, device)
+    if starts.device != device:
+        raise RuntimeError("starts must be on the cache's device")
     _vector(slots, "slots", (torch.int64,), None, device)
     _vector(places, "places", (torch.int32,), slots.numel(), device)
     _run(device, "keep_tokens", load_library().exl3_cache_keep, pages.data_ptr(), n, page_size, heads,
