@@ -469,7 +469,9 @@ __global__ void __launch_bounds__(512) linear_rows_kernel(LinearArgs a) {
 // memory for all waves; each wave decodes its own columns, one step ahead of the
 // products, and its words come through shared memory as above. 64 rows of 4096 by
 // 4096, 22 us: 5 to turn the rows, 12 here, 4 to join 16 shares (four waves of twice
-// the columns and 32 shares, which two waves a SIMD hide less of: 30).
+// the columns and 32 shares, which two waves a SIMD hide less of: 30). Latency and the
+// vector instructions of decoding bound it: 20 rows of 12288 by 4096 take 28 us, 64
+// 35.
 //
 // In step s rows s + DEPTH + 1 and words s + DEPTH + 2 are sent for, in as many
 // instructions each step (past the end the last ones again, which nobody uses), so
@@ -579,11 +581,6 @@ __global__ void __launch_bounds__(512, 2) linear_blocks_kernel(LinearArgs a) {
         next[c][of & 3] = of & 1 ? half_of<WIDE, CB, 1>(words.w[c][t], late, early, K)
                                  : half_of<WIDE, CB, 0>(words.w[c][t], late, early, K);
       }
-#pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
-      }
     }
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -602,20 +599,25 @@ __global__ void __launch_bounds__(512, 2) linear_blocks_kernel(LinearArgs a) {
     }
 }
 
-// Many rows: eight waves take 256 rows (128 of two parts) and 256 columns, so two
-// waves share 64 columns, each with half of the rows. Each decodes half of the
+// Many rows: eight waves take 32 SETS rows (half as many of two parts; 256, 224 or 192
+// of the parts, whichever wastes least) and 256 columns, so two waves share 64 columns, each with half of the rows. Each decodes half of the
 // columns' operands, in a step for the next one, and hands them to the other
 // through shared memory: vector instructions, four cycles each (and eight of a
 // matrix one's sixteen) on a SIMD that two waves share, are then as long as the
 // matrix ones. Products begin with a wave's own operands, and rows are read for the
 // next step as this one's are used up, so nothing is waited for after the barrier.
-template <int K, int CB, bool BF16, int PARTS>
+// 4096 rows of 4096 by 4096 (one round of the chip): 130 us here and 32 to turn the
+// rows, 0.85 PFLOP/s in all; the products alone would take 0.8 us of a step's 1.0, so
+// the power that matrix instructions draw bounds it (a library product of 8192 a side
+// reaches 1.21). 2055 rows of 4096 by 12288: 242 us and 18.
+template <int K, int CB, bool BF16, int PARTS, int SETS>
 __global__ void __launch_bounds__(512, 2) linear_wide_kernel(LinearArgs a) {
-  constexpr int MT = 8 / PARTS, SETS = 8, DEPTH = 2;     // of a wave
+  constexpr int MT = SETS / PARTS, DEPTH = 2;            // of a wave
   constexpr int ROWS = 2 * SETS * 64, ROW_SLOTS = DEPTH + 3;                 // vectors of a step's rows
   constexpr int SEGMENT = 2 * 32 * K, WORDS = 2 * SEGMENT, WORD_SLOTS = DEPTH + 2;  // bytes of a wave's words
+  constexpr int CHUNK = 8 * 4 * 64;                      // vectors of the eight waves' 16 output rows
   constexpr bool WIDE = K > 5;
-  __shared__ u32x4 rows_held[ROW_SLOTS * ROWS];
+  __shared__ u32x4 rows_held[ROW_SLOTS * ROWS > 2 * CHUNK ? ROW_SLOTS * ROWS : 2 * CHUNK];
   __shared__ u32x4 words_held[8 * WORD_SLOTS * WORDS / 16];
   __shared__ u32x4 operands[2][4][4][64];                // [step & 1][column group][column tile]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -639,13 +641,16 @@ __global__ void __launch_bounds__(512, 2) linear_wide_kernel(LinearArgs a) {
   int sent = 0;
   const uint32_t rows0 = shared_byte(rows_held + wave * 64), words0 = shared_byte(own_words);
   uint32_t rows_to = rows0, words_to = words0;
-  static_assert(ROWS == 2 * 512, "a step's rows are two of each thread");
+  // A step's rows are two of each thread, or of the second some waves have none and
+  // send for their words twice, so that all count alike.
+  static_assert(ROWS > 512 && ROWS <= 2 * 512 && 2 * SETS >= 12, "two of a thread; decoding takes eleven places of a step");
   auto send = [&](int part) __attribute__((always_inline)) {
-    if (part < 2) {
+    if (part == 0 || (part == 1 && wave < 2 * SETS - 8)) {
       to_shared(next_rows + part * 8192, 16 * tid, rows_to + part * 8192);
       return;
     }
     if (16 * lane < WORDS) to_shared(next_words, word_at, words_to);
+    if (part == 1) return;
     const bool on = ++sent < steps;
     next_rows += on ? 16 * ROWS : 0, next_words += on ? 2 * row_bytes : 0;
     rows_to = rows_to == rows0 + (ROW_SLOTS - 1) * (16 * ROWS) ? rows0 : rows_to + 16 * ROWS;
@@ -718,11 +723,6 @@ __global__ void __launch_bounds__(512, 2) linear_wide_kernel(LinearArgs a) {
         next[c][of & 3] = of & 1 ? half_of<WIDE, CB, 1>(words.w[c][t], late, early, K) : half_of<WIDE, CB, 0>(words.w[c][t], late, early, K);
       }
       if (s == 7 || s == 11) operands[parity ^ 1][quarter][2 * side + s / 8][lane] = next[s / 8];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
-      }
     }
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -747,9 +747,7 @@ __global__ void __launch_bounds__(512, 2) linear_wide_kernel(LinearArgs a) {
   // The output's transform: a lane holds channels 4 (lane / 16) .. + 3 of its tiles,
   // so two levels lie in its registers, two across lanes, two across the four tiles,
   // and one across the waves of 64 columns beside each other.
-  constexpr int CHUNK = 8 * 4 * 64;                      // vectors of the eight waves' 16 rows
-  f32x4* exchange = reinterpret_cast<f32x4*>(rows_held);
-  static_assert(ROW_SLOTS * ROWS >= 2 * CHUNK, "two chunks in the rows' memory");
+  f32x4* exchange = reinterpret_cast<f32x4*>(rows_held);  // two chunks of it
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
 #pragma unroll
@@ -868,23 +866,35 @@ Plan plan_of(int64_t rows, int64_t k, int64_t n, bool bf16) {
   while (p.variant < BLOCK_WIDE && rows > BLOCK_ROWS[p.variant]) p.variant = (Variant)(p.variant + 1);
   if (p.variant == BLOCK128 && !bf16) p.variant = BLOCK_WIDE;
   p.parts = p.variant >= BLOCK128 && bf16 ? 1 : 2;
-  p.block_rows = p.variant == BLOCK_WIDE ? 256 / p.parts : BLOCK_ROWS[p.variant];
-  p.blocks = (int)((rows + p.block_rows - 1) / p.block_rows);
-  p.sets = p.variant == ROWS_FEW ? 0 : p.block_rows * p.parts / 16;
   // Shares of the input channels that fill the chip: a wave of linear_rows_kernel
   // takes at least one block of 128, a workgroup of linear_blocks_kernel too; one of
   // linear_wide_kernel at least 640 channels, as the shares' sums go through memory
   // (300 rows of 4096 by 4096: 8 shares 58 us, 6 52; 200 rows: 16 45 us, 6 39).
-  int64_t most, want = CUS;
-  if (p.variant <= ROWS16) {
-    p.groups = (int)(n / 32);
-    most = k / (8 * HAD), want = 4 * CUS;
+  const bool few = p.variant <= ROWS16;
+  p.groups = (int)(few ? n / 32 : (n + 255) / 256);
+  const int64_t most = std::max<int64_t>(1, few ? k / (8 * HAD) : p.variant == BLOCK_WIDE ? k / (5 * HAD) : k / HAD);
+  auto cut = [&](int64_t block_rows) {
+    p.block_rows = (int)block_rows, p.blocks = (int)((rows + block_rows - 1) / block_rows);
+    p.splits = (int)std::min(most, std::max<int64_t>(1, (few ? 4 : 1) * CUS / ((int64_t)p.groups * p.blocks)));
+  };
+  if (p.variant < BLOCK_WIDE) {
+    cut(BLOCK_ROWS[p.variant]);
   } else {
-    p.groups = (int)((n + 255) / 256);
-    most = p.variant == BLOCK_WIDE ? k / (5 * HAD) : k / HAD;
+    // Blocks of 8, 7 or 6 sets (of two parts, 8 or 6) by the time of the last
+    // workgroup: rounds of the chip, times a step, which takes as long as the products
+    // of its sets and about two more, over the shares. (2055 rows of 4096 by 12288:
+    // 8 sets 273 us, 7 262, 6 352; 300 rows of 4096 by 4096: 52, 44 of 6; 4096 rows:
+    // 170, 250 of 6.)
+    int64_t least = INT64_MAX, best = 8;
+    for (int64_t sets = 8; sets >= 6; sets -= p.parts) {
+      cut(32 * sets / p.parts);
+      const int64_t rounds = ((int64_t)p.groups * p.blocks * p.splits + CUS - 1) / CUS;
+      const int64_t cost = rounds * (sets + 2) * 1024 / p.splits;
+      if (cost < least) least = cost, best = sets;
+    }
+    cut(32 * best / p.parts);
   }
-  most = std::max<int64_t>(1, most);
-  p.splits = (int)std::min(most, std::max<int64_t>(1, want / ((int64_t)p.groups * p.blocks)));
+  p.sets = p.variant == ROWS_FEW ? 0 : p.block_rows * p.parts / 16;
   p.z_bytes = k / 32 * p.sets * 1024 * p.blocks;
   p.scale_bytes = p.variant == ROWS_FEW ? 0 : (4 * rows + 15) & ~(int64_t)15;
   const bool direct = p.variant == BLOCK_WIDE && p.splits == 1;
@@ -904,7 +914,18 @@ void launch_product(const Plan& p, const LinearArgs& a, hipStream_t stream) {
     case BLOCK48: linear_blocks_kernel<K, CB, 3, 2><<<all, 512, 0, stream>>>(a); break;
     case BLOCK64: linear_blocks_kernel<K, CB, 4, 2><<<all, 512, 0, stream>>>(a); break;
     case BLOCK128: linear_blocks_kernel<K, CB, 8, 1><<<all, 512, 0, stream>>>(a); break;
-    case BLOCK_WIDE: linear_wide_kernel<K, CB, BF16, BF16 ? 1 : 2><<<all, 512, 0, stream>>>(a); break;
+    case BLOCK_WIDE:
+      if constexpr (BF16) {
+        if (p.block_rows == 224) {
+          linear_wide_kernel<K, CB, true, 1, 7><<<all, 512, 0, stream>>>(a);
+          break;
+        }
+      }
+      if (p.block_rows * p.parts == 192)
+        linear_wide_kernel<K, CB, BF16, BF16 ? 1 : 2, 6><<<all, 512, 0, stream>>>(a);
+      else
+        linear_wide_kernel<K, CB, BF16, BF16 ? 1 : 2, 8><<<all, 512, 0, stream>>>(a);
+      break;
   }
 }
 template <int CB, bool BF16>

@@ -290,3 +290,11 @@ def test_a_row_that_is_not_finite_is_alone(rows, dtype):
 def test_more_sizes(rows, k, n):
     for dtype in (torch.float16, torch.bfloat16):
         _check(rows, k, n, 1 + rows % 8, rows % 3, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows, k, n, K", [(200, 128, 33024, 5), (200, 1920, 16384, 2), (170, 256, 512, 8), (450, 640, 256, 4), (250, 1280, 384, 3)])
+def test_blocks_of_many_rows(rows, k, n, K):
+    """Blocks of 256, 224 and 192 rows, in one share and in more."""
+    for dtype in (torch.bfloat16, torch.float16):
+        _check(rows, k, n, K, 2 - K % 3, dtype)
