@@ -120,11 +120,15 @@ __device__ __forceinline__ uint32_t top_of(const float (&v)[32]) {
 // |z| <= sqrt(128) max |x su|: 22 bits of a value, and places down to 2^-39 of
 // the row's largest one, so the products are as exact as float32 makes them.
 // A workgroup takes a row, a quad of lanes a block of 128: two levels across its
-// lanes, five within one. A row with an infinity or a NaN is all NaN.
+// lanes, five within one. A row with an infinity or a NaN is all NaN. Sixteen rows
+// share each 256 bytes of z, so the chip's dies, which get workgroups in turn, take
+// runs of rows: what they write meets in one cache (the whole product with 4096 rows
+// of 4096 by 4096: row by row over the dies 170 us, so 159).
 template <bool BF16>
 __global__ void __launch_bounds__(1024) linear_turn_kernel(TurnArgs a) {
   __shared__ uint32_t tops[16];
-  const int row = blockIdx.x, tid = threadIdx.x, q = tid & 3, units = a.k / HAD, step = blockDim.x / 4;
+  const int die = blockIdx.x & 7, all = gridDim.x, row = die * (all / 8) + min(die, all % 8) + (int)(blockIdx.x >> 3);
+  const int tid = threadIdx.x, q = tid & 3, units = a.k / HAD, step = blockDim.x / 4;
   const uint16_t* x = a.x + row * a.stride;
   float v[32];
   uint32_t top = 0;
@@ -606,10 +610,10 @@ __global__ void __launch_bounds__(512, 2) linear_blocks_kernel(LinearArgs a) {
 // matrix one's sixteen) on a SIMD that two waves share, are then as long as the
 // matrix ones. Products begin with a wave's own operands, and rows are read for the
 // next step as this one's are used up, so nothing is waited for after the barrier.
-// 4096 rows of 4096 by 4096 (one round of the chip): 130 us here and 32 to turn the
-// rows, 0.85 PFLOP/s in all; the products alone would take 0.8 us of a step's 1.0, so
+// 4096 rows of 4096 by 4096 (one round of the chip): 159 us with the rows' turning,
+// 0.86 PFLOP/s; the products alone would take 0.8 us of a step's 1.0, so
 // the power that matrix instructions draw bounds it (a library product of 8192 a side
-// reaches 1.21). 2055 rows of 4096 by 12288: 242 us and 18.
+// reaches 1.21). 2055 rows of 4096 by 12288, 480 workgroups: 258 us, 0.80 PFLOP/s.
 template <int K, int CB, bool BF16, int PARTS, int SETS>
 __global__ void __launch_bounds__(512, 2) linear_wide_kernel(LinearArgs a) {
   constexpr int MT = SETS / PARTS, DEPTH = 2;            // of a wave
@@ -883,8 +887,8 @@ Plan plan_of(int64_t rows, int64_t k, int64_t n, bool bf16) {
     // Blocks of 8, 7 or 6 sets (of two parts, 8 or 6) by the time of the last
     // workgroup: rounds of the chip, times a step, which takes as long as the products
     // of its sets and about two more, over the shares. (2055 rows of 4096 by 12288:
-    // 8 sets 273 us, 7 262, 6 352; 300 rows of 4096 by 4096: 52, 44 of 6; 4096 rows:
-    // 170, 250 of 6.)
+    // 8 sets 273 us, 7 262, 6 352; 300 rows of 4096 by 4096: 8 sets 52, 6 44; 4096 rows:
+    // 170 and 250.)
     int64_t least = INT64_MAX, best = 8;
     for (int64_t sets = 8; sets >= 6; sets -= p.parts) {
       cut(32 * sets / p.parts);
@@ -944,7 +948,7 @@ void launch_rate(const Plan& p, const LinearArgs& a, hipStream_t stream) {
 
 template <bool BF16>
 int launch_linear(const Plan& p, const TurnArgs& t, const LinearArgs& a, int cb, hipStream_t s) {
-  const int threads = t.k <= 8192 ? 256 : t.k <= 16384 ? 512 : 1024;
+  const int threads = t.k <= 4096 ? 128 : t.k <= 8192 ? 256 : t.k <= 16384 ? 512 : 1024;
   if (p.variant != ROWS_FEW) {
     linear_turn_kernel<BF16><<<(unsigned)a.rows, threads, 0, s>>>(t);
     if (check_launch("exl3_linear")) return 1;
