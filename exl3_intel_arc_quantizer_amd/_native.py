@@ -1402,16 +1402,13 @@ def linear(x, trellis, su, sv, K: int, cb: int):
     _vector(sv, "svh", scales, n, device)
     # The kernel reads 16 bytes at a time; rows that start elsewhere are copied.
     rows = x if x.dim() == 2 else x.reshape(-1, k)
-    stride = rows.stride()
-    if stride[1] != 1 or stride[0] % 8 or stride[0] < 0 or rows.data_ptr() % 16:
+    stride, at, words_at, su_at, sv_at = rows.stride(), rows.data_ptr(), trellis.data_ptr(), su.data_ptr(), sv.data_ptr()
+    if stride[1] != 1 or stride[0] % 8 or at % 16:
         rows = rows.clone(memory_format=torch.contiguous_format)
-        stride = rows.stride()
-    if trellis.data_ptr() % 16:
-        trellis = trellis.clone()
-    if su.data_ptr() % 16:
-        su = su.clone()
-    if sv.data_ptr() % 16:
-        sv = sv.clone()
+        stride, at = rows.stride(), rows.data_ptr()
+    if (words_at | su_at | sv_at) % 16:
+        trellis, su, sv = (t.clone() if t.data_ptr() % 16 else t for t in (trellis, su, sv))
+        words_at, su_at, sv_at = trellis.data_ptr(), su.data_ptr(), sv.data_ptr()
     count = rows.shape[0]
     lib = load_library()
     code = _types()[x.dtype]
@@ -1420,8 +1417,7 @@ def linear(x, trellis, su, sv, K: int, cb: int):
         raise RuntimeError(f"quantized_linear: {count} rows of {k} by {n} are too many")
     out = x.new_empty((*shape[:-1], n))
     workspace = trellis.new_empty(size // 2)
-    _run(device, "quantized_linear", lib.exl3_linear, rows.data_ptr(), stride[0], count,
-         code, trellis.data_ptr(), su.data_ptr(), sv.data_ptr(),
+    _run(device, "quantized_linear", lib.exl3_linear, at, stride[0], count, code, words_at, su_at, sv_at,
          (su.dtype == torch.float16) + 2 * (sv.dtype == torch.float16), k, n, K, cb,
          out.data_ptr(), workspace.data_ptr(), size)
     return out

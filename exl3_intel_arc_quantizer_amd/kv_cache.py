@@ -105,8 +105,9 @@ def plan_step(cached: torch.Tensor, new: torch.Tensor, tables: torch.Tensor,
 
 
 def _unrecorded(what: str, *tensors) -> None:
-    if any(t is not None and records(t) for t in tensors):
-        raise RuntimeError(f"{what} has no gradient: detach its inputs")
+    for t in tensors:
+        if t is not None and records(t):
+            raise RuntimeError(f"{what} has no gradient: detach its inputs")
 
 
 def append_tokens(pages: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, *,

@@ -29,6 +29,7 @@ def quantized_linear(x: torch.Tensor, trellis: torch.Tensor, suh: torch.Tensor, 
     of 16 bytes, and rows that lie otherwise, are copied first. The call enqueues
     work on the current stream of x's device and keeps nothing. It has no
     gradient: train through ``x @ decode_weight_from_storage(...)``."""
-    if any(isinstance(t, torch.Tensor) and records(t) for t in (x, suh, svh)):
-        raise RuntimeError("quantized_linear has no gradient: detach its inputs")
+    for t in (x, suh, svh):
+        if isinstance(t, torch.Tensor) and records(t):
+            raise RuntimeError("quantized_linear has no gradient: detach its inputs")
     return _native.linear(x, trellis, suh, svh, K, cb)
