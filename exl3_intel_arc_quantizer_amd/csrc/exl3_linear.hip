@@ -118,7 +118,10 @@ __device__ __forceinline__ uint32_t top_of(const float (&v)[32]) {
 
 // A row is held as 2^p (hi + lo), both float16, with p from the bound
 // |z| <= sqrt(128) max |x su|: 22 bits of a value, and places down to 2^-39 of
-// the row's largest one, so the products are as exact as float32 makes them.
+// the row's largest one, so the products are as exact as float32 makes them. More
+// than 64 bfloat16 rows are held as hi alone, 11 bits: their own values have 8, the
+// output is rounded to 8, and a second part doubles the matrix work (2055 rows of
+// 4096 by 12288 258 us so, 491 of two parts).
 // A workgroup takes a row, a quad of lanes a block of 128: two levels across its
 // lanes, five within one. A row with an infinity or a NaN is all NaN. Sixteen rows
 // share each 256 bytes of z, so the chip's dies, which get workgroups in turn, take
@@ -603,17 +606,18 @@ __global__ void __launch_bounds__(512, 2) linear_blocks_kernel(LinearArgs a) {
     }
 }
 
-// Many rows: eight waves take 32 SETS rows (half as many of two parts; 256, 224 or 192
-// of the parts, whichever wastes least) and 256 columns, so two waves share 64 columns, each with half of the rows. Each decodes half of the
-// columns' operands, in a step for the next one, and hands them to the other
-// through shared memory: vector instructions, four cycles each (and eight of a
-// matrix one's sixteen) on a SIMD that two waves share, are then as long as the
-// matrix ones. Products begin with a wave's own operands, and rows are read for the
-// next step as this one's are used up, so nothing is waited for after the barrier.
-// 4096 rows of 4096 by 4096 (one round of the chip): 159 us with the rows' turning,
-// 0.86 PFLOP/s; the products alone would take 0.8 us of a step's 1.0, so
-// the power that matrix instructions draw bounds it (a library product of 8192 a side
-// reaches 1.21). 2055 rows of 4096 by 12288, 480 workgroups: 258 us, 0.80 PFLOP/s.
+// Many rows: eight waves take 32 SETS rows (of two parts half as many) and 256 columns,
+// so two waves share 64 columns, each with half of the rows. Each decodes half of the
+// columns' operands, in a step for the next one, and hands them to the other through
+// shared memory: vector instructions, four cycles each (and eight of a matrix one's
+// sixteen) on a SIMD that two waves share, are then as long as the matrix ones.
+// Products begin with a wave's own operands, and rows are read for the next step as
+// this one's are used up, so nothing is waited for after the barrier.
+//
+// 4096 rows of 4096 by 4096, one round of the chip: 159 us with the rows' turning, 0.86
+// PFLOP/s (a library product of 8192 a side reaches 1.21). Of a step's 1.0 us, 0.8 are
+// left without decoding and reading: the rate of the matrix instructions bounds it, then
+// their overlap with vector ones. 2055 rows of 4096 by 12288, 480 workgroups: 258 us.
 template <int K, int CB, bool BF16, int PARTS, int SETS>
 __global__ void __launch_bounds__(512, 2) linear_wide_kernel(LinearArgs a) {
   constexpr int MT = SETS / PARTS, DEPTH = 2;            // of a wave
@@ -804,7 +808,8 @@ struct JoinArgs {
 };
 
 // A wave takes a block of 128 outputs of a row, eight a lane; its four rows of
-// lanes take shares in turn, as their loads wait for each other.
+// lanes take shares in turn, as their loads wait for each other (16 shares of 64 rows
+// of 4096: 4 us; sixteen lanes a block, shares one after another, 7.8).
 template <bool BF16>
 __global__ void __launch_bounds__(256) linear_join_kernel(JoinArgs a) {
   const int64_t unit = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
