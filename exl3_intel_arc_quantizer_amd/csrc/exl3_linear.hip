@@ -284,9 +284,15 @@ __device__ __forceinline__ u32x4 operand_of(const uint32_t (&w)[2][WIDE ? 4 : 2]
 // compiler would wait for all of these before it reads any shared memory; the waits
 // are the caller's (counts of vmcnt, which the compiler's own waits beside them only
 // make stricter).
+//
+// m0, which the text writes, is named as clobbered; the compiler warns that it would
+// not keep a reserved register's value across such a statement, which is meant.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void to_shared(const void* from, uint32_t lane_at, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(lane_at), "s"(from) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(lane_at), "s"(from) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 __device__ __forceinline__ uint32_t shared_byte(const void* p) {
   return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p);
 }
