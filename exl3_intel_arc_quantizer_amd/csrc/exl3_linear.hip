@@ -55,6 +55,17 @@ __device__ __forceinline__ uint32_t pair_of(float a, float b) {
   return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
 }
 
+// Two values as float16 parts and what these leave. That is taken from the parts as
+// they are stored: where a value is a product the compiler otherwise forms its part
+// again, rounded once (v_fma_mixlo_f16), while the stored one is that of the rounded
+// product. One value in 8192 lies where they differ, by a whole place of the part.
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t& parts, uint32_t& rest) {
+  parts = pair_of(a, b);
+  asm("" : "+v"(parts));
+  const f16x2 h = __builtin_bit_cast(f16x2, parts);
+  rest = pair_of(a - (float)h[0], b - (float)h[1]);
+}
+
 // Scales of a layer: float32, or float16 as they are stored.
 struct Scales {
   const void* data;
@@ -173,10 +184,9 @@ __global__ void __launch_bounds__(1024) linear_turn_kernel(TurnArgs a) {
       u32x4 hi, lo;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float y = v[8 * s + 2 * e], w = v[8 * s + 2 * e + 1];
-        const _Float16 hy = (_Float16)y, hw = (_Float16)w;
-        hi[e] = __builtin_bit_cast(uint32_t, f16x2{hy, hw});
-        lo[e] = pair_of(y - (float)hy, w - (float)hw);
+        uint32_t parts, rest;
+        split_pair(v[8 * s + 2 * e], v[8 * s + 2 * e + 1], parts, rest);
+        hi[e] = parts, lo[e] = rest;
       }
       u32x4* z = out + (int64_t)(4 * unit + s) * a.sets * 64;
       z[0] = hi;
@@ -420,9 +430,7 @@ __global__ void __launch_bounds__(512) linear_rows_kernel(LinearArgs a) {
         lane_butterfly<16>(x, y);
         lane_butterfly<32>(x, y);
         x *= ROOT, y *= ROOT;
-        const _Float16 hx = (_Float16)x, hy = (_Float16)y;
-        to[4 * r] = __builtin_bit_cast(uint32_t, f16x2{hx, hy});
-        to[4 * (r + 4)] = pair_of(x - (float)hx, y - (float)hy);
+        split_pair(x, y, to[4 * r], to[4 * (r + 4)]);
       }
     }
     // The block's words (and what was loaded before them).
