@@ -96,7 +96,7 @@ def serve(tokens: int = 24, lengths=(40, 3, 75), device: str = "cuda", seed: int
         plan = plan_step(cached, new, tables, free, taken, page_size=PAGE, max_tokens=len(tree))
         shape = plan_tree(parents, plan.starts, plan.lengths, max_new=drafted)
         after = model.choices(tree, plan, shape.positions, pages, tables, drafted, shape.masks)
-        kept = accept_drafts(tree, after, parents, plan.starts, plan.lengths)
+        kept = accept_drafts(tree, after, parents, plan.starts, plan.lengths, max_new=drafted)
         keep_tokens(pages, plan.slots, plan.starts, kept.places)
         taken = release_pages(plan.lengths, kept.lengths, tables, free, plan.taken, page_size=PAGE)
         cached, chosen, steps = kept.lengths, kept.next, steps + 1

@@ -114,6 +114,8 @@ _SIGNATURES = {
     "exl3_plan_tree": (_c_int, [_c_vp, _c_vp, _c_vp, _c_int, _c_i64, _c_int, _c_vp, _c_vp, _c_vp]),
     "exl3_accept_drafts": (_c_int, [_c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_int,
                                     _c_i64, _c_vp, _c_vp, _c_vp, _c_vp]),
+    "exl3_accept_trees": (_c_int, [_c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_int,
+                                   _c_i64, _c_int, _c_vp, _c_vp, _c_vp, _c_vp]),
     "exl3_cache_keep": (_c_int, [_c_vp, _c_i64, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_vp, _c_int,
                                  _c_i64, _c_vp]),
     "exl3_release_pages": (_c_int, [_c_vp, _c_vp, _c_int, _c_vp, _c_int, _c_int, _c_vp, _c_int,
@@ -1312,8 +1314,8 @@ def plan_tree(parents, starts, lengths, words: int) -> tuple:
     return masks, positions
 
 
-def accept_drafts(tokens, choices, parents, starts, lengths, certain) -> tuple:
-    """Places, lengths and next tokens (exl3_accept_drafts)."""
+def accept_drafts(tokens, choices, parents, starts, lengths, certain, words: int) -> tuple:
+    """Places, lengths and next tokens (exl3_accept_trees)."""
     torch = _torch()
     requests, device = _ranges(starts, lengths), starts.device
     _vector(parents, "parents", (torch.int32,), None, device)
@@ -1324,9 +1326,9 @@ def accept_drafts(tokens, choices, parents, starts, lengths, certain) -> tuple:
         _vector(certain, "certain", (torch.int32,), requests, device)
     places, kept = torch.empty_like(parents), torch.empty_like(lengths)
     following = lengths.new_empty(requests, dtype=tokens.dtype)
-    _run(device, "accept_drafts", load_library().exl3_accept_drafts, tokens.data_ptr(),
+    _run(device, "accept_drafts", load_library().exl3_accept_trees, tokens.data_ptr(),
          choices.data_ptr(), tokens.dtype == torch.int64, parents.data_ptr(), starts.data_ptr(),
-         lengths.data_ptr(), None if certain is None else certain.data_ptr(), requests, count,
+         lengths.data_ptr(), None if certain is None else certain.data_ptr(), requests, count, words,
          places.data_ptr(), kept.data_ptr(), following.data_ptr())
     return places, kept, following
 

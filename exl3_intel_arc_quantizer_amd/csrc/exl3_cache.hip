@@ -725,10 +725,12 @@ __global__ void __launch_bounds__(TREE_THREADS) tree_kernel(TreeArgs a, int word
 // from the last of them down, as long as there is one, the first child that is
 // the token chosen after its parent. A wave takes a request; of up to 64 tokens a
 // lane holds one each, and a step is a vote (512 requests of up to 48 tokens 3.6 us,
-// one of 13 1.9: a launch and two loads).
+// one of 13 1.9: a launch and two loads). Requests of more than `most` tokens are
+// runs, as they were to tree_kernel: a token's parent is the one before it.
 template <typename ID>
 struct AcceptArgs {
   TreeArgs tree;
+  int most;                        // 64 of them at least
   const ID *tokens, *choices;
   const int32_t* certain;
   int32_t *places, *lengths;
@@ -763,13 +765,15 @@ __global__ void __launch_bounds__(64) accept_kernel(AcceptArgs<ID> a) {
     if (there) places[lane] = place;
   } else {
     // Lane i % 64 writes the places of i: first these, then those found.
+    const bool run = d.n > a.most;
     for (int i = lane; i < d.n; i += 64) places[i] = i < certain ? i : -1;
     for (bool found = true; found;) {
       const ID chosen = choices[at];
+      const int end = run ? min(at + 2, d.n) : d.n;      // of those that may follow
       found = false;
-      for (int base = (at + 1) & ~63; base < d.n && !found; base += 64) {
+      for (int base = (at + 1) & ~63; base < end && !found; base += 64) {
         const int i = base + lane;
-        const bool fits = i < d.n && i >= certain && i > at && parents[i] == at && tokens[i] == chosen;
+        const bool fits = i < end && i >= certain && i > at && (run || parents[i] == at) && tokens[i] == chosen;
         const uint64_t all = __ballot(fits);
         if (!all) continue;
         found = true;
@@ -1098,19 +1102,28 @@ int exl3_plan_tree(const int32_t* parents, const int32_t* starts, const int32_t*
   return check_launch("exl3_plan_tree");
 }
 
-int exl3_accept_drafts(const void* tokens, const void* choices, int wide, const int32_t* parents,
-                       const int32_t* starts, const int32_t* lengths, const int32_t* certain, int requests,
-                       int64_t max_tokens, int32_t* places, int32_t* kept, void* next, void* stream) {
+int exl3_accept_trees(const void* tokens, const void* choices, int wide, const int32_t* parents,
+                      const int32_t* starts, const int32_t* lengths, const int32_t* certain, int requests,
+                      int64_t max_tokens, int words, int32_t* places, int32_t* kept, void* next, void* stream) {
   if (check_drafts("exl3_accept_drafts", requests, max_tokens)) return 1;
+  if (words < 1 || 64 * words > MAX_TREE)
+    return set_error("exl3_accept_drafts: words must be in 1..%d, got %d", MAX_TREE / 64, words);
   const TreeArgs tree{parents, starts, lengths, max_tokens, requests};
   auto launch = [&](auto id) {
     typedef decltype(id) ID;
-    const AcceptArgs<ID> a{tree, static_cast<const ID*>(tokens), static_cast<const ID*>(choices), certain, places, kept,
-                           static_cast<ID*>(next)};
+    const AcceptArgs<ID> a{tree, 64 * words, static_cast<const ID*>(tokens), static_cast<const ID*>(choices), certain, places,
+                           kept, static_cast<ID*>(next)};
     accept_kernel<ID><<<(unsigned)requests + 8, 64, 0, (hipStream_t)stream>>>(a);
     return check_launch("exl3_accept_drafts");
   };
   return wide ? launch((int64_t)0) : launch((int32_t)0);
+}
+
+int exl3_accept_drafts(const void* tokens, const void* choices, int wide, const int32_t* parents,
+                       const int32_t* starts, const int32_t* lengths, const int32_t* certain, int requests,
+                       int64_t max_tokens, int32_t* places, int32_t* kept, void* next, void* stream) {
+  return exl3_accept_trees(tokens, choices, wide, parents, starts, lengths, certain, requests, max_tokens, MAX_TREE / 64, places,
+                           kept, next, stream);
 }
 
 int exl3_release_pages(const int32_t* before, const int32_t* after, int requests, int32_t* tables, int width,

@@ -19,7 +19,7 @@ with no host synchronisation in it. Drafted tokens of a request may be a tree:
     q = append_tokens(..., positions=tree.positions, ...)
     out = cache_attention(..., trees=tree.masks)
     ...                                               # the model's choice after every token
-    kept = accept_drafts(tokens, choices, parents, plan.starts, plan.lengths)
+    kept = accept_drafts(tokens, choices, parents, plan.starts, plan.lengths, max_new=most)
     taken = release_pages(plan.lengths, kept.lengths, tables, free_pages, plan.taken,
                           page_size=64)
     keep_tokens(pages, plan.slots, plan.starts, kept.places)     # every layer
@@ -189,9 +189,14 @@ def plan_tree(parents: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor
     counts as -1. ``max_new`` (at most 1024) bounds the tokens of a tree: masks
     have ceil(max_new / 64) words, and a request of more tokens than they have bits
     is no tree but a run: its positions count up. Tokens of no request get 0."""
+    return TreePlan(*_native.plan_tree(parents, starts, lengths, _tree_words(max_new)))
+
+
+def _tree_words(max_new: int) -> int:
+    """Words of a mask for trees of up to ``max_new`` tokens."""
     if not 1 <= max_new <= 64 * _native.MAX_TREE_WORDS:
         raise ValueError(f"max_new must be in 1..{64 * _native.MAX_TREE_WORDS}, got {max_new}")
-    return TreePlan(*_native.plan_tree(parents, starts, lengths, -(-max_new // 64)))
+    return -(-max_new // 64)
 
 
 class Accepted(NamedTuple):
@@ -204,7 +209,8 @@ class Accepted(NamedTuple):
 
 def accept_drafts(tokens: torch.Tensor, choices: torch.Tensor, parents: torch.Tensor,
                   starts: torch.Tensor, lengths: torch.Tensor, *,
-                  certain: Optional[torch.Tensor] = None) -> Accepted:
+                  certain: Optional[torch.Tensor] = None,
+                  max_new: Optional[int] = None) -> Accepted:
     """The drafted tokens that the model would have chosen itself.
 
     ``tokens`` are the step's token ids and ``choices`` the model's choice after
@@ -213,8 +219,13 @@ def accept_drafts(tokens: torch.Tensor, choices: torch.Tensor, parents: torch.Te
     (int32, (requests,); at least, and if left out, the first: the one that the
     last step chose) are kept, then from the last of them down, as long as there is
     one, the first token after those whose parent is the last kept and which is the
-    choice after it. ``next`` is -1 for requests without new tokens."""
-    return Accepted(*_native.accept_drafts(tokens, choices, parents, starts, lengths, certain))
+    choice after it. ``next`` is -1 for requests without new tokens.
+
+    ``max_new`` is the bound that ``plan_tree`` was given (1024 if left out).
+    Requests of more tokens than its masks have bits attended as a run, whatever
+    their parents say, and are accepted as one: of each token the next one follows."""
+    words = _native.MAX_TREE_WORDS if max_new is None else _tree_words(max_new)
+    return Accepted(*_native.accept_drafts(tokens, choices, parents, starts, lengths, certain, words))
 
 
 def keep_tokens(pages: torch.Tensor, slots: torch.Tensor, starts: torch.Tensor,

@@ -365,14 +365,22 @@ int exl3_plan_tree(const int32_t* parents, const int32_t* starts, const int32_t*
                    int requests, int64_t max_tokens, int words, int64_t* masks, int32_t* positions,
                    void* stream);
 
-/* The drafted tokens that the model would have chosen itself. choices[t] is its
+/* The drafted tokens that the model would have chosen itself, of trees that
+ * exl3_plan_tree planned with masks of `words` words. choices[t] is its
  * choice after token t; both are int64 if `wide`, else int32. A request keeps its
  * first certain[r] tokens (at least its first; certain NULL: that one), and then
  * from the last of them down, as long as there is one, the first token past them
  * whose parent is the last kept and which is the choice after it. places[t] is a
  * token's place among those kept, -1 if it is not (or of no request); kept[r] the
  * request's tokens cached before plus those kept, next[r] the choice after the
- * last kept, -1 where there are no new tokens. */
+ * last kept, -1 where there are no new tokens. Of requests of more than 64 words
+ * tokens, which are no trees, a token's parent is the one before it. */
+int exl3_accept_trees(const void* tokens, const void* choices, int wide, const int32_t* parents,
+                      const int32_t* starts, const int32_t* lengths, const int32_t* certain,
+                      int requests, int64_t max_tokens, int words, int32_t* places, int32_t* kept,
+                      void* next, void* stream);
+
+/* exl3_accept_trees with the most words, 16. */
 int exl3_accept_drafts(const void* tokens, const void* choices, int wide, const int32_t* parents,
                        const int32_t* starts, const int32_t* lengths, const int32_t* certain,
                        int requests, int64_t max_tokens, int32_t* places, int32_t* kept, void* next,
