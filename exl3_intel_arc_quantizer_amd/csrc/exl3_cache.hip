@@ -795,8 +795,10 @@ __global__ void __launch_bounds__(64) accept_kernel(AcceptArgs<ID> a) {
 // pages from ceil(after / P) to ceil(before / P) of its row, in the order of the
 // requests and their rows, onto the stack of which `taken` is the top. One
 // workgroup: prefix sums over the requests, then the entries as one list, counted
-// and then written (entries without a page are not). Bound by latency (512
-// requests of a page or two each 5.6 us, one 2.3).
+// and then written (entries without a page are not). Pages that have no place on the
+// stack, of which fewer were taken than come back, stay where they are: nothing else
+// would know of them. Bound by latency (512 requests of a page or two each 5.6 us,
+// one 2.3).
 struct ReleaseArgs {
   const int32_t *before, *after, *taken;
   int32_t *tables, *free_pages, *taken_out;
@@ -843,9 +845,9 @@ __global__ void __launch_bounds__(STEP_THREADS) release_kernel(ReleaseArgs a) {
     }
     int64_t sum;
     const int64_t rank = done + block_sum(page >= 0, parts, &sum) - 1, to = top + rank;
-    if (page >= 0) {
+    if (page >= 0 && to >= 0 && to < a.free_count) {
       a.tables[entry] = -1;
-      if (to >= 0 && to < a.free_count) a.free_pages[to] = page;
+      a.free_pages[to] = page;
     }
     done += sum;
   }

@@ -244,5 +244,10 @@ def release_pages(before: torch.Tensor, after: torch.Tensor, tables: torch.Tenso
     ``after`` of them (int32, (requests,); 0 ends a request): their entries of
     ``tables`` become -1 and the pages, in order, the last of ``free_pages`` before
     entry ``taken``, both in place. Returns the new ``taken``; the step plans'
-    ``free_pages`` are thus a stack, from which the next ``plan_step`` takes."""
+    ``free_pages`` are thus a stack, from which the next ``plan_step`` takes.
+
+    Only as many pages as were taken from it have a place on the stack. Of more (pages
+    that a caller put into the tables from elsewhere) the first ones stay in their
+    rows, where the caller finds them: entries past the kept tokens that are not -1,
+    to be read before the next ``plan_step``, which writes over those it needs."""
     return _native.release_pages(before, after, tables, free_pages, taken, page_size)

@@ -397,7 +397,9 @@ int exl3_cache_keep(void* pages, int64_t num_pages, int page_size, int kv_heads,
 /* Gives back the pages of requests that held before[r] tokens and keep after[r]
  * of them (none: all its pages): entries ceil(after / page_size) to ceil(before /
  * page_size) of its row become -1, and their pages (where there are any) the last
- * of free_pages before *taken, in order; *taken_out = *taken less their number. */
+ * of free_pages before *taken, in order; *taken_out = *taken less their number, 0
+ * at least. Pages that have no place there, the first ones where more come back than
+ * were taken, stay in their rows. */
 int exl3_release_pages(const int32_t* before, const int32_t* after, int requests, int32_t* tables,
                        int width, int page_size, int32_t* free_pages, int free_count,
                        const int32_t* taken, int32_t* taken_out, void* stream);
