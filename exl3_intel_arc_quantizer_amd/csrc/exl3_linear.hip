@@ -883,6 +883,9 @@ struct Plan {
 
 constexpr int CUS = 256;
 
+// Threads of linear_turn_kernel, by its rows' blocks of 128, four each.
+int turn_threads(int64_t k) { return k <= 4096 ? 128 : k <= 8192 ? 256 : k <= 16384 ? 512 : 1024; }
+
 Plan plan_of(int64_t rows, int64_t k, int64_t n, bool bf16) {
   Plan p{};
   p.variant = ROWS_FEW;
@@ -967,9 +970,8 @@ void launch_rate(const Plan& p, const LinearArgs& a, hipStream_t stream) {
 
 template <bool BF16>
 int launch_linear(const Plan& p, const TurnArgs& t, const LinearArgs& a, int cb, hipStream_t s) {
-  const int threads = t.k <= 4096 ? 128 : t.k <= 8192 ? 256 : t.k <= 16384 ? 512 : 1024;
   if (p.variant != ROWS_FEW) {
-    linear_turn_kernel<BF16><<<(unsigned)a.rows, threads, 0, s>>>(t);
+    linear_turn_kernel<BF16><<<(unsigned)a.rows, turn_threads(t.k), 0, s>>>(t);
     if (check_launch("exl3_linear")) return 1;
   }
   cb == 0 ? launch_rate<0, BF16>(p, a, s) : cb == 1 ? launch_rate<1, BF16>(p, a, s) : launch_rate<2, BF16>(p, a, s);
@@ -988,6 +990,7 @@ extern "C" {
 
 int64_t exl3_linear_workspace(int64_t rows, int64_t k, int64_t n, int type) {
   if (rows < 0 || rows > 1 << 22 || k < HAD || n < HAD || k % HAD || n % HAD || k > 1 << 24 || n > 1 << 24) return -1;
+  if (rows * turn_threads(k) > UINT32_MAX) return -1;    // a launch has fewer than 2^32 threads
   if (!rows) return 0;
   const Plan p = plan_of(rows, k, n, type == 2);
   return p.z_bytes + p.scale_bytes + p.partial_bytes;
