@@ -1487,6 +1487,19 @@ constexpr int MAX_WORDS = 16;                            // of a row's mask, 64 
 //   128 dims, 24 requests        157  184                        280  266   39  33 (41  38)
 //             100                376  696
 //   64 dims,  24 (24 each)        79   92  (96 rows)              78   92   32  32
+// Over the bounds (waves of 32 rows, blocks; 4 heads; 24 requests of up to 8192
+// positions with equal trees and with trees of up to so many rows, and 100 such requests
+// of up to 4096; a graph's start of some 6 us in each):
+//   rows               64        96       128       160       192       256
+//   128 dims, equal   95 137   134 145   172 155   206 193   237 197   285 211
+//             ragged 103 138   108 135   123 153   159 202   172 189   191 189
+//             100    161 381   188 399   215 436   264 480   372 552   362 495
+//   64 dims,  equal   64  75    90  87   110  96   124 131   152 141   184 151
+//             ragged  76  90    78  90    88  94    92 104   115 115   126 123
+//             100    101 125   130 151   157 159   177 186   194 201   242 313
+// 2 and 8 heads alike. How even the trees are the host does not know: up to 160 rows of
+// 128 dims ragged ones gain more (a fifth) than equal ones lose (7 to 11 %), at 192 less
+// (9 and 20); of 64 dims ragged ones gain up to 160, equal ones lose from 128 on.
 enum Variant { ROWS8, ROWS16, ROWS32, TILES };
 Variant variant_of(int64_t rows, int head_dim, int requests, bool trees) {
   if (head_dim == 256) return rows <= 32 ? ROWS8 : TILES;

@@ -130,9 +130,12 @@ __device__ __forceinline__ uint32_t top_of(const float (&v)[32]) {
 // A row is held as 2^p (hi + lo), both float16, with p from the bound
 // |z| <= sqrt(128) max |x su|: 22 bits of a value, and places down to 2^-39 of
 // the row's largest one, so the products are as exact as float32 makes them. More
-// than 64 bfloat16 rows are held as hi alone, 11 bits: their own values have 8, the
-// output is rounded to 8, and a second part doubles the matrix work (2055 rows of
-// 4096 by 12288 258 us so, 491 of two parts).
+// than 64 bfloat16 rows are held as hi alone, 11 bits, for time: a second part doubles
+// the matrix work, which bounds them (2055 rows of 4096 by 12288 258 us so, 491 of two
+// parts; the products of 37 rows take half as long as their decoding). What is left
+// out is an eighth of the output's own rounding to 8 bits, of both signs like it:
+// errors grow by under one per cent. So the 65th row changes what the others of its
+// call count with. Float16 outputs, rounded to 11 bits, keep both parts.
 // A workgroup takes a row, a quad of lanes a block of 128: two levels across its
 // lanes, five within one. A row with an infinity or a NaN is all NaN. Sixteen rows
 // share each 256 bytes of z, so the chip's dies, which get workgroups in turn, take
@@ -330,8 +333,11 @@ __device__ __forceinline__ float row_butterfly(float v, int lane) {
 // channels; a workgroup's eight waves add up in shared memory. Words come through
 // shared memory, each wave's own, a block ahead (2 KB at 4 bits), as a lane's dwords
 // lie 16 bytes from its neighbour's, and the vector cache then takes four of them at a
-// time. One row of 4096 by 4096, 8.6 MB of words: 6.8 us and 3.2 to join; launches and
-// latency bound it (by 12288, 25 MB: 12.5 us, 2 TB/s).
+// time. One row of 4096 by 4096, 8.4 MB of words, takes 8.9 us in a graph, the join
+// with it (in a profiler's trace, each with its own start and end, 6.6 to 6.8 and 3.6):
+// launches and the first loads bound it, a wave having one block. Larger weights are
+// bound by the instructions of decoding, whatever their bits: 8192 by 28672 at 2, 4 and
+// 8 bits (59, 117 and 235 MB) 45, 47 and 51 us, 4096 by 131072 at 4 (268 MB) 87.
 //
 // FUSED (up to FEW rows): the wave transforms its blocks of the rows itself, two
 // channels a lane, with a power of two of their own, which saves a launch; each of
@@ -489,10 +495,10 @@ __global__ void __launch_bounds__(512) linear_rows_kernel(LinearArgs a) {
 // waves, 256 columns, of a share of the input channels. Rows come through shared
 // memory for all waves; each wave decodes its own columns, one step ahead of the
 // products, and its words come through shared memory as above. 64 rows of 4096 by
-// 4096, 22 us: 5 to turn the rows, 12 here, 4 to join 16 shares (four waves of twice
+// 4096, 21 us: 5 to turn the rows, 12 here, 4 to join 16 shares (four waves of twice
 // the columns and 32 shares, which two waves a SIMD hide less of: 30). Latency and the
-// vector instructions of decoding bound it: 20 rows of 12288 by 4096 take 28 us, 64
-// 35.
+// vector instructions of decoding bound it: 20 rows of 12288 by 4096 take 27 us, 64
+// 33.
 //
 // In step s rows s + DEPTH + 1 and words s + DEPTH + 2 are sent for, in as many
 // instructions each step (past the end the last ones again, which nobody uses), so
@@ -628,7 +634,7 @@ __global__ void __launch_bounds__(512, 2) linear_blocks_kernel(LinearArgs a) {
 // Products begin with a wave's own operands, and rows are read for the next step as
 // this one's are used up, so nothing is waited for after the barrier.
 //
-// 4096 rows of 4096 by 4096, one round of the chip: 159 us with the rows' turning, 0.86
+// 4096 rows of 4096 by 4096, one round of the chip: 159 to 161 us with the rows' turning, 0.86
 // PFLOP/s (a library product of 8192 a side reaches 1.21). Of a step's 1.0 us, 0.8 are
 // left without decoding and reading: the rate of the matrix instructions bounds it, then
 // their overlap with vector ones. 2055 rows of 4096 by 12288, 480 workgroups: 258 us.
@@ -869,10 +875,12 @@ constexpr int BLOCK_ROWS[] = {FEW, 8, 16, 32, 48, 64, 128};
 
 // How a call is cut: the variant of the fewest rows that takes them all (two float16
 // parts). Times in a graph, us, of the one chosen and of the next larger one, at 4
-// bits: 1 row of 4096 by 4096 9.0 and 12.6, 4 rows 10.3 and 13.0; 8 rows of 4096 by
-// 12288 17.7 and 18.7; 16 rows of 12288 by 4096 24.4 and 27.0; 32 rows of 4096 by 4096
-// 16.9 and 18.3; 48 rows of 4096 by 12288 32.1 and 33.1; 128 rows of 4096 by 4096
-// (bfloat16) 28.0 and 30.1.
+// bits: 1 row of 4096 by 4096 9.0 and 12.3, 4 rows 10.2 and 12.5; 8 rows of 4096 by
+// 12288 17.0 and 18.5; 16 rows of 12288 by 4096 23.7 and 26.2; 32 rows of 4096 by 4096
+// 16.1 and 16.5; 48 rows of 4096 by 12288 30.1 and 30.8; 64 rows of 4096 by 4096
+// (float16) 20.8 and 28.7; 128 rows (bfloat16) 27.2 and 32.8. Of larger weights 2 to 4
+// rows would gain by the variant of 8, whose waves do not each turn the rows: 4 rows of
+// 4096 by 12288 17.7 and 16.7; 2 and 4 rows of 8192 by 28672 53 and 66, and 45.
 struct Plan {
   Variant variant;
   int parts;                       // float16 parts of a value: 2, or 1 of more than 64 bfloat16 rows
@@ -895,7 +903,10 @@ Plan plan_of(int64_t rows, int64_t k, int64_t n, bool bf16) {
   // Shares of the input channels that fill the chip: a wave of linear_rows_kernel
   // takes at least one block of 128, a workgroup of linear_blocks_kernel too; one of
   // linear_wide_kernel at least 640 channels, as the shares' sums go through memory
-  // (300 rows of 4096 by 4096: 8 shares 58 us, 6 52; 200 rows: 16 45 us, 6 39).
+  // (300 rows of 4096 by 4096 in shares of 384, 640 and 1024 channels at least: 48, 44
+  // and 48 us; in float16 47 each, at 1280 53). Fewer workgroups would take smaller
+  // ones: 200 rows 36, 40 and 44, 130 rows 30, 34 and 40, 520 of 4096 by 1024 35, 40
+  // and 46.
   const bool few = p.variant <= ROWS16;
   p.groups = (int)(few ? n / 32 : (n + 255) / 256);
   const int64_t most = std::max<int64_t>(1, few ? k / (8 * HAD) : p.variant == BLOCK_WIDE ? k / (5 * HAD) : k / HAD);
@@ -909,8 +920,9 @@ Plan plan_of(int64_t rows, int64_t k, int64_t n, bool bf16) {
     // Blocks of 8, 7 or 6 sets (of two parts, 8 or 6) by the time of the last
     // workgroup: rounds of the chip, times a step, which takes as long as the products
     // of its sets and about two more, over the shares. (2055 rows of 4096 by 12288:
-    // 8 sets 273 us, 7 262, 6 352; 300 rows of 4096 by 4096: 8 sets 52, 6 44; 4096 rows:
-    // 170 and 250.)
+    // 8 sets 265 us, 7 254, 6 344; 300 rows of 4096 by 4096: 51, 47, 44; 4096 rows: 162,
+    // 256, 242; two parts, 520 rows of 4096 by 12288: 8 sets 130, 6 210. The sums of more
+    // shares are not counted: 200 rows of 4096 by 4096 39, 38, 41.)
     int64_t least = INT64_MAX, best = 8;
     for (int64_t sets = 8; sets >= 6; sets -= p.parts) {
       cut(32 * sets / p.parts);
